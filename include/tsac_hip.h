@@ -490,6 +490,150 @@ int tsac_hip_attention_causal(const uint16_t* qkv, size_t heads, size_t head_wid
                               size_t sequences, size_t max_length, const uint16_t* rotations,
                               float scale, uint16_t* out, void* stream);
 
+/* ---- drafted decoding: a paged cache, attention over it, verification -----------
+ * No counterpart in the reference, whose decode takes one known-next token at a
+ * time. Several drafted tokens of a sequence, a chain or a tree, go through the
+ * model in one step: their keys and values are written behind the cached ones,
+ * each row attends to the cache and to the drafted rows on its own line, the
+ * drafts are held against the model's probabilities, and the rows of those
+ * accepted stay. Sums here have no fixed reference order: the range coder's
+ * distributions come from the entry points above.
+ *
+ * Calls are ordered on `stream`, run on the current device, neither allocate nor
+ * wait, and may be captured into a graph. Sizes and pointers are checked on the
+ * host. What is in device memory is checked by the kernels: a call that finds a
+ * number, length or page out of range stays inside the given memory, does what
+ * its declaration says, and writes one of these to `status` (device memory, or
+ * NULL; 0 beforehand, never cleared by a call). */
+#define TSAC_HIP_PAGES_INVALID 1   /* a sequence, length, path or page out of range */
+#define TSAC_HIP_PAGES_EXHAUSTED 2 /* fewer free pages than the call needs */
+
+/* 16-bit element types of keys, values, queries and outputs, and of probabilities. */
+#define TSAC_HIP_TYPE_BF16 0
+#define TSAC_HIP_TYPE_FP16 1
+#define TSAC_HIP_TYPE_FP32 2 /* probabilities only */
+
+/* A cache of keys and values in pages of page_rows positions (a power of two, 16
+ * to 1024), shared by `layers` layers and `sequences` sequences. All pointers are
+ * device memory of the caller's. keys and values: [layers][pages][page_rows]
+ * [heads][head_width] 16-bit elements, head_width 64 or 128, at the given strides
+ * (in elements, multiples of 8; the heads of a row lie one after the other; 16-byte
+ * aligned). table[s * table_stride + i] is the page of positions i * page_rows on
+ * of sequence s, for i < held[s]; lengths[s] positions are in use. references[p]
+ * counts the sequences that hold page p; 0 is free. Before the first call: held,
+ * lengths and references all 0. At most 65535 sequences, 255 layers and 2^20 pages
+ * a sequence. */
+typedef struct tsac_hip_paged_cache
+{
+    void* keys;
+    void* values;
+    size_t layer_stride, page_stride, row_stride;
+    uint32_t layers, pages, page_rows, heads, head_width;
+    int32_t type; /* TSAC_HIP_TYPE_BF16 or TSAC_HIP_TYPE_FP16 */
+    int32_t* table;
+    size_t table_stride;
+    int32_t* held;
+    int32_t* lengths;
+    int32_t* references;
+    uint32_t sequences;
+} tsac_hip_paged_cache;
+
+/* Pages for rows[i] positions past the length of sequence sequences[i] (device
+ * arrays of `count` <= 8192 numbers; sequences NULL: 0 .. count-1), the lowest free
+ * ones in the order of the list. All or nothing: a sequence listed twice or out of
+ * range, a negative number, a table too short (INVALID) or a pool too small
+ * (EXHAUSTED) leaves everything as it was. */
+int tsac_hip_pages_reserve(const tsac_hip_paged_cache* cache, const int32_t* sequences, const int32_t* rows,
+                           size_t count, int32_t* status, void* stream);
+
+/* Makes targets[i], which holds nothing, a copy of sources[i]: it shares the pages
+ * that are full and gets a copy of the last one's used rows, in every layer, in a
+ * page of its own. Positions below the length of a fork are not to be written
+ * afterwards. One source may have several targets; a target listed twice, that is a
+ * source too or holds pages is INVALID. All or nothing, as tsac_hip_pages_reserve;
+ * a table entry out of range is passed on as -1 (INVALID). */
+int tsac_hip_pages_fork(const tsac_hip_paged_cache* cache, const int32_t* sources, const int32_t* targets,
+                        size_t count, int32_t* status, void* stream);
+
+/* Gives back the pages of each listed sequence (NULL: 0 .. count-1): counts them
+ * down, clears its table entries to -1, its length and what it holds to 0. A
+ * sequence listed twice is freed once; one out of range, or a page that is not
+ * counted, is passed over (INVALID). */
+int tsac_hip_pages_free(const tsac_hip_paged_cache* cache, const int32_t* sequences, size_t count, int32_t* status,
+                        void* stream);
+
+/* Rows starts[s] .. starts[s+1]-1 (device, [sequences + 1], ascending) of keys and
+ * values, [layers][rows][heads][head_width] at their strides (elements, multiples of
+ * 8; 16-byte aligned), to the positions from lengths[s] on of sequence s, in layers
+ * layer .. layer + layers - 1. max_rows: the most rows of one sequence; further ones
+ * are not written. lengths stay. A row without a page, or whose page another sequence
+ * holds too, is passed over (INVALID). */
+int tsac_hip_pages_write(const tsac_hip_paged_cache* cache, uint32_t layer, uint32_t layers, const void* keys,
+                         const void* values, size_t layer_stride, size_t row_stride, size_t rows,
+                         const int32_t* starts, size_t max_rows, int32_t* status, void* stream);
+
+/* Keeps accepted[s] of the rows behind lengths[s], in every layer: position
+ * lengths[s] + k takes what is at lengths[s] + path[s * path_stride + k], for
+ * k < accepted[s]; the path ascends and stays below the sequence's starts[s+1] -
+ * starts[s] rows. lengths_out[s] = lengths[s] + accepted[s]; it may be the cache's
+ * own lengths. A sequence whose path is not one is left as it was (INVALID), a row
+ * without a page of its own is not moved (INVALID). Pages stay held. */
+int tsac_hip_pages_keep(const tsac_hip_paged_cache* cache, const int32_t* starts, const int32_t* path,
+                        size_t path_stride, const int32_t* accepted, int32_t* lengths_out, int32_t* status,
+                        void* stream);
+
+/* Ancestor bits of drafted rows: parents[r] is the place, within its sequence, of row
+ * r's parent, which precedes it; anything else makes the row a root. Bit j of
+ * mask[r][words] is set for the row itself and every row above it. max_rows (at most
+ * 1024 and 64 * words): rows past it in a sequence are left as they were. */
+int tsac_hip_tree_mask(const int32_t* parents, size_t rows, const int32_t* starts, size_t sequences,
+                       size_t max_rows, uint64_t* mask, size_t words, void* stream);
+
+/* Attention of rows starts[s] .. starts[s+1]-1 of query [rows][heads][head_width] over
+ * sequence s of one layer of the cache, where the rows' own keys and values are
+ * written already: every row sees the lengths[s] cached positions, and of the
+ * sequence's rows those whose bit is set in mask[row][words] or, with mask NULL,
+ * itself and those in front of it. Query head h reads head h / (heads /
+ * cache->heads). out [rows][heads][head_width] = softmax(scale q k) v; a row that sees
+ * no key (or none with a score above -infinity) is 0. Keys and values that a row does
+ * not see do not reach it, whatever they are; a position whose page is out of range
+ * or not held is seen by none. Strides in elements, multiples of 8; 16-byte aligned.
+ * max_rows: the most rows of one sequence, at most 65536; further rows are left as
+ * they were. max_length: about the longest lengths[s] plus its rows (it shapes the
+ * launch; any value gives the result). Workspace: tsac_hip_attention_paged_workspace
+ * bytes of device memory, 16-byte aligned, not shared by calls that overlap. */
+size_t tsac_hip_attention_paged_workspace(const tsac_hip_paged_cache* cache, size_t rows, size_t heads,
+                                          size_t max_rows, size_t max_length);
+int tsac_hip_attention_paged(const tsac_hip_paged_cache* cache, uint32_t layer, const void* query,
+                             size_t query_stride, size_t rows, size_t heads, const int32_t* starts, size_t max_rows,
+                             size_t max_length, const uint64_t* mask, size_t words, float scale, void* out,
+                             size_t out_stride, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Holds drafted tokens against the target's probabilities with given random numbers,
+ * so that what is accepted and followed by `next` is distributed as the target's
+ * own samples. Rows starts[s] .. starts[s+1]-1 are the nodes of sequence s: node 0 is
+ * the last token it has, each other a drafted token behind its parent, which
+ * precedes it (parents as for tsac_hip_tree_mask; a node with none is not reached).
+ * target [rows][alphabet]: the target's distribution behind each node; draft: the
+ * drafter's, from which every child of the node was drawn, or NULL where a drafted
+ * token was certain. Values of `type`, strides in elements; what is negative or not
+ * finite counts as 0. Children are tried in order, child c with uniforms[c] in
+ * [0, 1): accepted if u q(x) W < max(0, p(x) - S q(x)), S = 0 and W = 1 at first; if
+ * not, S += W and W = sum max(0, p - S q). Without draft: accepted if u W < p(x); if
+ * not, W -= p(x) and p(x) = 0. Where no child is accepted, next[s] is the lowest token
+ * whose inclusive sum of max(0, p - S q) (or p) exceeds draws[s] in [0, 1) times the
+ * whole sum; if that is 0, of the row of p as it is; if that is 0 too, -1. path
+ * [sequences][max_nodes]: node 0 and the accepted ones, then -1; accepted[s]: their
+ * number. A sequence without nodes: 0, -1. Sums are 64-bit and of one order. At most
+ * 1024 nodes a sequence (further ones are not looked at) and 2^20 tokens.
+ * Workspace as for tsac_hip_attention_paged. */
+size_t tsac_hip_verify_drafts_workspace(size_t sequences, size_t max_nodes, size_t alphabet, int type);
+int tsac_hip_verify_drafts(const void* target, size_t target_stride, const void* draft, size_t draft_stride,
+                           int type, size_t alphabet, size_t rows, const int32_t* tokens, const int32_t* parents,
+                           const int32_t* starts, size_t sequences, size_t max_nodes, const float* uniforms,
+                           const float* draws, int32_t* path, int32_t* accepted, int32_t* next, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
 /* ---- calibration (no counterpart in the reference) ------------------------- */
 
 /* The attainable rates roofline fractions are read against, for benchmarks on

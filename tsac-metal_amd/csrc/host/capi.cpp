@@ -1,6 +1,7 @@
 // C ABI of the probability model (include/tsac_hip.h). Exceptions stop here and
 // become a nonzero status plus a thread-local message.
 #include "../../../include/tsac_hip.h"
+#include "../kernels/paged.hpp"
 #include "audio.hpp"
 #include "runtime.hpp"
 #include "source.hpp"
@@ -602,6 +603,83 @@ LinearPath path_of(int path)
            : path == TSAC_HIP_PATH_GEMM  ? LinearPath::gemm
            : path == TSAC_HIP_PATH_SMALL ? LinearPath::small
                                          : LinearPath::automatic;
+}
+
+// A cache description's sizes and pointers; what its device arrays hold, the kernels check.
+PagedCache paged_cache_of(const tsac_hip_paged_cache* c)
+{
+    require(c != nullptr, "missing argument");
+    require(c->type == TSAC_HIP_TYPE_BF16 || c->type == TSAC_HIP_TYPE_FP16, "paged cache: type must be BF16 or FP16");
+    require(c->head_width == 64 || c->head_width == 128, "paged cache: head width must be 64 or 128");
+    require(c->page_rows >= 16 && c->page_rows <= 1024 && !(c->page_rows & (c->page_rows - 1)),
+            "paged cache: page rows must be a power of two from 16 to 1024");
+    require(c->heads > 0 && c->heads <= 4096 && c->layers > 0 && c->layers <= unsigned(max_layers) && c->pages > 0 &&
+                c->pages < (1u << 31) && c->sequences <= unsigned(max_sequences),
+            "paged cache: size out of range");
+    require(c->table_stride > 0 && c->table_stride <= std::size_t(max_table_pages), "paged cache: table out of range");
+    const std::size_t row = std::size_t(c->heads) * c->head_width;
+    require(c->row_stride >= row && c->row_stride < (std::size_t(1) << 24) && c->row_stride % 8 == 0 &&
+                c->page_stride % 8 == 0 && c->layer_stride % 8 == 0,
+            "paged cache: strides must be multiples of 8 elements, rows apart");
+    require(c->keys && c->values && c->table && c->held && c->lengths && c->references, "missing argument");
+    require((reinterpret_cast<std::uintptr_t>(c->keys) | reinterpret_cast<std::uintptr_t>(c->values)) % 16 == 0,
+            "paged cache: keys and values must be 16-byte aligned");
+    PagedCache p;
+    p.keys = static_cast<uint16_t*>(c->keys);
+    p.values = static_cast<uint16_t*>(c->values);
+    p.layer_stride = c->layer_stride;
+    p.page_stride = c->page_stride;
+    p.row_stride = c->row_stride;
+    p.layers = int(c->layers);
+    p.pages = int(c->pages);
+    p.page_rows = int(c->page_rows);
+    p.heads = int(c->heads);
+    p.head_width = int(c->head_width);
+    p.half = c->type == TSAC_HIP_TYPE_FP16;
+    p.table = c->table;
+    p.table_stride = c->table_stride;
+    p.held = c->held;
+    p.lengths = c->lengths;
+    p.references = c->references;
+    p.sequences = int(c->sequences);
+    return p;
+}
+
+void require_aligned(const void* pointer, std::size_t stride, const char* message)
+{
+    require(reinterpret_cast<std::uintptr_t>(pointer) % 16 == 0 && stride % 8 == 0, message);
+}
+
+constexpr std::size_t max_new_rows = std::size_t(1) << 24; // of one call
+
+PagedRows paged_rows_of(const PagedCache& cache, std::size_t rows, std::size_t heads, std::size_t max_rows,
+                        std::size_t max_length)
+{
+    require(rows < max_new_rows && max_rows <= 65536 && max_length < (std::size_t(1) << 30),
+            "paged attention: rows or length out of range");
+    require(heads > 0 && heads <= 65536 && heads % std::size_t(cache.heads) == 0,
+            "paged attention: heads must be a multiple of the cache's");
+    PagedRows r;
+    r.rows = int(rows);
+    r.heads = int(heads);
+    r.max_rows = int(max_rows);
+    r.max_length = max_length;
+    return r;
+}
+
+Drafts drafts_of(std::size_t sequences, std::size_t max_nodes, std::size_t alphabet, int type)
+{
+    require(type >= TSAC_HIP_TYPE_BF16 && type <= TSAC_HIP_TYPE_FP32, "verify: invalid type");
+    require(alphabet > 0 && alphabet <= (std::size_t(1) << 20), "verify: alphabets of 1 to 2^20 tokens");
+    require(max_nodes <= std::size_t(max_draft_nodes) && (max_nodes > 0 || !sequences),
+            "verify: trees of 1 to 1024 nodes");
+    require(sequences < (std::size_t(1) << 24), "verify: too many sequences");
+    Drafts d;
+    d.type = type;
+    d.alphabet = int(alphabet);
+    d.sequences = int(sequences);
+    d.max_nodes = int(max_nodes);
+    return d;
 }
 } // namespace
 
@@ -1345,6 +1423,184 @@ int tsac_hip_attention_causal(const uint16_t* qkv, size_t heads, size_t head_wid
         {
             attention_prefill(qkv, heads * head_width, heads, head_width, start, length, replay,
                               sequences, max_length, rotations, scale, out, as_stream(stream));
+        });
+}
+
+int tsac_hip_pages_reserve(const tsac_hip_paged_cache* cache, const int32_t* sequences, const int32_t* rows,
+                           size_t count, int32_t* status, void* stream)
+{
+    return guarded(
+        [&]
+        {
+            const PagedCache c = paged_cache_of(cache);
+            require(rows || !count, "missing argument");
+            require(count <= std::size_t(max_listed_sequences) && (sequences || count <= std::size_t(c.sequences)),
+                    "pages: too many sequences in one call");
+            pages_reserve(c, sequences, rows, count, status, as_stream(stream));
+        });
+}
+
+int tsac_hip_pages_fork(const tsac_hip_paged_cache* cache, const int32_t* sources, const int32_t* targets,
+                        size_t count, int32_t* status, void* stream)
+{
+    return guarded(
+        [&]
+        {
+            const PagedCache c = paged_cache_of(cache);
+            require((sources && targets) || !count, "missing argument");
+            require(count <= std::size_t(max_listed_sequences), "pages: too many sequences in one call");
+            pages_fork(c, sources, targets, count, status, as_stream(stream));
+        });
+}
+
+int tsac_hip_pages_free(const tsac_hip_paged_cache* cache, const int32_t* sequences, size_t count, int32_t* status,
+                        void* stream)
+{
+    return guarded(
+        [&]
+        {
+            const PagedCache c = paged_cache_of(cache);
+            require(count <= std::size_t(max_sequences) && (sequences || count <= std::size_t(c.sequences)),
+                    "pages: too many sequences in one call");
+            pages_free(c, sequences, count, status, as_stream(stream));
+        });
+}
+
+int tsac_hip_pages_write(const tsac_hip_paged_cache* cache, uint32_t layer, uint32_t layers, const void* keys,
+                         const void* values, size_t layer_stride, size_t row_stride, size_t rows,
+                         const int32_t* starts, size_t max_rows, int32_t* status, void* stream)
+{
+    return guarded(
+        [&]
+        {
+            const PagedCache c = paged_cache_of(cache);
+            require(starts && ((keys && values) || !rows), "missing argument");
+            require(layer <= unsigned(c.layers) && layers <= unsigned(c.layers) - layer, "pages: layers out of range");
+            require(rows < max_new_rows && max_rows < max_new_rows, "pages: too many rows in one call");
+            require_aligned(keys, row_stride, "pages: rows must be 16-byte aligned");
+            require_aligned(values, layer_stride, "pages: rows must be 16-byte aligned");
+            NewRows fresh;
+            fresh.keys = static_cast<const uint16_t*>(keys);
+            fresh.values = static_cast<const uint16_t*>(values);
+            fresh.layer_stride = layer_stride;
+            fresh.row_stride = row_stride;
+            fresh.rows = int(rows);
+            pages_write(c, int(layer), int(layers), fresh, starts, int(std::min(rows, max_rows)), status,
+                        as_stream(stream));
+        });
+}
+
+int tsac_hip_pages_keep(const tsac_hip_paged_cache* cache, const int32_t* starts, const int32_t* path,
+                        size_t path_stride, const int32_t* accepted, int32_t* lengths_out, int32_t* status,
+                        void* stream)
+{
+    return guarded(
+        [&]
+        {
+            const PagedCache c = paged_cache_of(cache);
+            require(starts && path && accepted && lengths_out, "missing argument");
+            pages_keep(c, starts, path, path_stride, accepted, lengths_out, status, as_stream(stream));
+        });
+}
+
+int tsac_hip_tree_mask(const int32_t* parents, size_t rows, const int32_t* starts, size_t sequences,
+                       size_t max_rows, uint64_t* mask, size_t words, void* stream)
+{
+    return guarded(
+        [&]
+        {
+            require(starts && ((parents && mask) || !rows), "missing argument");
+            require(rows < max_new_rows && sequences <= std::size_t(max_sequences), "tree mask: size out of range");
+            require(words > 0 && words <= std::size_t(max_draft_nodes) / 64 && max_rows <= 64 * words,
+                    "tree mask: at most 64 rows a word, 16 words");
+            tree_mask(parents, int(rows), starts, int(sequences), int(max_rows), mask, words, as_stream(stream));
+        });
+}
+
+size_t tsac_hip_attention_paged_workspace(const tsac_hip_paged_cache* cache, size_t rows, size_t heads,
+                                          size_t max_rows, size_t max_length)
+{
+    size_t bytes = 0;
+    guarded(
+        [&]
+        {
+            const PagedCache c = paged_cache_of(cache);
+            bytes = attention_paged_workspace(c, paged_rows_of(c, rows, heads, max_rows, max_length));
+        });
+    return bytes;
+}
+
+int tsac_hip_attention_paged(const tsac_hip_paged_cache* cache, uint32_t layer, const void* query,
+                             size_t query_stride, size_t rows, size_t heads, const int32_t* starts, size_t max_rows,
+                             size_t max_length, const uint64_t* mask, size_t words, float scale, void* out,
+                             size_t out_stride, void* workspace, size_t workspace_bytes, void* stream)
+{
+    return guarded(
+        [&]
+        {
+            const PagedCache c = paged_cache_of(cache);
+            PagedRows r = paged_rows_of(c, rows, heads, max_rows, max_length);
+            require(starts && ((query && out) || !rows), "missing argument");
+            require(layer < unsigned(c.layers), "paged attention: layer out of range");
+            require(!mask || (words > 0 && words <= 1024), "paged attention: 1 to 1024 mask words a row");
+            require_aligned(query, query_stride, "paged attention: rows must be 16-byte aligned");
+            require_aligned(out, out_stride, "paged attention: rows must be 16-byte aligned");
+            require(reinterpret_cast<std::uintptr_t>(workspace) % 16 == 0,
+                    "paged attention: the workspace must be 16-byte aligned");
+            const std::size_t row = heads * std::size_t(c.head_width);
+            require(rows <= 1 || (query_stride >= row && out_stride >= row), "paged attention: rows overlap");
+            r.query = static_cast<const uint16_t*>(query);
+            r.query_stride = query_stride;
+            r.out = static_cast<uint16_t*>(out);
+            r.out_stride = out_stride;
+            r.starts = starts;
+            r.mask = mask;
+            r.words = words;
+            r.scale = scale;
+            attention_paged(c, int(layer), r, workspace, workspace_bytes, as_stream(stream));
+        });
+}
+
+size_t tsac_hip_verify_drafts_workspace(size_t sequences, size_t max_nodes, size_t alphabet, int type)
+{
+    size_t bytes = 0;
+    guarded([&] { bytes = verify_drafts_workspace(drafts_of(sequences, max_nodes, alphabet, type)); });
+    return bytes;
+}
+
+int tsac_hip_verify_drafts(const void* target, size_t target_stride, const void* draft, size_t draft_stride,
+                           int type, size_t alphabet, size_t rows, const int32_t* tokens, const int32_t* parents,
+                           const int32_t* starts, size_t sequences, size_t max_nodes, const float* uniforms,
+                           const float* draws, int32_t* path, int32_t* accepted, int32_t* next, void* workspace,
+                           size_t workspace_bytes, void* stream)
+{
+    return guarded(
+        [&]
+        {
+            Drafts d = drafts_of(sequences, max_nodes, alphabet, type);
+            require((target && tokens && parents && uniforms) || !rows, "missing argument");
+            require((starts && draws && path && accepted && next) || !sequences, "missing argument");
+            require(rows < max_new_rows, "verify: too many rows");
+            require(rows <= 1 || (target_stride >= alphabet && (!draft || draft_stride >= alphabet)),
+                    "verify: rows overlap");
+            const std::size_t size = type == TSAC_HIP_TYPE_FP32 ? 4 : 2;
+            require((reinterpret_cast<std::uintptr_t>(target) | reinterpret_cast<std::uintptr_t>(draft)) % size == 0 &&
+                        reinterpret_cast<std::uintptr_t>(workspace) % 16 == 0,
+                    "verify: misaligned pointer");
+            d.target = target;
+            d.target_stride = target_stride;
+            d.draft = draft;
+            d.draft_stride = draft_stride;
+            d.rows = int(rows);
+            d.tokens = tokens;
+            d.parents = parents;
+            d.starts = starts;
+            d.uniforms = uniforms;
+            d.draws = draws;
+            d.path = path;
+            d.accepted = accepted;
+            d.next = next;
+            verify_drafts(d, workspace, workspace_bytes, as_stream(stream));
         });
 }
 

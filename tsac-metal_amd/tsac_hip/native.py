@@ -41,10 +41,15 @@ EXPORTS = (
     "tsac_hip_prepared_dac_destroy", "tsac_hip_model_create_from_source", "tsac_hip_dac_create_from_source",
     "tsac_hip_pcm16_read", "tsac_hip_wave_read", "tsac_hip_wave_write", "tsac_hip_audio_header",
     "tsac_hip_parse_header", "tsac_hip_cli_parse", "tsac_hip_cli_help",
+    "tsac_hip_pages_reserve", "tsac_hip_pages_fork", "tsac_hip_pages_free", "tsac_hip_pages_write",
+    "tsac_hip_pages_keep", "tsac_hip_tree_mask", "tsac_hip_attention_paged_workspace", "tsac_hip_attention_paged",
+    "tsac_hip_verify_drafts_workspace", "tsac_hip_verify_drafts",
 )
 
 PATH_AUTO, PATH_GEMV, PATH_GEMM, PATH_GEMM_TILES, PATH_SMALL = 0, 1, 2, 3, 4
 PASS_ENCODE, PASS_DECODE = 0, 1
+TYPE_BF16, TYPE_FP16, TYPE_FP32 = 0, 1, 2
+PAGES_INVALID, PAGES_EXHAUSTED = 1, 2
 
 
 class HipError(RuntimeError):
@@ -124,6 +129,13 @@ class CliOptions(C.Structure):
 class EncodeOptions(C.Structure):
     _fields_ = [("method", C.c_uint8), ("codebooks", C.c_uint8), ("separate_channels", C.c_uint8),
                 ("entropy_batch", C.c_uint16)]
+
+
+class PagedCacheDesc(C.Structure):
+    _fields_ = [("keys", vp), ("values", vp), ("layer_stride", sz), ("page_stride", sz), ("row_stride", sz),
+                ("layers", C.c_uint32), ("pages", C.c_uint32), ("page_rows", C.c_uint32), ("heads", C.c_uint32),
+                ("head_width", C.c_uint32), ("type", C.c_int32), ("table", vp), ("table_stride", sz), ("held", vp),
+                ("lengths", vp), ("references", vp), ("sequences", C.c_uint32)]
 
 
 def header(frames, batch, groups, codebooks, model_channels=2, method=1) -> Header:
@@ -208,6 +220,21 @@ def library() -> C.CDLL:
         lib.tsac_hip_parse_header.argtypes = [u8p, sz, C.POINTER(Limits), C.POINTER(Header)]
         lib.tsac_hip_cli_parse.argtypes = [sz, C.POINTER(C.c_char_p), C.POINTER(CliOptions)]
         lib.tsac_hip_cli_help.restype = C.c_char_p
+        cache = C.POINTER(PagedCacheDesc)
+        lib.tsac_hip_pages_reserve.argtypes = [cache, vp, vp, sz, vp, vp]
+        lib.tsac_hip_pages_fork.argtypes = [cache, vp, vp, sz, vp, vp]
+        lib.tsac_hip_pages_free.argtypes = [cache, vp, sz, vp, vp]
+        lib.tsac_hip_pages_write.argtypes = [cache, C.c_uint32, C.c_uint32, vp, vp, sz, sz, sz, vp, sz, vp, vp]
+        lib.tsac_hip_pages_keep.argtypes = [cache, vp, vp, sz, vp, vp, vp, vp]
+        lib.tsac_hip_tree_mask.argtypes = [vp, sz, vp, sz, sz, vp, sz, vp]
+        lib.tsac_hip_attention_paged_workspace.argtypes = [cache, sz, sz, sz, sz]
+        lib.tsac_hip_attention_paged_workspace.restype = sz
+        lib.tsac_hip_attention_paged.argtypes = [cache, C.c_uint32, vp, sz, sz, sz, vp, sz, sz, vp, sz, C.c_float, vp, sz,
+                                                 vp, sz, vp]
+        lib.tsac_hip_verify_drafts_workspace.argtypes = [sz, sz, sz, C.c_int]
+        lib.tsac_hip_verify_drafts_workspace.restype = sz
+        lib.tsac_hip_verify_drafts.argtypes = [vp, sz, vp, sz, C.c_int, sz, sz, vp, vp, vp, sz, sz, vp, vp, vp, vp, vp,
+                                               vp, sz, vp]
         _lib = lib
     return _lib
 
@@ -820,6 +847,191 @@ def attention_causal(qkv, heads, head_width, start, length, replay, sequences, m
     check(library().tsac_hip_attention_causal(
         _dp(qkv), heads, head_width, _dp(start), _dp(length), _dp(replay), sequences, max_length,
         _dp(rotations) if rotations is not None else None, scale, _dp(out), _stream(stream)))
+
+
+# ---------------------------------------------------------------- drafted decoding
+
+def _need(condition, message):
+    if not condition:
+        raise HipError(message)
+
+
+def _array(tensor, device, kind, count, name):
+    """The address of a contiguous device tensor of at least `count` elements (kind: its dtype's name)."""
+    _need(tensor.device == device, f"{name}: on {tensor.device}, not on {device}")
+    _need(str(tensor.dtype) == kind and tensor.is_contiguous(), f"{name}: must be contiguous {kind}")
+    _need(tensor.numel() >= count, f"{name}: {tensor.numel()} elements, {count} needed")
+    return tensor.data_ptr()
+
+
+_INT, _FLOAT, _LONG = "torch.int32", "torch.float32", "torch.int64"
+#: Element types by dtype; int16 holds BF16 bits, as in the other operators.
+_ROW_TYPES = {"torch.bfloat16": TYPE_BF16, "torch.int16": TYPE_BF16, "torch.float16": TYPE_FP16}
+
+
+def _current(device):
+    import torch
+
+    _need(device.type == "cuda" and device.index == torch.cuda.current_device(),
+          f"tensors are on {device}, which is not the current device")
+    return _stream()
+
+
+def _rows(tensor, device, heads, width, type_, name):
+    """(address, row stride) of [rows][heads][width], the heads of a row one after the other."""
+    _need(tensor.device == device and _ROW_TYPES.get(str(tensor.dtype)) == type_, f"{name}: another device or type")
+    shape, strides = tensor.shape, tensor.stride()
+    _need(len(shape) == 3 and shape[1] == heads and shape[2] == width, f"{name}: must be [rows][{heads}][{width}]")
+    _need((strides[2] == 1 and (heads == 1 or strides[1] == width)) or not shape[0], f"{name}: heads must be contiguous")
+    return tensor.data_ptr(), strides[0] if shape[0] > 1 else heads * width
+
+
+class PagedCache:
+    """A paged cache over a program's own tensors (tsac_hip_paged_cache): keys and values
+    [layers][pages][page_rows][heads][head_width] of one type and layout, table
+    [sequences][pages a sequence], held, lengths and references int32, on one device."""
+
+    def __init__(self, keys, values, table, held, lengths, references):
+        shape, strides = keys.shape, keys.stride()
+        _need(len(shape) == 5 and values.shape == shape and values.stride() == strides and values.dtype == keys.dtype,
+              "keys and values: must be [layers][pages][page_rows][heads][head_width], laid out alike")
+        _need(str(keys.dtype) in _ROW_TYPES, "keys and values: must be bfloat16, float16 or int16")
+        self.layers, self.pages, self.page_rows, self.heads, self.head_width = shape
+        self.type, self.device, self.sequences = _ROW_TYPES[str(keys.dtype)], keys.device, table.shape[0]
+        _need(strides[4] == 1 and (shape[3] == 1 or strides[3] == shape[4]), "keys and values: heads must be contiguous")
+        _need(values.device == keys.device and table.dim() == 2, "table: must be [sequences][pages a sequence]")
+        self.tensors = (keys, values, table, held, lengths, references)  # what the addresses below belong to
+        n, d = self.sequences, self.device
+        self.desc = PagedCacheDesc(
+            keys.data_ptr(), values.data_ptr(), strides[0], strides[1], strides[2], *shape, self.type,
+            _array(table, d, _INT, 0, "table"), table.shape[1], _array(held, d, _INT, n, "held"),
+            _array(lengths, d, _INT, n, "lengths"), _array(references, d, _INT, self.pages, "references"), n)
+        self._desc = C.byref(self.desc)
+
+    def _ints(self, tensor, count, name):
+        return _array(tensor, self.device, _INT, count, name)
+
+    def _status(self, status):
+        return None if status is None else self._ints(status, 1, "status")
+
+    def reserve(self, rows, sequences=None, status=None):
+        """Pages for rows[i] further positions of sequences[i] (all, if None)."""
+        n = rows.numel()
+        check(library().tsac_hip_pages_reserve(
+            self._desc, None if sequences is None else self._ints(sequences, n, "sequences"),
+            self._ints(rows, n, "rows"), n, self._status(status), _current(self.device)))
+
+    def fork(self, sources, targets, status=None):
+        """Makes targets[i] a copy of sources[i], sharing the full pages."""
+        n = sources.numel()
+        _need(targets.numel() == n, "sources and targets: one target a source")
+        check(library().tsac_hip_pages_fork(self._desc, self._ints(sources, n, "sources"),
+                                            self._ints(targets, n, "targets"), n, self._status(status),
+                                            _current(self.device)))
+
+    def free(self, sequences=None, status=None):
+        """Gives back the pages of the listed sequences (all, if None)."""
+        n = self.sequences if sequences is None else sequences.numel()
+        check(library().tsac_hip_pages_free(
+            self._desc, None if sequences is None else self._ints(sequences, n, "sequences"), n, self._status(status),
+            _current(self.device)))
+
+    def write(self, keys, values, starts, max_rows, layer=0, status=None):
+        """New rows, [layers][rows][heads][head_width] or, of one layer, [rows][heads][head_width], behind
+        each sequence's length."""
+        if keys.dim() == 3:
+            keys, values = keys[None], values[None]
+        _need(keys.dim() == 4 and keys.shape == values.shape and keys.stride() == values.stride(),
+              "keys and values: must be [layers][rows][heads][head_width], laid out alike")
+        _need(_ROW_TYPES.get(str(values.dtype)) == self.type and values.device == self.device,
+              "values: another device or type")
+        layers = keys.shape[0]
+        if not layers:
+            return
+        pointer, stride = _rows(keys[0], self.device, self.heads, self.head_width, self.type, "keys")
+        check(library().tsac_hip_pages_write(
+            self._desc, layer, layers, pointer, values.data_ptr(), keys.stride(0) if layers > 1 else 0, stride,
+            keys.shape[1], self._ints(starts, self.sequences + 1, "starts"), max_rows, self._status(status),
+            _current(self.device)))
+
+    def keep(self, starts, path, accepted, lengths=None, status=None):
+        """Moves each sequence's accepted rows (path [sequences][nodes], accepted) to the front of the
+        new ones, in every layer; lengths (the cache's own, if None) takes the new lengths."""
+        n = self.sequences
+        _need(path.dim() == 2, "path: must be [sequences][nodes]")
+        lengths = self.tensors[4] if lengths is None else lengths
+        check(library().tsac_hip_pages_keep(
+            self._desc, self._ints(starts, n + 1, "starts"), self._ints(path, n * path.shape[1], "path"),
+            path.shape[1], self._ints(accepted, n, "accepted"), self._ints(lengths, n, "lengths"),
+            self._status(status), _current(self.device)))
+
+
+def tree_mask(parents, starts, max_rows, mask):
+    """Ancestor bits (int64 mask [rows][words]) of drafted rows."""
+    device, rows, words = parents.device, parents.numel(), mask.shape[1]
+    check(library().tsac_hip_tree_mask(
+        _array(parents, device, _INT, rows, "parents"), rows, _array(starts, device, _INT, 1, "starts"),
+        starts.numel() - 1, max_rows, _array(mask, device, _LONG, rows * words, "mask"), words, _current(device)))
+
+
+def attention_paged_workspace(cache, rows, heads, max_rows, max_length) -> int:
+    return int(library().tsac_hip_attention_paged_workspace(cache._desc, rows, heads, max_rows, max_length))
+
+
+def _workspace(bytes_, workspace, device):
+    """(address, size): the caller's, or a new one, kept until the call is queued."""
+    import torch
+
+    if workspace is None:
+        if not bytes_:
+            return None, 0, None
+        workspace = torch.empty(bytes_, dtype=torch.uint8, device=device)
+    _need(workspace.device == device and workspace.is_contiguous(), "workspace: must be contiguous, on the same device")
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
+
+
+def attention_paged(cache, layer, query, starts, max_rows, max_length, mask, scale, out, workspace=None):
+    """Attention of new rows (query and out [rows][heads][head_width]) over the cache; mask int64
+    [rows][words] (tree_mask) or None for a chain. A new workspace a call, if none is given."""
+    device, heads, rows = cache.device, query.shape[1], query.shape[0]
+    lib = library()
+    q, q_stride = _rows(query, device, heads, cache.head_width, cache.type, "query")
+    o, o_stride = _rows(out, device, heads, cache.head_width, cache.type, "out")
+    _need(out.shape[0] == rows, "out: must have the query's rows")
+    words = 0 if mask is None else mask.shape[1]
+    need = lib.tsac_hip_attention_paged_workspace(cache._desc, rows, heads, max_rows, max_length)
+    space, size, keep = _workspace(need, workspace, device)
+    check(lib.tsac_hip_attention_paged(
+        cache._desc, layer, q, q_stride, rows, heads, _array(starts, device, _INT, cache.sequences + 1, "starts"),
+        max_rows, max_length, None if mask is None else _array(mask, device, _LONG, rows * words, "mask"), words, scale,
+        o, o_stride, space, size, _current(device)))
+    del keep
+
+
+_PROBABILITY_TYPES = dict(_ROW_TYPES, **{"torch.float32": TYPE_FP32})
+
+
+def verify_drafts(target, draft, tokens, parents, starts, max_nodes, uniforms, draws, path, accepted, next,
+                  workspace=None):
+    """Drafted trees against the target's distributions (target, draft [rows][alphabet], or draft None);
+    path int32 [sequences][max_nodes], accepted and next int32 [sequences] are written."""
+    device, (rows, alphabet), sequences = target.device, target.shape, starts.numel() - 1
+    type_ = _PROBABILITY_TYPES.get(str(target.dtype))
+    _need(type_ is not None and (alphabet <= 1 or target.stride(1) == 1), "target: must be rows of probabilities")
+    if draft is not None:
+        _need(draft.dtype == target.dtype and draft.shape == target.shape and draft.device == device and
+              (alphabet <= 1 or draft.stride(1) == 1), "draft: must be as target")
+    lib = library()
+    need = lib.tsac_hip_verify_drafts_workspace(sequences, max_nodes, alphabet, type_)
+    space, size, keep = _workspace(need, workspace, device)
+    check(lib.tsac_hip_verify_drafts(
+        target.data_ptr(), target.stride(0), None if draft is None else draft.data_ptr(),
+        0 if draft is None else draft.stride(0), type_, alphabet, rows, _array(tokens, device, _INT, rows, "tokens"),
+        _array(parents, device, _INT, rows, "parents"), _array(starts, device, _INT, 1, "starts"), sequences, max_nodes,
+        _array(uniforms, device, _FLOAT, rows, "uniforms"), _array(draws, device, _FLOAT, sequences, "draws"),
+        _array(path, device, _INT, sequences * max_nodes, "path"), _array(accepted, device, _INT, sequences, "accepted"),
+        _array(next, device, _INT, sequences, "next"), space, size, _current(device)))
+    del keep
 
 
 def probe_read(data, stream=None):
