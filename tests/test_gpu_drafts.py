@@ -3,10 +3,10 @@ through the C ABI, against plain implementations in 64 bits written from the def
 
 Attention's tolerance, element by element, with u half a step of the 16-bit type (2^-8 for BF16,
 2^-11 for half): the output's rounding is u |out|; each weight's rounding before the second product
-u sum w|v|; a score's error (32-bit sums of head_width products, their scaling and the exponential's
-argument) d = (head_width + 8) 2^-24 sum|q k| scale log2(e) moves a weight and its share of the sum by 2 d,
+u sum w|v|, and as the rounded weights are summed, sum w e v - out sum w e with |e| <= u, u |out| more; a
+score's error (32-bit sums of head_width products, their scaling and the exponential's argument) d = (head_width + 8) 2^-24 sum|q k| scale log2(e) moves a weight and its share of the sum by 2 d,
 the exponential itself and 32-bit sums of T terms by (T + 16) 2^-24:
-|error| <= u |out| + (u + 2 d + (T + 16) 2^-24) sum w|v|, times 1 + 2^-6 for products of these."""
+|error| <= 2 u |out| + (u + 2 d + (T + 16) 2^-24) sum w|v|, times 1 + 2^-6 for products of these."""
 import math
 import random
 
@@ -155,7 +155,7 @@ class Batch:
                     out[row, h] = w @ vv
                     spread = w @ vv.abs()
                     d = (self.width + 8) * 2.0 ** -24 * float((kk.abs() @ q[i, h].abs()).max()) * abs(self.scale) * 1.4427
-                    room[row, h] = (u * out[row, h].abs() + (u + 2 * d + (len(keep) + 16) * 2.0 ** -24) * spread) * (
+                    room[row, h] = (2 * u * out[row, h].abs() + (u + 2 * d + (len(keep) + 16) * 2.0 ** -24) * spread) * (
                         1 + 2.0 ** -6)
         return out, room
 
