@@ -23,6 +23,7 @@
 #include "paged.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace tsac_hip
 {
@@ -87,6 +88,11 @@ template <bool Half> __device__ __forceinline__ float widen(uint16_t bits)
     }
 }
 
+__device__ __forceinline__ float maximum(float a, float b, float c)
+{
+    return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
+}
+
 // Largest over the four lanes that hold a query.
 __device__ __forceinline__ float query_max(float value)
 {
@@ -124,6 +130,7 @@ struct Launch
     int parts;  // 16 rows each, of a sequence and head
     int splits, chunk; // chunks, keys of a chunk
     int units;         // sequences x chunks x key/value heads
+    int together;      // of them that one die takes
     float scale_log2;  // above or at 0
     bool negative;     // scale is below: queries are taken negative
 };
@@ -171,25 +178,33 @@ __device__ __forceinline__ int chunk_end(const Launch& l, const Place& p)
     return p.split == l.splits - 1 ? p.total : min(p.total, (p.split + 1) * l.chunk);
 }
 
+// A number that no kernel writes meanwhile, through the scalar cache: as a vector load, which the
+// compiler makes it beside assembly that touches memory, its wait would be one for all loads
+// of keys and values in flight (64 nodes over 131,001 positions: 187 us so).
+__device__ __forceinline__ int scalar_load(const int* from)
+{
+    return *(const __attribute__((address_space(4))) int*)reinterpret_cast<std::uintptr_t>(from);
+}
+
 // Where 16 keys from a position start, as an offset into keys and values; `there` if they lie in
 // a page of the pool, otherwise the offset is some page's.
 __device__ __forceinline__ std::size_t locate(const Launch& l, const Place& p, int position, bool& there)
 {
     const int index = position >> l.page_shift;
-    const int page = index < p.limit ? l.table[p.sequence * l.table_stride + index] : -1;
-    there = page >= 0 && page < l.pages;
-    return (there ? page : 0) * l.page_stride +
-           std::size_t(position & ((1 << l.page_shift) - 1)) * l.row_stride;
+    const int read = scalar_load(l.table + p.sequence * l.table_stride + max(min(index, p.limit - 1), 0));
+    there = index < p.limit && read >= 0 && read < l.pages;
+    return (there ? read : 0) * l.page_stride + std::size_t(position & ((1 << l.page_shift) - 1)) * l.row_stride;
 }
 
-// One 16-row part's running sums. A lane has row lane % 16 and of its output the coordinates
-// (4 * (lane / 16) + i) * step + j.
-template <int HW> struct Sums
+// One 16-row part's running sums. A lane has row lane % 16 and 4 * HW / 16 of its coordinates:
+// those 16 * j + 4 * (lane / 16) + i (Across), or (4 * (lane / 16) + i) * (HW / 16) + j.
+template <int HW, bool Across> struct Sums
 {
     static constexpr int step = HW / 16;
-    static constexpr int words = 4 * step + 2; // of a record, [word][lane]
-    f32x4 out[step];                           // [j][i]
-    f32x4 total;                               // four times the same
+    static constexpr int words = 4 * step + 2; // a lane's, joined within a workgroup
+    static constexpr int record = 16 * HW + 32; // floats of a chunk's record: [row][HW], references, sums
+    f32x4 out[step]; // [j][i]
+    f32x4 total;     // four times the same
     float reference;
 
     __device__ __forceinline__ void clear()
@@ -214,7 +229,8 @@ template <int HW> struct Sums
             out[j] *= factor;
         }
     }
-    __device__ __forceinline__ void store(float* to, int lane) const
+    // [word][lane]
+    __device__ __forceinline__ void hand_over(float* to, int lane) const
     {
 #pragma unroll
         for (int j = 0; j < step; ++j)
@@ -244,51 +260,70 @@ template <int HW> struct Sums
             }
         }
     }
+    // put(first coordinate, values): runs of them in ascending order.
+    template <class Put> __device__ __forceinline__ void each(int lane, Put put) const
+    {
+        constexpr int runs = Across ? step : 4, length = Across ? 4 : step;
+#pragma unroll
+        for (int r = 0; r < runs; ++r)
+        {
+            float values[length];
+#pragma unroll
+            for (int k = 0; k < length; ++k)
+            {
+                values[k] = Across ? out[r][k] : out[k][r];
+            }
+            put(Across ? 16 * r + 4 * (lane / 16) : (4 * (lane / 16) + r) * step, values);
+        }
+    }
+    __device__ __forceinline__ void store(float* to, int lane) const
+    {
+        const int row = lane % 16;
+        each(lane,
+             [&](int first, const auto& values)
+             {
+                 __builtin_memcpy(__builtin_assume_aligned(to + row * HW + first, 16), values, sizeof values);
+             });
+        if (lane < 16)
+        {
+            to[16 * HW + row] = reference;
+            to[16 * HW + 16 + row] = total[0];
+        }
+    }
 };
 
-// A lane's part i of one row, divided by the row's sum. A row that no key reached is 0.
-template <int HW, bool Half>
-__device__ __forceinline__ void write_part(const Launch& l, const Place& p, int row, int lane, int i, const float* values,
-                                           float total)
+// Coordinates of one row from `first` on, divided by the row's sum. A row that no key reached is 0.
+template <int HW, bool Half, int Count>
+__device__ __forceinline__ void write_row(const Launch& l, const Place& p, int row, int first, const float (&values)[Count],
+                                          float total)
 {
-    constexpr int step = HW / 16;
     const int node = row / l.group, head = p.head * l.group + row % l.group;
     const float inverse = 1.0f / total;
-    unsigned word[step / 2];
+    unsigned word[Count / 2];
 #pragma unroll
-    for (int j = 0; j < step / 2; ++j)
+    for (int k = 0; k < Count / 2; ++k)
     {
-        word[j] = total == 0 ? 0u : pack<Half>(values[2 * j] * inverse, values[2 * j + 1] * inverse);
+        word[k] = total == 0 ? 0u : pack<Half>(values[2 * k] * inverse, values[2 * k + 1] * inverse);
     }
-    uint16_t* const to = l.out + std::size_t(p.first + node) * l.out_stride + std::size_t(head) * HW +
-                         (4 * (lane / 16) + i) * step;
-    __builtin_memcpy(__builtin_assume_aligned(to, 2 * step), word, 2 * step);
+    uint16_t* const to = l.out + std::size_t(p.first + node) * l.out_stride + std::size_t(head) * HW + first;
+    __builtin_memcpy(__builtin_assume_aligned(to, sizeof word), word, sizeof word);
 }
 
 // A part's sums: to the output, or as the chunk's record.
-template <int HW, bool Half>
-__device__ __forceinline__ void finish(const Launch& l, const Place& p, int unit, int row, int lane, const Sums<HW>& sums)
+template <int HW, bool Half, bool Across>
+__device__ __forceinline__ void finish(const Launch& l, const Place& p, int unit, int row, int lane,
+                                       const Sums<HW, Across>& sums)
 {
     if (chunks_of(l, p) > 1)
     {
-        sums.store(l.partial + (std::size_t(unit) * l.parts + row / 16) * (Sums<HW>::words * 64), lane);
+        sums.store(l.partial + (std::size_t(unit) * l.parts + row / 16) * Sums<HW, Across>::record, lane);
         return;
     }
     const int mine = row + lane % 16;
-    if (mine / l.group >= p.nodes)
+    if (mine / l.group < p.nodes)
     {
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-    {
-        float part[Sums<HW>::step];
-#pragma unroll
-        for (int j = 0; j < Sums<HW>::step; ++j)
-        {
-            part[j] = sums.out[j][i];
-        }
-        write_part<HW, Half>(l, p, mine, lane, i, part, sums.total[0]);
+        sums.each(lane, [&](int first, const auto& values)
+                  { write_row<HW, Half>(l, p, mine, first, values, sums.total[0]); });
     }
 }
 
@@ -339,14 +374,14 @@ __device__ __forceinline__ unsigned seen(const Launch& l, const Place& p, int at
 }
 
 // A value row that is not finite, of new row `key` of the block, for the rows that see it.
-template <int HW, bool Half>
+template <int HW, bool Half, bool Across>
 __device__ __forceinline__ void add_poisoned(const Launch& l, const Place& p, int at, int key, float weight, bool live,
-                                             int lane, Sums<HW>& sums)
+                                             int lane, Sums<HW, Across>& sums)
 {
     constexpr int step = HW / 16;
     bool there;
     const std::size_t base = locate(l, p, at + key / 16 * 16, there) + std::size_t(p.head) * HW;
-    const uint16_t* const from = l.values + base + std::size_t(key % 16) * l.row_stride + lane / 16 * 4 * step;
+    const uint16_t* const from = l.values + base + std::size_t(key % 16) * l.row_stride;
     if (live && there)
     {
 #pragma unroll
@@ -355,7 +390,8 @@ __device__ __forceinline__ void add_poisoned(const Launch& l, const Place& p, in
 #pragma unroll
             for (int j = 0; j < step; ++j)
             {
-                const uint16_t bits = from[i * step + j];
+                const int first = 4 * (lane / 16) + i;
+                const uint16_t bits = from[Across ? 16 * j + first : first * step + j];
                 sums.out[j][i] += nonfinite<Half>(bits) ? weight * widen<Half>(bits) : 0.0f;
             }
         }
@@ -394,17 +430,17 @@ __device__ __forceinline__ unsigned clean(unsigned (&value)[4][HW / 32], int hal
     return poisoned;
 }
 
-// Adds a block's keys to `Parts` parts of 16 rows. key(half, d) and value(j) give the operands;
-// next() runs once the keys are used up.
-// Masks are looked at where the block is not `whole`: not all of it exists, or it reaches into
-// what some row does not see.
-template <int HW, bool Half, int Parts, class Key, class Values, class Next>
-__device__ __forceinline__ void attend(const Launch& l, const Place& p, int at, bool whole, unsigned exist,
-                                       unsigned poisoned, int lane, const u32x4 (&query)[Parts][HW / 32],
-                                       const int (&node)[Parts], Sums<HW> (&sums)[Parts], Key key, Values value, Next next)
+// What masks ask of a block: which keys exist, and which new ones have values that are not finite.
+struct Marks
 {
-    constexpr int depth = HW / 32, step = HW / 16;
-    f32x4 score[Parts][2];
+    unsigned exist, poisoned;
+};
+
+// A block's scores for `Parts` parts of 16 rows, unscaled: keys 16 * half + 4 * (lane / 16) + i.
+template <int HW, bool Half, int Parts>
+__device__ __forceinline__ void score_block(const u32x4 (&key)[2][HW / 32], const u32x4 (&query)[Parts][HW / 32],
+                                            f32x4 (&score)[Parts][2])
+{
 #pragma unroll
     for (int half = 0; half < 2; ++half)
     {
@@ -414,41 +450,31 @@ __device__ __forceinline__ void attend(const Launch& l, const Place& p, int at, 
             score[t][half] = f32x4{0, 0, 0, 0};
         }
 #pragma unroll
-        for (int d = 0; d < depth; ++d)
+        for (int d = 0; d < HW / 32; ++d)
         {
-            const u32x4 k = key(half, d);
 #pragma unroll
             for (int t = 0; t < Parts; ++t)
             {
-                score[t][half] = product<Half>(k, query[t][d], score[t][half]);
+                score[t][half] = product<Half>(key[half][d], query[t][d], score[t][half]);
             }
         }
     }
-    next();
-    unsigned live[Parts];
-    if (!whole)
-    {
-#pragma unroll
-        for (int t = 0; t < Parts; ++t)
-        {
-            live[t] = seen(l, p, at, exist, node[t]) >> 4 * (lane / 16);
-#pragma unroll
-            for (int slot = 0; slot < 8; ++slot)
-            {
-                f32x4& s = score[t][slot / 4];
-                s[slot % 4] = live[t] >> (16 * (slot / 4) + slot % 4) & 1 ? s[slot % 4] : minus_infinity;
-            }
-        }
-    }
-    // The reference moves only when a score passes it by 2^8: weights stay in range without it,
-    // and most blocks need neither the exchange nor the scaling.
+}
+
+// Moves the running references, if need be, before a block's scores are weighed: only when a
+// score passes one by 2^8. Weights stay in range without it, and most blocks need neither the
+// exchange nor the scaling.
+template <int HW, bool Across, int Parts>
+__device__ __forceinline__ void settle(const Launch& l, const f32x4 (&score)[Parts][2], Sums<HW, Across> (&sums)[Parts])
+{
     float most[Parts];
     bool move = false;
 #pragma unroll
     for (int t = 0; t < Parts; ++t)
     {
         const f32x4 a = score[t][0], b = score[t][1];
-        most[t] = fmaxf(fmaxf(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])), fmaxf(b[0], b[1])), fmaxf(b[2], b[3]));
+        // Of scores that are not numbers it is none either, and so is the row.
+        most[t] = maximum(maximum(maximum(a[0], a[1], a[2]), a[3], b[0]), maximum(b[1], b[2], b[3]), b[3]);
         // Not a product with -infinity, which a scale of 0 would make no number.
         most[t] = most[t] == minus_infinity ? most[t] : most[t] * l.scale_log2;
         move = move || most[t] > sums[t].reference + 8.0f;
@@ -461,10 +487,17 @@ __device__ __forceinline__ void attend(const Launch& l, const Place& p, int at, 
             sums[t].move(fmaxf(query_max(most[t]), sums[t].reference));
         }
     }
-    u32x4 weight[Parts];
+}
+
+// Weights of a block's scores against the references.
+template <int HW, bool Half, bool Across, int Parts>
+__device__ __forceinline__ void weigh(const Launch& l, const f32x4 (&score)[Parts][2],
+                                      const Sums<HW, Across> (&sums)[Parts], u32x4 (&weight)[Parts])
+{
 #pragma unroll
     for (int t = 0; t < Parts; ++t)
     {
+        // Where no key had a score the reference is -infinity, and so are the scores.
         const float reference = sums[t].reference == minus_infinity ? 0.0f : sums[t].reference;
         float e[8];
 #pragma unroll
@@ -472,46 +505,27 @@ __device__ __forceinline__ void attend(const Launch& l, const Place& p, int at, 
         {
             e[slot] = __builtin_amdgcn_exp2f(__builtin_fmaf(score[t][slot / 4][slot % 4], l.scale_log2, -reference));
         }
-        if (!whole)
-        {
-#pragma unroll
-            for (int slot = 0; slot < 8; ++slot)
-            {
-                e[slot] = live[t] >> (16 * (slot / 4) + slot % 4) & 1 ? e[slot] : 0.0f;
-            }
-        }
 #pragma unroll
         for (int w = 0; w < 4; ++w)
         {
             weight[t][w] = pack<Half>(e[2 * w], e[2 * w + 1]);
         }
-        if (poisoned)
-        {
-            const unsigned mine = seen(l, p, at, exist, node[t]);
-            for (unsigned left = poisoned; left; left &= left - 1)
-            {
-                const int k = __builtin_ctz(left);
-                float x = e[0];
-#pragma unroll
-                for (int slot = 1; slot < 8; ++slot)
-                {
-                    x = 4 * (k / 16) + k % 4 == slot ? e[slot] : x;
-                }
-                x = __shfl(x, k % 16 / 4 * 16 + lane % 16);
-                add_poisoned<HW, Half>(l, p, at, k, x, mine >> k & 1, lane, sums[t]);
-            }
-        }
     }
-    // The sum of a row's weights, as they are rounded, is one more product.
+}
+
+// Adds a block's weighted values; value(j) gives the j-th coordinates of its keys. The
+// sum of a row's weights, as they are rounded, is one more product.
+template <int HW, bool Half, bool Across, int Parts, class Values>
+__device__ __forceinline__ void add_block(const u32x4 (&weight)[Parts], Sums<HW, Across> (&sums)[Parts], Values value)
+{
     constexpr unsigned one = Half ? 0x3c003c00u : 0x3f803f80u;
-    const u32x4 ones = {one, one, one, one};
 #pragma unroll
     for (int t = 0; t < Parts; ++t)
     {
-        sums[t].total = product<Half>(ones, weight[t], sums[t].total);
+        sums[t].total = product<Half>(u32x4{one, one, one, one}, weight[t], sums[t].total);
     }
 #pragma unroll
-    for (int j = 0; j < step; ++j)
+    for (int j = 0; j < HW / 16; ++j)
     {
         const u32x4 v = value(j);
 #pragma unroll
@@ -522,23 +536,97 @@ __device__ __forceinline__ void attend(const Launch& l, const Place& p, int at, 
     }
 }
 
+// A block with masks: the keys that a row does not see weigh nothing, whatever they are.
+template <int HW, bool Half, bool Across, int Parts, class Values>
+__device__ __forceinline__ void attend_masked(const Launch& l, const Place& p, int at, Marks marks, int lane,
+                                              const u32x4 (&key)[2][HW / 32], const u32x4 (&query)[Parts][HW / 32],
+                                              const int (&node)[Parts], Sums<HW, Across> (&sums)[Parts], Values value)
+{
+    f32x4 score[Parts][2];
+    score_block<HW, Half>(key, query, score);
+    unsigned live[Parts];
+#pragma unroll
+    for (int t = 0; t < Parts; ++t)
+    {
+        live[t] = seen(l, p, at, marks.exist, node[t]);
+#pragma unroll
+        for (int slot = 0; slot < 8; ++slot)
+        {
+            f32x4& x = score[t][slot / 4];
+            x[slot % 4] = live[t] >> (16 * (slot / 4) + 4 * (lane / 16) + slot % 4) & 1 ? x[slot % 4] : minus_infinity;
+        }
+    }
+    settle(l, score, sums);
+    u32x4 weight[Parts];
+#pragma unroll
+    for (int t = 0; t < Parts; ++t)
+    {
+        const float reference = sums[t].reference == minus_infinity ? 0.0f : sums[t].reference;
+        float e[8];
+#pragma unroll
+        for (int slot = 0; slot < 8; ++slot)
+        {
+            // Chosen once more: a scale of 0 makes no number of -infinity.
+            const float x =
+                __builtin_amdgcn_exp2f(__builtin_fmaf(score[t][slot / 4][slot % 4], l.scale_log2, -reference));
+            e[slot] = live[t] >> (16 * (slot / 4) + 4 * (lane / 16) + slot % 4) & 1 ? x : 0.0f;
+        }
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+        {
+            weight[t][w] = pack<Half>(e[2 * w], e[2 * w + 1]);
+        }
+        for (unsigned left = marks.poisoned; left; left &= left - 1)
+        {
+            const int k = __builtin_ctz(left);
+            float x = e[0];
+#pragma unroll
+            for (int slot = 1; slot < 8; ++slot)
+            {
+                x = 4 * (k / 16) + k % 4 == slot ? e[slot] : x;
+            }
+            x = __shfl(x, k % 16 / 4 * 16 + lane % 16);
+            add_poisoned<HW, Half>(l, p, at, k, x, live[t] >> k & 1, lane, sums[t]);
+        }
+    }
+    add_block<HW, Half>(weight, sums, value);
+}
+
+// A lane's byte offsets from where 16 keys lie. Rows are under 2^25 bytes apart, so that these
+// fit 32 bits and what is common to the wave stays in scalar registers.
+struct Offsets
+{
+    unsigned key, value, row; // row: the same for all lanes
+};
+template <int HW> __device__ __forceinline__ Offsets offsets_of(const Launch& l, int lane)
+{
+    constexpr unsigned step = HW / 16;
+    return {2 * (lane % 16 * l.row_stride + lane / 16 * 8), 2 * (lane / 16 * 4 * l.row_stride + lane % 16 * step),
+            2 * l.row_stride};
+}
+
+// Half a block's keys, 16 of them, in operand order.
+template <int HW>
+__device__ __forceinline__ void load_keys(const uint16_t* from, const Offsets& o, u32x4 (&key)[HW / 32])
+{
+    const char* const mine = reinterpret_cast<const char*>(from) + o.key;
+#pragma unroll
+    for (int d = 0; d < HW / 32; ++d)
+    {
+        key[d] = *reinterpret_cast<const u32x4*>(mine + 64 * d);
+    }
+}
+
 // Half a block's values as a lane loads them, 16 keys: `step` coordinates of four keys.
 template <int HW>
-__device__ __forceinline__ void load_values(const uint16_t* from, unsigned row_stride, int lane, unsigned (&value)[4][HW / 32])
+__device__ __forceinline__ void load_values(const uint16_t* from, const Offsets& o, unsigned (&value)[4][HW / 32])
 {
-    constexpr int step = HW / 16;
-    const uint16_t* const mine = from + 4 * (lane / 16) * row_stride + lane % 16 * step;
+    using Part = std::conditional_t<HW == 128, u32x4, u32x2>;
+    const char* row = reinterpret_cast<const char*>(from);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 4; ++i, row += o.row)
     {
-        if constexpr (step == 8)
-        {
-            *reinterpret_cast<u32x4*>(value[i]) = *reinterpret_cast<const u32x4*>(mine + i * row_stride);
-        }
-        else
-        {
-            *reinterpret_cast<u32x2*>(value[i]) = *reinterpret_cast<const u32x2*>(mine + i * row_stride);
-        }
+        *reinterpret_cast<Part*>(value[i]) = *reinterpret_cast<const Part*>(row + o.value);
     }
 }
 
@@ -548,18 +636,110 @@ template <int HW> __device__ __forceinline__ unsigned pair(const unsigned (&valu
     return __builtin_amdgcn_perm(value[i + 1][j / 2], value[i][j / 2], j % 2 ? 0x07060302u : 0x05040100u);
 }
 
-// Workgroups go round the eight dies: a unit's tiles, which read the same keys, follow one
-// another on one die.
+// 16 bytes a lane, from each lane's address to `to`, lane after lane; the wave waits for it with
+// its other loads (s_waitcnt vmcnt). Written out because the compiler would wait for it before any
+// other read of LDS. M0 is reserved, so that clang warns where it is named; nothing else uses it.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void load_to_lds(const void* from, void* to)
+{
+    const unsigned address =
+        unsigned(reinterpret_cast<std::uintptr_t>((__attribute__((address_space(3))) const void*)to));
+    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from),
+                 "s"(__builtin_amdgcn_readfirstlane(address))
+                 : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+// Four keys of coordinate lane % 16 of the 16 that start at each four lanes' rows: lanes 4 r .. 4 r + 3
+// of 16 name row r.
+__device__ __forceinline__ u32x2 read_transposed(const char* from)
+{
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(
+        u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)from));
+}
+
+// clean() for a stage's values where they lie in LDS, eight keys a wave, for the whole workgroup.
+template <int HW, bool Half>
+__device__ __forceinline__ void clean_stage(const Launch& l, const Place& p, int at, int end, int warp, int lane,
+                                            char* values, Marks* marked)
+{
+    constexpr int lanes = HW / 8, pieces = HW / 64; // lanes of a row
+    const int first = at + 8 * warp;                // of the wave's keys
+    bool there;
+    locate(l, p, first / 16 * 16, there);
+    const unsigned exist = there ? low_bits(end - first) & 0xff : 0u, cached = low_bits(p.length - first);
+    Marks marks = {exist, 0};
+#pragma unroll
+    for (int i = 0; i < pieces; ++i)
+    {
+        const int key = i * (64 / lanes) + lane / lanes;
+        u32x4& v = *reinterpret_cast<u32x4*>(values + (warp * pieces + i) * 1024 + lane * 16);
+        u32x4 x = v;
+        const bool here = exist >> key & 1, fresh = !(cached >> key & 1);
+        bool wrong = false;
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+        {
+            const unsigned keep = (nonfinite<Half>(uint16_t(x[w])) ? 0u : 0xffffu) |
+                                  (nonfinite<Half>(uint16_t(x[w] >> 16)) ? 0u : 0xffff0000u);
+            wrong = wrong || keep != ~0u;
+            x[w] = !here ? 0u : fresh ? x[w] & keep : x[w];
+        }
+        v = x;
+        const uint64_t bad = __ballot(wrong && here && fresh);
+#pragma unroll
+        for (int k = 0; k < 64 / lanes; ++k)
+        {
+            marks.poisoned |= (bad >> k * lanes & ((1ull << lanes) - 1) ? 1u : 0u) << (i * (64 / lanes) + k);
+        }
+    }
+    if (lane == 0)
+    {
+        marked[warp] = marks;
+    }
+    __syncthreads();
+}
+
+// Whether every page from one position to another is there, for the whole workgroup.
+template <int Threads>
+__device__ __forceinline__ bool all_there(const Launch& l, const Place& p, int from, int to, int& flag)
+{
+    const int first = from >> l.page_shift, last = (to - 1) >> l.page_shift;
+    bool good = true;
+    for (int i = first + int(threadIdx.x); i <= last; i += Threads)
+    {
+        const int page = i < p.limit ? l.table[p.sequence * l.table_stride + i] : -1;
+        good = good && page >= 0 && page < l.pages;
+    }
+    if (threadIdx.x == 0)
+    {
+        flag = 1;
+    }
+    __syncthreads();
+    if (!good)
+    {
+        flag = 0;
+    }
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane(flag);
+}
+
+// Workgroups go round the eight dies. A unit's tiles, which read the same keys, follow one another
+// on one die, and so do `together` heads of a chunk, which read the rows of the same positions:
+// where a die reads one head alone, its requests meet in two of its cache's sixteen channels.
 __device__ __forceinline__ void unit_of(const Launch& l, int& unit, int& tile)
 {
-    unit = blockIdx.x / (8 * l.tiles) * 8 + blockIdx.x % 8;
-    tile = blockIdx.x / 8 % l.tiles;
+    const int die = blockIdx.x % 8, i = blockIdx.x / 8, j = i / l.tiles;
+    tile = i % l.tiles;
+    unit = (j / l.together * 8 + die) * l.together + j % l.together;
 }
 
 // A tile is `Parts` x 16 rows; a wave takes every fourth block of the chunk.
 template <int HW, bool Half, int Parts> __global__ __launch_bounds__(64 * waves, Parts == 1 ? 3 : 2) void direct_kernel(Launch l)
 {
-    constexpr int depth = HW / 32, record = Sums<HW>::words * 64;
+    constexpr int depth = HW / 32, words = Sums<HW, false>::words * 64;
     extern __shared__ float joined[];
     const int lane = threadIdx.x % 64, warp = __builtin_amdgcn_readfirstlane(int(threadIdx.x / 64));
     int unit, tile;
@@ -574,7 +754,7 @@ template <int HW, bool Half, int Parts> __global__ __launch_bounds__(64 * waves,
     const int open = l.mask ? p.length : p.length + p.row / l.group + 1;
     u32x4 query[Parts][depth];
     int node[Parts];
-    Sums<HW> sums[Parts];
+    Sums<HW, false> sums[Parts];
 #pragma unroll
     for (int t = 0; t < Parts; ++t)
     {
@@ -583,7 +763,9 @@ template <int HW, bool Half, int Parts> __global__ __launch_bounds__(64 * waves,
     }
 
     // A block's keys are asked for as soon as the last one's are used up, and so are its values:
-    // one set of registers each, and either is under way while the other is worked on.
+    // one set of registers each, and either is under way while the other is worked on. Where
+    // they lie is looked up a block earlier.
+    const Offsets offsets = offsets_of<HW>(l, lane);
     u32x4 key[2][depth];
     unsigned value[2][4][HW / 32];
     std::size_t base[2];
@@ -596,17 +778,12 @@ template <int HW, bool Half, int Parts> __global__ __launch_bounds__(64 * waves,
             base[half] = locate(l, p, at + 16 * half, there[half]) + std::size_t(p.head) * HW;
         }
     };
-    const auto load_keys = [&]
+    const auto load_both_keys = [&]
     {
 #pragma unroll
         for (int half = 0; half < 2; ++half)
         {
-#pragma unroll
-            for (int d = 0; d < depth; ++d)
-            {
-                key[half][d] = *reinterpret_cast<const u32x4*>(l.keys + base[half] + lane % 16 * l.row_stride +
-                                                               lane / 16 * 8 + 32 * d);
-            }
+            load_keys<HW>(l.keys + base[half], offsets, key[half]);
         }
     };
     const auto load_both_values = [&]
@@ -614,46 +791,58 @@ template <int HW, bool Half, int Parts> __global__ __launch_bounds__(64 * waves,
 #pragma unroll
         for (int half = 0; half < 2; ++half)
         {
-            load_values<HW>(l.values + base[half], l.row_stride, lane, value[half]);
+            load_values<HW>(l.values + base[half], offsets, value[half]);
         }
+    };
+    const auto value_of = [&](int j)
+    {
+        return u32x4{pair<HW>(value[0], 0, j), pair<HW>(value[0], 2, j), pair<HW>(value[1], 0, j),
+                     pair<HW>(value[1], 2, j)};
     };
     constexpr int stride = block * waves;
     int at = begin + block * warp;
-    if (at < end)
+    const int whole = min(open, end) - block; // the last block that all rows see whole
+    if (at <= whole)
     {
         find(at);
-        load_keys();
+        load_both_keys();
         load_both_values();
+        bool here = there[0] && there[1]; // of the block in registers
+        find(at + stride);
+        while (at <= whole && here)
+        {
+            const bool more = at + stride <= whole;
+            f32x4 score[Parts][2];
+            score_block<HW, Half>(key, query, score);
+            if (more)
+            {
+                load_both_keys();
+            }
+            settle(l, score, sums);
+            u32x4 weight[Parts];
+            weigh<HW, Half>(l, score, sums, weight);
+            add_block<HW, Half>(weight, sums, value_of);
+            at += stride;
+            if (more)
+            {
+                load_both_values();
+                here = there[0] && there[1];
+                find(at + stride);
+            }
+        }
     }
+    // What is left: blocks with masks, and all behind a page that is not there.
     for (; at < end; at += stride)
     {
-        unsigned exist = ~0u, poisoned = 0;
-        const bool whole = at + block <= min(open, end) && there[0] && there[1];
-        if (!whole)
-        {
-            exist = low_bits(end - at) & ((there[0] ? 0xffffu : 0u) | (there[1] ? 0xffff0000u : 0u));
-            const unsigned cached = low_bits(p.length - at);
-            poisoned = clean<HW, Half>(value[0], 0, exist, cached, lane) | clean<HW, Half>(value[1], 1, exist, cached, lane);
-        }
-        attend<HW, Half, Parts>(
-            l, p, at, whole, exist, poisoned, lane, query, node, sums, [&](int half, int d) { return key[half][d]; },
-            [&](int j)
-            {
-                return u32x4{pair<HW>(value[0], 0, j), pair<HW>(value[0], 2, j), pair<HW>(value[1], 0, j),
-                             pair<HW>(value[1], 2, j)};
-            },
-            [&]
-            {
-                if (at + stride < end)
-                {
-                    find(at + stride);
-                    load_keys();
-                }
-            });
-        if (at + stride < end)
-        {
-            load_both_values();
-        }
+        find(at);
+        load_both_keys();
+        load_both_values();
+        Marks marks;
+        marks.exist = low_bits(end - at) & ((there[0] ? 0xffffu : 0u) | (there[1] ? 0xffff0000u : 0u));
+        const unsigned cached = low_bits(p.length - at);
+        marks.poisoned = clean<HW, Half>(value[0], 0, marks.exist, cached, lane) |
+                         clean<HW, Half>(value[1], 1, marks.exist, cached, lane);
+        attend_masked<HW, Half>(l, p, at, marks, lane, key, query, node, sums, value_of);
     }
 
     // Waves 2 and 3 to 0 and 1, then 1 to 0.
@@ -665,7 +854,7 @@ template <int HW, bool Half, int Parts> __global__ __launch_bounds__(64 * waves,
 #pragma unroll
             for (int t = 0; t < Parts; ++t)
             {
-                sums[t].store(joined + ((warp - half) * Parts + t) * record, lane);
+                sums[t].hand_over(joined + ((warp - half) * Parts + t) * words, lane);
             }
         }
         __syncthreads();
@@ -674,7 +863,7 @@ template <int HW, bool Half, int Parts> __global__ __launch_bounds__(64 * waves,
 #pragma unroll
             for (int t = 0; t < Parts; ++t)
             {
-                sums[t].join(joined + (warp * Parts + t) * record, lane);
+                sums[t].join(joined + (warp * Parts + t) * words, lane);
             }
         }
         __syncthreads();
@@ -692,15 +881,41 @@ template <int HW, bool Half, int Parts> __global__ __launch_bounds__(64 * waves,
     }
 }
 
-// A tile is 128 rows, 32 a wave. Two blocks lie in LDS in operand order while the next two are
-// under way to registers, a quarter a wave: 16 keys, and 16 keys' values paired.
-template <int HW, bool Half> __global__ __launch_bounds__(64 * waves, 2) void staged_kernel(Launch l)
+constexpr int staging_waves = 8;
+constexpr int staged_keys = 2 * block; // of a stage
+constexpr int stages = 4;              // in LDS
+
+// At most `count` of the wave's memory operations still under way (they complete in order).
+template <int Count> __device__ __forceinline__ void wait_memory()
 {
-    constexpr int depth = HW / 32, step = HW / 16, parts = 2, rows = 16 * parts * waves, keys = 2 * block;
-    // [buffer][block][half, d or j][lane] 16 bytes each.
-    __shared__ u32x4 key_tile[2][2][2 * depth][64];
-    __shared__ u32x4 value_tile[2][2][step][64];
-    __shared__ unsigned exists[2][2][2], poison[2][2][2]; // [buffer][block][half]
+    static_assert(Count < 16);
+    __builtin_amdgcn_s_waitcnt(Count | 7 << 4 | 15 << 8);
+}
+
+// How far the 16-byte pieces of a key row and the 32-byte pieces of a value row are shifted in LDS (by
+// exclusive or), so that a piece of 16 rows meets every bank: 16 keys' pieces are read at a time,
+// and 16 value rows' transposed.
+template <int HW> __device__ __forceinline__ int key_shift(int row)
+{
+    return HW == 128 ? row & 15 : row >> 1 & 7;
+}
+template <int HW> __device__ __forceinline__ int value_shift(int row)
+{
+    return HW == 128 ? row & 7 : row >> 1 & 3;
+}
+
+// A tile is 256 / Teams rows, 32 a wave; a team of waves takes all stages, or every second
+// block. Stages of 64 keys go from memory straight into a ring of four in LDS, eight rows a wave, in
+// whole rows (4 TB/s where a load took 64 bytes of 16 rows, 5.5 so).
+template <int HW, bool Half, int Teams> __global__ __launch_bounds__(64 * staging_waves, 2) void staged_kernel(Launch l)
+{
+    constexpr int depth = HW / 32, step = HW / 16, parts = 2, team = staging_waves / Teams, rows = 16 * parts * team;
+    constexpr int keys = staged_keys, row_bytes = 2 * HW, key_bytes = keys * row_bytes;
+    constexpr int stage_bytes = 2 * key_bytes;
+    constexpr int pieces = HW / 64; // 1 KiB each, of keys and of values, that a wave loads of a stage
+    extern __shared__ __attribute__((aligned(128))) char ring[]; // [stage]: keys [key][HW], values [key][HW]
+    __shared__ Marks marked[staging_waves]; // of eight keys each
+    __shared__ int flag;
     const int lane = threadIdx.x % 64, warp = __builtin_amdgcn_readfirstlane(int(threadIdx.x / 64));
     int unit, tile;
     unit_of(l, unit, tile);
@@ -709,13 +924,17 @@ template <int HW, bool Half> __global__ __launch_bounds__(64 * waves, 2) void st
     {
         return;
     }
-    const int begin = p.split * l.chunk, end = chunk_end(l, p);
-    const int row = p.row + 16 * parts * warp;
+    const int begin = p.split * l.chunk, end = chunk_end(l, p), count = (max(end - begin, 0) + keys - 1) / keys;
+    const int row = p.row + 16 * parts * (warp % team);
     const bool idle = row >= p.nodes * l.group;
-    const int open = l.mask ? p.length : p.length + row / l.group + 1;
+    // Up to here stages are whole for every row of the tile, if the chunk's pages are all there.
+    const int open = min(end, l.mask ? p.length : p.length + p.row / l.group + 1);
+    const int whole =
+        all_there<64 * staging_waves>(l, p, begin, open, flag) ? max(open - begin, 0) / keys : 0; // stages
+
     u32x4 query[parts][depth];
     int node[parts];
-    Sums<HW> sums[parts];
+    Sums<HW, true> sums[parts];
 #pragma unroll
     for (int t = 0; t < parts; ++t)
     {
@@ -723,88 +942,232 @@ template <int HW, bool Half> __global__ __launch_bounds__(64 * waves, 2) void st
         sums[t].clear();
     }
 
-    // A wave's quarter: half `half` of block `which`.
-    const int which = warp / 2, half = warp % 2;
-    u32x4 key[depth];
-    unsigned value[4][HW / 32];
-    bool there = false;
-    const auto load = [&](int at)
-    {
-        const std::size_t base =
-            locate(l, p, at + block * which + 16 * half, there) + std::size_t(p.head) * HW;
+    // A wave's eighth: eight rows of keys and of values, of 16-key half `half`. A row's 16-byte
+    // pieces of keys and 32-byte pieces of values are shifted by its number.
+    const int half = warp / 2;
+    constexpr int lanes = HW / 8, rows_a_piece = 64 / lanes; // lanes of a row; rows that one load takes
+    unsigned key_offset[pieces], value_offset[pieces];       // bytes, of a lane
 #pragma unroll
-        for (int d = 0; d < depth; ++d)
+    for (int i = 0; i < pieces; ++i)
+    {
+        const int r = 8 * (warp % 2) + i * rows_a_piece + lane / lanes, place = lane % lanes;
+        key_offset[i] = 2 * (r * l.row_stride) + 16 * (place ^ key_shift<HW>(r));
+        value_offset[i] = 2 * (r * l.row_stride) + 16 * (place ^ 2 * value_shift<HW>(r));
+    }
+    bool there;
+    std::size_t base = 0; // where the wave's half of the next stage to load lies
+    const auto find = [&](int stage)
+    { base = locate(l, p, begin + keys * stage + 16 * half, there) + std::size_t(p.head) * HW; };
+    const auto load = [&](int stage)
+    {
+        char* const to = ring + stage % stages * stage_bytes + warp * pieces * 1024;
+        const char* const from_keys = reinterpret_cast<const char*>(l.keys + base);
+        const char* const from_values = reinterpret_cast<const char*>(l.values + base);
+#pragma unroll
+        for (int i = 0; i < pieces; ++i)
         {
-            key[d] = *reinterpret_cast<const u32x4*>(l.keys + base + lane % 16 * l.row_stride + lane / 16 * 8 + 32 * d);
+            load_to_lds(from_keys + key_offset[i], to + i * 1024);
+            load_to_lds(from_values + value_offset[i], to + key_bytes + i * 1024);
         }
-        load_values<HW>(l.values + base, l.row_stride, lane, value);
+        find(stage + 1);
     };
-    const auto stage = [&](int at, int buffer)
+    int issued = 0; // stages asked for
+    const auto load_up_to = [&](int last)
     {
-        const int mine = at + block * which;
-        const unsigned here = half ? 0xffff0000u : 0xffffu;
-        unsigned exist = here, poisoned = 0;
-        if (mine + block > min(p.length, end) || !there)
+        for (; issued <= min(last, count - 1); ++issued)
         {
-            exist = there ? low_bits(end - mine) & here : 0u;
-            poisoned = clean<HW, Half>(value, half, exist, low_bits(p.length - mine), lane);
+            load(issued);
         }
-        if (lane == 0)
+    };
+    // Stage `next` is in LDS, as are those in front of it, for all waves, and what they have read
+    // of LDS is in registers.
+    const auto arrive = [&](int next)
+    {
+        switch (issued - 1 - next)
         {
-            exists[buffer][which][half] = exist;
-            poison[buffer][which][half] = poisoned;
+        case 3: wait_memory<3 * 2 * pieces>(); break;
+        case 2: wait_memory<2 * 2 * pieces>(); break;
+        case 1: wait_memory<2 * pieces>(); break;
+        default: wait_memory<0>(); break;
         }
+        __syncthreads();
+    };
+    find(0);
+    // One team works on block 0 of a stage while the stage in front of it is still read for block 1
+    // by others; of two teams each is done with a stage once it has its values.
+    constexpr int ahead = Teams == 1 ? 2 : 3;
+    load_up_to(ahead);
+    arrive(Teams - 1);
+
+    u32x4 key[2][depth], value[step];
+    const int key_row = lane % 16, value_row = lane % 16 / 4 + 4 * (lane / 16); // of a half, by the lane's address
+    const int key_lane = key_row * row_bytes, keys_shift = 16 * (lane / 16 ^ key_shift<HW>(key_row));
+    const int value_lane = value_row * row_bytes + lane % 4 * 8, values_shift = 32 * value_shift<HW>(value_row);
+    const auto read_keys = [&](int stage, int b)
+    {
+        const char* const from = ring + stage % stages * stage_bytes + b * block * row_bytes + key_lane;
 #pragma unroll
         for (int d = 0; d < depth; ++d)
         {
-            key_tile[buffer][which][half * depth + d][lane] = key[d];
+            const char* const piece = from + (64 * d ^ keys_shift);
+            key[0][d] = *reinterpret_cast<const u32x4*>(piece);
+            key[1][d] = *reinterpret_cast<const u32x4*>(piece + 16 * row_bytes);
         }
+        asm volatile("" ::: "memory"); // here, not where they are used
+    };
+    const auto read_values = [&](int stage, int b)
+    {
+        const char* const from = ring + stage % stages * stage_bytes + key_bytes + b * block * row_bytes + value_lane;
 #pragma unroll
         for (int j = 0; j < step; ++j)
         {
-            const u32x2 v = {pair<HW>(value, 0, j), pair<HW>(value, 2, j)};
-            reinterpret_cast<u32x2*>(&value_tile[buffer][which][j][lane])[half] = v;
+            const char* const piece = from + (32 * j ^ values_shift);
+            const u32x2 low = read_transposed(piece), high = read_transposed(piece + 16 * row_bytes);
+            value[j] = u32x4{low[0], low[1], high[0], high[1]};
         }
+        asm volatile("" ::: "memory");
     };
-    int buffer = 0;
-    if (begin < end)
+    const auto value_of = [&](int j) { return value[j]; };
+    const int mine = Teams == 1 ? 0 : warp / team; // the first block of a stage that the wave takes
+    int stage = 0;
+    if (idle)
     {
-        load(begin);
-        stage(begin, 0);
-    }
-    __syncthreads();
-    for (int at = begin; at < end; at += keys, buffer ^= 1)
-    {
-        const bool more = at + keys < end;
-        if (more)
+        for (; stage < whole; ++stage)
         {
-            load(at + keys);
+            arrive(stage + Teams);
+            load_up_to(stage + ahead + 1);
         }
-        if (!idle)
+    }
+    else if (whole)
+    {
+        // The next block's scores are products while this block's weights are exponentials: a wave
+        // has work for both units at any time. Keys and values are read from LDS a phase before
+        // they are used.
+        f32x4 score[parts][2], next[parts][2];
+        u32x4 weight[parts];
+        read_keys(0, mine);
+        score_block<HW, Half>(key, query, score);
+        read_keys(Teams == 1 ? 0 : 1, Teams == 1 ? 1 : mine);
+        settle(l, score, sums);
+        const auto turn = [&](f32x4(&now)[parts][2], f32x4(&then)[parts][2], int block_stage, int b, int key_stage, int key_b,
+                              bool last, auto between)
         {
+            read_values(block_stage, b);
+            score_block<HW, Half>(key, query, then);
+            weigh<HW, Half>(l, now, sums, weight);
 #pragma unroll
-            for (int b = 0; b < 2; ++b)
+            for (int i = 0; i < 4 * parts * depth; ++i)
             {
-                const unsigned exist =
-                    __builtin_amdgcn_readfirstlane(exists[buffer][b][0] | exists[buffer][b][1]);
-                const unsigned poisoned =
-                    __builtin_amdgcn_readfirstlane(poison[buffer][b][0] | poison[buffer][b][1]);
-                if (exist)
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); // a product
+                __builtin_amdgcn_sched_group_barrier(0x002, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x400, 1, 0); // an exponential
+            }
+            between();
+            read_keys(key_stage, key_b);
+            add_block<HW, Half>(weight, sums, value_of);
+            if (!last)
+            {
+                settle(l, then, sums);
+            }
+        };
+        // While there are stages to ask for, nothing of a turn depends on their number.
+        const auto steady = [&]
+        {
+            wait_memory<2 * pieces>();
+            __syncthreads();
+            load(issued);
+            ++issued;
+        };
+        const auto drain = [&]
+        {
+            arrive(stage + Teams);
+            load_up_to(stage + ahead + 1);
+        };
+        const int enough = min(whole - 1, count - ahead - 1); // up to here a stage is asked for in each
+        if constexpr (Teams == 1)
+        {
+            for (; stage < enough; ++stage)
+            {
+                turn(score, next, stage, 0, stage + 1, 0, false, steady);
+                turn(next, score, stage, 1, stage + 1, 1, false, [] {});
+            }
+#pragma unroll 1
+            for (; stage < whole; ++stage)
+            {
+                turn(score, next, stage, 0, stage + 1, 0, false, drain);
+                turn(next, score, stage, 1, stage + 1, 1, stage + 1 == whole, [] {});
+            }
+        }
+        else
+        {
+            for (; stage + 1 < enough; stage += 2)
+            {
+                turn(score, next, stage, mine, stage + 2, mine, false, steady);
+                turn(next, score, stage + 1, mine, stage + 3, mine, false, steady);
+            }
+#pragma unroll 1
+            for (; stage < whole; ++stage)
+            {
+                turn(score, next, stage, mine, stage + 2, mine, stage + 1 == whole, drain);
+#pragma unroll
+                for (int t = 0; t < parts; ++t)
                 {
-                    attend<HW, Half, parts>(
-                        l, p, at + block * b, exist == ~0u && at + block * (b + 1) <= open, exist, poisoned, lane, query,
-                        node, sums, [&](int h, int d) { return key_tile[buffer][b][h * depth + d][lane]; },
-                        [&](int j) { return value_tile[buffer][b][j][lane]; }, [] {});
+                    score[t][0] = next[t][0];
+                    score[t][1] = next[t][1];
                 }
             }
         }
-        if (more)
+    }
+    for (; stage < count; ++stage)
+    {
+        const int at = begin + keys * stage;
+        arrive(stage);
+        load_up_to(stage + stages - 1);
+        clean_stage<HW, Half>(l, p, at, end, warp, lane, ring + stage % stages * stage_bytes + key_bytes, marked);
+#pragma unroll 1
+        for (int b = mine; b < 2 && !idle; b += Teams)
         {
-            stage(at + keys, buffer ^ 1);
+            Marks marks = {0, 0};
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+            {
+                marks.exist |= marked[4 * b + w].exist << 8 * w;
+                marks.poisoned |= marked[4 * b + w].poisoned << 8 * w;
+            }
+            marks.exist = __builtin_amdgcn_readfirstlane(marks.exist);
+            marks.poisoned = __builtin_amdgcn_readfirstlane(marks.poisoned);
+            if (marks.exist)
+            {
+                read_keys(stage, b);
+                read_values(stage, b);
+                attend_masked<HW, Half>(l, p, at + block * b, marks, lane, key, query, node, sums, value_of);
+            }
+        }
+    }
+    __syncthreads();
+    if constexpr (Teams == 2)
+    {
+        constexpr int words = Sums<HW, true>::words * 64;
+        float* const joined = reinterpret_cast<float*>(ring) + warp % team * parts * words;
+        if (warp >= team && !idle)
+        {
+#pragma unroll
+            for (int t = 0; t < parts; ++t)
+            {
+                sums[t].hand_over(joined + t * words, lane);
+            }
         }
         __syncthreads();
+        if (warp < team && !idle)
+        {
+#pragma unroll
+            for (int t = 0; t < parts; ++t)
+            {
+                sums[t].join(joined + t * words, lane);
+            }
+        }
     }
-    if (!idle)
+    if (warp < team)
     {
 #pragma unroll
         for (int t = 0; t < parts; ++t)
@@ -817,54 +1180,77 @@ template <int HW, bool Half> __global__ __launch_bounds__(64 * waves, 2) void st
     }
 }
 
-// Joins the chunks of 16 rows of a (sequence, head), in ascending order: a wave takes
-// coordinates i of a lane's four.
+// Joins the chunks of 16 rows of a (sequence, head), in ascending order.
 template <int HW, bool Half> __global__ __launch_bounds__(256) void join_kernel(Launch l, int tile_rows)
 {
-    constexpr int step = HW / 16, record = Sums<HW>::words * 64;
-    const int lane = threadIdx.x % 64, i = threadIdx.x / 64;
+    constexpr int step = HW / 16, record = Sums<HW, true>::record; // coordinates of a thread
+    const int mine = threadIdx.x / 16, first = threadIdx.x % 16 * step;
     const int part = blockIdx.x % l.parts, pair = blockIdx.x / l.parts;
     const int head = pair % l.heads, sequence = pair / l.heads;
-    const auto unit = [&](int split) { return (sequence * l.splits + split) * l.heads + head; };
+    const int unit = sequence * l.splits * l.heads + head; // of the first chunk
     Place p;
     // The chunks are those of the tile that the rows were in.
-    if (!place_of(l, unit(0), 16 * part / tile_rows * tile_rows, tile_rows, p))
+    if (!place_of(l, unit, 16 * part / tile_rows * tile_rows, tile_rows, p))
     {
         return;
     }
-    const int chunks = chunks_of(l, p), row = 16 * part + lane % 16;
+    const int chunks = chunks_of(l, p), row = 16 * part + mine;
     if (chunks == 1 || row / l.group >= p.nodes)
     {
         return;
     }
-    const float* const first = l.partial + (std::size_t(unit(0)) * l.parts + part) * record + lane;
+    const float* const records = l.partial + (std::size_t(unit) * l.parts + part) * record;
     const std::size_t apart = std::size_t(l.heads) * l.parts * record;
-    float reference = minus_infinity;
-    for (int split = 0; split < chunks; ++split)
+    // Eight chunks are read at a time, the last one again past the end, where it counts nothing.
+    constexpr int together = 8;
+    float reference = minus_infinity, total = 0, out[step] = {};
+    for (int base = 0; base < chunks; base += together)
     {
-        reference = fmaxf(reference, first[split * apart + 4 * step * 64]);
-    }
-    float total = 0, out[step] = {};
-#pragma unroll 4
-    for (int split = 0; split < chunks; ++split)
-    {
-        const float* const from = first + split * apart;
-        const float other = from[4 * step * 64];
-        const float factor = other == reference ? 1.0f : __builtin_amdgcn_exp2f(other - reference);
-        total += from[(4 * step + 1) * 64] * factor;
+        float other[together], part_total[together], part_out[together][step];
 #pragma unroll
-        for (int j = 0; j < step; ++j)
+        for (int c = 0; c < together; ++c)
         {
-            out[j] += from[(i * step + j) * 64] * factor;
+            const float* const from = records + min(base + c, chunks - 1) * apart;
+            other[c] = from[16 * HW + mine];
+            part_total[c] = from[16 * HW + 16 + mine];
+            __builtin_memcpy(part_out[c], __builtin_assume_aligned(from + mine * HW + first, 16), sizeof part_out[c]);
+        }
+        float most = reference;
+#pragma unroll
+        for (int c = 0; c < together; ++c)
+        {
+            most = fmaxf(most, other[c]);
+        }
+        const float ours = reference == most ? 1.0f : __builtin_amdgcn_exp2f(reference - most);
+        reference = most;
+        total *= ours;
+#pragma unroll
+        for (int k = 0; k < step; ++k)
+        {
+            out[k] *= ours;
+        }
+#pragma unroll
+        for (int c = 0; c < together; ++c)
+        {
+            const float factor = other[c] == most ? 1.0f : __builtin_amdgcn_exp2f(other[c] - most);
+            if (base + c < chunks)
+            {
+                total += part_total[c] * factor;
+#pragma unroll
+                for (int k = 0; k < step; ++k)
+                {
+                    out[k] += part_out[c][k] * factor;
+                }
+            }
         }
     }
-    write_part<HW, Half>(l, p, row, lane, i, out, total);
+    write_row<HW, Half>(l, p, row, first, out, total);
 }
 
 // The launch's shape: it depends on what the host knows, sizes and not lengths.
 struct Shape
 {
-    int parts_a_tile; // 16-row parts of a workgroup's tile: 1 or 2 (direct), 8 (staged)
+    int parts_a_tile; // 16-row parts of a workgroup's tile: 1 or 2 (direct), 8 or 16 (staged)
     int tiles, parts, splits, chunk;
     std::size_t units, record;
 };
@@ -874,10 +1260,10 @@ Shape shape_of(const PagedCache& cache, const PagedRows& rows)
     Shape s;
     const std::size_t group = std::size_t(rows.heads / cache.heads), queries = std::size_t(rows.max_rows) * group;
     s.parts = int((queries + 15) / 16);
-    s.parts_a_tile = s.parts <= 2 ? s.parts : 8;
+    s.parts_a_tile = s.parts <= 2 ? s.parts : s.parts <= 8 ? 8 : 16;
     s.tiles = (s.parts + s.parts_a_tile - 1) / s.parts_a_tile;
     const std::size_t pairs = std::size_t(cache.sequences) * cache.heads;
-    const std::size_t slots = (s.parts_a_tile == 1 ? 3 : 2) * std::size_t(compute_units());
+    const std::size_t slots = (s.parts_a_tile == 1 ? 3 : s.parts_a_tile == 2 ? 2 : 1) * std::size_t(compute_units());
     const std::size_t wanted = std::max<std::size_t>(1, slots / (pairs * s.tiles));
     const std::size_t most = std::max<std::size_t>(1, (rows.max_length + 255) / 256);
     s.splits = int(std::min(wanted, most));
@@ -885,21 +1271,33 @@ Shape shape_of(const PagedCache& cache, const PagedRows& rows)
     s.chunk = int(((rows.max_length + s.splits - 1) / s.splits + keys - 1) / keys * keys);
     s.chunk = std::max<int>(s.chunk, keys);
     s.units = pairs * s.splits;
-    s.record = 64 * std::size_t(cache.head_width / 4 + 2);
+    s.record = 16 * std::size_t(cache.head_width) + 32;
     return s;
 }
 
 template <int HW, bool Half> void launch(const Launch& l, const Shape& s, std::size_t pairs, hipStream_t stream)
 {
-    const unsigned grid = unsigned((s.units + 7) / 8 * 8 * std::size_t(s.tiles));
-    const std::size_t lds = 2 * Sums<HW>::words * 64 * 4;
+    const std::size_t groups = s.units / l.together;
+    const unsigned grid = unsigned((groups + 7) / 8 * 8 * l.together * s.tiles);
+    const auto run = [&](auto kernel, int threads, std::size_t lds)
+    {
+        if (lds > 65536)
+        {
+            check_hip(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                          hipFuncAttributeMaxDynamicSharedMemorySize, int(lds)),
+                      "paged attention LDS");
+        }
+        kernel<<<grid, threads, lds, stream>>>(l);
+        check_hip(hipGetLastError(), "paged attention launch");
+    };
+    constexpr std::size_t direct = 2 * Sums<HW, false>::words * 64 * 4, staged = stages * staged_keys * HW * 4;
     switch (s.parts_a_tile)
     {
-    case 1: direct_kernel<HW, Half, 1><<<grid, 64 * waves, lds, stream>>>(l); break;
-    case 2: direct_kernel<HW, Half, 2><<<grid, 64 * waves, 2 * lds, stream>>>(l); break;
-    default: staged_kernel<HW, Half><<<grid, 64 * waves, 0, stream>>>(l); break;
+    case 1: run(direct_kernel<HW, Half, 1>, 64 * waves, direct); break;
+    case 2: run(direct_kernel<HW, Half, 2>, 64 * waves, 2 * direct); break;
+    case 8: run(staged_kernel<HW, Half, 2>, 64 * staging_waves, staged); break;
+    default: run(staged_kernel<HW, Half, 1>, 64 * staging_waves, staged); break;
     }
-    check_hip(hipGetLastError(), "paged attention launch");
     if (s.splits > 1)
     {
         join_kernel<HW, Half><<<unsigned(pairs * s.parts), 256, 0, stream>>>(l, 16 * s.parts_a_tile);
@@ -928,7 +1326,7 @@ void attention_paged(const PagedCache& cache, int layer, const PagedRows& rows, 
     const Shape s = shape_of(cache, rows);
     const std::size_t pairs = std::size_t(cache.sequences) * cache.heads;
     // 2^32 work-items along x are a grid's limit.
-    require((s.units + 8) * s.tiles < (std::size_t(1) << 23) && pairs * s.parts < (std::size_t(1) << 23),
+    require((s.units + 8 * cache.heads) * s.tiles < (std::size_t(1) << 23) && pairs * s.parts < (std::size_t(1) << 23),
             "paged attention: too many workgroups for one launch");
     require(s.splits == 1 || (workspace && bytes >= s.units * s.parts * s.record * 4),
             "paged attention: the workspace is too small");
@@ -960,6 +1358,12 @@ void attention_paged(const PagedCache& cache, int layer, const PagedRows& rows, 
     l.splits = s.splits;
     l.chunk = s.chunk;
     l.units = int(s.units);
+    // As many heads as leave each die eight groups.
+    l.together = cache.heads;
+    while (cache.heads % l.together || (l.together > 1 && s.units / l.together < 64))
+    {
+        --l.together;
+    }
     l.negative = rows.scale < 0;
     l.scale_log2 = (l.negative ? -rows.scale : rows.scale) * 1.44269504088896340736f;
     const auto by_type = [&](auto width)
