@@ -1055,13 +1055,6 @@ template <int HW, bool Half, int Teams> __global__ __launch_bounds__(64 * stagin
             read_values(block_stage, b);
             score_block<HW, Half>(key, query, then);
             weigh<HW, Half>(l, now, sums, weight);
-#pragma unroll
-            for (int i = 0; i < 4 * parts * depth; ++i)
-            {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); // a product
-                __builtin_amdgcn_sched_group_barrier(0x002, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x400, 1, 0); // an exponential
-            }
             between();
             read_keys(key_stage, key_b);
             add_block<HW, Half>(weight, sums, value_of);

@@ -12,9 +12,8 @@ namespace tsac_hip
 {
 namespace
 {
-constexpr int taking_threads = 1024;
-constexpr int taking_waves = taking_threads / 64;
-constexpr int scanned = 4; // reference counts a thread reads at a time
+constexpr int most_threads = 1024; // of a workgroup that takes pages
+constexpr int scanned = 4;         // reference counts a thread reads at a time
 
 __device__ __forceinline__ void report(int* status, int what)
 {
@@ -24,177 +23,218 @@ __device__ __forceinline__ void report(int* status, int what)
     }
 }
 
-// Inclusive sum over the wave's lanes.
-__device__ __forceinline__ long long wave_scan(long long value, int lane)
+// Lanes below this one whose bit is set.
+__device__ __forceinline__ int lanes_below(uint64_t bits)
 {
-#pragma unroll
-    for (int step = 1; step < 64; step *= 2)
-    {
-        const long long below = __shfl_up(value, step);
-        value += lane >= step ? below : 0;
-    }
-    return value;
+    return __builtin_amdgcn_mbcnt_hi(unsigned(bits >> 32), __builtin_amdgcn_mbcnt_lo(unsigned(bits), 0));
 }
 
 struct TakingShared
 {
     int before[max_listed_sequences + 1]; // pages taken by the entries in front of each one
     unsigned seen[max_sequences / 32 + 1];
-    long long sums[taking_waves];
-    int bad, stopped;
+    int sums[2][most_threads / 64];
+    int bad;
 };
 
-// Exclusive sums of each entry's need into `before`, for the whole workgroup; returns the total.
-template <class Need> __device__ long long sum_needs(TakingShared& shared, int count, Need need)
+// A list of sequences is checked and worked on by one workgroup of `Threads`, an entry a thread
+// and round. The first round's reference counts are asked for at the start: they need nothing
+// else, and each wait for memory here is a fifth of a small call.
+template <int Threads> struct Taking
 {
+    static constexpr int waves = Threads / 64;
+    TakingShared& shared;
+    const PagedCache& cache;
+    int count;
+    int first_counts[scanned];
     const int lane = threadIdx.x % 64, warp = threadIdx.x / 64;
-    long long total = 0;
-    for (int base = 0; base < count; base += taking_threads)
-    {
-        const int i = base + threadIdx.x;
-        const long long mine = i < count ? need(i) : 0;
-        const long long inclusive = wave_scan(mine, lane);
-        if (lane == 63)
-        {
-            shared.sums[warp] = inclusive;
-        }
-        __syncthreads();
-        long long front = total, all = 0;
-        for (int w = 0; w < taking_waves; ++w)
-        {
-            front += w < warp ? shared.sums[w] : 0;
-            all += shared.sums[w];
-        }
-        if (i < count)
-        {
-            // Beyond 2^31 the call fails: there are fewer pages.
-            shared.before[i] = int(front + inclusive - mine);
-        }
-        total += all;
-        __syncthreads();
-    }
-    if (threadIdx.x == 0)
-    {
-        shared.before[count] = int(total);
-    }
-    __syncthreads();
-    return total;
-}
 
-// Hands the `total` lowest free pages to take(entry, index within the entry's need, page), in
-// order, and counts them once; false, with what was handed out given to undo(), if there are
-// too few. The counts are read four a thread; the scan ends as soon as enough are found.
-template <class Take, class Undo>
-__device__ bool take_pages(TakingShared& shared, int count, int total, int* references, int pages, Take take, Undo undo)
-{
-    const int lane = threadIdx.x % 64, warp = threadIdx.x / 64;
-    int found = 0;
-    const auto entry = [&](int rank)
+    __device__ Taking(TakingShared& s, const PagedCache& c, int n) : shared(s), cache(c), count(n)
     {
-        int low = 0, high = count; // the last entry with before <= rank
+        read_counts(0, first_counts);
+    }
+    // Counts from `base` on, of the thread's pages; not 0 past the last page.
+    __device__ __forceinline__ void read_counts(long long base, int (&counts)[scanned]) const
+    {
+        const long long first = base + threadIdx.x * scanned;
+#pragma unroll
+        for (int j = 0; j < scanned; ++j)
+        {
+            counts[j] = first + j < cache.pages ? cache.references[first + j] : 1;
+        }
+    }
+    // Whether every entry passes, and names a sequence that no other one does.
+    template <class Sequence, class Check> __device__ bool check(Sequence sequence, Check check_entry)
+    {
+        for (int i = threadIdx.x; i < count; i += Threads)
+        {
+            const int s = sequence(i);
+            if (s >= 0 && s < cache.sequences)
+            {
+                shared.seen[s / 32] = 0;
+            }
+        }
+        if (threadIdx.x == 0)
+        {
+            shared.bad = 0;
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < count; i += Threads)
+        {
+            const int s = sequence(i);
+            if (s < 0 || s >= cache.sequences || (atomicOr(&shared.seen[s / 32], 1u << s % 32) >> s % 32 & 1) ||
+                !check_entry(i, s))
+            {
+                shared.bad = 1;
+            }
+        }
+        __syncthreads();
+        return !shared.bad;
+    }
+    // Exclusive sums of each entry's need (below 2^21) into `before`; returns the total.
+    template <class Need> __device__ long long sum_needs(Need need)
+    {
+        long long total = 0;
+        for (int base = 0, round = 0; base < count; base += Threads, round ^= 1)
+        {
+            const int i = base + int(threadIdx.x), mine = i < count ? need(i) : 0;
+            int inclusive = mine;
+#pragma unroll
+            for (int step = 1; step < 64; step *= 2)
+            {
+                const int below = __shfl_up(inclusive, step);
+                inclusive += lane >= step ? below : 0;
+            }
+            if (lane == 63)
+            {
+                shared.sums[round][warp] = inclusive;
+            }
+            __syncthreads();
+            int front = 0, all = 0;
+#pragma unroll
+            for (int w = 0; w < waves; ++w)
+            {
+                front += w < warp ? shared.sums[round][w] : 0;
+                all += shared.sums[round][w];
+            }
+            if (i < count)
+            {
+                // Past 2^31 the call fails: there are fewer pages.
+                shared.before[i] = int(total + front + inclusive - mine);
+            }
+            total += all;
+        }
+        if (threadIdx.x == 0)
+        {
+            shared.before[count] = int(total);
+        }
+        __syncthreads();
+        return total;
+    }
+    // The last entry with before <= rank.
+    __device__ __forceinline__ int entry(int rank) const
+    {
+        int low = 0, high = count;
         while (high - low > 1)
         {
             const int middle = (low + high) / 2;
             (shared.before[middle] <= rank ? low : high) = middle;
         }
         return low;
-    };
-    for (long long base = 0; base < pages && found < total; base += taking_threads * scanned)
+    }
+    // Hands the `total` lowest free pages to take(entry, index within the entry's need, page), in
+    // order, and counts them once; false, with what was handed out given to undo(), if there are
+    // too few. The scan ends as soon as enough are found.
+    template <class Take, class Undo> __device__ bool take_pages(long long total, Take take, Undo undo)
     {
-        const long long first = base + threadIdx.x * scanned;
-        unsigned free = 0;
+        if (total > cache.pages)
+        {
+            return false;
+        }
+        int found = 0;
+        int counts[scanned];
 #pragma unroll
         for (int j = 0; j < scanned; ++j)
         {
-            free |= (first + j < pages && references[first + j] == 0 ? 1u : 0u) << j;
+            counts[j] = first_counts[j];
         }
-        const long long inclusive = wave_scan(__popc(free), lane);
-        if (lane == 63)
+        for (long long base = 0; base < cache.pages && found < total;)
         {
-            shared.sums[warp] = inclusive;
-        }
-        __syncthreads();
-        int rank = found + int(inclusive) - __popc(free), all = 0;
-        for (int w = 0; w < taking_waves; ++w)
-        {
-            rank += w < warp ? int(shared.sums[w]) : 0;
-            all += int(shared.sums[w]);
-        }
+            // Free pages of the lanes below, and of the thread's in front.
+            int rank = 0, mine = 0;
 #pragma unroll
-        for (int j = 0; j < scanned; ++j)
-        {
-            if (free >> j & 1)
+            for (int j = 0; j < scanned; ++j)
             {
-                if (rank < total)
+                rank += lanes_below(__ballot(counts[j] == 0));
+                mine += __popcll(__ballot(counts[j] == 0));
+            }
+            const int round = base / (Threads * scanned) % 2;
+            if (lane == 0)
+            {
+                shared.sums[round][warp] = mine;
+            }
+            __syncthreads();
+            int all = 0;
+            rank += found;
+#pragma unroll
+            for (int w = 0; w < waves; ++w)
+            {
+                rank += w < warp ? shared.sums[round][w] : 0;
+                all += shared.sums[round][w];
+            }
+#pragma unroll
+            for (int j = 0; j < scanned; ++j)
+            {
+                if (counts[j] == 0)
                 {
-                    const int i = entry(rank), page = int(first + j);
-                    take(i, rank - shared.before[i], page);
-                    references[page] = 1;
+                    if (rank < total)
+                    {
+                        const int i = entry(rank), page = int(base + threadIdx.x * scanned + j);
+                        take(i, rank - shared.before[i], page);
+                        cache.references[page] = 1;
+                    }
+                    ++rank;
                 }
-                ++rank;
+            }
+            found += all;
+            base += Threads * scanned;
+            if (base < cache.pages && found < total)
+            {
+                read_counts(base, counts);
             }
         }
-        found += all;
+        if (found >= total)
+        {
+            return true;
+        }
         __syncthreads();
+        for (int rank = threadIdx.x; rank < found; rank += Threads)
+        {
+            const int i = entry(rank);
+            cache.references[undo(i, rank - shared.before[i])] = 0;
+        }
+        return false;
     }
-    if (found >= total)
-    {
-        return true;
-    }
-    for (int rank = threadIdx.x; rank < found; rank += taking_threads)
-    {
-        const int i = entry(rank);
-        references[undo(i, rank - shared.before[i])] = 0;
-    }
-    return false;
-}
+};
 
-__device__ __forceinline__ void clear_seen(TakingShared& shared)
-{
-    for (int i = threadIdx.x; i < max_sequences / 32 + 1; i += taking_threads)
-    {
-        shared.seen[i] = 0;
-    }
-    if (threadIdx.x == 0)
-    {
-        shared.bad = 0;
-    }
-    __syncthreads();
-}
-
-__global__ __launch_bounds__(taking_threads) void reserve_kernel(PagedCache cache, const int* __restrict__ sequences,
-                                                                 const int* __restrict__ rows, int count, int* status)
+template <int Threads>
+__global__ __launch_bounds__(Threads) void reserve_kernel(PagedCache cache, const int* __restrict__ sequences,
+                                                          const int* __restrict__ rows, int count, int* status)
 {
     extern __shared__ char memory[];
-    auto& shared = *reinterpret_cast<TakingShared*>(memory);
-    clear_seen(shared);
+    Taking<Threads> taking(*reinterpret_cast<TakingShared*>(memory), cache, count);
     const auto sequence = [&](int i) { return sequences ? sequences[i] : i; };
-    // Checked below before it is used.
-    const auto need = [&](int i) -> long long
-    {
-        const int s = sequence(i);
-        const long long last = (long long)cache.lengths[s] + rows[i];
-        const long long pages = (last + cache.page_rows - 1) / cache.page_rows - cache.held[s];
-        return pages > 0 ? pages : 0;
-    };
-    for (int i = threadIdx.x; i < count; i += taking_threads)
-    {
-        const int s = sequence(i);
-        bool ok = s >= 0 && s < cache.sequences;
-        if (ok)
-        {
-            ok = !(atomicOr(&shared.seen[s / 32], 1u << s % 32) >> s % 32 & 1) && rows[i] >= 0 && cache.lengths[s] >= 0 &&
-                 cache.held[s] >= 0 && std::size_t(cache.held[s]) <= cache.table_stride &&
-                 std::size_t((cache.lengths[s] + (long long)rows[i] + cache.page_rows - 1) / cache.page_rows) <=
-                     cache.table_stride;
-        }
-        if (!ok)
-        {
-            shared.bad = 1;
-        }
-    }
-    __syncthreads();
-    if (shared.bad)
+    // Pages that positions up to length + rows take.
+    const auto pages = [&](int i, int s) -> long long
+    { return ((long long)cache.lengths[s] + rows[i] + cache.page_rows - 1) / cache.page_rows; };
+    const bool good = taking.check(sequence,
+                                   [&](int i, int s)
+                                   {
+                                       return rows[i] >= 0 && cache.lengths[s] >= 0 && cache.held[s] >= 0 &&
+                                              std::size_t(cache.held[s]) <= cache.table_stride &&
+                                              std::size_t(pages(i, s)) <= cache.table_stride;
+                                   });
+    if (!good)
     {
         if (threadIdx.x == 0)
         {
@@ -202,22 +242,26 @@ __global__ __launch_bounds__(taking_threads) void reserve_kernel(PagedCache cach
         }
         return;
     }
-    const long long total = sum_needs(shared, count, need);
+    const long long total = taking.sum_needs(
+        [&](int i)
+        {
+            const int s = sequence(i);
+            const int more = int(pages(i, s)) - cache.held[s];
+            return more > 0 ? more : 0;
+        });
     const auto slot = [&](int i, int j) -> int&
     {
         const int s = sequence(i);
         return cache.table[s * cache.table_stride + cache.held[s] + j];
     };
-    const bool enough =
-        total <= cache.pages && take_pages(
-                                    shared, count, int(total), cache.references, cache.pages,
-                                    [&](int i, int j, int page) { slot(i, j) = page; },
-                                    [&](int i, int j)
-                                    {
-                                        const int page = slot(i, j);
-                                        slot(i, j) = -1;
-                                        return page;
-                                    });
+    const bool enough = taking.take_pages(
+        total, [&](int i, int j, int page) { slot(i, j) = page; },
+        [&](int i, int j)
+        {
+            const int page = slot(i, j);
+            slot(i, j) = -1;
+            return page;
+        });
     if (!enough)
     {
         if (threadIdx.x == 0)
@@ -227,9 +271,9 @@ __global__ __launch_bounds__(taking_threads) void reserve_kernel(PagedCache cach
         return;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < count; i += taking_threads)
+    for (int i = threadIdx.x; i < count; i += Threads)
     {
-        cache.held[sequence(i)] += shared.before[i + 1] - shared.before[i];
+        cache.held[sequence(i)] += taking.shared.before[i + 1] - taking.shared.before[i];
     }
 }
 
@@ -241,38 +285,36 @@ static_assert(max_table_pages < arrival && 2 * max_layers + 1 < forking / arriva
 
 // Checks the list, takes a page for each source's last partial one and makes the targets
 // hold their pages; what is shared and copied follows in fork_copy_kernel.
-__global__ __launch_bounds__(taking_threads) void fork_kernel(PagedCache cache, const int* __restrict__ sources,
-                                                              const int* __restrict__ targets, int count, int* status)
+template <int Threads>
+__global__ __launch_bounds__(Threads) void fork_kernel(PagedCache cache, const int* __restrict__ sources,
+                                                       const int* __restrict__ targets, int count, int* status)
 {
     extern __shared__ char memory[];
     auto& shared = *reinterpret_cast<TakingShared*>(memory);
-    clear_seen(shared);
-    for (int i = threadIdx.x; i < count; i += taking_threads)
-    {
-        const int t = targets[i];
-        if (t < 0 || t >= cache.sequences || (atomicOr(&shared.seen[t / 32], 1u << t % 32) >> t % 32 & 1) ||
-            cache.held[t] != 0)
-        {
-            shared.bad = 1;
-        }
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < count; i += taking_threads)
+    Taking<Threads> taking(shared, cache, count);
+    // The words that sources are looked for in, too.
+    for (int i = threadIdx.x; i < count; i += Threads)
     {
         const int s = sources[i];
-        bool ok = s >= 0 && s < cache.sequences && !(shared.seen[s / 32] >> s % 32 & 1);
-        if (ok)
+        if (s >= 0 && s < cache.sequences)
         {
-            ok = cache.lengths[s] >= 0 && cache.held[s] >= 0 && std::size_t(cache.held[s]) <= cache.table_stride &&
-                 (cache.lengths[s] + (long long)cache.page_rows - 1) / cache.page_rows <= cache.held[s];
+            shared.seen[s / 32] = 0;
         }
-        if (!ok)
+    }
+    bool good = taking.check([&](int i) { return targets[i]; }, [&](int, int t) { return cache.held[t] == 0; });
+    for (int i = threadIdx.x; i < count; i += Threads)
+    {
+        const int s = sources[i];
+        if (s < 0 || s >= cache.sequences || (shared.seen[s / 32] >> s % 32 & 1) || cache.lengths[s] < 0 ||
+            cache.held[s] < 0 || std::size_t(cache.held[s]) > cache.table_stride ||
+            (cache.lengths[s] + (long long)cache.page_rows - 1) / cache.page_rows > cache.held[s])
         {
             shared.bad = 1;
         }
     }
     __syncthreads();
-    if (shared.bad)
+    good = good && !shared.bad;
+    if (!good)
     {
         if (threadIdx.x == 0)
         {
@@ -280,12 +322,11 @@ __global__ __launch_bounds__(taking_threads) void fork_kernel(PagedCache cache, 
         }
         return;
     }
-    const auto partial = [&](int i) -> long long { return cache.lengths[sources[i]] % cache.page_rows != 0; };
-    const long long total = sum_needs(shared, count, partial);
+    const long long total = taking.sum_needs([&](int i) { return cache.lengths[sources[i]] % cache.page_rows != 0; });
     const auto slot = [&](int i) -> int&
     { return cache.table[targets[i] * cache.table_stride + cache.lengths[sources[i]] / cache.page_rows]; };
-    const bool enough = take_pages(
-        shared, count, int(total), cache.references, cache.pages, [&](int i, int, int page) { slot(i) = page; },
+    const bool enough = taking.take_pages(
+        total, [&](int i, int, int page) { slot(i) = page; },
         [&](int i, int)
         {
             const int page = slot(i);
@@ -300,7 +341,7 @@ __global__ __launch_bounds__(taking_threads) void fork_kernel(PagedCache cache, 
         }
         return;
     }
-    for (int i = threadIdx.x; i < count; i += taking_threads)
+    for (int i = threadIdx.x; i < count; i += Threads)
     {
         const int length = cache.lengths[sources[i]];
         cache.lengths[targets[i]] = length;
@@ -509,22 +550,25 @@ __device__ __forceinline__ int kept_rows(const int* path, int accepted, int node
     return *bad ? -1 : accepted;
 }
 
-constexpr int moved = 8; // rows a thread moves at a time
+constexpr int moved = 4;       // rows a thread moves at a time
+constexpr int placed = 256;    // rows whose places are looked up at a time
 
-// blockIdx: 256 vectors of a row, the sequence, (layer, keys or values). A thread moves one
-// vector of every kept row, in ascending order: row k comes from node path[k] >= k, so that
-// reading `moved` rows before writing them never meets a row that was written already.
+// blockIdx: vectors of a row, the sequence, (layer, keys or values). Threads stand side by side for
+// up to 256 vectors of a row, and rows apart for the rest; rows are moved in ascending order, as
+// many at a time as there are threads for, all read before any is written: row k comes from node
+// path[k] >= k, so that no row is read that was written.
 __global__ __launch_bounds__(copying_threads) void keep_kernel(PagedCache cache, const int* __restrict__ starts,
                                                                const int* __restrict__ path, std::size_t path_stride,
                                                                const int* __restrict__ accepted, int* lengths,
                                                                int* status)
 {
     __shared__ int bad;
+    __shared__ long long from[placed], to[placed]; // offsets of rows, -1: not moved
     const int s = blockIdx.y;
-    const int length = cache.lengths[s];
+    const int length = cache.lengths[s], count = accepted[s];
     const int nodes = starts[s + 1] - starts[s];
     path += s * path_stride;
-    const int kept = kept_rows(path, accepted[s], nodes, path_stride, &bad);
+    const int kept = kept_rows(path, count, nodes, path_stride, &bad);
     const bool reporter = threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.z == 0;
     if (lengths && reporter)
     {
@@ -538,49 +582,58 @@ __global__ __launch_bounds__(copying_threads) void keep_kernel(PagedCache cache,
         }
         return;
     }
-    const int vector = blockIdx.x * copying_threads + threadIdx.x;
-    if (vector >= cache.heads * cache.head_width / 8)
-    {
-        return;
-    }
+    const int vectors = cache.heads * cache.head_width / 8, first = int(blockIdx.x) * copying_threads;
+    const int wide = min(vectors - first, copying_threads), apart = copying_threads / wide;
+    const int vector = first + int(threadIdx.x) % wide, row = int(threadIdx.x) / wide;
     uint16_t* const memory =
         (blockIdx.z % 2 ? cache.values : cache.keys) + blockIdx.z / 2 * cache.layer_stride + 8 * std::size_t(vector);
-    const auto at = [&](int row) -> uint16_t*
+    const auto place = [&](int node) -> long long
     {
-        const int page = writable_page(cache, s, (long long)length + row);
-        return page < 0 ? nullptr
-                        : memory + page * cache.page_stride + (length + (long long)row) % cache.page_rows * cache.row_stride;
+        const long long position = (long long)length + node;
+        const int page = writable_page(cache, s, position);
+        return page < 0 ? -1
+                        : (long long)(page * cache.page_stride + position % cache.page_rows * cache.row_stride);
     };
-    int k = 0;
-    while (k < kept && path[k] == k)
+    for (int base = 0; base < kept; base += placed)
     {
-        ++k;
-    }
-    for (; k < kept; k += moved)
-    {
-        uint4 value[moved];
-        uint16_t* to[moved];
-#pragma unroll
-        for (int j = 0; j < moved; ++j)
+        const int rows = min(kept - base, placed);
+        __syncthreads();
+        for (int k = threadIdx.x; k < rows; k += copying_threads)
         {
-            const uint16_t* const from = k + j < kept ? at(path[k + j]) : nullptr;
-            to[j] = from ? at(k + j) : nullptr;
-            if (to[j])
-            {
-                value[j] = *reinterpret_cast<const uint4*>(from);
-            }
-            else if (k + j < kept)
+            const int node = path[base + k];
+            // Rows that are in place already stay.
+            const long long source = node == base + k ? -1 : place(node), target = node == base + k ? -1 : place(base + k);
+            from[k] = source;
+            to[k] = source < 0 ? -1 : target;
+            if (node != base + k && (source < 0 || target < 0))
             {
                 report(status, status_invalid);
             }
         }
-#pragma unroll
-        for (int j = 0; j < moved; ++j)
+        __syncthreads();
+        for (int k = 0; k < rows; k += moved * apart)
         {
-            if (to[j])
+            uint4 value[moved];
+#pragma unroll
+            for (int j = 0; j < moved; ++j)
             {
-                *reinterpret_cast<uint4*>(to[j]) = value[j];
+                const int mine = k + j * apart + row;
+                if (row < apart && mine < rows && to[mine] >= 0)
+                {
+                    value[j] = *reinterpret_cast<const uint4*>(memory + from[mine]);
+                }
             }
+            __syncthreads(); // one thread's row is another one's source
+#pragma unroll
+            for (int j = 0; j < moved; ++j)
+            {
+                const int mine = k + j * apart + row;
+                if (row < apart && mine < rows && to[mine] >= 0)
+                {
+                    *reinterpret_cast<uint4*>(memory + to[mine]) = value[j];
+                }
+            }
+            __syncthreads();
         }
     }
 }
@@ -639,7 +692,11 @@ void pages_reserve(const PagedCache& cache, const int* sequences, const int* row
     {
         return;
     }
-    reserve_kernel<<<1, taking_threads, sizeof(TakingShared), stream>>>(cache, sequences, rows, int(count), status);
+    // Four waves for lists that fit them: their barriers are short (3 sequences of a pool of 300 pages
+    // with sixteen waves: 8.0 us).
+    (count <= 256 ? reserve_kernel<256><<<1, 256, sizeof(TakingShared), stream>>>(cache, sequences, rows, int(count), status)
+                  : reserve_kernel<most_threads><<<1, most_threads, sizeof(TakingShared), stream>>>(
+                        cache, sequences, rows, int(count), status));
     check_hip(hipGetLastError(), "pages reserve launch");
 }
 
@@ -650,7 +707,9 @@ void pages_fork(const PagedCache& cache, const int* sources, const int* targets,
     {
         return;
     }
-    fork_kernel<<<1, taking_threads, sizeof(TakingShared), stream>>>(cache, sources, targets, int(count), status);
+    (count <= 256 ? fork_kernel<256><<<1, 256, sizeof(TakingShared), stream>>>(cache, sources, targets, int(count), status)
+                  : fork_kernel<most_threads><<<1, most_threads, sizeof(TakingShared), stream>>>(cache, sources, targets,
+                                                                                                 int(count), status));
     check_hip(hipGetLastError(), "pages fork launch");
     const dim3 grid{unsigned(count), unsigned(2 * cache.layers + 1)};
     fork_copy_kernel<<<grid, copying_threads, 0, stream>>>(cache, sources, targets, status);

@@ -856,33 +856,57 @@ def _need(condition, message):
         raise HipError(message)
 
 
-def _array(tensor, device, kind, count, name):
-    """The address of a contiguous device tensor of at least `count` elements (kind: its dtype's name)."""
-    _need(tensor.device == device, f"{name}: on {tensor.device}, not on {device}")
-    _need(str(tensor.dtype) == kind and tensor.is_contiguous(), f"{name}: must be contiguous {kind}")
-    _need(tensor.numel() >= count, f"{name}: {tensor.numel()} elements, {count} needed")
-    return tensor.data_ptr()
-
-
 _INT, _FLOAT, _LONG = "torch.int32", "torch.float32", "torch.int64"
 #: Element types by dtype; int16 holds BF16 bits, as in the other operators.
 _ROW_TYPES = {"torch.bfloat16": TYPE_BF16, "torch.int16": TYPE_BF16, "torch.float16": TYPE_FP16}
+_PROBABILITY_TYPES = dict(_ROW_TYPES, **{"torch.float32": TYPE_FP32})
+_kinds = {}  # names of the dtypes met so far
+
+
+def _kind(tensor):
+    kind = _kinds.get(tensor.dtype)
+    if kind is None:
+        kind = _kinds[tensor.dtype] = str(tensor.dtype)
+    return kind
+
+
+def _array(tensor, device, kind, count, name):
+    """The address of a contiguous device tensor of at least `count` elements (kind: its dtype's name).
+    Messages are put together only where they are raised: a call of one kernel takes few microseconds."""
+    if tensor.device != device:
+        raise HipError(f"{name}: on {tensor.device}, not on {device}")
+    if _kind(tensor) != kind or not tensor.is_contiguous():
+        raise HipError(f"{name}: must be contiguous {kind}")
+    if tensor.numel() < count:
+        raise HipError(f"{name}: {tensor.numel()} elements, {count} needed")
+    return tensor.data_ptr()
+
+
+_cuda = None  # (current device, current stream's handle by device), once torch is imported
 
 
 def _current(device):
-    import torch
+    """The current stream's handle; the tensors have to be on the current device."""
+    global _cuda
+    if _cuda is None:
+        import torch
 
-    _need(device.type == "cuda" and device.index == torch.cuda.current_device(),
-          f"tensors are on {device}, which is not the current device")
-    return _stream()
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        _cuda = (torch.cuda.current_device, raw or (lambda index: torch.cuda.current_stream(index).cuda_stream))
+    if device.type != "cuda" or device.index != _cuda[0]():
+        raise HipError(f"tensors are on {device}, which is not the current device")
+    return _cuda[1](device.index)
 
 
 def _rows(tensor, device, heads, width, type_, name):
     """(address, row stride) of [rows][heads][width], the heads of a row one after the other."""
-    _need(tensor.device == device and _ROW_TYPES.get(str(tensor.dtype)) == type_, f"{name}: another device or type")
     shape, strides = tensor.shape, tensor.stride()
-    _need(len(shape) == 3 and shape[1] == heads and shape[2] == width, f"{name}: must be [rows][{heads}][{width}]")
-    _need((strides[2] == 1 and (heads == 1 or strides[1] == width)) or not shape[0], f"{name}: heads must be contiguous")
+    if tensor.device != device or _ROW_TYPES.get(_kind(tensor)) != type_:
+        raise HipError(f"{name}: another device or type")
+    if len(shape) != 3 or shape[1] != heads or shape[2] != width:
+        raise HipError(f"{name}: must be [rows][{heads}][{width}]")
+    if shape[0] and (strides[2] != 1 or (heads > 1 and strides[1] != width)):
+        raise HipError(f"{name}: heads must be contiguous")
     return tensor.data_ptr(), strides[0] if shape[0] > 1 else heads * width
 
 
@@ -895,9 +919,9 @@ class PagedCache:
         shape, strides = keys.shape, keys.stride()
         _need(len(shape) == 5 and values.shape == shape and values.stride() == strides and values.dtype == keys.dtype,
               "keys and values: must be [layers][pages][page_rows][heads][head_width], laid out alike")
-        _need(str(keys.dtype) in _ROW_TYPES, "keys and values: must be bfloat16, float16 or int16")
+        _need(_kind(keys) in _ROW_TYPES, "keys and values: must be bfloat16, float16 or int16")
         self.layers, self.pages, self.page_rows, self.heads, self.head_width = shape
-        self.type, self.device, self.sequences = _ROW_TYPES[str(keys.dtype)], keys.device, table.shape[0]
+        self.type, self.device, self.sequences = _ROW_TYPES[_kind(keys)], keys.device, table.shape[0]
         _need(strides[4] == 1 and (shape[3] == 1 or strides[3] == shape[4]), "keys and values: heads must be contiguous")
         _need(values.device == keys.device and table.dim() == 2, "table: must be [sequences][pages a sequence]")
         self.tensors = (keys, values, table, held, lengths, references)  # what the addresses below belong to
@@ -907,6 +931,7 @@ class PagedCache:
             _array(table, d, _INT, 0, "table"), table.shape[1], _array(held, d, _INT, n, "held"),
             _array(lengths, d, _INT, n, "lengths"), _array(references, d, _INT, self.pages, "references"), n)
         self._desc = C.byref(self.desc)
+        self._workspaces = {}  # bytes by (rows, heads, max_rows, max_length)
 
     def _ints(self, tensor, count, name):
         return _array(tensor, self.device, _INT, count, name)
@@ -939,20 +964,22 @@ class PagedCache:
     def write(self, keys, values, starts, max_rows, layer=0, status=None):
         """New rows, [layers][rows][heads][head_width] or, of one layer, [rows][heads][head_width], behind
         each sequence's length."""
-        if keys.dim() == 3:
-            keys, values = keys[None], values[None]
-        _need(keys.dim() == 4 and keys.shape == values.shape and keys.stride() == values.stride(),
-              "keys and values: must be [layers][rows][heads][head_width], laid out alike")
-        _need(_ROW_TYPES.get(str(values.dtype)) == self.type and values.device == self.device,
-              "values: another device or type")
-        layers = keys.shape[0]
-        if not layers:
-            return
-        pointer, stride = _rows(keys[0], self.device, self.heads, self.head_width, self.type, "keys")
+        shape, strides = keys.shape, keys.stride()
+        if values.shape != shape or values.stride() != strides:
+            raise HipError("keys and values: must be laid out alike")
+        if keys.device != self.device or values.device != self.device or \
+                _ROW_TYPES.get(_kind(keys)) != self.type or _ROW_TYPES.get(_kind(values)) != self.type:
+            raise HipError("keys and values: another device or type")
+        if len(shape) == 3:
+            shape, strides = (1, *shape), (0, *strides)
+        layers, rows, heads, width = shape
+        if heads != self.heads or width != self.head_width or \
+                (layers * rows and (strides[3] != 1 or (heads > 1 and strides[2] != width))):
+            raise HipError(f"keys and values: must be [layers][rows][{self.heads}][{self.head_width}], heads contiguous")
         check(library().tsac_hip_pages_write(
-            self._desc, layer, layers, pointer, values.data_ptr(), keys.stride(0) if layers > 1 else 0, stride,
-            keys.shape[1], self._ints(starts, self.sequences + 1, "starts"), max_rows, self._status(status),
-            _current(self.device)))
+            self._desc, layer, layers, keys.data_ptr(), values.data_ptr(), strides[0] if layers > 1 else 0,
+            strides[1] if rows > 1 else heads * width, rows, self._ints(starts, self.sequences + 1, "starts"), max_rows,
+            self._status(status), _current(self.device)))
 
     def keep(self, starts, path, accepted, lengths=None, status=None):
         """Moves each sequence's accepted rows (path [sequences][nodes], accepted) to the front of the
@@ -999,7 +1026,12 @@ def attention_paged(cache, layer, query, starts, max_rows, max_length, mask, sca
     o, o_stride = _rows(out, device, heads, cache.head_width, cache.type, "out")
     _need(out.shape[0] == rows, "out: must have the query's rows")
     words = 0 if mask is None else mask.shape[1]
-    need = lib.tsac_hip_attention_paged_workspace(cache._desc, rows, heads, max_rows, max_length)
+    shape = (rows, heads, max_rows, max_length)
+    need = cache._workspaces.get(shape)
+    if need is None:
+        if len(cache._workspaces) >= 1024:
+            cache._workspaces.clear()
+        need = cache._workspaces[shape] = lib.tsac_hip_attention_paged_workspace(cache._desc, *shape)
     space, size, keep = _workspace(need, workspace, device)
     check(lib.tsac_hip_attention_paged(
         cache._desc, layer, q, q_stride, rows, heads, _array(starts, device, _INT, cache.sequences + 1, "starts"),
@@ -1008,15 +1040,12 @@ def attention_paged(cache, layer, query, starts, max_rows, max_length, mask, sca
     del keep
 
 
-_PROBABILITY_TYPES = dict(_ROW_TYPES, **{"torch.float32": TYPE_FP32})
-
-
 def verify_drafts(target, draft, tokens, parents, starts, max_nodes, uniforms, draws, path, accepted, next,
                   workspace=None):
     """Drafted trees against the target's distributions (target, draft [rows][alphabet], or draft None);
     path int32 [sequences][max_nodes], accepted and next int32 [sequences] are written."""
     device, (rows, alphabet), sequences = target.device, target.shape, starts.numel() - 1
-    type_ = _PROBABILITY_TYPES.get(str(target.dtype))
+    type_ = _PROBABILITY_TYPES.get(_kind(target))
     _need(type_ is not None and (alphabet <= 1 or target.stride(1) == 1), "target: must be rows of probabilities")
     if draft is not None:
         _need(draft.dtype == target.dtype and draft.shape == target.shape and draft.device == device and
