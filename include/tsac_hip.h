@@ -625,9 +625,9 @@ int tsac_hip_attention_paged(const tsac_hip_paged_cache* cache, uint32_t layer, 
  * whole sum; if that is 0, of the row of p as it is; if that is 0 too, -1. path
  * [sequences][max_nodes]: node 0 and the accepted ones, then -1; accepted[s]: their
  * number. A sequence without nodes: 0, -1. Sums are 64-bit and of one order. At most
- * 1024 nodes a sequence (further ones are not looked at) and 2^20 tokens.
+ * 1024 nodes a sequence (further ones are not looked at), 65535 sequences and 2^20 tokens.
  * Workspace as for tsac_hip_attention_paged. */
-size_t tsac_hip_verify_drafts_workspace(size_t sequences, size_t max_nodes, size_t alphabet, int type);
+size_t tsac_hip_verify_drafts_workspace(size_t sequences, size_t alphabet);
 int tsac_hip_verify_drafts(const void* target, size_t target_stride, const void* draft, size_t draft_stride,
                            int type, size_t alphabet, size_t rows, const int32_t* tokens, const int32_t* parents,
                            const int32_t* starts, size_t sequences, size_t max_nodes, const float* uniforms,

@@ -673,7 +673,7 @@ Drafts drafts_of(std::size_t sequences, std::size_t max_nodes, std::size_t alpha
     require(alphabet > 0 && alphabet <= (std::size_t(1) << 20), "verify: alphabets of 1 to 2^20 tokens");
     require(max_nodes <= std::size_t(max_draft_nodes) && (max_nodes > 0 || !sequences),
             "verify: trees of 1 to 1024 nodes");
-    require(sequences < (std::size_t(1) << 24), "verify: too many sequences");
+    require(sequences <= std::size_t(max_sequences), "verify: too many sequences");
     Drafts d;
     d.type = type;
     d.alphabet = int(alphabet);
@@ -1561,10 +1561,10 @@ int tsac_hip_attention_paged(const tsac_hip_paged_cache* cache, uint32_t layer, 
         });
 }
 
-size_t tsac_hip_verify_drafts_workspace(size_t sequences, size_t max_nodes, size_t alphabet, int type)
+size_t tsac_hip_verify_drafts_workspace(size_t sequences, size_t alphabet)
 {
     size_t bytes = 0;
-    guarded([&] { bytes = verify_drafts_workspace(drafts_of(sequences, max_nodes, alphabet, type)); });
+    guarded([&] { bytes = verify_drafts_workspace(drafts_of(sequences, 1, alphabet, TSAC_HIP_TYPE_BF16)); });
     return bytes;
 }
 

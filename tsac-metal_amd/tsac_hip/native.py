@@ -231,7 +231,7 @@ def library() -> C.CDLL:
         lib.tsac_hip_attention_paged_workspace.restype = sz
         lib.tsac_hip_attention_paged.argtypes = [cache, C.c_uint32, vp, sz, sz, sz, vp, sz, sz, vp, sz, C.c_float, vp, sz,
                                                  vp, sz, vp]
-        lib.tsac_hip_verify_drafts_workspace.argtypes = [sz, sz, sz, C.c_int]
+        lib.tsac_hip_verify_drafts_workspace.argtypes = [sz, sz]
         lib.tsac_hip_verify_drafts_workspace.restype = sz
         lib.tsac_hip_verify_drafts.argtypes = [vp, sz, vp, sz, C.c_int, sz, sz, vp, vp, vp, sz, sz, vp, vp, vp, vp, vp,
                                                vp, sz, vp]
@@ -1051,7 +1051,7 @@ def verify_drafts(target, draft, tokens, parents, starts, max_nodes, uniforms, d
         _need(draft.dtype == target.dtype and draft.shape == target.shape and draft.device == device and
               (alphabet <= 1 or draft.stride(1) == 1), "draft: must be as target")
     lib = library()
-    need = lib.tsac_hip_verify_drafts_workspace(sequences, max_nodes, alphabet, type_)
+    need = lib.tsac_hip_verify_drafts_workspace(sequences, alphabet)
     space, size, keep = _workspace(need, workspace, device)
     check(lib.tsac_hip_verify_drafts(
         target.data_ptr(), target.stride(0), None if draft is None else draft.data_ptr(),
