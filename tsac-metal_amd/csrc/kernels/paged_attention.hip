@@ -638,14 +638,16 @@ template <int HW> __device__ __forceinline__ unsigned pair(const unsigned (&valu
 
 // 16 bytes a lane, from each lane's address to `to`, lane after lane; the wave waits for it with
 // its other loads (s_waitcnt vmcnt). Written out because the compiler would wait for it before any
-// other read of LDS. M0 is reserved, so that clang warns where it is named; nothing else uses it.
+// other read of LDS. A load to LDS needs a wait state behind a write of M0, which the compiler
+// does not put into assembly. M0 is reserved, so that clang warns where it is named; nothing else
+// uses it.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void load_to_lds(const void* from, void* to)
 {
     const unsigned address =
         unsigned(reinterpret_cast<std::uintptr_t>((__attribute__((address_space(3))) const void*)to));
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from),
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from),
                  "s"(__builtin_amdgcn_readfirstlane(address))
                  : "memory", "m0");
 }
@@ -890,6 +892,7 @@ template <int Count> __device__ __forceinline__ void wait_memory()
 {
     static_assert(Count < 16);
     __builtin_amdgcn_s_waitcnt(Count | 7 << 4 | 15 << 8);
+    asm volatile("" ::: "memory"); // no read of LDS moves in front
 }
 
 // How far the 16-byte pieces of a key row and the 32-byte pieces of a value row are shifted in LDS (by
