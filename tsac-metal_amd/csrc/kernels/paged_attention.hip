@@ -11,15 +11,13 @@
 // keys, are taken 16 at a time, the keys 32 at a time (a block). Scores are computed transposed
 // (keys x queries), so that a lane holds eight keys of one query; the weights then are the
 // second product's operand as they lie, with keys in the order of the registers. Its other
-// operand needs eight keys of one coordinate per lane: a lane loads 8 (or 4) coordinates of
-// eight keys and pairs halves with one byte permute a register, so that a row of the cache is
-// read in whole lines and nothing is transposed through memory.
+// operand needs eight keys of one coordinate per lane: LDS transposes values as they are read.
 //
-// Up to 32 query rows (direct_kernel) the cache's bytes are what costs: a wave takes all rows
-// and every fourth block of its workgroup's chunk of keys, straight from memory into operand
-// registers. More rows (staged_kernel) cost products and exponentials: a wave takes 32 rows, and
-// the four of a workgroup share blocks that they stage in LDS in operand order. Chunks are
-// joined in ascending order by join_kernel.
+// Rows of the cache go from memory straight into LDS, in whole lines. Up to 32 query rows
+// (narrow_kernel) the cache's bytes are what costs: a wave takes all rows and every eighth block
+// of its workgroup's chunk of keys, through LDS of its own. More rows (staged_kernel) cost
+// products and exponentials: a wave takes 32 rows, and all eight of a workgroup read the same
+// stages of keys. Chunks are joined in ascending order by join_kernel.
 #include "paged.hpp"
 
 #include <algorithm>
@@ -37,7 +35,7 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2_ __attribute__((ext_vector_type(2)));
 
-constexpr int waves = 4;  // of a workgroup
+constexpr int waves = 8;  // of a workgroup
 constexpr int block = 32; // keys of one step
 constexpr float minus_infinity = -__builtin_inff();
 
@@ -196,9 +194,9 @@ __device__ __forceinline__ std::size_t locate(const Launch& l, const Place& p, i
     return (there ? read : 0) * l.page_stride + std::size_t(position & ((1 << l.page_shift) - 1)) * l.row_stride;
 }
 
-// One 16-row part's running sums. A lane has row lane % 16 and 4 * HW / 16 of its coordinates:
-// those 16 * j + 4 * (lane / 16) + i (Across), or (4 * (lane / 16) + i) * (HW / 16) + j.
-template <int HW, bool Across> struct Sums
+// One 16-row part's running sums. A lane has row lane % 16 and its coordinates
+// 16 * j + 4 * (lane / 16) + i.
+template <int HW> struct Sums
 {
     static constexpr int step = HW / 16;
     static constexpr int words = 4 * step + 2; // a lane's, joined within a workgroup
@@ -260,30 +258,14 @@ template <int HW, bool Across> struct Sums
             }
         }
     }
-    // put(first coordinate, values): runs of them in ascending order.
-    template <class Put> __device__ __forceinline__ void each(int lane, Put put) const
-    {
-        constexpr int runs = Across ? step : 4, length = Across ? 4 : step;
-#pragma unroll
-        for (int r = 0; r < runs; ++r)
-        {
-            float values[length];
-#pragma unroll
-            for (int k = 0; k < length; ++k)
-            {
-                values[k] = Across ? out[r][k] : out[k][r];
-            }
-            put(Across ? 16 * r + 4 * (lane / 16) : (4 * (lane / 16) + r) * step, values);
-        }
-    }
     __device__ __forceinline__ void store(float* to, int lane) const
     {
         const int row = lane % 16;
-        each(lane,
-             [&](int first, const auto& values)
-             {
-                 __builtin_memcpy(__builtin_assume_aligned(to + row * HW + first, 16), values, sizeof values);
-             });
+#pragma unroll
+        for (int j = 0; j < step; ++j)
+        {
+            *reinterpret_cast<f32x4*>(to + row * HW + 16 * j + 4 * (lane / 16)) = out[j];
+        }
         if (lane < 16)
         {
             to[16 * HW + row] = reference;
@@ -310,20 +292,24 @@ __device__ __forceinline__ void write_row(const Launch& l, const Place& p, int r
 }
 
 // A part's sums: to the output, or as the chunk's record.
-template <int HW, bool Half, bool Across>
+template <int HW, bool Half>
 __device__ __forceinline__ void finish(const Launch& l, const Place& p, int unit, int row, int lane,
-                                       const Sums<HW, Across>& sums)
+                                       const Sums<HW>& sums)
 {
     if (chunks_of(l, p) > 1)
     {
-        sums.store(l.partial + (std::size_t(unit) * l.parts + row / 16) * Sums<HW, Across>::record, lane);
+        sums.store(l.partial + (std::size_t(unit) * l.parts + row / 16) * Sums<HW>::record, lane);
         return;
     }
     const int mine = row + lane % 16;
     if (mine / l.group < p.nodes)
     {
-        sums.each(lane, [&](int first, const auto& values)
-                  { write_row<HW, Half>(l, p, mine, first, values, sums.total[0]); });
+#pragma unroll
+        for (int j = 0; j < Sums<HW>::step; ++j)
+        {
+            const float values[4] = {sums.out[j][0], sums.out[j][1], sums.out[j][2], sums.out[j][3]};
+            write_row<HW, Half>(l, p, mine, 16 * j + 4 * (lane / 16), values, sums.total[0]);
+        }
     }
 }
 
@@ -374,9 +360,9 @@ __device__ __forceinline__ unsigned seen(const Launch& l, const Place& p, int at
 }
 
 // A value row that is not finite, of new row `key` of the block, for the rows that see it.
-template <int HW, bool Half, bool Across>
+template <int HW, bool Half>
 __device__ __forceinline__ void add_poisoned(const Launch& l, const Place& p, int at, int key, float weight, bool live,
-                                             int lane, Sums<HW, Across>& sums)
+                                             int lane, Sums<HW>& sums)
 {
     constexpr int step = HW / 16;
     bool there;
@@ -390,44 +376,11 @@ __device__ __forceinline__ void add_poisoned(const Launch& l, const Place& p, in
 #pragma unroll
             for (int j = 0; j < step; ++j)
             {
-                const int first = 4 * (lane / 16) + i;
-                const uint16_t bits = from[Across ? 16 * j + first : first * step + j];
+                const uint16_t bits = from[16 * j + 4 * (lane / 16) + i];
                 sums.out[j][i] += nonfinite<Half>(bits) ? weight * widen<Half>(bits) : 0.0f;
             }
         }
     }
-}
-
-// Drops from half a block's values, slots 4 * half .. of the lane, those of keys that do not exist
-// (a weight of zero would not drop one that is not finite), and those not finite of new rows,
-// which only some queries see. Returns the bits of the latter's keys.
-template <int HW, bool Half>
-__device__ __forceinline__ unsigned clean(unsigned (&value)[4][HW / 32], int half, unsigned exist, unsigned cached, int lane)
-{
-    unsigned poisoned = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-    {
-        const int key = 16 * half + 4 * (lane / 16) + i;
-        const bool there = exist >> key & 1, fresh = !(cached >> key & 1);
-        bool wrong = false;
-#pragma unroll
-        for (int w = 0; w < HW / 32; ++w)
-        {
-            unsigned& v = value[i][w];
-            const unsigned keep = (nonfinite<Half>(uint16_t(v)) ? 0u : 0xffffu) |
-                                  (nonfinite<Half>(uint16_t(v >> 16)) ? 0u : 0xffff0000u);
-            wrong = wrong || keep != ~0u;
-            v = !there ? 0u : fresh ? v & keep : v;
-        }
-        const uint64_t lanes = __ballot(wrong && there && fresh);
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-        {
-            poisoned |= (lanes >> 16 * q & 0xffff ? 1u : 0u) << (16 * half + 4 * q + i);
-        }
-    }
-    return poisoned;
 }
 
 // What masks ask of a block: which keys exist, and which new ones have values that are not finite.
@@ -464,8 +417,8 @@ __device__ __forceinline__ void score_block(const u32x4 (&key)[2][HW / 32], cons
 // Moves the running references, if need be, before a block's scores are weighed: only when a
 // score passes one by 2^8. Weights stay in range without it, and most blocks need neither the
 // exchange nor the scaling.
-template <int HW, bool Across, int Parts>
-__device__ __forceinline__ void settle(const Launch& l, const f32x4 (&score)[Parts][2], Sums<HW, Across> (&sums)[Parts])
+template <int HW, int Parts>
+__device__ __forceinline__ void settle(const Launch& l, const f32x4 (&score)[Parts][2], Sums<HW> (&sums)[Parts])
 {
     float most[Parts];
     bool move = false;
@@ -490,9 +443,9 @@ __device__ __forceinline__ void settle(const Launch& l, const f32x4 (&score)[Par
 }
 
 // Weights of a block's scores against the references.
-template <int HW, bool Half, bool Across, int Parts>
+template <int HW, bool Half, int Parts>
 __device__ __forceinline__ void weigh(const Launch& l, const f32x4 (&score)[Parts][2],
-                                      const Sums<HW, Across> (&sums)[Parts], u32x4 (&weight)[Parts])
+                                      const Sums<HW> (&sums)[Parts], u32x4 (&weight)[Parts])
 {
 #pragma unroll
     for (int t = 0; t < Parts; ++t)
@@ -513,10 +466,10 @@ __device__ __forceinline__ void weigh(const Launch& l, const f32x4 (&score)[Part
     }
 }
 
-// Adds a block's weighted values; value(j) gives the j-th coordinates of its keys. The
+// Adds a block's weighted values; value[j]: coordinate 16 * j + lane % 16 of its keys. The
 // sum of a row's weights, as they are rounded, is one more product.
-template <int HW, bool Half, bool Across, int Parts, class Values>
-__device__ __forceinline__ void add_block(const u32x4 (&weight)[Parts], Sums<HW, Across> (&sums)[Parts], Values value)
+template <int HW, bool Half, int Parts>
+__device__ __forceinline__ void add_block(const u32x4 (&weight)[Parts], Sums<HW> (&sums)[Parts], const u32x4 (&value)[HW / 16])
 {
     constexpr unsigned one = Half ? 0x3c003c00u : 0x3f803f80u;
 #pragma unroll
@@ -527,7 +480,7 @@ __device__ __forceinline__ void add_block(const u32x4 (&weight)[Parts], Sums<HW,
 #pragma unroll
     for (int j = 0; j < HW / 16; ++j)
     {
-        const u32x4 v = value(j);
+        const u32x4 v = value[j];
 #pragma unroll
         for (int t = 0; t < Parts; ++t)
         {
@@ -537,10 +490,10 @@ __device__ __forceinline__ void add_block(const u32x4 (&weight)[Parts], Sums<HW,
 }
 
 // A block with masks: the keys that a row does not see weigh nothing, whatever they are.
-template <int HW, bool Half, bool Across, int Parts, class Values>
+template <int HW, bool Half, int Parts>
 __device__ __forceinline__ void attend_masked(const Launch& l, const Place& p, int at, Marks marks, int lane,
                                               const u32x4 (&key)[2][HW / 32], const u32x4 (&query)[Parts][HW / 32],
-                                              const int (&node)[Parts], Sums<HW, Across> (&sums)[Parts], Values value)
+                                              const int (&node)[Parts], Sums<HW> (&sums)[Parts], const u32x4 (&value)[HW / 16])
 {
     f32x4 score[Parts][2];
     score_block<HW, Half>(key, query, score);
@@ -592,62 +545,18 @@ __device__ __forceinline__ void attend_masked(const Launch& l, const Place& p, i
     add_block<HW, Half>(weight, sums, value);
 }
 
-// A lane's byte offsets from where 16 keys lie. Rows are under 2^25 bytes apart, so that these
-// fit 32 bits and what is common to the wave stays in scalar registers.
-struct Offsets
-{
-    unsigned key, value, row; // row: the same for all lanes
-};
-template <int HW> __device__ __forceinline__ Offsets offsets_of(const Launch& l, int lane)
-{
-    constexpr unsigned step = HW / 16;
-    return {2 * (lane % 16 * l.row_stride + lane / 16 * 8), 2 * (lane / 16 * 4 * l.row_stride + lane % 16 * step),
-            2 * l.row_stride};
-}
-
-// Half a block's keys, 16 of them, in operand order.
-template <int HW>
-__device__ __forceinline__ void load_keys(const uint16_t* from, const Offsets& o, u32x4 (&key)[HW / 32])
-{
-    const char* const mine = reinterpret_cast<const char*>(from) + o.key;
-#pragma unroll
-    for (int d = 0; d < HW / 32; ++d)
-    {
-        key[d] = *reinterpret_cast<const u32x4*>(mine + 64 * d);
-    }
-}
-
-// Half a block's values as a lane loads them, 16 keys: `step` coordinates of four keys.
-template <int HW>
-__device__ __forceinline__ void load_values(const uint16_t* from, const Offsets& o, unsigned (&value)[4][HW / 32])
-{
-    using Part = std::conditional_t<HW == 128, u32x4, u32x2>;
-    const char* row = reinterpret_cast<const char*>(from);
-#pragma unroll
-    for (int i = 0; i < 4; ++i, row += o.row)
-    {
-        *reinterpret_cast<Part*>(value[i]) = *reinterpret_cast<const Part*>(row + o.value);
-    }
-}
-
-// Coordinate j of keys i and i + 1, out of a lane's values.
-template <int HW> __device__ __forceinline__ unsigned pair(const unsigned (&value)[4][HW / 32], int i, int j)
-{
-    return __builtin_amdgcn_perm(value[i + 1][j / 2], value[i][j / 2], j % 2 ? 0x07060302u : 0x05040100u);
-}
-
-// 16 bytes a lane, from each lane's address to `to`, lane after lane; the wave waits for it with
-// its other loads (s_waitcnt vmcnt). Written out because the compiler would wait for it before any
-// other read of LDS. A load to LDS needs a wait state behind a write of M0, which the compiler
-// does not put into assembly. M0 is reserved, so that clang warns where it is named; nothing else
+// 16 bytes a lane, from `offset` bytes behind `from`, to `to`, lane after lane; the wave waits for it
+// with its other loads (s_waitcnt vmcnt). Written out because the compiler would wait for it
+// before any other read of LDS. A load to LDS needs a wait state behind a write of M0, which the
+// compiler does not put into assembly. M0 is reserved, so that clang warns where it is named; nothing else
 // uses it.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
-__device__ __forceinline__ void load_to_lds(const void* from, void* to)
+__device__ __forceinline__ void load_to_lds(const void* from, unsigned offset, void* to)
 {
     const unsigned address =
         unsigned(reinterpret_cast<std::uintptr_t>((__attribute__((address_space(3))) const void*)to));
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from),
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(from),
                  "s"(__builtin_amdgcn_readfirstlane(address))
                  : "memory", "m0");
 }
@@ -662,22 +571,19 @@ __device__ __forceinline__ u32x2 read_transposed(const char* from)
         u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)from));
 }
 
-// clean() for a stage's values where they lie in LDS, eight keys a wave, for the whole workgroup.
-template <int HW, bool Half>
-__device__ __forceinline__ void clean_stage(const Launch& l, const Place& p, int at, int end, int warp, int lane,
-                                            char* values, Marks* marked)
+// Drops from `Pieces` KiB of values in LDS, whole rows, those of keys that do not exist (a weight of
+// zero would not drop one that is not finite), and those not finite of new rows, which only some
+// queries see. Returns the bits of the latter's keys.
+template <int HW, bool Half, int Pieces>
+__device__ __forceinline__ unsigned clean(char* values, unsigned exist, unsigned cached, int lane)
 {
-    constexpr int lanes = HW / 8, pieces = HW / 64; // lanes of a row
-    const int first = at + 8 * warp;                // of the wave's keys
-    bool there;
-    locate(l, p, first / 16 * 16, there);
-    const unsigned exist = there ? low_bits(end - first) & 0xff : 0u, cached = low_bits(p.length - first);
-    Marks marks = {exist, 0};
-#pragma unroll
-    for (int i = 0; i < pieces; ++i)
+    constexpr int lanes = HW / 8, rows_a_piece = 64 / lanes; // lanes of a row
+    unsigned poisoned = 0;
+#pragma unroll 1
+    for (int i = 0; i < Pieces; ++i)
     {
-        const int key = i * (64 / lanes) + lane / lanes;
-        u32x4& v = *reinterpret_cast<u32x4*>(values + (warp * pieces + i) * 1024 + lane * 16);
+        const int key = i * rows_a_piece + lane / lanes;
+        u32x4& v = *reinterpret_cast<u32x4*>(values + i * 1024 + lane * 16);
         u32x4 x = v;
         const bool here = exist >> key & 1, fresh = !(cached >> key & 1);
         bool wrong = false;
@@ -692,14 +598,28 @@ __device__ __forceinline__ void clean_stage(const Launch& l, const Place& p, int
         v = x;
         const uint64_t bad = __ballot(wrong && here && fresh);
 #pragma unroll
-        for (int k = 0; k < 64 / lanes; ++k)
+        for (int k = 0; k < rows_a_piece; ++k)
         {
-            marks.poisoned |= (bad >> k * lanes & ((1ull << lanes) - 1) ? 1u : 0u) << (i * (64 / lanes) + k);
+            poisoned |= (bad >> k * lanes & ((1ull << lanes) - 1) ? 1u : 0u) << (i * rows_a_piece + k);
         }
     }
+    return poisoned;
+}
+
+// clean() for a stage, eight keys a wave, for the whole workgroup.
+template <int HW, bool Half>
+__device__ __forceinline__ void clean_stage(const Launch& l, const Place& p, int at, int end, int warp, int lane,
+                                            char* values, Marks* marked)
+{
+    const int first = at + 8 * warp; // of the wave's keys
+    bool there;
+    locate(l, p, first / 16 * 16, there);
+    const unsigned exist = there ? low_bits(end - first) & 0xff : 0u;
+    const unsigned poisoned =
+        clean<HW, Half, HW / 64>(values + warp * (HW / 64) * 1024, exist, low_bits(p.length - first), lane);
     if (lane == 0)
     {
-        marked[warp] = marks;
+        marked[warp] = Marks{exist, poisoned};
     }
     __syncthreads();
 }
@@ -738,11 +658,84 @@ __device__ __forceinline__ void unit_of(const Launch& l, int& unit, int& tile)
     unit = (j / l.together * 8 + die) * l.together + j % l.together;
 }
 
-// A tile is `Parts` x 16 rows; a wave takes every fourth block of the chunk.
-template <int HW, bool Half, int Parts> __global__ __launch_bounds__(64 * waves, Parts == 1 ? 3 : 2) void direct_kernel(Launch l)
+// How far the 16-byte pieces of a key row and the 32-byte pieces of a value row are shifted in LDS (by
+// exclusive or), so that a piece of 16 rows meets every bank: 16 keys' pieces are read at a time,
+// and 16 value rows' transposed.
+template <int HW> __device__ __forceinline__ int key_shift(int row)
 {
-    constexpr int depth = HW / 32, words = Sums<HW, false>::words * 64;
-    extern __shared__ float joined[];
+    return HW == 128 ? row & 15 : row >> 1 & 7;
+}
+template <int HW> __device__ __forceinline__ int value_shift(int row)
+{
+    return HW == 128 ? row & 7 : row >> 1 & 3;
+}
+
+// At most `count` of the wave's memory operations still under way (they complete in order).
+template <int Count> __device__ __forceinline__ void wait_memory()
+{
+    static_assert(Count < 16);
+    __builtin_amdgcn_s_waitcnt(Count | 7 << 4 | 15 << 8);
+    asm volatile("" ::: "memory"); // no read of LDS moves in front
+}
+
+__device__ __forceinline__ void wait_lds()
+{
+    __builtin_amdgcn_s_waitcnt(15 | 3 << 14 | 7 << 4);
+    asm volatile("" ::: "memory");
+}
+
+// Reads a block's operands from where its rows lie in LDS.
+template <int HW> struct Reading
+{
+    static constexpr int row_bytes = 2 * HW;
+    int key_lane, key_shifted, value_lane, value_shifted;
+
+    __device__ explicit Reading(int lane)
+    {
+        const int key_row = lane % 16, value_row = lane % 16 / 4 + 4 * (lane / 16); // of a half, by the lane's address
+        key_lane = key_row * row_bytes;
+        key_shifted = 16 * (lane / 16 ^ key_shift<HW>(key_row));
+        value_lane = value_row * row_bytes + lane % 4 * 8;
+        value_shifted = 32 * value_shift<HW>(value_row);
+    }
+    __device__ __forceinline__ void keys(const char* rows, u32x4 (&key)[2][HW / 32]) const
+    {
+        const char* const from = rows + key_lane;
+#pragma unroll
+        for (int d = 0; d < HW / 32; ++d)
+        {
+            const char* const piece = from + (64 * d ^ key_shifted);
+            key[0][d] = *reinterpret_cast<const u32x4*>(piece);
+            key[1][d] = *reinterpret_cast<const u32x4*>(piece + 16 * row_bytes);
+        }
+        asm volatile("" ::: "memory"); // here, not where they are used
+    }
+    __device__ __forceinline__ void values(const char* rows, u32x4 (&value)[HW / 16]) const
+    {
+        const char* const from = rows + value_lane;
+#pragma unroll
+        for (int j = 0; j < HW / 16; ++j)
+        {
+            const char* const piece = from + (32 * j ^ value_shifted);
+            const u32x2 low = read_transposed(piece), high = read_transposed(piece + 16 * row_bytes);
+            value[j] = u32x4{low[0], low[1], high[0], high[1]};
+        }
+        asm volatile("" ::: "memory");
+    }
+};
+
+// A tile is `Parts` x 16 rows, and a wave takes every eighth block of the chunk. A block's keys and
+// values come into the wave's own 16 KiB of LDS in whole rows, and the next ones are asked for
+// once these are in registers: a unit has up to 128 KiB under way, and its waves wait for nothing
+// but their own loads. A token of each of 8 sequences, 264 MB of keys and values: 52 us, 5.0 TB/s,
+// and 5 us for the join; with operands loaded from memory into registers, 64 bytes of a row at a
+// time, 58 us.
+template <int HW, bool Half, int Parts> __global__ __launch_bounds__(64 * waves, 2) void narrow_kernel(Launch l)
+{
+    constexpr int depth = HW / 32, step = HW / 16, row_bytes = 2 * HW, lanes = HW / 8, rows_a_piece = 64 / lanes;
+    constexpr int half_pieces = 16 / rows_a_piece, pieces = 2 * half_pieces; // loads of a block's keys, or values
+    constexpr int words = Sums<HW>::words * 64;
+    extern __shared__ __attribute__((aligned(128))) char memory[]; // [wave]: keys [key][HW], values [key][HW]
     const int lane = threadIdx.x % 64, warp = __builtin_amdgcn_readfirstlane(int(threadIdx.x / 64));
     int unit, tile;
     unit_of(l, unit, tile);
@@ -753,24 +746,19 @@ template <int HW, bool Half, int Parts> __global__ __launch_bounds__(64 * waves,
     }
     const int begin = p.split * l.chunk, end = chunk_end(l, p);
     // Every row sees what lies in front of this.
-    const int open = l.mask ? p.length : p.length + p.row / l.group + 1;
-    u32x4 query[Parts][depth];
-    int node[Parts];
-    Sums<HW, false> sums[Parts];
-#pragma unroll
-    for (int t = 0; t < Parts; ++t)
-    {
-        load_query<HW>(l, p, p.row + 16 * t, lane, query[t], node[t]);
-        sums[t].clear();
-    }
+    const int open = min(end, l.mask ? p.length : p.length + p.row / l.group + 1);
 
-    // A block's keys are asked for as soon as the last one's are used up, and so are its values:
-    // one set of registers each, and either is under way while the other is worked on. Where
-    // they lie is looked up a block earlier.
-    const Offsets offsets = offsets_of<HW>(l, lane);
-    u32x4 key[2][depth];
-    unsigned value[2][4][HW / 32];
-    std::size_t base[2];
+    char* const own = memory + warp * (2 * block * row_bytes);
+    char* const own_values = own + block * row_bytes;
+    unsigned key_offset[half_pieces], value_offset[half_pieces]; // bytes, of a lane, from a half's start
+#pragma unroll
+    for (int i = 0; i < half_pieces; ++i)
+    {
+        const int r = i * rows_a_piece + lane / lanes, place = lane % lanes;
+        key_offset[i] = 2 * (r * l.row_stride) + 16 * (place ^ key_shift<HW>(r));
+        value_offset[i] = 2 * (r * l.row_stride) + 16 * (place ^ 2 * value_shift<HW>(r));
+    }
+    std::size_t base[2]; // where the halves of the next block to load lie
     bool there[2];
     const auto find = [&](int at)
     {
@@ -780,76 +768,97 @@ template <int HW, bool Half, int Parts> __global__ __launch_bounds__(64 * waves,
             base[half] = locate(l, p, at + 16 * half, there[half]) + std::size_t(p.head) * HW;
         }
     };
-    const auto load_both_keys = [&]
+    const auto load = [&](const uint16_t* rows, const unsigned (&offset)[half_pieces], char* to)
     {
 #pragma unroll
         for (int half = 0; half < 2; ++half)
         {
-            load_keys<HW>(l.keys + base[half], offsets, key[half]);
-        }
-    };
-    const auto load_both_values = [&]
-    {
 #pragma unroll
-        for (int half = 0; half < 2; ++half)
-        {
-            load_values<HW>(l.values + base[half], offsets, value[half]);
+            for (int i = 0; i < half_pieces; ++i)
+            {
+                load_to_lds(rows + base[half], offset[i], to + (half * half_pieces + i) * 1024);
+            }
         }
     };
-    const auto value_of = [&](int j)
-    {
-        return u32x4{pair<HW>(value[0], 0, j), pair<HW>(value[0], 2, j), pair<HW>(value[1], 0, j),
-                     pair<HW>(value[1], 2, j)};
-    };
-    constexpr int stride = block * waves;
     int at = begin + block * warp;
-    const int whole = min(open, end) - block; // the last block that all rows see whole
-    if (at <= whole)
+    constexpr int stride = block * waves;
+    bool here[2] = {}; // `there` of the block that is worked on
+    if (at < end)
     {
         find(at);
-        load_both_keys();
-        load_both_values();
-        bool here = there[0] && there[1]; // of the block in registers
+        load(l.keys, key_offset, own);
+        load(l.values, value_offset, own_values);
+        here[0] = there[0];
+        here[1] = there[1];
         find(at + stride);
-        while (at <= whole && here)
-        {
-            const bool more = at + stride <= whole;
-            f32x4 score[Parts][2];
-            score_block<HW, Half>(key, query, score);
-            if (more)
-            {
-                load_both_keys();
-            }
-            settle(l, score, sums);
-            u32x4 weight[Parts];
-            weigh<HW, Half>(l, score, sums, weight);
-            add_block<HW, Half>(weight, sums, value_of);
-            at += stride;
-            if (more)
-            {
-                load_both_values();
-                here = there[0] && there[1];
-                find(at + stride);
-            }
-        }
     }
-    // What is left: blocks with masks, and all behind a page that is not there.
+    u32x4 query[Parts][depth];
+    int node[Parts];
+    Sums<HW> sums[Parts];
+#pragma unroll
+    for (int t = 0; t < Parts; ++t)
+    {
+        load_query<HW>(l, p, p.row + 16 * t, lane, query[t], node[t]);
+        sums[t].clear();
+    }
+    u32x4 key[2][depth], value[step];
+    const Reading<HW> reading(lane);
+    // The block at `at` into registers, and the next one asked for.
+    const auto take = [&](auto clean_values)
+    {
+        const bool more = at + stride < end;
+        wait_memory<pieces>(); // the keys
+        reading.keys(own, key);
+        wait_lds();
+        if (more)
+        {
+            load(l.keys, key_offset, own);
+            wait_memory<pieces>(); // the values
+        }
+        else
+        {
+            wait_memory<0>();
+        }
+        clean_values();
+        reading.values(own_values, value);
+        wait_lds();
+        if (more)
+        {
+            load(l.values, value_offset, own_values);
+            here[0] = there[0];
+            here[1] = there[1];
+            find(at + 2 * stride);
+        }
+    };
+    for (; at + block <= open && here[0] && here[1]; at += stride)
+    {
+        take([] {});
+        f32x4 score[Parts][2];
+        score_block<HW, Half>(key, query, score);
+        settle(l, score, sums);
+        u32x4 weight[Parts];
+        weigh<HW, Half>(l, score, sums, weight);
+        add_block<HW, Half>(weight, sums, value);
+    }
+    // From the first block on that asks for masks.
+#pragma unroll 1
     for (; at < end; at += stride)
     {
-        find(at);
-        load_both_keys();
-        load_both_values();
-        Marks marks;
-        marks.exist = low_bits(end - at) & ((there[0] ? 0xffffu : 0u) | (there[1] ? 0xffff0000u : 0u));
-        const unsigned cached = low_bits(p.length - at);
-        marks.poisoned = clean<HW, Half>(value[0], 0, marks.exist, cached, lane) |
-                         clean<HW, Half>(value[1], 1, marks.exist, cached, lane);
-        attend_masked<HW, Half>(l, p, at, marks, lane, key, query, node, sums, value_of);
+        Marks marks = {low_bits(end - at) & ((here[0] ? 0xffffu : 0u) | (here[1] ? 0xffff0000u : 0u)), 0};
+        take(
+            [&]
+            {
+                marks.poisoned = clean<HW, Half, pieces>(own_values, marks.exist, low_bits(p.length - at), lane);
+                wait_lds();
+            });
+        attend_masked<HW, Half>(l, p, at, marks, lane, key, query, node, sums, value);
     }
 
-    // Waves 2 and 3 to 0 and 1, then 1 to 0.
-#pragma unroll
-    for (int half = 2; half >= 1; half /= 2)
+    // Half the waves to the other half, down to one.
+    float* const joined = reinterpret_cast<float*>(memory);
+    __syncthreads();
+#pragma unroll 1
+    for (int half = waves / 2; half >= 1; half /= 2)
     {
         if (warp >= half && warp < 2 * half)
         {
@@ -883,41 +892,20 @@ template <int HW, bool Half, int Parts> __global__ __launch_bounds__(64 * waves,
     }
 }
 
-constexpr int staging_waves = 8;
 constexpr int staged_keys = 2 * block; // of a stage
 constexpr int stages = 4;              // in LDS
-
-// At most `count` of the wave's memory operations still under way (they complete in order).
-template <int Count> __device__ __forceinline__ void wait_memory()
-{
-    static_assert(Count < 16);
-    __builtin_amdgcn_s_waitcnt(Count | 7 << 4 | 15 << 8);
-    asm volatile("" ::: "memory"); // no read of LDS moves in front
-}
-
-// How far the 16-byte pieces of a key row and the 32-byte pieces of a value row are shifted in LDS (by
-// exclusive or), so that a piece of 16 rows meets every bank: 16 keys' pieces are read at a time,
-// and 16 value rows' transposed.
-template <int HW> __device__ __forceinline__ int key_shift(int row)
-{
-    return HW == 128 ? row & 15 : row >> 1 & 7;
-}
-template <int HW> __device__ __forceinline__ int value_shift(int row)
-{
-    return HW == 128 ? row & 7 : row >> 1 & 3;
-}
 
 // A tile is 256 / Teams rows, 32 a wave; a team of waves takes all stages, or every second
 // block. Stages of 64 keys go from memory straight into a ring of four in LDS, eight rows a wave, in
 // whole rows (4 TB/s where a load took 64 bytes of 16 rows, 5.5 so).
-template <int HW, bool Half, int Teams> __global__ __launch_bounds__(64 * staging_waves, 2) void staged_kernel(Launch l)
+template <int HW, bool Half, int Teams> __global__ __launch_bounds__(64 * waves, 2) void staged_kernel(Launch l)
 {
-    constexpr int depth = HW / 32, step = HW / 16, parts = 2, team = staging_waves / Teams, rows = 16 * parts * team;
+    constexpr int depth = HW / 32, step = HW / 16, parts = 2, team = waves / Teams, rows = 16 * parts * team;
     constexpr int keys = staged_keys, row_bytes = 2 * HW, key_bytes = keys * row_bytes;
     constexpr int stage_bytes = 2 * key_bytes;
     constexpr int pieces = HW / 64; // 1 KiB each, of keys and of values, that a wave loads of a stage
     extern __shared__ __attribute__((aligned(128))) char ring[]; // [stage]: keys [key][HW], values [key][HW]
-    __shared__ Marks marked[staging_waves]; // of eight keys each
+    __shared__ Marks marked[waves]; // of eight keys each
     __shared__ int flag;
     const int lane = threadIdx.x % 64, warp = __builtin_amdgcn_readfirstlane(int(threadIdx.x / 64));
     int unit, tile;
@@ -933,11 +921,11 @@ template <int HW, bool Half, int Teams> __global__ __launch_bounds__(64 * stagin
     // Up to here stages are whole for every row of the tile, if the chunk's pages are all there.
     const int open = min(end, l.mask ? p.length : p.length + p.row / l.group + 1);
     const int whole =
-        all_there<64 * staging_waves>(l, p, begin, open, flag) ? max(open - begin, 0) / keys : 0; // stages
+        all_there<64 * waves>(l, p, begin, open, flag) ? max(open - begin, 0) / keys : 0; // stages
 
     u32x4 query[parts][depth];
     int node[parts];
-    Sums<HW, true> sums[parts];
+    Sums<HW> sums[parts];
 #pragma unroll
     for (int t = 0; t < parts; ++t)
     {
@@ -969,8 +957,8 @@ template <int HW, bool Half, int Teams> __global__ __launch_bounds__(64 * stagin
 #pragma unroll
         for (int i = 0; i < pieces; ++i)
         {
-            load_to_lds(from_keys + key_offset[i], to + i * 1024);
-            load_to_lds(from_values + value_offset[i], to + key_bytes + i * 1024);
+            load_to_lds(from_keys, key_offset[i], to + i * 1024);
+            load_to_lds(from_values, value_offset[i], to + key_bytes + i * 1024);
         }
         find(stage + 1);
     };
@@ -1003,34 +991,11 @@ template <int HW, bool Half, int Teams> __global__ __launch_bounds__(64 * stagin
     arrive(Teams - 1);
 
     u32x4 key[2][depth], value[step];
-    const int key_row = lane % 16, value_row = lane % 16 / 4 + 4 * (lane / 16); // of a half, by the lane's address
-    const int key_lane = key_row * row_bytes, keys_shift = 16 * (lane / 16 ^ key_shift<HW>(key_row));
-    const int value_lane = value_row * row_bytes + lane % 4 * 8, values_shift = 32 * value_shift<HW>(value_row);
+    const Reading<HW> reading(lane);
     const auto read_keys = [&](int stage, int b)
-    {
-        const char* const from = ring + stage % stages * stage_bytes + b * block * row_bytes + key_lane;
-#pragma unroll
-        for (int d = 0; d < depth; ++d)
-        {
-            const char* const piece = from + (64 * d ^ keys_shift);
-            key[0][d] = *reinterpret_cast<const u32x4*>(piece);
-            key[1][d] = *reinterpret_cast<const u32x4*>(piece + 16 * row_bytes);
-        }
-        asm volatile("" ::: "memory"); // here, not where they are used
-    };
+    { reading.keys(ring + stage % stages * stage_bytes + b * block * row_bytes, key); };
     const auto read_values = [&](int stage, int b)
-    {
-        const char* const from = ring + stage % stages * stage_bytes + key_bytes + b * block * row_bytes + value_lane;
-#pragma unroll
-        for (int j = 0; j < step; ++j)
-        {
-            const char* const piece = from + (32 * j ^ values_shift);
-            const u32x2 low = read_transposed(piece), high = read_transposed(piece + 16 * row_bytes);
-            value[j] = u32x4{low[0], low[1], high[0], high[1]};
-        }
-        asm volatile("" ::: "memory");
-    };
-    const auto value_of = [&](int j) { return value[j]; };
+    { reading.values(ring + stage % stages * stage_bytes + key_bytes + b * block * row_bytes, value); };
     const int mine = Teams == 1 ? 0 : warp / team; // the first block of a stage that the wave takes
     int stage = 0;
     if (idle)
@@ -1060,7 +1025,7 @@ template <int HW, bool Half, int Teams> __global__ __launch_bounds__(64 * stagin
             weigh<HW, Half>(l, now, sums, weight);
             between();
             read_keys(key_stage, key_b);
-            add_block<HW, Half>(weight, sums, value_of);
+            add_block<HW, Half>(weight, sums, value);
             if (!last)
             {
                 settle(l, then, sums);
@@ -1136,14 +1101,14 @@ template <int HW, bool Half, int Teams> __global__ __launch_bounds__(64 * stagin
             {
                 read_keys(stage, b);
                 read_values(stage, b);
-                attend_masked<HW, Half>(l, p, at + block * b, marks, lane, key, query, node, sums, value_of);
+                attend_masked<HW, Half>(l, p, at + block * b, marks, lane, key, query, node, sums, value);
             }
         }
     }
     __syncthreads();
     if constexpr (Teams == 2)
     {
-        constexpr int words = Sums<HW, true>::words * 64;
+        constexpr int words = Sums<HW>::words * 64;
         float* const joined = reinterpret_cast<float*>(ring) + warp % team * parts * words;
         if (warp >= team && !idle)
         {
@@ -1179,7 +1144,7 @@ template <int HW, bool Half, int Teams> __global__ __launch_bounds__(64 * stagin
 // Joins the chunks of 16 rows of a (sequence, head), in ascending order.
 template <int HW, bool Half> __global__ __launch_bounds__(256) void join_kernel(Launch l, int tile_rows)
 {
-    constexpr int step = HW / 16, record = Sums<HW, true>::record; // coordinates of a thread
+    constexpr int step = HW / 16, record = Sums<HW>::record; // coordinates of a thread
     const int mine = threadIdx.x / 16, first = threadIdx.x % 16 * step;
     const int part = blockIdx.x % l.parts, pair = blockIdx.x / l.parts;
     const int head = pair % l.heads, sequence = pair / l.heads;
@@ -1246,7 +1211,7 @@ template <int HW, bool Half> __global__ __launch_bounds__(256) void join_kernel(
 // The launch's shape: it depends on what the host knows, sizes and not lengths.
 struct Shape
 {
-    int parts_a_tile; // 16-row parts of a workgroup's tile: 1 or 2 (direct), 8 or 16 (staged)
+    int parts_a_tile; // 16-row parts of a workgroup's tile: 1 or 2 (narrow), 8 or 16 (staged)
     int tiles, parts, splits, chunk;
     std::size_t units, record;
 };
@@ -1259,9 +1224,9 @@ Shape shape_of(const PagedCache& cache, const PagedRows& rows)
     s.parts_a_tile = s.parts <= 2 ? s.parts : s.parts <= 8 ? 8 : 16;
     s.tiles = (s.parts + s.parts_a_tile - 1) / s.parts_a_tile;
     const std::size_t pairs = std::size_t(cache.sequences) * cache.heads;
-    const std::size_t slots = (s.parts_a_tile == 1 ? 3 : s.parts_a_tile == 2 ? 2 : 1) * std::size_t(compute_units());
-    const std::size_t wanted = std::max<std::size_t>(1, slots / (pairs * s.tiles));
-    const std::size_t most = std::max<std::size_t>(1, (rows.max_length + 255) / 256);
+    // One workgroup a compute unit, of at least 1,024 keys each.
+    const std::size_t wanted = std::max<std::size_t>(1, std::size_t(compute_units()) / (pairs * s.tiles));
+    const std::size_t most = std::max<std::size_t>(1, rows.max_length / 1024);
     s.splits = int(std::min(wanted, most));
     constexpr std::size_t keys = block * waves;
     s.chunk = int(((rows.max_length + s.splits - 1) / s.splits + keys - 1) / keys * keys);
@@ -1286,13 +1251,13 @@ template <int HW, bool Half> void launch(const Launch& l, const Shape& s, std::s
         kernel<<<grid, threads, lds, stream>>>(l);
         check_hip(hipGetLastError(), "paged attention launch");
     };
-    constexpr std::size_t direct = 2 * Sums<HW, false>::words * 64 * 4, staged = stages * staged_keys * HW * 4;
+    constexpr std::size_t narrow = waves * 2 * block * HW * 2, staged = stages * staged_keys * HW * 4;
     switch (s.parts_a_tile)
     {
-    case 1: run(direct_kernel<HW, Half, 1>, 64 * waves, direct); break;
-    case 2: run(direct_kernel<HW, Half, 2>, 64 * waves, 2 * direct); break;
-    case 8: run(staged_kernel<HW, Half, 2>, 64 * staging_waves, staged); break;
-    default: run(staged_kernel<HW, Half, 1>, 64 * staging_waves, staged); break;
+    case 1: run(narrow_kernel<HW, Half, 1>, 64 * waves, narrow); break;
+    case 2: run(narrow_kernel<HW, Half, 2>, 64 * waves, narrow); break;
+    case 8: run(staged_kernel<HW, Half, 2>, 64 * waves, staged); break;
+    default: run(staged_kernel<HW, Half, 1>, 64 * waves, staged); break;
     }
     if (s.splits > 1)
     {
