@@ -216,6 +216,48 @@ def test_attention_over_many_chunks(torch, native, lengths, nodes, heads, kv_hea
         assert bool(((got - out).abs() <= room).all()), guess
 
 
+@pytest.mark.parametrize("kind,heads,kv_heads,width", [("bfloat16", 32, 16, 64), ("float16", 32, 8, 128)])
+@pytest.mark.parametrize("tree", [False, True])
+def test_attention_of_many_tall_tiles(torch, native, kind, heads, kv_heads, width, tree):
+    """As many (sequence, head) pairs as units, each of more than 128 query rows; a sequence's garbage behind
+    its end, a value of one node that is not finite."""
+    lengths = [(37 * i) % 301 for i in range(32)]
+    counts = [70 - i if i != 9 else 0 for i in range(32)]
+    b = Batch(torch, native, lengths, counts, heads, kv_heads, width, 16, kind, seed=21)
+    trees = [random_tree(b.rng, n) for n in counts]
+    used = torch.zeros(b.keys.shape[1:3], dtype=torch.bool)
+    table = b.table.cpu()
+    for s in range(32):
+        for t in range(lengths[s] + counts[s]):
+            used[int(table[s, t // 16]), t % 16] = True
+    b.keys[0][~used] = math.nan
+    b.values[0][~used] = math.inf
+    if tree:
+        page, row = int(table[3, (lengths[3] + 9) // 16]), (lengths[3] + 9) % 16
+        b.values[0, page, row, 0, 5] = math.inf
+    rows = [line(t, i) for t in trees for i in range(len(t))]
+    got = b.attend(pack_masks(torch, rows, 2) if tree else None)
+    if tree:
+        reached = torch.zeros(got.shape, dtype=torch.bool)
+        for i in range(counts[3]):
+            reached[b.starts_list[3] + i, :heads // kv_heads, 5] = 9 in line(trees[3], i)
+        assert torch.equal(got.cpu() == math.inf, reached) and bool(got.cpu()[~reached].isfinite().all())
+        b.values[0, page, row, 0, 5] = 0.0
+        out, room = b.expected(lambda s, i: line(trees[s], i))
+        assert bool((((got.double().cpu() - out).abs() <= room) | reached).all())
+    else:
+        b.check(got, chain)
+
+
+@pytest.mark.parametrize("nodes", [3, 40])
+def test_rows_behind_the_last_sequence_stay(torch, native, nodes):
+    b = Batch(torch, native, [50, 20, 9], [nodes, nodes, nodes], 4, 2, 64, 16, seed=6)
+    full = b.attend().clone()
+    b.starts = ints(torch, [0, nodes, 2 * nodes, 2 * nodes])
+    got = b.attend()
+    assert torch.equal(got[:2 * nodes], full[:2 * nodes]) and bool((got[2 * nodes:] == 7).all())
+
+
 @pytest.mark.parametrize("magnitude,scale", [(30.0, None), (1.0, 0.0), (1.0, -1.0), (60.0, 1.0)])
 def test_attention_of_large_and_equal_scores(torch, native, magnitude, scale):
     """Scores far apart move the reference many times; equal ones weigh the same."""
@@ -835,6 +877,63 @@ def test_verification_of_wide_alphabets(torch, native, drafts, alphabet):
             assert got[s] == verify_plain(back[part], drafts_back[part] if drafts else None, tokens[part], trees[s],
                                           uniforms[part], draws[s])
             first += n
+
+
+@pytest.mark.parametrize("drafts", [True, False])
+@pytest.mark.parametrize("alphabet", [1, 40000, 65537])
+def test_verification_of_sparse_rows(torch, native, drafts, alphabet):
+    """Alphabets of one token, and wide ones whose mass lies in few places, all sums exact: at the ends, around the
+    boundaries of what is summed together, nowhere."""
+    def row(*places):
+        values = np.zeros(alphabet, np.float32)
+        for at, value in places:
+            values[at % alphabet] = value
+        return values
+
+    last = alphabet - 1
+    rows = [row((0, 1.0)), row((last, 1.0)), row((0, 0.5), (last, 0.5)), row(), row((0, math.nan), (last, math.inf)),
+            row((8191, 0.25), (8192, 0.25), (32767, 0.25), (last, 0.25)), row((511, 0.5), (512, 0.25), (513, 0.25))]
+    trees, tokens, p, q, uniforms, draws = [], [], [], [], [], []
+    for i, target in enumerate(rows):
+        for j, draft in enumerate(rows):
+            for token, u, d in ((0, 0.0, 0.0), (last, 0.5, 0.5), (8192 % alphabet, 0.75, 1 - 2.0 ** -24)):
+                trees.append([-1, 0, 0])
+                tokens += [0, token, last]
+                p += [target, draft, target]
+                q += [draft, draft, draft]
+                uniforms += [0.0, u, 0.25]
+                draws.append(d)
+    for at in range(0, len(trees), 21):
+        nodes = slice(3 * at, 3 * (at + 21))
+        args = [np.stack(p[nodes]), np.stack(q[nodes]) if drafts else None]
+        u, d = np.array(uniforms[nodes], np.float32), np.array(draws[at:at + 21], np.float32)
+        got, back, drafts_back = run_verify(torch, native, *args, trees[at:at + 21], tokens[nodes], u, d)
+        for s in range(21):
+            part = slice(3 * s, 3 * s + 3)
+            want = verify_plain(back[part], drafts_back[part] if drafts else None, tokens[nodes][part], [-1, 0, 0],
+                                u[part], d[s])
+            assert got[s] == want, (at + s, got[s], want)
+
+
+def test_the_workspace_of_verification_is_checked(torch, native):
+    rows, alphabet = 3, 70000
+    p = torch.full((rows, alphabet), 1.0 / alphabet, device="cuda")
+    outputs = [torch.full(shape, 99, dtype=torch.int32, device="cuda") for shape in ((1, 3), (1,), (1,))]
+    need = native.library().tsac_hip_verify_drafts_workspace(1, alphabet)
+    assert need > 0 and native.library().tsac_hip_verify_drafts_workspace(1, 1000) == 0
+
+    def call(space):
+        native.verify_drafts(p, None, ints(torch, [0, 5, 6]), ints(torch, [-1, 0, 0]), ints(torch, [0, 3]), 3,
+                             torch.full((3,), 0.5, device="cuda"), torch.tensor([0.25], device="cuda"), *outputs,
+                             workspace=space)
+        torch.cuda.synchronize()
+        return [x.tolist() for x in outputs]
+
+    with pytest.raises(native.HipError, match="workspace"):
+        call(torch.empty(need - 16, dtype=torch.uint8, device="cuda"))
+    assert outputs[0].tolist() == [[99] * 3]
+    dirty = torch.full((need,), 255, dtype=torch.uint8, device="cuda")
+    assert call(dirty) == call(None) == call(dirty)
 
 
 def test_verification_at_the_edges(torch, native):

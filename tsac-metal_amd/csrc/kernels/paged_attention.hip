@@ -1221,15 +1221,20 @@ Shape shape_of(const PagedCache& cache, const PagedRows& rows)
     Shape s;
     const std::size_t group = std::size_t(rows.heads / cache.heads), queries = std::size_t(rows.max_rows) * group;
     s.parts = int((queries + 15) / 16);
-    // A wave of the narrow kernel has registers for 32 rows. 128-row tiles leave two teams to share a
-    // block's rows; 256-row tiles read a chunk's keys half as often.
-    s.parts_a_tile = s.parts <= 2 ? s.parts : s.parts <= 8 ? 8 : 16;
-    s.tiles = (s.parts + s.parts_a_tile - 1) / s.parts_a_tile;
     const std::size_t pairs = std::size_t(cache.sequences) * cache.heads;
+    // A wave of the narrow kernel has registers for 32 rows: 64 us, call and join included, for 32
+    // over 8,190 positions of 8 sequences, 8 heads, where the staged kernel takes 65; 11 for 18 with
+    // 12 rows over 1,021 of 3, 16 heads. Above that tiles of 128 rows, of which more start at once (2
+    // prompts of 500 rows over 2,580 positions, 16 heads: 34 us for 40, with the join), or of 256,
+    // which read a chunk's keys half as often, where these fill the units by themselves (4 of 500
+    // rows over 6,001, four query heads to each of 8: 228 us for 246).
+    const bool tall = s.parts > 8 && pairs * ((s.parts + 15) / 16) >= std::size_t(compute_units());
+    s.parts_a_tile = s.parts <= 2 ? s.parts : tall ? 16 : 8;
+    s.tiles = (s.parts + s.parts_a_tile - 1) / s.parts_a_tile;
     // One workgroup a compute unit, of at least 1,024 keys each. Two a unit, with fewer keys: 57 us
     // for 53 (8 sequences of one token over 8,190 positions, 8 heads), 134 for 108 (32 trees of 32
-    // nodes over 4,093, with the join), 190 for 166 (64 nodes over 131,001, with the join). Of 512
-    // keys: 12.3 us with the join for 11.5 (3 lanes of 4 tokens over 1,024).
+    // nodes over 4,093, with the join), 190 for 166 (64 nodes over 131,001, with the join, 256-row tiles). Of 512
+    // keys: 12.3 us with the join for 11.5 (3 trees of 12 nodes over 1,021).
     const std::size_t wanted = std::max<std::size_t>(1, std::size_t(compute_units()) / (pairs * s.tiles));
     const std::size_t most = std::max<std::size_t>(1, rows.max_length / 1024);
     s.splits = int(std::min(wanted, most));
