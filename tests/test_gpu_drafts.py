@@ -592,6 +592,20 @@ def test_calls_that_cannot_be_met_change_nothing(torch, native):
     p.free([])
 
 
+def test_a_refused_fork_leaves_numbers_that_make_no_sense(torch, native):
+    """What a target holds may look like anything; nothing is shared, copied or counted for it."""
+    p = Pool(torch, native)
+    p.reserve([0], [40])
+    p.grow(0, 40)
+    for held, length in (((1 << 30) | 3, 1 << 29), ((1 << 30) | 2, 40), (2 ** 31 - 1, 2 ** 31 - 1), ((1 << 30) | 9, -5)):
+        p.held[4], p.lengths[4] = held, length
+        p.model.held[4], p.model.lengths[4] = 0, length
+        p.cache.fork(ints(torch, [0]), ints(torch, [4]), status=p.status)
+        assert p.held.tolist()[4] == held
+        p.held[4] = 0
+        p.same(native.PAGES_INVALID)
+
+
 def test_forks_share_full_pages_and_copy_the_last(torch, native):
     p = Pool(torch, native, kind="float16")
     for s, n in ((0, 50), (1, 32), (2, 5)):

@@ -412,7 +412,15 @@ __global__ __launch_bounds__(copying_threads) void fork_copy_kernel(PagedCache c
     {
         return; // refused
     }
+    // A refused call leaves `held` as it was, and that may look like a mark: what it has to agree with
+    // where it is one keeps the table's bounds.
     const int length = cache.lengths[target];
+    const long long pages = (length + (long long)cache.page_rows - 1) / cache.page_rows;
+    if (length < 0 || length != cache.lengths[source] || pages != (mark & (arrival - 1)) ||
+        std::size_t(pages) > cache.table_stride || pages > cache.held[source])
+    {
+        return;
+    }
     const int full = length / cache.page_rows, rest = length % cache.page_rows;
     const int* const from = cache.table + source * cache.table_stride;
     int* const to = cache.table + target * cache.table_stride;
