@@ -760,6 +760,20 @@ def test_paths_that_are_none_move_nothing(torch, native):
     p.same(native.PAGES_INVALID)
 
 
+@pytest.mark.parametrize("in_place", [False, True])
+def test_a_negative_length_is_kept_as_it_is(torch, native, in_place):
+    p = Pool(torch, native, sequences=2)
+    p.reserve([0, 1], [40, 40])
+    p.grow(1, 20)
+    p.lengths[0] = p.model.lengths[0] = -7
+    out = p.lengths if in_place else torch.zeros(2, dtype=torch.int32, device="cuda")
+    p.cache.keep(ints(torch, [0, 4, 8]), ints(torch, [[0, 1], [0, 1]]), ints(torch, [2, 2]), None if in_place else out,
+                 status=p.status)
+    assert out.tolist() == [-7, 22]
+    p.model.lengths[1] = 22 if in_place else 20
+    p.same(native.PAGES_INVALID)
+
+
 # ---------------------------------------------------------------- verification
 
 def verify_plain(p, q, tokens, parents, uniforms, draw):

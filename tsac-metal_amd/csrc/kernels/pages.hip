@@ -582,7 +582,7 @@ __global__ __launch_bounds__(copying_threads) void keep_kernel(PagedCache cache,
     const bool reporter = threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.z == 0;
     if (lengths && reporter)
     {
-        lengths[s] = length + (kept > 0 ? kept : 0);
+        lengths[s] = length + (kept > 0 && length >= 0 ? kept : 0);
     }
     if (kept < 0 || length < 0)
     {
@@ -657,7 +657,7 @@ __global__ __launch_bounds__(64) void keep_lengths_kernel(const int* __restrict_
     const int s = blockIdx.x;
     const int kept =
         kept_rows(path + s * path_stride, accepted[s], starts[s + 1] - starts[s], path_stride, &bad);
-    if (threadIdx.x == 0 && kept > 0)
+    if (threadIdx.x == 0 && kept > 0 && lengths[s] >= 0)
     {
         lengths[s] += kept;
     }
