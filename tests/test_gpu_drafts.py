@@ -347,6 +347,59 @@ def test_numbers_out_of_range_stay_inside(torch, native):
         b.attend()
 
 
+@pytest.mark.parametrize("nodes", [1, 60])
+@pytest.mark.parametrize("length", [49, 5000, 1 << 30, 2 ** 31 - 1])
+def test_a_length_past_what_is_held_ends_there(torch, native, nodes, length):
+    b = Batch(torch, native, [48, 20], [nodes, nodes], 8, 4, 128, 16, seed=12)
+    want, room = b.expected(lambda s, i: set() if s == 0 else chain(s, i))
+    b.held[0] = 3
+    b.cache.tensors[4].copy_(ints(torch, [length, 20]))
+    got = b.attend(max_length=9000).double().cpu()
+    assert bool(((got - want).abs() <= room).all())
+
+
+@pytest.mark.parametrize("nodes,lengths", [(1, [5000, 70]), (30, [5000, 70]), (60, [9, 4100])])
+def test_wide_heads_in_graphs(torch, native, nodes, lengths):
+    """Two captured calls with a workspace each, replayed one after the other and side by side with eager ones."""
+    batches = [Batch(torch, native, lengths, [nodes, max(1, nodes - 3)], 8, 4, 128, 32, kind, seed=13 + i)
+               for i, kind in enumerate(("bfloat16", "float16"))]
+    need = [native.attention_paged_workspace(b.cache, b.rows, b.heads, b.max_rows, b.max_length) for b in batches]
+    spaces = [torch.empty(max(n, 16), dtype=torch.uint8, device="cuda") for n in need]
+    outs = [torch.zeros(b.rows, b.heads, b.width, dtype=b.query.dtype, device="cuda") for b in batches]
+    queries = [b.query.clone() for b in batches]
+
+    def call(i):
+        b = batches[i]
+        native.attention_paged(b.cache, 0, queries[i], b.starts, b.max_rows, b.max_length, None, b.scale, outs[i],
+                               workspace=spaces[i])
+
+    eager = [b.attend().clone() for b in batches]
+    graphs = []
+    for i in range(2):
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            call(i)
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i]):
+            call(i)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for step in range(4):
+        for i in range(2):
+            queries[i].copy_(batches[i].query)
+            outs[i].zero_()
+            spaces[i].fill_(255)
+        torch.cuda.synchronize()
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+        again = batches[step % 2].attend()
+        torch.cuda.synchronize()
+        assert torch.equal(again, eager[step % 2])
+        assert torch.equal(outs[0], eager[0]) and torch.equal(outs[1], eager[1]), step
+
+
 def test_more_rows_than_announced_are_left_alone(torch, native):
     b = Batch(torch, native, [50, 20], [10, 3], 4, 2, 64, 16, seed=4)
     full = b.attend().clone()

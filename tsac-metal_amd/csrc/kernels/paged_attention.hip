@@ -162,6 +162,8 @@ __device__ __forceinline__ bool place_of(const Launch& l, int unit, int row, int
     }
     // Without a mask a row sees the rows up to its own.
     p.total = p.length + (l.mask ? p.nodes : min((row + count - 1) / l.group, p.nodes - 1) + 1);
+    // What no page holds nobody sees, however long a sequence says it is.
+    p.total = min(p.total, max(p.limit, 0) << l.page_shift);
     return true;
 }
 
