@@ -550,17 +550,26 @@ __device__ __forceinline__ void attend_masked(const Launch& l, const Place& p, i
 // 16 bytes a lane, from `offset` bytes behind `from`, to `to`, lane after lane; the wave waits for it
 // with its other loads (s_waitcnt vmcnt). Written out because the compiler would wait for it
 // before any other read of LDS. A load to LDS needs a wait state behind a write of M0, which the
-// compiler does not put into assembly. M0 is reserved, so that clang warns where it is named; nothing else
+// compiler does not put into assembly. `Once`: lines that no other workgroup reads. M0 is reserved, so that clang warns where it is named; nothing else
 // uses it.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
-__device__ __forceinline__ void load_to_lds(const void* from, unsigned offset, void* to)
+template <bool Once> __device__ __forceinline__ void load_to_lds(const void* from, unsigned offset, void* to)
 {
-    const unsigned address =
-        unsigned(reinterpret_cast<std::uintptr_t>((__attribute__((address_space(3))) const void*)to));
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(from),
-                 "s"(__builtin_amdgcn_readfirstlane(address))
-                 : "memory", "m0");
+    const unsigned address = __builtin_amdgcn_readfirstlane(
+        unsigned(reinterpret_cast<std::uintptr_t>((__attribute__((address_space(3))) const void*)to)));
+    if constexpr (Once)
+    {
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(offset), "s"(from),
+                     "s"(address)
+                     : "memory", "m0");
+    }
+    else
+    {
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(from),
+                     "s"(address)
+                     : "memory", "m0");
+    }
 }
 #pragma clang diagnostic pop
 
@@ -732,7 +741,8 @@ template <int HW> struct Reading
 // but their own loads. A token of each of 8 sequences, 264 MB of keys and values: 52 us, 5.0 TB/s,
 // and 5 us for the join; with operands loaded from memory into registers, 64 bytes of a row at a
 // time, 58 us.
-template <int HW, bool Half, int Parts> __global__ __launch_bounds__(64 * waves, 2) void narrow_kernel(Launch l)
+template <int HW, bool Half, int Parts, bool Once>
+__global__ __launch_bounds__(64 * waves, 2) void narrow_kernel(Launch l)
 {
     constexpr int depth = HW / 32, step = HW / 16, row_bytes = 2 * HW, lanes = HW / 8, rows_a_piece = 64 / lanes;
     constexpr int half_pieces = 16 / rows_a_piece, pieces = 2 * half_pieces; // loads of a block's keys, or values
@@ -778,7 +788,7 @@ template <int HW, bool Half, int Parts> __global__ __launch_bounds__(64 * waves,
 #pragma unroll
             for (int i = 0; i < half_pieces; ++i)
             {
-                load_to_lds(rows + base[half], offset[i], to + (half * half_pieces + i) * 1024);
+                load_to_lds<Once>(rows + base[half], offset[i], to + (half * half_pieces + i) * 1024);
             }
         }
     };
@@ -900,7 +910,8 @@ constexpr int stages = 4;              // in LDS
 // A tile is 256 / Teams rows, 32 a wave; a team of waves takes all stages, or every second
 // block. Stages of 64 keys go from memory straight into a ring of four in LDS, eight rows a wave, in
 // whole rows (4 TB/s where a load took 64 bytes of 16 rows, 5.5 so).
-template <int HW, bool Half, int Teams> __global__ __launch_bounds__(64 * waves, 2) void staged_kernel(Launch l)
+template <int HW, bool Half, int Teams, bool Once>
+__global__ __launch_bounds__(64 * waves, 2) void staged_kernel(Launch l)
 {
     constexpr int depth = HW / 32, step = HW / 16, parts = 2, team = waves / Teams, rows = 16 * parts * team;
     constexpr int keys = staged_keys, row_bytes = 2 * HW, key_bytes = keys * row_bytes;
@@ -959,8 +970,8 @@ template <int HW, bool Half, int Teams> __global__ __launch_bounds__(64 * waves,
 #pragma unroll
         for (int i = 0; i < pieces; ++i)
         {
-            load_to_lds(from_keys, key_offset[i], to + i * 1024);
-            load_to_lds(from_values, value_offset[i], to + key_bytes + i * 1024);
+            load_to_lds<Once>(from_keys, key_offset[i], to + i * 1024);
+            load_to_lds<Once>(from_values, value_offset[i], to + key_bytes + i * 1024);
         }
         find(stage + 1);
     };
@@ -1216,6 +1227,7 @@ struct Shape
     int parts_a_tile; // 16-row parts of a workgroup's tile: 1 or 2 (narrow), 8 or 16 (staged)
     int tiles, parts, splits, chunk;
     std::size_t units, record;
+    bool once; // keys and values go past the caches
 };
 
 Shape shape_of(const PagedCache& cache, const PagedRows& rows)
@@ -1245,6 +1257,11 @@ Shape shape_of(const PagedCache& cache, const PagedRows& rows)
     s.chunk = std::max<int>(s.chunk, keys);
     s.units = pairs * s.splits;
     s.record = 16 * std::size_t(cache.head_width) + 32;
+    // One tile reads a unit's keys and values, and they are more than the dies' caches of 4 MiB hold:
+    // 8 sequences of one token over 8,190 positions, 8 heads: 47 us for 52, 32 trees of 32 nodes over
+    // 4,093: 93 for 106. With another tile to come, 2 prompts of 500 rows: 31 for 29; of 12 MB 11.6
+    // for 11.0.
+    s.once = s.tiles == 1 && pairs * rows.max_length * cache.head_width * 4 > (std::size_t(8) << 22);
     return s;
 }
 
@@ -1264,13 +1281,18 @@ template <int HW, bool Half> void launch(const Launch& l, const Shape& s, std::s
         check_hip(hipGetLastError(), "paged attention launch");
     };
     constexpr std::size_t narrow = waves * 2 * block * HW * 2, staged = stages * staged_keys * HW * 4;
-    switch (s.parts_a_tile)
+    const auto run_either = [&](auto read_once)
     {
-    case 1: run(narrow_kernel<HW, Half, 1>, 64 * waves, narrow); break;
-    case 2: run(narrow_kernel<HW, Half, 2>, 64 * waves, narrow); break;
-    case 8: run(staged_kernel<HW, Half, 2>, 64 * waves, staged); break;
-    default: run(staged_kernel<HW, Half, 1>, 64 * waves, staged); break;
-    }
+        constexpr bool once = decltype(read_once)::value;
+        switch (s.parts_a_tile)
+        {
+        case 1: run(narrow_kernel<HW, Half, 1, once>, 64 * waves, narrow); break;
+        case 2: run(narrow_kernel<HW, Half, 2, once>, 64 * waves, narrow); break;
+        case 8: run(staged_kernel<HW, Half, 2, once>, 64 * waves, staged); break;
+        default: run(staged_kernel<HW, Half, 1, once>, 64 * waves, staged); break;
+        }
+    };
+    s.once ? run_either(std::true_type{}) : run_either(std::false_type{});
     if (s.splits > 1)
     {
         join_kernel<HW, Half><<<unsigned(pairs * s.parts), 256, 0, stream>>>(l, 16 * s.parts_a_tile);
