@@ -370,7 +370,11 @@ __device__ __forceinline__ void share_pages(const PagedCache& cache, const int* 
     }
 }
 
-// Copies the rows of the last page, of one layer's keys or values.
+typedef unsigned Vector __attribute__((ext_vector_type(4)));
+
+// Copies the rows of the last page, of one layer's keys or values. Stores go past the caches, which
+// keep the source for its other targets: 64 targets of 8 sources 28 us, with plain stores 49 (and with
+// loads past them too, 50).
 __device__ __forceinline__ void copy_rows(const PagedCache& cache, int part, int old, int fresh, int rest, int* status)
 {
     if (old < 0 || old >= cache.pages || fresh < 0 || fresh >= cache.pages)
@@ -386,14 +390,13 @@ __device__ __forceinline__ void copy_rows(const PagedCache& cache, int part, int
     for (int i = threadIdx.x; i < rest * vectors; i += copying_threads)
     {
         const std::size_t at = i / vectors * cache.row_stride + i % vectors * 8;
-        const uint4 value = *reinterpret_cast<const uint4*>(memory + old * cache.page_stride + at);
-        *reinterpret_cast<uint4*>(memory + fresh * cache.page_stride + at) = value;
+        const auto value = *reinterpret_cast<const Vector*>(memory + old * cache.page_stride + at);
+        __builtin_nontemporal_store(value, reinterpret_cast<Vector*>(memory + fresh * cache.page_stride + at));
     }
 }
 
 // blockIdx: the entry of the list, then (layer, keys or values), past the last of them the
-// sharing. A workgroup a page and layer reads and writes at once: 64 targets of pages of 64 rows, 12
-// layers of 8 x 128, 211 MB read and written in 48 us, 4.4 TB/s (a large copy 4.9).
+// sharing. 64 targets of pages of 64 rows, 12 layers of 8 x 128: 105 MB are written in 28 us, 3.8 TB/s.
 __global__ __launch_bounds__(copying_threads) void fork_copy_kernel(PagedCache cache, const int* __restrict__ sources,
                                                                     const int* __restrict__ targets, int* status)
 {
