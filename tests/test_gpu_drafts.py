@@ -249,6 +249,19 @@ def test_attention_of_many_tall_tiles(torch, native, kind, heads, kv_heads, widt
         b.check(got, chain)
 
 
+@pytest.mark.parametrize("kind,heads,kv_heads,width", [("bfloat16", 32, 8, 128), ("float16", 24, 4, 64)])
+@pytest.mark.parametrize("tree", [False, True])
+def test_tall_tiles_over_chunks(torch, native, kind, heads, kv_heads, width, tree):
+    """A launch that is shaped for a long context takes tiles of 256 rows over chunks of it, whatever there is."""
+    b = Batch(torch, native, [4900, 2303], [41, 36], heads, kv_heads, width, 64, kind, seed=31)
+    trees = [random_tree(b.rng, n) for n in b.counts]
+    mask = pack_masks(torch, [line(t, i) for t in trees for i in range(len(t))], 1) if tree else None
+    out, room = b.expected((lambda s, i: line(trees[s], i)) if tree else chain)
+    for guess in (70000, 140000):
+        got = b.attend(mask, max_length=guess).double().cpu()
+        assert bool(((got - out).abs() <= room).all()), guess
+
+
 @pytest.mark.parametrize("nodes", [3, 40])
 def test_rows_behind_the_last_sequence_stay(torch, native, nodes):
     b = Batch(torch, native, [50, 20, 9], [nodes, nodes, nodes], 4, 2, 64, 16, seed=6)

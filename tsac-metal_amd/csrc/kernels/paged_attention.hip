@@ -1239,10 +1239,13 @@ Shape shape_of(const PagedCache& cache, const PagedRows& rows)
     // A wave of the narrow kernel has registers for 32 rows: 64 us, call and join included, for 32
     // over 8,190 positions of 8 sequences, 8 heads, where the staged kernel takes 65; 11 for 18 with
     // 12 rows over 1,021 of 3, 16 heads. Above that tiles of 128 rows, of which more start at once (2
-    // prompts of 500 rows over 2,580 positions, 16 heads: 34 us for 40, with the join), or of 256,
-    // which read a chunk's keys half as often, where these fill the units by themselves (4 of 500
-    // rows over 6,001, four query heads to each of 8: 228 us for 246).
-    const bool tall = s.parts > 8 && pairs * ((s.parts + 15) / 16) >= std::size_t(compute_units());
+    // prompts of 500 rows over 2,580 positions, 16 heads: 34 us for 40, with the join; 2 trees of 64
+    // nodes over 16,381, four query heads to each of 8: 59 for 65), or of 256, which read a chunk's
+    // keys half as often, where these give each unit 2,048 keys (4 prompts of 500 rows over 6,001:
+    // 228 us for 246; 64 nodes over 131,001: 192 for 206).
+    const std::size_t tall_tiles = pairs * ((s.parts + 15) / 16);
+    const bool tall =
+        s.parts > 8 && tall_tiles * std::max<std::size_t>(1, rows.max_length / 2048) >= std::size_t(compute_units());
     s.parts_a_tile = s.parts <= 2 ? s.parts : tall ? 16 : 8;
     s.tiles = (s.parts + s.parts_a_tile - 1) / s.parts_a_tile;
     // One workgroup a compute unit, of at least 1,024 keys each. Two a unit, with fewer keys: 57 us
