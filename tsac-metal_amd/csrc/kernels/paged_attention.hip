@@ -738,9 +738,9 @@ template <int HW> struct Reading
 // A tile is `Parts` x 16 rows, and a wave takes every eighth block of the chunk. A block's keys and
 // values come into the wave's own 16 KiB of LDS in whole rows, and the next ones are asked for
 // once these are in registers: a unit has up to 128 KiB under way, and its waves wait for nothing
-// but their own loads. A token of each of 8 sequences, 264 MB of keys and values: 52 us, 5.0 TB/s,
-// and 5 us for the join; with operands loaded from memory into registers, 64 bytes of a row at a
-// time, 58 us.
+// but their own loads. A token of each of 8 sequences, 264 MB of keys and values: 47 us, 5.6 TB/s,
+// and 5 us for the join. Before loads went past the caches it was 52 us so, and 58 with operands
+// loaded from memory into registers, 64 bytes of a row at a time.
 template <int HW, bool Half, int Parts, bool Once>
 __global__ __launch_bounds__(64 * waves, 2) void narrow_kernel(Launch l)
 {
@@ -909,7 +909,9 @@ constexpr int stages = 4;              // in LDS
 
 // A tile is 256 / Teams rows, 32 a wave; a team of waves takes all stages, or every second
 // block. Stages of 64 keys go from memory straight into a ring of four in LDS, eight rows a wave, in
-// whole rows (4 TB/s where a load took 64 bytes of 16 rows, 5.5 so).
+// whole rows (4 TB/s where a load took 64 bytes of 16 rows, 5.5 so). 32 trees of 32 nodes over 4,093
+// positions, 497 MB: 95 us, 5.2 TB/s; 64 nodes over 131,001, 137 GFLOP and 538 MB: 155 us and 11 for
+// the join, 890 TFLOP/s with the matrix units busy 45% of the time.
 template <int HW, bool Half, int Teams, bool Once>
 __global__ __launch_bounds__(64 * waves, 2) void staged_kernel(Launch l)
 {
@@ -1248,7 +1250,8 @@ Shape shape_of(const PagedCache& cache, const PagedRows& rows)
         s.parts > 8 && tall_tiles * std::max<std::size_t>(1, rows.max_length / 2048) >= std::size_t(compute_units());
     s.parts_a_tile = s.parts <= 2 ? s.parts : tall ? 16 : 8;
     s.tiles = (s.parts + s.parts_a_tile - 1) / s.parts_a_tile;
-    // One workgroup a compute unit, of at least 1,024 keys each. Two a unit, with fewer keys: 57 us
+    // One workgroup a compute unit, of at least 1,024 keys each. Two a unit, with fewer keys (all
+    // before loads went past the caches): 57 us
     // for 53 (8 sequences of one token over 8,190 positions, 8 heads), 134 for 108 (32 trees of 32
     // nodes over 4,093, with the join), 190 for 166 (64 nodes over 131,001, with the join, 256-row tiles). Of 512
     // keys: 12.3 us with the join for 11.5 (3 trees of 12 nodes over 1,021).
