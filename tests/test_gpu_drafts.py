@@ -249,6 +249,22 @@ def test_attention_of_many_tall_tiles(torch, native, kind, heads, kv_heads, widt
         b.check(got, chain)
 
 
+@pytest.mark.parametrize("kind,heads,kv_heads,width", [("bfloat16", 16, 8, 128), ("float16", 32, 16, 64)])
+@pytest.mark.parametrize("nodes,longest", [(1, 400), (12, 100), (20, 150), (31, 33)])
+@pytest.mark.parametrize("guess", [300, 8000])
+def test_attention_of_many_short_sequences(torch, native, kind, heads, kv_heads, width, nodes, longest, guess):
+    """More (sequence, head) pairs than units: of one to four 16-row parts each, empty ones among them, whether the
+    launch is shaped for short sequences or for long ones."""
+    rng = np.random.default_rng(nodes)
+    lengths = [int(x) for x in rng.integers(0, longest, 36)]
+    counts = [0 if i % 7 == 3 else max(1, nodes - i % 4) for i in range(36)]
+    b = Batch(torch, native, lengths, counts, heads, kv_heads, width, 16, kind, seed=41)
+    trees = [random_tree(b.rng, n) for n in counts]
+    mask = pack_masks(torch, [line(t, i) for t in trees for i in range(len(t))], 1)
+    b.values[0, int(b.table[5, 0]), 0, 0, 3] = math.nan if lengths[5] else 0.0  # cached: reaches all of its rows
+    b.check(b.attend(mask, max_length=guess), lambda s, i: line(trees[s], i))
+
+
 @pytest.mark.parametrize("kind,heads,kv_heads,width", [("bfloat16", 32, 8, 128), ("float16", 24, 4, 64)])
 @pytest.mark.parametrize("tree", [False, True])
 def test_tall_tiles_over_chunks(torch, native, kind, heads, kv_heads, width, tree):

@@ -35,8 +35,9 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2_ __attribute__((ext_vector_type(2)));
 
-constexpr int waves = 8;  // of a workgroup
-constexpr int block = 32; // keys of one step
+constexpr int waves = 8;     // of a workgroup
+constexpr int few_waves = 2; // where there are many, of short sequences
+constexpr int block = 32;    // keys of one step
 constexpr float minus_infinity = -__builtin_inff();
 
 template <bool Half> __device__ __forceinline__ f32x4 product(u32x4 a, u32x4 b, f32x4 c)
@@ -550,8 +551,8 @@ __device__ __forceinline__ void attend_masked(const Launch& l, const Place& p, i
 // 16 bytes a lane, from `offset` bytes behind `from`, to `to`, lane after lane; the wave waits for it
 // with its other loads (s_waitcnt vmcnt). Written out because the compiler would wait for it
 // before any other read of LDS. A load to LDS needs a wait state behind a write of M0, which the
-// compiler does not put into assembly. `Once`: lines that no other workgroup reads. M0 is reserved, so that clang warns where it is named; nothing else
-// uses it.
+// compiler does not put into assembly. M0 is reserved, so that clang warns where it is named; nothing
+// else uses it. `Once`: past the caches.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 template <bool Once> __device__ __forceinline__ void load_to_lds(const void* from, unsigned offset, void* to)
@@ -735,14 +736,14 @@ template <int HW> struct Reading
     }
 };
 
-// A tile is `Parts` x 16 rows, and a wave takes every eighth block of the chunk. A block's keys and
+// A tile is `Parts` x 16 rows, and a wave takes every eighth (or, of two, second) block of the chunk. A block's keys and
 // values come into the wave's own 16 KiB of LDS in whole rows, and the next ones are asked for
-// once these are in registers: a unit has up to 128 KiB under way, and its waves wait for nothing
+// once these are in registers: eight waves have up to 128 KiB under way, and its waves wait for nothing
 // but their own loads. A token of each of 8 sequences, 264 MB of keys and values: 47 us, 5.6 TB/s,
 // and 5 us for the join. Before loads went past the caches it was 52 us so, and 58 with operands
 // loaded from memory into registers, 64 bytes of a row at a time.
-template <int HW, bool Half, int Parts, bool Once>
-__global__ __launch_bounds__(64 * waves, 2) void narrow_kernel(Launch l)
+template <int HW, bool Half, int Parts, int Waves, bool Once>
+__global__ __launch_bounds__(64 * Waves, 2) void narrow_kernel(Launch l)
 {
     constexpr int depth = HW / 32, step = HW / 16, row_bytes = 2 * HW, lanes = HW / 8, rows_a_piece = 64 / lanes;
     constexpr int half_pieces = 16 / rows_a_piece, pieces = 2 * half_pieces; // loads of a block's keys, or values
@@ -793,7 +794,7 @@ __global__ __launch_bounds__(64 * waves, 2) void narrow_kernel(Launch l)
         }
     };
     int at = begin + block * warp;
-    constexpr int stride = block * waves;
+    constexpr int stride = block * Waves;
     bool here[2] = {}; // `there` of the block that is worked on
     if (at < end)
     {
@@ -870,7 +871,7 @@ __global__ __launch_bounds__(64 * waves, 2) void narrow_kernel(Launch l)
     float* const joined = reinterpret_cast<float*>(memory);
     __syncthreads();
 #pragma unroll 1
-    for (int half = waves / 2; half >= 1; half /= 2)
+    for (int half = Waves / 2; half >= 1; half /= 2)
     {
         if (warp >= half && warp < 2 * half)
         {
@@ -911,7 +912,7 @@ constexpr int stages = 4;              // in LDS
 // block. Stages of 64 keys go from memory straight into a ring of four in LDS, eight rows a wave, in
 // whole rows (4 TB/s where a load took 64 bytes of 16 rows, 5.5 so). 32 trees of 32 nodes over 4,093
 // positions, 497 MB: 95 us, 5.2 TB/s; 64 nodes over 131,001, 137 GFLOP and 538 MB: 155 us and 11 for
-// the join, 890 TFLOP/s with the matrix units busy 45% of the time.
+// the join, 885 TFLOP/s with the matrix units busy 45% of the time.
 template <int HW, bool Half, int Teams, bool Once>
 __global__ __launch_bounds__(64 * waves, 2) void staged_kernel(Launch l)
 {
@@ -1229,7 +1230,8 @@ struct Shape
     int parts_a_tile; // 16-row parts of a workgroup's tile: 1 or 2 (narrow), 8 or 16 (staged)
     int tiles, parts, splits, chunk;
     std::size_t units, record;
-    bool once; // keys and values go past the caches
+    int narrow_waves; // of a workgroup
+    bool once;        // keys and values go past the caches
 };
 
 Shape shape_of(const PagedCache& cache, const PagedRows& rows)
@@ -1248,13 +1250,22 @@ Shape shape_of(const PagedCache& cache, const PagedRows& rows)
     const std::size_t tall_tiles = pairs * ((s.parts + 15) / 16);
     const bool tall =
         s.parts > 8 && tall_tiles * std::max<std::size_t>(1, rows.max_length / 2048) >= std::size_t(compute_units());
-    s.parts_a_tile = s.parts <= 2 ? s.parts : tall ? 16 : 8;
+    // Where there are more (sequence, head) pairs than units, and short ones, workgroups of two waves
+    // with a quarter of the LDS start and end apart, and take two tiles of 32 rows too. 256 sequences, 8
+    // heads of 128, a token each: over 100 positions 27 us for 67, over 500 81 for 111; 128 over 2,000
+    // 152 for 156, but 256 over 4,000 589 for 570. 256 of 48 rows over 100: 64 for 91 staged (but 128
+    // rows 118 for 117). 16 heads of 64: 256 over 100 24 for 51, over 500 83 for 83, but 128 over 1,000
+    // 90 for 76. With fewer pairs (16 sequences, 8 heads of 128, 2,000 positions): 34 for 33.
+    const bool many = pairs > std::size_t(compute_units()) &&
+                      rows.max_length <= std::size_t(cache.head_width == 128 ? 2048 : 512);
+    s.narrow_waves = many ? few_waves : waves;
+    s.parts_a_tile = s.parts == 1 ? 1 : s.parts <= (many ? 4 : 2) ? 2 : tall ? 16 : 8;
     s.tiles = (s.parts + s.parts_a_tile - 1) / s.parts_a_tile;
-    // One workgroup a compute unit, of at least 1,024 keys each. Two a unit, with fewer keys (all
-    // before loads went past the caches): 57 us
-    // for 53 (8 sequences of one token over 8,190 positions, 8 heads), 134 for 108 (32 trees of 32
-    // nodes over 4,093, with the join), 190 for 166 (64 nodes over 131,001, with the join, 256-row tiles). Of 512
-    // keys: 12.3 us with the join for 11.5 (3 trees of 12 nodes over 1,021).
+    // One workgroup a compute unit, of at least 1,024 keys each. Two a unit, with fewer keys (before
+    // loads went past the caches): 57 us for 53 (8 sequences of one token over 8,190 positions, 8
+    // heads), 134 for 108 (32 trees of 32 nodes over 4,093, with the join), 190 for 166 (64 nodes over
+    // 131,001, with the join, 256-row tiles). Of 512 keys: 12.3 us with the join for 11.5 (3 trees of
+    // 12 nodes over 1,021).
     const std::size_t wanted = std::max<std::size_t>(1, std::size_t(compute_units()) / (pairs * s.tiles));
     const std::size_t most = std::max<std::size_t>(1, rows.max_length / 1024);
     s.splits = int(std::min(wanted, most));
@@ -1286,14 +1297,22 @@ template <int HW, bool Half> void launch(const Launch& l, const Shape& s, std::s
         kernel<<<grid, threads, lds, stream>>>(l);
         check_hip(hipGetLastError(), "paged attention launch");
     };
-    constexpr std::size_t narrow = waves * 2 * block * HW * 2, staged = stages * staged_keys * HW * 4;
+    constexpr std::size_t narrow_wave = 2 * block * HW * 2, staged = stages * staged_keys * HW * 4;
     const auto run_either = [&](auto read_once)
     {
         constexpr bool once = decltype(read_once)::value;
         switch (s.parts_a_tile)
         {
-        case 1: run(narrow_kernel<HW, Half, 1, once>, 64 * waves, narrow); break;
-        case 2: run(narrow_kernel<HW, Half, 2, once>, 64 * waves, narrow); break;
+        case 1:
+            s.narrow_waves == waves
+                ? run(narrow_kernel<HW, Half, 1, waves, once>, 64 * waves, waves * narrow_wave)
+                : run(narrow_kernel<HW, Half, 1, few_waves, once>, 64 * few_waves, few_waves * narrow_wave);
+            break;
+        case 2:
+            s.narrow_waves == waves
+                ? run(narrow_kernel<HW, Half, 2, waves, once>, 64 * waves, waves * narrow_wave)
+                : run(narrow_kernel<HW, Half, 2, few_waves, once>, 64 * few_waves, few_waves * narrow_wave);
+            break;
         case 8: run(staged_kernel<HW, Half, 2, once>, 64 * waves, staged); break;
         default: run(staged_kernel<HW, Half, 1, once>, 64 * waves, staged); break;
         }
