@@ -1261,13 +1261,17 @@ Shape shape_of(const PagedCache& cache, const PagedRows& rows)
     s.narrow_waves = many ? few_waves : waves;
     s.parts_a_tile = s.parts == 1 ? 1 : s.parts <= (many ? 4 : 2) ? 2 : tall ? 16 : 8;
     s.tiles = (s.parts + s.parts_a_tile - 1) / s.parts_a_tile;
-    // One workgroup a compute unit, of at least 1,024 keys each. Two a unit, with fewer keys (before
-    // loads went past the caches): 57 us for 53 (8 sequences of one token over 8,190 positions, 8
-    // heads), 134 for 108 (32 trees of 32 nodes over 4,093, with the join), 190 for 166 (64 nodes over
-    // 131,001, with the join, 256-row tiles). Of 512 keys: 12.3 us with the join for 11.5 (3 trees of
-    // 12 nodes over 1,021).
+    // One workgroup a compute unit. Two a unit, with fewer keys (before loads went past the caches): 57
+    // us for 53 (8 sequences of one token over 8,190 positions, 8 heads), 134 for 108 (32 trees of 32
+    // nodes over 4,093, with the join), 190 for 166 (64 nodes over 131,001, with the join, 256-row tiles).
     const std::size_t wanted = std::max<std::size_t>(1, std::size_t(compute_units()) / (pairs * s.tiles));
-    const std::size_t most = std::max<std::size_t>(1, rows.max_length / 1024);
+    // With fewer, a chunk has 256 keys or more: 64 nodes of 8 heads to one over 3,000 positions 23 us, with
+    // chunks of 512 27, of 1,024 37; 500 rows over 1,000, 16 heads of 64: 23, 24, 25. In the narrow
+    // kernel it has 512, two blocks a wave, and there is a chunk less, for what the join costs: a
+    // token over 3,000 positions, 4 heads of 128, 15 us, with chunks of 1,024 19; but 3 trees of 12
+    // nodes over 1,021, 16 heads of 64, 10 in one chunk, 12 in two.
+    const std::size_t most = std::max<std::size_t>(
+        1, s.parts_a_tile > 2 ? rows.max_length / 256 : std::max<std::size_t>(2, rows.max_length / 512) - 1);
     s.splits = int(std::min(wanted, most));
     constexpr std::size_t keys = block * waves;
     s.chunk = int(((rows.max_length + s.splits - 1) / s.splits + keys - 1) / keys * keys);
