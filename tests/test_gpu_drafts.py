@@ -294,6 +294,48 @@ def test_attention_of_large_and_equal_scores(torch, native, magnitude, scale):
     b.check(b.attend(), chain)
 
 
+@pytest.mark.parametrize("width", [64, 128])
+@pytest.mark.parametrize("nodes,tree", [(1, False), (12, True), (40, False), (40, True)])
+@pytest.mark.parametrize("gap", [10.0, 14.0, 16.0, 17.5, 18.0])
+def test_small_weights_in_half_precision_count(torch, native, width, nodes, tree, gap):
+    """Every sixteenth key scores `gap` above the others and has a value of 0, so that all of the output comes
+    from weights of e^-gap. As operands in half, of which the largest is 2^7 or more, they are off by half a step:
+    2^-11 of them or, below the smallest normal number, 2^-25, which is 2^-32 of the largest weight. Everything else
+    as above, with f the weights against the largest one and u_f = max(u f, 2^-32): the output's rounding is u |out|
+    (no outputs are subnormal here) and
+    |error| <= u |out| + sum (u_f + f (2 d + (T + 16) 2^-24)) |v| / sum f + |out| sum u_f / sum f, times 1 + 2^-6."""
+    heads, kv = 4, 2
+    b = Batch(torch, native, [600, 33], [nodes, nodes], heads, kv, width, 16, "float16", seed=61)
+    g = torch.Generator(device="cuda").manual_seed(62)
+    # Scores are the keys' first coordinates: exact but for the scale, a power of two or one rounding.
+    b.query.zero_()
+    b.query[:, :, 0] = 8.0
+    b.scale = 0.125
+    b.keys[..., 0] = torch.rand(b.keys.shape[:-1], generator=g, device="cuda").half() * 0.25
+    b.keys[0, :, 3, :, 0] = gap
+    b.values.copy_(8000 + 22000 * torch.rand(b.values.shape, generator=g, device="cuda"))
+    b.values[0, :, 3] = 0
+    trees = [random_tree(b.rng, n) for n in b.counts]
+    sees = (lambda s, i: line(trees[s], i)) if tree else chain
+    got = b.attend(pack_masks(torch, [line(t, i) for t in trees for i in range(len(t))], 1) if tree else None)
+    got = got.double().cpu()
+    for s, (length, count) in enumerate(zip(b.lengths, b.counts)):
+        where = [b.position(s, t) for t in range(length + count)]
+        keys, values = (torch.stack([w[side] for w in where]).double().cpu() for side in range(2))
+        for i in range(count):
+            keep = [t for t in range(length + count) if t < length or t - length in sees(s, i)]
+            for h in range(heads):
+                score, v = keys[keep, h // 2, 0], values[keep, h // 2]
+                f = torch.exp(score - score.max())
+                out = f @ v / f.sum()
+                d = (width + 8) * 2.0 ** -24 * gap * 1.4427
+                step = torch.clamp(f * UNIT["float16"], min=2.0 ** -32)
+                room = ((step + f * (2 * d + (len(keep) + 16) * 2.0 ** -24)) @ v + out * step.sum()) / f.sum()
+                room = (room + UNIT["float16"] * out) * (1 + 2.0 ** -6)
+                error = (got[b.starts_list[s] + i, h] - out).abs()
+                assert float(out.min()) > 2.0 ** -14 and bool((error <= room).all()), (s, i, h, float((error / out).max()))
+
+
 def test_rows_without_keys_are_zero(torch, native):
     b = Batch(torch, native, [0, 40, 0], [6, 6, 40], 4, 2, 64)
     seen = {(0, 2): {2}, (0, 5): {0, 3}, (2, 39): {0}}

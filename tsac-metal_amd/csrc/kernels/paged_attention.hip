@@ -417,10 +417,16 @@ __device__ __forceinline__ void score_block(const u32x4 (&key)[2][HW / 32], cons
     }
 }
 
+// The weight of a score that a reference is moved to, as a power of two: weights and their sums have it as a
+// factor, which leaves their quotient. Weights in half are subnormal below 2^-14 and nothing below
+// 2^-25, and a long context can have most of its sum in such ones: with 2^7, of the 2^16 there is, they are
+// lost below 2^-32 of the largest. BF16 has the range of 32 bits.
+template <bool Half> constexpr float weight_log2 = Half ? 7.0f : 0.0f;
+
 // Moves the running references, if need be, before a block's scores are weighed: only when a
-// score passes one by 2^8. Weights stay in range without it, and most blocks need neither the
+// score passes what one was moved to by 2^8. Weights stay in range without it, and most blocks need neither the
 // exchange nor the scaling.
-template <int HW, int Parts>
+template <int HW, bool Half, int Parts>
 __device__ __forceinline__ void settle(const Launch& l, const f32x4 (&score)[Parts][2], Sums<HW> (&sums)[Parts])
 {
     float most[Parts];
@@ -433,14 +439,14 @@ __device__ __forceinline__ void settle(const Launch& l, const f32x4 (&score)[Par
         most[t] = maximum(maximum(maximum(a[0], a[1], a[2]), a[3], b[0]), maximum(b[1], b[2], b[3]), b[3]);
         // Not a product with -infinity, which a scale of 0 would make no number.
         most[t] = most[t] == minus_infinity ? most[t] : most[t] * l.scale_log2;
-        move = move || most[t] > sums[t].reference + 8.0f;
+        move = move || most[t] > sums[t].reference + (8.0f + weight_log2<Half>);
     }
     if (__any(move))
     {
 #pragma unroll
         for (int t = 0; t < Parts; ++t)
         {
-            sums[t].move(fmaxf(query_max(most[t]), sums[t].reference));
+            sums[t].move(fmaxf(query_max(most[t]) - weight_log2<Half>, sums[t].reference));
         }
     }
 }
@@ -512,7 +518,7 @@ __device__ __forceinline__ void attend_masked(const Launch& l, const Place& p, i
             x[slot % 4] = live[t] >> (16 * (slot / 4) + 4 * (lane / 16) + slot % 4) & 1 ? x[slot % 4] : minus_infinity;
         }
     }
-    settle(l, score, sums);
+    settle<HW, Half>(l, score, sums);
     u32x4 weight[Parts];
 #pragma unroll
     for (int t = 0; t < Parts; ++t)
@@ -848,7 +854,7 @@ __global__ __launch_bounds__(64 * Waves, 2) void narrow_kernel(Launch l)
         take([] {});
         f32x4 score[Parts][2];
         score_block<HW, Half>(key, query, score);
-        settle(l, score, sums);
+        settle<HW, Half>(l, score, sums);
         u32x4 weight[Parts];
         weigh<HW, Half>(l, score, sums, weight);
         add_block<HW, Half>(weight, sums, value);
@@ -1032,7 +1038,7 @@ __global__ __launch_bounds__(64 * waves, 2) void staged_kernel(Launch l)
         read_keys(0, mine);
         score_block<HW, Half>(key, query, score);
         read_keys(Teams == 1 ? 0 : 1, Teams == 1 ? 1 : mine);
-        settle(l, score, sums);
+        settle<HW, Half>(l, score, sums);
         const auto turn = [&](f32x4(&now)[parts][2], f32x4(&then)[parts][2], int block_stage, int b, int key_stage, int key_b,
                               bool last, auto between)
         {
@@ -1044,7 +1050,7 @@ __global__ __launch_bounds__(64 * waves, 2) void staged_kernel(Launch l)
             add_block<HW, Half>(weight, sums, value);
             if (!last)
             {
-                settle(l, then, sums);
+                settle<HW, Half>(l, then, sums);
             }
         };
         // While there are stages to ask for, nothing of a turn depends on their number.
