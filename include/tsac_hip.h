@@ -551,7 +551,7 @@ int tsac_hip_pages_reserve(const tsac_hip_paged_cache* cache, const int32_t* seq
  * page of its own. Positions below the length of a fork are not to be written
  * afterwards. One source may have several targets; a target listed twice, that is a
  * source too or holds pages is INVALID. All or nothing, as tsac_hip_pages_reserve;
- * a table entry out of range is passed on as -1 (INVALID). */
+ * a table entry out of range, the last one too, is passed on as -1 (INVALID). */
 int tsac_hip_pages_fork(const tsac_hip_paged_cache* cache, const int32_t* sources, const int32_t* targets,
                         size_t count, int32_t* status, void* stream);
 

@@ -745,6 +745,41 @@ def test_forks_share_full_pages_and_copy_the_last(torch, native):
     assert not p.references.any()
 
 
+@pytest.mark.parametrize("number", [-1, 1 << 30, "pool"])
+@pytest.mark.parametrize("index", [1, 3])  # a full page, the last one of two rows
+def test_a_fork_passes_on_entries_out_of_range(torch, native, number, index):
+    """As -1, without a page in their place: what the source does not see the fork does not either."""
+    p = Pool(torch, native)
+    p.reserve([0], [50])
+    p.grow(0, 50)
+    bad = p.keys.shape[1] if number == "pool" else number
+    p.table[0, index] = p.model.table[0][index] = bad
+    p.cache.fork(ints(torch, [0]), ints(torch, [4]), status=p.status)
+    m = p.model
+    m.table[4] = [-1 if i == index else page for i, page in enumerate(m.table[0])]
+    m.held[4], m.lengths[4] = 4, 50
+    for page in m.table[4][:3]:
+        if page >= 0:
+            m.references[page] += 1
+    if index != 3:
+        m.table[4][3] = 4
+        m.references[4] = 1
+        p.want_keys[:, 4, :2], p.want_values[:, 4, :2] = p.want_keys[:, 3, :2], p.want_values[:, 3, :2]
+    p.same(native.PAGES_INVALID)
+    query = torch.randn(2, 2, 64, device="cuda").to(p.keys.dtype)
+    query[1] = query[0]
+    out = torch.full_like(query, 7.0)
+    cached = torch.zeros(2, 1, dtype=torch.int64, device="cuda")  # of the new rows none is seen
+    native.attention_paged(p.cache, 1, query, ints(torch, [0, 1, 1, 1, 1, 2, 2, 2]), 1, 51, cached, 0.125, out)
+    assert torch.equal(out[0], out[1]) and bool((out[0] != 7).any())
+    p.cache.free(ints(torch, [4]), status=p.status)
+    for page in m.table[4][:4]:
+        if page >= 0:
+            m.references[page] -= 1
+    m.table[4], m.held[4], m.lengths[4] = [-1] * 9, 0, 0
+    p.same(native.PAGES_INVALID)
+
+
 @pytest.mark.parametrize("seed", range(4))
 def test_pages_through_many_calls(torch, native, seed):
     """A random history against the plain bookkeeping, refusals among it."""

@@ -351,9 +351,21 @@ __global__ __launch_bounds__(Threads) void fork_kernel(PagedCache cache, const i
 
 constexpr int copying_threads = 256;
 
-// Shares the full pages.
-__device__ __forceinline__ void share_pages(const PagedCache& cache, const int* from, int* to, int full, int* status)
+// Shares the full pages. A last one that is out of range has nothing to copy: the page that was taken for
+// the copy, and has another sequence's old rows, is given back.
+__device__ __forceinline__ void share_pages(const PagedCache& cache, const int* from, int* to, int full, int rest,
+                                            int* status)
 {
+    if (threadIdx.x == 0 && rest && (from[full] < 0 || from[full] >= cache.pages))
+    {
+        const int fresh = to[full];
+        if (fresh >= 0 && fresh < cache.pages)
+        {
+            cache.references[fresh] = 0;
+        }
+        to[full] = -1;
+        report(status, status_invalid);
+    }
     for (int j = threadIdx.x; j < full; j += copying_threads)
     {
         int page = from[j];
@@ -375,15 +387,11 @@ typedef unsigned Vector __attribute__((ext_vector_type(4)));
 // Copies the rows of the last page, of one layer's keys or values. Stores go past the caches, which
 // keep the source for its other targets: 64 targets of 8 sources 28 us, with plain stores 49 (and with
 // loads past them too, 50).
-__device__ __forceinline__ void copy_rows(const PagedCache& cache, int part, int old, int fresh, int rest, int* status)
+__device__ __forceinline__ void copy_rows(const PagedCache& cache, int part, int old, int fresh, int rest)
 {
     if (old < 0 || old >= cache.pages || fresh < 0 || fresh >= cache.pages)
     {
-        if (threadIdx.x == 0)
-        {
-            report(status, status_invalid);
-        }
-        return;
+        return; // reported by share_pages
     }
     uint16_t* const memory = (part % 2 ? cache.values : cache.keys) + part / 2 * cache.layer_stride;
     const int vectors = cache.heads * cache.head_width / 8;
@@ -429,11 +437,11 @@ __global__ __launch_bounds__(copying_threads) void fork_copy_kernel(PagedCache c
     int* const to = cache.table + target * cache.table_stride;
     if (int(blockIdx.y) == 2 * cache.layers)
     {
-        share_pages(cache, from, to, full, status);
+        share_pages(cache, from, to, full, rest, status);
     }
     else if (rest)
     {
-        copy_rows(cache, blockIdx.y, from[full], to[full], rest, status);
+        copy_rows(cache, blockIdx.y, from[full], to[full], rest);
     }
     if (threadIdx.x == 0)
     {
