@@ -173,3 +173,30 @@ def test_bindings_check_their_tensors():
     with pytest.raises(native.HipError, match="draft"):
         native.verify_drafts(torch.zeros(4, 9), torch.zeros(4, 8), ints(4), ints(4), ints(2), 4, torch.zeros(4),
                              torch.zeros(1), ints(1, 4), ints(1), ints(1))
+
+
+def test_bindings_check_what_is_read_at_a_pitch():
+    """A path of another width than the nodes announced would be written at one pitch and kept at another; words
+    of a mask are its second axis."""
+    torch = pytest.importorskip("torch")
+
+    def ints(*shape):
+        return torch.zeros(shape, dtype=torch.int32)
+
+    def verify(path, max_nodes):
+        native.verify_drafts(torch.zeros(4, 9), None, ints(4), ints(4), ints(3), max_nodes, torch.zeros(4),
+                             torch.zeros(2), path, ints(2), ints(2))
+
+    for path, max_nodes in ((ints(2, 64), 32), (ints(4, 4), 8), (ints(64), 32), (ints(2, 4, 8), 4)):
+        with pytest.raises(native.HipError, match="path"):
+            verify(path, max_nodes)
+    with pytest.raises(native.HipError, match="path: 4 elements"):
+        verify(ints(1, 4), 4)
+    pool = torch.zeros(2, 8, 16, 2, 64, dtype=torch.bfloat16)
+    cache = native.PagedCache(pool, pool.clone(), ints(3, 4), ints(3), ints(3), ints(8))
+    rows = torch.zeros(5, 2, 64, dtype=torch.bfloat16)
+    for mask in (torch.zeros(5, dtype=torch.int64), torch.zeros(5, 1, 2, dtype=torch.int64)):
+        with pytest.raises(native.HipError, match="mask"):
+            native.attention_paged(cache, 0, rows, ints(4), 5, 64, mask, 1.0, rows.clone())
+        with pytest.raises(native.HipError, match="mask"):
+            native.tree_mask(ints(5), ints(4), 5, mask)

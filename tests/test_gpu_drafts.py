@@ -1218,6 +1218,46 @@ def test_verification_in_a_graph_and_on_a_stream(torch, native):
             first += n
 
 
+def test_a_path_wider_than_the_trees_is_kept_from(torch, native):
+    """One buffer of 64 nodes a sequence for trees of fewer, written by verification and read by keep; another
+    width than what is announced is refused, as a call would write it at one pitch and the other read it at
+    another."""
+    rng = np.random.default_rng(12)
+    p = Pool(torch, native, sequences=3, pages=30, layers=2)
+    counts, lengths = [12, 20, 9], [5, 0, 30]
+    for s in range(3):
+        p.reserve([s], [lengths[s] + counts[s]])
+        p.grow(s, lengths[s])
+    q, _, trees, tokens = drafted(rng, counts, 50, 3, False)
+    target = torch.from_numpy(q).cuda()
+    starts, uniforms = ints(torch, [0] + np.cumsum(counts).tolist()), torch.zeros(sum(counts), device="cuda")
+    buffer = torch.full((3, 64), 77, dtype=torch.int32, device="cuda")
+    accepted, following = ints(torch, [0] * 3), ints(torch, [0] * 3)
+
+    def verify(max_nodes):
+        native.verify_drafts(target, None, ints(torch, tokens), ints(torch, sum(trees, [])), starts, max_nodes,
+                             uniforms, torch.rand(3, device="cuda"), buffer, accepted, following)
+
+    with pytest.raises(native.HipError, match="path"):
+        verify(20)
+    assert bool((buffer == 77).all())
+    verify(64)
+    p.cache.keep(starts, buffer, accepted, status=p.status)
+    old_keys, old_values = p.want_keys.clone(), p.want_values.clone()
+    first = 0
+    for s, n in enumerate(counts):
+        path, _ = verify_plain(q[first:first + n], None, tokens[first:first + n], trees[s], np.zeros(n), 0.5)
+        assert len(path) > 1 and buffer[s].tolist() == path + [-1] * (64 - len(path))
+        for k, node in enumerate(path):
+            a, b = lengths[s] + node, lengths[s] + k
+            to, frm = (p.model.table[s][b // 16], b % 16), (p.model.table[s][a // 16], a % 16)
+            p.want_keys[:, to[0], to[1]] = old_keys[:, frm[0], frm[1]]
+            p.want_values[:, to[0], to[1]] = old_values[:, frm[0], frm[1]]
+        p.model.lengths[s] += len(path)
+        first += n
+    p.same()
+
+
 # ---------------------------------------------------------------- together
 
 def test_a_drafted_decode(torch, native):

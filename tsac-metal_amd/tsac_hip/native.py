@@ -995,6 +995,7 @@ class PagedCache:
 
 def tree_mask(parents, starts, max_rows, mask):
     """Ancestor bits (int64 mask [rows][words]) of drafted rows."""
+    _need(mask.dim() == 2, "mask: must be [rows][words]")
     device, rows, words = parents.device, parents.numel(), mask.shape[1]
     check(library().tsac_hip_tree_mask(
         _array(parents, device, _INT, rows, "parents"), rows, _array(starts, device, _INT, 1, "starts"),
@@ -1025,6 +1026,7 @@ def attention_paged(cache, layer, query, starts, max_rows, max_length, mask, sca
     q, q_stride = _rows(query, device, heads, cache.head_width, cache.type, "query")
     o, o_stride = _rows(out, device, heads, cache.head_width, cache.type, "out")
     _need(out.shape[0] == rows, "out: must have the query's rows")
+    _need(mask is None or mask.dim() == 2, "mask: must be [rows][words]")
     words = 0 if mask is None else mask.shape[1]
     shape = (rows, heads, max_rows, max_length)
     need = cache._workspaces.get(shape)
@@ -1045,6 +1047,8 @@ def verify_drafts(target, draft, tokens, parents, starts, max_nodes, uniforms, d
     """Drafted trees against the target's distributions (target, draft [rows][alphabet], or draft None);
     path int32 [sequences][max_nodes], accepted and next int32 [sequences] are written."""
     device, (rows, alphabet), sequences = target.device, target.shape, starts.numel() - 1
+    # keep() reads it at its own width.
+    _need(path.dim() == 2 and path.shape[1] == max_nodes, "path: must be [sequences][max_nodes]")
     type_ = _PROBABILITY_TYPES.get(_kind(target))
     _need(type_ is not None and (alphabet <= 1 or target.stride(1) == 1), "target: must be rows of probabilities")
     if draft is not None:
