@@ -1067,6 +1067,23 @@ def test_verification_of_wide_alphabets(torch, native, drafts, alphabet):
 
 
 @pytest.mark.parametrize("drafts", [True, False])
+@pytest.mark.parametrize("sequences", [40, 70, 140])
+def test_verification_of_many_sequences_over_wide_alphabets(torch, native, drafts, sequences):
+    """As many as fill the units in several chunks of the alphabet each, or by themselves."""
+    rng = np.random.default_rng(sequences)
+    counts, alphabet = [5 if s % 9 else 0 for s in range(sequences)], 33001
+    p, q, trees, tokens = drafted(rng, counts, alphabet, 3, drafts, spread=4.0)
+    uniforms, draws = rng.random(sum(counts), np.float32), rng.random(sequences, np.float32)
+    got, back, drafts_back = run_verify(torch, native, p, q, trees, tokens, uniforms, draws, "bfloat16", 7)
+    first = 0
+    for s, n in enumerate(counts):
+        part = slice(first, first + n)
+        assert got[s] == verify_plain(back[part], drafts_back[part] if drafts else None, tokens[part], trees[s],
+                                      uniforms[part], draws[s]), s
+        first += n
+
+
+@pytest.mark.parametrize("drafts", [True, False])
 @pytest.mark.parametrize("alphabet", [1, 40000, 65537])
 def test_verification_of_sparse_rows(torch, native, drafts, alphabet):
     """Alphabets of one token, and wide ones whose mass lies in few places, all sums exact: at the ends, around the

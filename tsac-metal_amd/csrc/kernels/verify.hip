@@ -746,12 +746,17 @@ __global__ __launch_bounds__(256) void draw_kernel(Drafts d, const Walk* __restr
 }
 
 // Chunks of the alphabet of one sequence, a workgroup each; what follows is drawn by a second launch
-// then, 4 to 5 us. Of 4 sequences over 128,001 values without drafts: 8 and 5 us, in one chunk 24.
-// Of 32 over 32,000, trees of 32 nodes: 24 and 4 us in three chunks, 25 in one.
-int chunks_of(int sequences, int alphabet)
+// then, 4 to 5 us. Every one follows the path for itself and with drafts sums whole rows for it, so that
+// they gain where all run at once: a workgroup a unit with drafts, two without, and none below four chunks. Over
+// 128,001 values in BF16, several chunks and one: with drafts, trees of 16 nodes of up to four children, 4
+// sequences 56 us and 66, 32 of them 67 and 73 (15 chunks each: 81), 64 72 and 75 (144); without, 4 sequences 12
+// and 28, 64 19 and 33 (15 chunks: 24), 128 26 and 33 (8: 29), 256 42 and 35. Over 50,257 with drafts 128
+// sequences are 44 in two chunks, 42 in one.
+int chunks_of(int sequences, int alphabet, bool draft)
 {
-    const int wanted = alphabet / 8192, room = std::max(1, 4 * compute_units() / std::max(1, sequences));
-    return wanted < 4 ? 1 : std::min(wanted, room);
+    const int room = (draft ? 1 : 2) * compute_units() / std::max(1, sequences);
+    const int chunks = std::min(alphabet / 8192, room);
+    return chunks < 4 ? 1 : chunks;
 }
 
 struct Workspace
@@ -770,7 +775,7 @@ struct Workspace
         {
             return;
         }
-        if (chunks_of(d.sequences, d.alphabet) > 1)
+        if (chunks_of(d.sequences, d.alphabet, false) > 1) // with drafts there are no more
         {
             walks = room(d.sequences * sizeof(Walk));
             sums = room(std::size_t(d.sequences) * ((d.alphabet + segment - 1) / segment) * 8);
@@ -792,13 +797,13 @@ void verify_drafts(const Drafts& drafts, void* workspace, std::size_t bytes, hip
     }
     const Workspace space(drafts);
     require(!space.bytes || (workspace && bytes >= space.bytes), "verify: the workspace is too small");
-    const int chunks = chunks_of(drafts.sequences, drafts.alphabet);
+    const int chunks = chunks_of(drafts.sequences, drafts.alphabet, drafts.draft != nullptr);
     char* const memory = static_cast<char*>(workspace);
     auto* const walks = reinterpret_cast<Walk*>(memory + space.walks);
     auto* const sums = reinterpret_cast<double*>(memory + space.sums);
     // Four waves where each has a segment or two (3 sequences over 1,024 values: 7.6 us, with eight 8.1,
     // with sixteen 9.7), eight where a walk sums no rows, only the chunk it ends with (64 sequences
-    // over 128,001: 20 us, with sixteen 30), sixteen otherwise (32 over 32,000: 25 us, with eight 28).
+    // over 128,001, 15 chunks: 20 us, with sixteen 30), sixteen otherwise (32 over 32,000: 25 us, with eight 28).
     const unsigned threads = drafts.alphabet <= 8 * segment ? 256 : chunks > 1 && !drafts.draft ? 512 : 1024;
     const auto launch = [&](auto type, auto draft)
     {
