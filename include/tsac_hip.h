@@ -599,7 +599,8 @@ int tsac_hip_tree_mask(const int32_t* parents, size_t rows, const int32_t* start
  * not see do not reach it, whatever they are; a position whose page is out of range
  * or not held is seen by none. Strides in elements, multiples of 8; 16-byte aligned.
  * max_rows: the most rows of one sequence, at most 65536; further rows are left as
- * they were. max_length: about the longest lengths[s] plus its rows (it shapes the
+ * they were. At most 2^30 query rows a cached head (max_rows times heads / cache->heads)
+ * and, at 128 or fewer of them a workgroup, workgroups a call. max_length: about the longest lengths[s] plus its rows (it shapes the
  * launch; any value gives the result). Workspace: tsac_hip_attention_paged_workspace
  * bytes of device memory, 16-byte aligned, not shared by calls that overlap. */
 size_t tsac_hip_attention_paged_workspace(const tsac_hip_paged_cache* cache, size_t rows, size_t heads,

@@ -200,3 +200,15 @@ def test_bindings_check_what_is_read_at_a_pitch():
             native.attention_paged(cache, 0, rows, ints(4), 5, 64, mask, 1.0, rows.clone())
         with pytest.raises(native.HipError, match="mask"):
             native.tree_mask(ints(5), ints(4), 5, mask)
+
+
+def test_attention_of_too_many_rows():
+    """More query rows of a cached head than the kernels count."""
+    lib = native.library()
+
+    def attend(sequences, heads, max_rows, stride):
+        return lib.tsac_hip_attention_paged(desc(sequences=sequences), 0, POINTER, stride, 4, heads, POINTER, max_rows, 64,
+                                            None, 0, 1.0, POINTER, stride, POINTER, 1 << 30, None)
+
+    refused(attend(1, 32768, 65536, 32768 * 64), "rows")  # 2^30 of each of two heads
+    assert lib.tsac_hip_attention_paged_workspace(desc(sequences=1), 4, 32768, 65536, 64) == 0

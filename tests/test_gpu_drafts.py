@@ -265,6 +265,35 @@ def test_attention_of_many_short_sequences(torch, native, kind, heads, kv_heads,
     b.check(b.attend(mask, max_length=guess), lambda s, i: line(trees[s], i))
 
 
+def test_attention_of_more_workgroups_than_a_launch_holds(torch, native):
+    """A batch of single rows and one prompt, announced as 65,536 rows a sequence: the tiles that have rows are
+    those of the smaller announcement, the last sequences in a second launch."""
+    rng = np.random.default_rng(7)
+    sequences = 2100
+    lengths = [int(x) for x in rng.integers(0, 30, sequences)]
+    counts = [1] * sequences
+    counts[-3], counts[5], counts[2050] = 300, 0, 40
+    b = Batch(torch, native, lengths, counts, 16, 8, 64, 16, seed=51)
+    want = b.attend().clone()
+    assert b.max_rows == 300 and bool((want != 7).all())
+    b.max_rows = 65536
+    assert torch.equal(b.attend(), want)
+
+
+def test_attention_of_more_workgroups_than_a_call_holds(torch, native):
+    sequences, heads = 65535, 16384
+    keys = torch.zeros(1, 1, 16, 2, 64, dtype=torch.bfloat16, device="cuda")
+    table, held, lengths = (torch.zeros(*shape, dtype=torch.int32, device="cuda")
+                            for shape in ((sequences, 1), (sequences,), (sequences,)))
+    cache = native.PagedCache(keys, keys.clone(), table, held, lengths, ints(torch, [0]))
+    query = torch.zeros(1, heads, 64, dtype=torch.bfloat16, device="cuda")
+    out, starts = torch.full_like(query, 7.0), torch.zeros(sequences + 1, dtype=torch.int32, device="cuda")
+    with pytest.raises(native.HipError, match="too many"):
+        native.attention_paged(cache, 0, query, starts, 65536, 64, None, 1.0, out)
+    torch.cuda.synchronize()
+    assert bool((out == 7).all())
+
+
 @pytest.mark.parametrize("kind,heads,kv_heads,width", [("bfloat16", 32, 8, 128), ("float16", 24, 4, 64)])
 @pytest.mark.parametrize("tree", [False, True])
 def test_tall_tiles_over_chunks(torch, native, kind, heads, kv_heads, width, tree):

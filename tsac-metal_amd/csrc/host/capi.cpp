@@ -659,6 +659,7 @@ PagedRows paged_rows_of(const PagedCache& cache, std::size_t rows, std::size_t h
             "paged attention: rows or length out of range");
     require(heads > 0 && heads <= 65536 && heads % std::size_t(cache.heads) == 0,
             "paged attention: heads must be a multiple of the cache's");
+    require(max_rows * (heads / std::size_t(cache.heads)) < (std::size_t(1) << 30), "paged attention: rows out of range");
     PagedRows r;
     r.rows = int(rows);
     r.heads = int(heads);

@@ -130,6 +130,7 @@ struct Launch
     int splits, chunk; // chunks, keys of a chunk
     int units;         // sequences x chunks x key/value heads
     int together;      // of them that one die takes
+    unsigned first;    // workgroup of the launch
     float scale_log2;  // above or at 0
     bool negative;     // scale is below: queries are taken negative
 };
@@ -671,7 +672,8 @@ __device__ __forceinline__ bool all_there(const Launch& l, const Place& p, int f
 // where a die reads one head alone, its requests meet in two of its cache's sixteen channels.
 __device__ __forceinline__ void unit_of(const Launch& l, int& unit, int& tile)
 {
-    const int die = blockIdx.x % 8, i = blockIdx.x / 8, j = i / l.tiles;
+    const unsigned index = l.first + blockIdx.x;
+    const int die = index % 8, i = index / 8, j = i / l.tiles;
     tile = i % l.tiles;
     unit = (j / l.together * 8 + die) * l.together + j % l.together;
 }
@@ -1292,10 +1294,14 @@ Shape shape_of(const PagedCache& cache, const PagedRows& rows)
     return s;
 }
 
-template <int HW, bool Half> void launch(const Launch& l, const Shape& s, std::size_t pairs, hipStream_t stream)
+// Workgroups of one launch, of which 2^32 work-items along x are the limit, and of one call. Those without rows
+// end at once: 8.6 million take 16 ms.
+constexpr std::size_t launch_limit = (std::size_t(1) << 23) - 8, call_limit = std::size_t(1) << 30;
+
+template <int HW, bool Half> void launch(Launch l, const Shape& s, std::size_t pairs, hipStream_t stream)
 {
     const std::size_t groups = s.units / l.together;
-    const unsigned grid = unsigned((groups + 7) / 8 * 8 * l.together * s.tiles);
+    const std::size_t grid = (groups + 7) / 8 * 8 * l.together * s.tiles;
     const auto run = [&](auto kernel, int threads, std::size_t lds)
     {
         if (lds > 65536)
@@ -1304,8 +1310,12 @@ template <int HW, bool Half> void launch(const Launch& l, const Shape& s, std::s
                                           hipFuncAttributeMaxDynamicSharedMemorySize, int(lds)),
                       "paged attention LDS");
         }
-        kernel<<<grid, threads, lds, stream>>>(l);
-        check_hip(hipGetLastError(), "paged attention launch");
+        for (std::size_t first = 0; first < grid; first += launch_limit)
+        {
+            l.first = unsigned(first);
+            kernel<<<unsigned(std::min(grid - first, launch_limit)), threads, lds, stream>>>(l);
+            check_hip(hipGetLastError(), "paged attention launch");
+        }
     };
     constexpr std::size_t narrow_wave = 2 * block * HW * 2, staged = stages * staged_keys * HW * 4;
     const auto run_either = [&](auto read_once)
@@ -1355,9 +1365,7 @@ void attention_paged(const PagedCache& cache, int layer, const PagedRows& rows, 
     }
     const Shape s = shape_of(cache, rows);
     const std::size_t pairs = std::size_t(cache.sequences) * cache.heads;
-    // 2^32 work-items along x are a grid's limit.
-    require((s.units + 8 * cache.heads) * s.tiles < (std::size_t(1) << 23) && pairs * s.parts < (std::size_t(1) << 23),
-            "paged attention: too many workgroups for one launch");
+    require((s.units + 8 * cache.heads) * s.tiles < call_limit, "paged attention: too many rows, sequences and heads");
     require(s.splits == 1 || (workspace && bytes >= s.units * s.parts * s.record * 4),
             "paged attention: the workspace is too small");
     Launch l{};
