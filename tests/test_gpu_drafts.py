@@ -886,6 +886,39 @@ def test_written_rows_lie_behind_the_length(torch, native, kind, layers):
     assert torch.equal(p.keys[:, page, row], p.want_keys[:, page, row]) and not p.keys[first, page, 0].any()
 
 
+@pytest.mark.parametrize("announced", [700, 5, 1 << 20])
+def test_written_rows_of_ragged_batches(torch, native, announced):
+    """Most sequences with a row or none and one with hundreds, by a search over starts 64 at a time; rows in front
+    of the first sequence and behind the last one are nobody's."""
+    rng = np.random.default_rng(3)
+    n, rows = 4200, 16
+    counts = [int(c) for c in rng.integers(0, 3, n)]
+    counts[64], counts[63], counts[4097], counts[-1] = 700, 0, 9, 4
+    starts = 3 + np.concatenate([[0], np.cumsum(counts)])
+    lengths = [int(x) for x in rng.integers(0, 20, n)]
+    held = [-(-(a + b) // rows) for a, b in zip(lengths, counts)]
+    pages = sum(held)
+    table, at = -np.ones((n, max(held)), np.int32), 0
+    order = rng.permutation(pages)
+    for s, h in enumerate(held):
+        table[s, :h] = order[at:at + h]
+        at += h
+    keys = torch.zeros(2, pages, rows, 1, 64, dtype=torch.bfloat16, device="cuda")
+    cache = native.PagedCache(keys, torch.zeros_like(keys), ints(torch, table), ints(torch, held), ints(torch, lengths),
+                              ints(torch, [1] * pages))
+    fresh = torch.randn(2, 2, int(starts[-1]) + 5, 1, 64, device="cuda").bfloat16()
+    status = ints(torch, [0])
+    cache.write(fresh[0], fresh[1], ints(torch, starts), announced, status=status)
+    assert int(status) == 0
+    want = torch.zeros_like(keys), torch.zeros_like(keys)
+    to = [(table[s, (lengths[s] + i) // rows], (lengths[s] + i) % rows, starts[s] + i)
+          for s in range(n) for i in range(min(counts[s], announced))]
+    page, place, row = (torch.tensor(np.array(x), device="cuda") for x in zip(*to))
+    for side in range(2):
+        want[side][:, page, place] = fresh[side][:, row]
+        assert torch.equal(cache.tensors[side], want[side])
+
+
 def test_shared_pages_are_not_written(torch, native):
     p = Pool(torch, native)
     p.reserve([0], [48])
