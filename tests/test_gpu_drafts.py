@@ -774,6 +774,18 @@ def test_forks_share_full_pages_and_copy_the_last(torch, native):
     assert not p.references.any()
 
 
+def test_freed_sequences_have_no_length(torch, native):
+    """Whatever they held: a length without pages, a negative number of them, a sequence listed twice."""
+    p = Pool(torch, native)
+    p.reserve([0, 1], [40, 20])
+    p.grow(0, 40)
+    p.held[2], p.lengths[2] = 0, 50
+    p.held[3], p.lengths[3] = -3, -8
+    p.cache.free(ints(torch, [2, 0, 3, 0]), status=p.status)
+    p.model.free([0])
+    p.same()
+
+
 @pytest.mark.parametrize("number", [-1, 1 << 30, "pool"])
 @pytest.mark.parametrize("index", [1, 3])  # a full page, the last one of two rows
 def test_a_fork_passes_on_entries_out_of_range(torch, native, number, index):

@@ -471,10 +471,7 @@ __global__ __launch_bounds__(copying_threads) void free_kernel(PagedCache cache,
     if (threadIdx.x == 0)
     {
         held = atomicExch(&cache.held[s], 0);
-        if (held)
-        {
-            cache.lengths[s] = 0;
-        }
+        cache.lengths[s] = 0;
     }
     __syncthreads();
     int* const table = cache.table + s * cache.table_stride;
