@@ -593,6 +593,15 @@ def test_masks_at_word_boundaries(torch, native):
     assert bool((mask[100:] == -1).all()) and torch.equal(mask[:100], pack_masks(torch, rows[:100], 16))
 
 
+def test_masks_of_a_thousand_nodes(torch, native):
+    rng = np.random.default_rng(1)
+    trees = [list(range(-1, 1023)), [-1] + [0] * 1023, random_tree(rng, 1000)]
+    mask = torch.full((3050, 16), -1, dtype=torch.int64, device="cuda")
+    native.tree_mask(ints(torch, sum(trees, []) + [0] * 2), ints(torch, [0, 1024, 2048, 3048]), 1024, mask)
+    rows = [line(t, i) for t in trees for i in range(len(t))]
+    assert torch.equal(mask[:3048], pack_masks(torch, rows, 16)) and bool((mask[3048:] == -1).all())
+
+
 # ---------------------------------------------------------------- pages
 
 class Model:
@@ -974,6 +983,52 @@ def test_accepted_rows_are_kept(torch, native, in_place, heads, rows):
     p.same()
 
 
+@pytest.mark.parametrize("heads", [3, 20, 40])
+def test_rows_of_any_width_are_written_forked_and_kept(torch, native, heads):
+    """24, 160 and 320 vectors a row: threads without one, several a thread, more than one workgroup has in keep().
+    One tree of 1,024 nodes of which more are kept than are looked up at a time, one in place but for its end."""
+    p = Pool(torch, native, sequences=4, pages=170, width=80, heads=heads, layers=2)
+    lengths, counts = [7, 33, 0, 0], [1024, 600, 0, 0]
+    paths = [sorted(random.Random(5).sample(range(1024), 700)), list(range(515)) + [530, 599], [], []]
+    for s in range(2):
+        p.reserve([s], [lengths[s] + counts[s]])
+        p.grow(s, lengths[s])
+    starts = [0] + np.cumsum(counts).tolist()
+    fresh = torch.randn(2, 2, starts[-1], heads, 64, device="cuda").bfloat16()
+    p.cache.write(fresh[0], fresh[1], ints(torch, starts), 1024, status=p.status)
+    path = -np.ones((4, 1024), np.int32)
+    for s, nodes in enumerate(paths):
+        path[s, :len(nodes)] = nodes
+        for i in range(counts[s]):
+            t = lengths[s] + i
+            p.want_keys[:, p.model.table[s][t // 16], t % 16] = fresh[0, :, starts[s] + i]
+            p.want_values[:, p.model.table[s][t // 16], t % 16] = fresh[1, :, starts[s] + i]
+    p.same()
+    p.cache.keep(ints(torch, starts), ints(torch, path), ints(torch, [len(x) for x in paths]), status=p.status)
+    for s, nodes in enumerate(paths):
+        for k, node in enumerate(nodes):
+            t = lengths[s] + k
+            p.want_keys[:, p.model.table[s][t // 16], t % 16] = fresh[0, :, starts[s] + node]
+            p.want_values[:, p.model.table[s][t // 16], t % 16] = fresh[1, :, starts[s] + node]
+        p.model.lengths[s] += len(nodes)
+    p.same()
+    p.fork([0, 1], [3, 2])
+
+
+def test_hundreds_of_forks(torch, native):
+    p = Pool(torch, native, sequences=700, pages=640, width=5, heads=3, layers=1)
+    for s, n in ((0, 50), (1, 32), (2, 5)):
+        p.reserve([s], [n])
+        p.grow(s, n)
+    targets = list(range(699, 99, -1))
+    p.fork([t % 3 for t in targets], targets)
+    assert int(p.references.max()) == 201
+    p.free(targets[::2] + targets[1:400:2])
+    p.fork([699 - 2 * 250] * 300, targets[:600:2])  # of those still held
+    p.free(list(range(700)))
+    assert not p.references.any()
+
+
 def test_paths_that_are_none_move_nothing(torch, native):
     p = Pool(torch, native, sequences=6)
     lengths = [20] * 6
@@ -1244,6 +1299,57 @@ def test_verification_at_the_edges(torch, native):
         got, _, _ = run_verify(torch, native, p, q, [parents], tokens, uniforms, draws)
         reached = [v if 0 <= v < i else -1 for i, v in enumerate(parents)]
         assert got[0] == verify_plain(p, q, tokens, reached, uniforms, draw), (parents, tokens)
+
+
+@pytest.mark.parametrize("drafts", [True, False])
+@pytest.mark.parametrize("alphabet", [1500, 33001])
+@pytest.mark.parametrize("last", [True, False])
+def test_verification_of_a_thousand_siblings(torch, native, drafts, alphabet, last):
+    """A root of 1,023 children, repeated tokens among them, all refused or all but the last. Every sum is exact:
+    half of p lies on 1,024 tokens that q has twice as often, half on one that q lacks."""
+    places = np.arange(1024) * ((alphabet - 1) // 1024) % (alphabet - 1)
+    p, q = np.zeros((1024, alphabet), np.float32), np.zeros((1024, alphabet), np.float32)
+    p[:, places], p[:, -1], q[:, places] = 2.0 ** -11, 0.5, 2.0 ** -10
+    rng = np.random.default_rng(alphabet)
+    tokens = [0] + [int(places[i]) for i in rng.integers(0, 700, 1022)] + [alphabet - 1 if last else int(places[3])]
+    trees, uniforms = [[-1] + [0] * 1023], np.full(1024, 0.999, np.float32)
+    if last and not drafts:
+        uniforms[-1] = 0.25  # of what is left, 0.5 and what was not drafted
+    for draw in (0.0, 0.3, 0.77, 1 - 2.0 ** -24):
+        draws = np.array([draw], np.float32)
+        got, back, back_q = run_verify(torch, native, p, q if drafts else None, trees, tokens, uniforms, draws, "bfloat16")
+        want = verify_plain(p, q if drafts else None, tokens, trees[0], uniforms, draws[0])
+        assert want[0] == ([0, 1023] if last else [0]) and got[0] == want
+
+
+@pytest.mark.parametrize("drafts", [True, False])
+@pytest.mark.parametrize("alphabet", [41, 33001])
+def test_verification_of_deep_trees(torch, native, drafts, alphabet):
+    """A chain and a tree of 1,024 nodes each, followed to the end and as far as random numbers go."""
+    rng = np.random.default_rng(alphabet)
+    rows, counts = 2048, [1024, 1024]
+    p = np.zeros((rows, alphabet), np.float32)
+    q = np.zeros((rows, alphabet), np.float32)
+    tokens = rng.integers(0, alphabet, rows)
+    places = rng.integers(0, alphabet, (rows, 8))
+    tree = [-1] + [int(rng.integers(max(0, i - 200), i)) for i in range(1, 1024)]
+    trees = [list(range(-1, 1023)), tree]
+    for r in range(rows):
+        np.add.at(p[r], places[r], rng.integers(1, 9, 8).astype(np.float32) / 64)
+        np.add.at(q[r], places[r], rng.integers(1, 9, 8).astype(np.float32) / 64)
+    for first, parents in ((0, trees[0]), (1024, trees[1])):
+        for i in range(1, 1024):
+            p[first + parents[i], tokens[first + i]] += 0.25
+            q[first + parents[i], tokens[first + i]] += 0.25
+    for scale in (0.0, 0.3, 1.0):
+        uniforms = (rng.random(rows, np.float32) * scale).astype(np.float32)
+        draws = rng.random(2, np.float32)
+        got, back, _ = run_verify(torch, native, p, q if drafts else None, trees, tokens.tolist(), uniforms, draws)
+        for s in range(2):
+            part = slice(1024 * s, 1024 * s + 1024)
+            want = verify_plain(p[part], q[part] if drafts else None, tokens[part], trees[s], uniforms[part], draws[s])
+            assert got[s] == want, (scale, s)
+        assert scale or len(got[0][0]) == 1024
 
 
 def test_nodes_past_the_announced_ones_are_not_looked_at(torch, native):
