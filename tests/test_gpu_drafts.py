@@ -365,6 +365,15 @@ def test_small_weights_in_half_precision_count(torch, native, width, nodes, tree
                 assert float(out.min()) > 2.0 ** -14 and bool((error <= room).all()), (s, i, h, float((error / out).max()))
 
 
+@pytest.mark.parametrize("nodes", [1, 70])
+def test_attention_past_32_bits_of_offset(torch, native, nodes):
+    """Two layers of 2,100 pages of 2^20 elements: the second's last page lies past 2^32 elements, and 2^33 bytes."""
+    b = Batch(torch, native, [3000, 900], [nodes, nodes], 16, 8, 128, 1024, layers=2, seed=71, spare=2094)
+    b.table[0, 0] = b.keys.shape[1] - 1
+    assert b.keys[1].storage_offset() + b.keys.stride(1) * int(b.table[0, 0]) > 2 ** 32
+    b.check(b.attend(layer=1), chain, layer=1)
+
+
 def test_rows_without_keys_are_zero(torch, native):
     b = Batch(torch, native, [0, 40, 0], [6, 6, 40], 4, 2, 64)
     seen = {(0, 2): {2}, (0, 5): {0, 3}, (2, 39): {0}}
@@ -1015,6 +1024,30 @@ def test_rows_of_any_width_are_written_forked_and_kept(torch, native, heads):
     p.fork([0, 1], [3, 2])
 
 
+def test_pages_past_32_bits_of_offset(torch, native):
+    """Rows written, kept and forked in the last pages of a pool of 2^32 elements and more a layer."""
+    layers, pages, rows = 2, 2100, 1024
+    keys, values = (torch.empty(layers, pages, rows, 8, 128, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    references = torch.ones(pages, dtype=torch.int32, device="cuda")
+    references[-3:] = 0
+    table = torch.full((2, 4), -1, dtype=torch.int32, device="cuda")
+    held, lengths, status = ints(torch, [0, 0]), ints(torch, [0, 0]), ints(torch, [0])
+    cache = native.PagedCache(keys, values, table, held, lengths, references)
+    cache.reserve(ints(torch, [1100]), ints(torch, [1]), status=status)
+    assert table[1].tolist() == [pages - 3, pages - 2, -1, -1]
+    fresh = torch.randn(2, layers, 1100, 8, 128, device="cuda").bfloat16()
+    starts = ints(torch, [0, 0, 1100])
+    cache.write(fresh[0], fresh[1], starts, 1100, status=status)
+    path = ints(torch, [[0] * 1030, [*range(1020), *range(1090, 1100)]])
+    cache.keep(starts, path, ints(torch, [0, 1030]), status=status)
+    cache.fork(ints(torch, [1]), ints(torch, [0]), status=status)
+    assert int(status) == 0 and lengths.tolist() == [1030] * 2 and table[0].tolist() == [pages - 3, pages - 1, -1, -1]
+    kept = fresh[:, :, path[1].long()]
+    for side, pool in enumerate((keys, values)):
+        for page in (pages - 2, pages - 1):
+            assert torch.equal(torch.cat([pool[:, pages - 3], pool[:, page, :6]], 1), kept[side])
+
+
 def test_hundreds_of_forks(torch, native):
     p = Pool(torch, native, sequences=700, pages=640, width=5, heads=3, layers=1)
     for s, n in ((0, 50), (1, 32), (2, 5)):
@@ -1350,6 +1383,28 @@ def test_verification_of_deep_trees(torch, native, drafts, alphabet):
             want = verify_plain(p[part], q[part] if drafts else None, tokens[part], trees[s], uniforms[part], draws[s])
             assert got[s] == want, (scale, s)
         assert scale or len(got[0][0]) == 1024
+
+
+@pytest.mark.parametrize("drafts", [True, False])
+def test_verification_past_32_bits_of_offset(torch, native, drafts):
+    """The last rows of 4,100 over 2^20 tokens: their values lie past 2^32 elements."""
+    rng = np.random.default_rng(9)
+    rows, alphabet, nodes = 4100, 1 << 20, 4
+    p, q, trees, tokens = drafted(rng, [nodes], alphabet, 3, drafts, spread=6.0)
+    target = torch.empty(rows, alphabet, dtype=torch.bfloat16, device="cuda")
+    draft = torch.empty_like(target) if drafts else None
+    target[-nodes:] = torch.from_numpy(p).cuda()
+    if drafts:
+        draft[-nodes:] = torch.from_numpy(q).cuda()
+    uniforms, draws = rng.random(rows, np.float32), rng.random(1, np.float32)
+    ids, parents = np.zeros(rows, np.int32), np.zeros(rows, np.int32)
+    ids[-nodes:], parents[-nodes:] = tokens, trees[0]
+    path, accepted, following = ints(torch, [[9] * nodes]), ints(torch, [9]), ints(torch, [9])
+    native.verify_drafts(target, draft, ints(torch, ids), ints(torch, parents), ints(torch, [rows - nodes, rows]), nodes,
+                         torch.from_numpy(uniforms).cuda(), torch.from_numpy(draws).cuda(), path, accepted, following)
+    back, back_q = (None if x is None else x[-nodes:].double().cpu().numpy() for x in (target, draft))
+    want, token = verify_plain(back, back_q, tokens, trees[0], uniforms[-nodes:], draws[0])
+    assert path[0, :int(accepted)].tolist() == want and int(following) == token
 
 
 def test_nodes_past_the_announced_ones_are_not_looked_at(torch, native):
