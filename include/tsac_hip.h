@@ -504,7 +504,8 @@ int tsac_hip_attention_causal(const uint16_t* qkv, size_t heads, size_t head_wid
  * host. What is in device memory is checked by the kernels: a call that finds a
  * number, length or page out of range stays inside the given memory, does what
  * its declaration says, and writes one of these to `status` (device memory, or
- * NULL; 0 beforehand, never cleared by a call). */
+ * NULL; 0 beforehand, never cleared by a call). A call that leaves everything as it
+ * was may still set table entries past what a sequence holds to -1. */
 #define TSAC_HIP_PAGES_INVALID 1   /* a sequence, length, path or page out of range */
 #define TSAC_HIP_PAGES_EXHAUSTED 2 /* fewer free pages than the call needs */
 
@@ -601,7 +602,8 @@ int tsac_hip_tree_mask(const int32_t* parents, size_t rows, const int32_t* start
  * max_rows: the most rows of one sequence, at most 65536; further rows are left as
  * they were. At most 2^30 query rows a cached head (max_rows times heads / cache->heads)
  * and, at 128 or fewer of them a workgroup, workgroups a call. max_length: about the longest lengths[s] plus its rows (it shapes the
- * launch; any value gives the result). Workspace: tsac_hip_attention_paged_workspace
+ * launch; any value gives the result, to rounding: sums are 32-bit and in an order that
+ * follows the launch's, the weights of values rounded to the cache's type). Workspace: tsac_hip_attention_paged_workspace
  * bytes of device memory, 16-byte aligned, not shared by calls that overlap. */
 size_t tsac_hip_attention_paged_workspace(const tsac_hip_paged_cache* cache, size_t rows, size_t heads,
                                           size_t max_rows, size_t max_length);
@@ -624,7 +626,7 @@ int tsac_hip_attention_paged(const tsac_hip_paged_cache* cache, uint32_t layer, 
  * not, W -= p(x) and p(x) = 0. Where no child is accepted, next[s] is the lowest token
  * whose inclusive sum of max(0, p - S q) (or p) exceeds draws[s] in [0, 1) times the
  * whole sum; if that is 0, of the row of p as it is; if that is 0 too, -1. path
- * [sequences][max_nodes]: node 0 and the accepted ones, then -1; accepted[s]: their
+ * [sequences][max_nodes], of that width: node 0 and the accepted ones, then -1; accepted[s]: their
  * number. A sequence without nodes: 0, -1. Sums are 64-bit and of one order. At most
  * 1024 nodes a sequence (further ones are not looked at), 65535 sequences and 2^20 tokens.
  * Workspace as for tsac_hip_attention_paged. */

