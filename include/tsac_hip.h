@@ -595,7 +595,8 @@ int tsac_hip_tree_mask(const int32_t* parents, size_t rows, const int32_t* start
  * written already: every row sees the lengths[s] cached positions, and of the
  * sequence's rows those whose bit is set in mask[row][words] or, with mask NULL,
  * itself and those in front of it. Query head h reads head h / (heads /
- * cache->heads). out [rows][heads][head_width] = softmax(scale q k) v; a row that sees
+ * cache->heads). out [rows][heads][head_width] = softmax(scale q k) v, for scale q k
+ * below 2^27 in size (past it, and infinite, what 32 bits give); a row that sees
  * no key (or none with a score above -infinity) is 0. Keys and values that a row does
  * not see do not reach it, whatever they are; a position whose page is out of range
  * or not held is seen by none. Strides in elements, multiples of 8; 16-byte aligned.

@@ -374,6 +374,45 @@ def test_attention_past_32_bits_of_offset(torch, native, nodes):
     b.check(b.attend(layer=1), chain, layer=1)
 
 
+@pytest.mark.parametrize("kind", ["float16", "bfloat16"])
+@pytest.mark.parametrize("width", [64, 128])
+@pytest.mark.parametrize("nodes,tree", [(1, False), (40, False), (40, True)])
+@pytest.mark.parametrize("size", [10, 23, 25, 26])
+def test_scores_that_are_large_and_close(torch, native, kind, width, nodes, tree, size):
+    """Scores 2^size + 8 j, j from 0 to 5, rising with the position, exact in 32 bits, though as powers of two their
+    neighbours lie up to 8 apart. With f the weights against the largest and u_f = max(u f, 2^-32) in half, u f in
+    BF16, exponents of up to 58 are off by half a step of theirs and the factor log2 e by one: d = 58 * 2^-23, and
+    |error| <= u |out| + sum (u_f + f (d + (T + 16) 2^-24)) |v| / sum f + |out| sum u_f / sum f, times 1 + 2^-6."""
+    heads, kv, u = 4, 2, UNIT[kind]
+    b = Batch(torch, native, [1500, 33], [nodes, nodes], heads, kv, width, 16, kind, seed=81, scale=1.0)
+    g = torch.Generator(device="cuda").manual_seed(82)
+    b.query.zero_()
+    b.query[:, :, 0], b.query[:, :, 1] = 2.0 ** 15, 1.0
+    b.keys.zero_()
+    b.keys[..., 0] = 2.0 ** (size - 15)
+    b.keys[..., 1] = 8.0 * torch.randint(0, 6, b.keys.shape[:-1], generator=g, device="cuda").to(b.keys.dtype)
+    for i, page in enumerate(b.table[0].tolist()):  # rising, so that every wave or team meets one after another
+        b.keys[0, page, :, :, 1] = 8.0 * min(5, i // 16) if page >= 0 else 0.0
+    trees = [random_tree(b.rng, n) for n in b.counts]
+    sees = (lambda s, i: line(trees[s], i)) if tree else chain
+    got = b.attend(pack_masks(torch, [line(t, i) for t in trees for i in range(len(t))], 1) if tree else None)
+    got = got.double().cpu()
+    for s, (length, count) in enumerate(zip(b.lengths, b.counts)):
+        where = [b.position(s, t) for t in range(length + count)]
+        keys, values = (torch.stack([w[side] for w in where]).double().cpu() for side in range(2))
+        for i in range(0, count, 7):
+            keep = [t for t in range(length + count) if t < length or t - length in sees(s, i)]
+            for h in range(heads):
+                score, v = keys[keep, h // 2, 1], values[keep, h // 2]
+                f = torch.exp(score - score.max())
+                out = f @ v / f.sum()
+                step = torch.clamp(f * u, min=2.0 ** -32) if kind == "float16" else f * u
+                room = (step + f * (58 * 2.0 ** -23 + (len(keep) + 16) * 2.0 ** -24)) @ v.abs() / f.sum()
+                room = (room + (u + step.sum() / f.sum()) * out.abs()) * (1 + 2.0 ** -6)
+                error = (got[b.starts_list[s] + i, h] - out).abs()
+                assert bool((error <= room).all()), (s, i, h, float((error / room).max()))
+
+
 def test_rows_without_keys_are_zero(torch, native):
     b = Batch(torch, native, [0, 40, 0], [6, 6, 40], 4, 2, 64)
     seen = {(0, 2): {2}, (0, 5): {0, 3}, (2, 39): {0}}

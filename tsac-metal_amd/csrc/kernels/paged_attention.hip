@@ -426,7 +426,8 @@ template <bool Half> constexpr float weight_log2 = Half ? 7.0f : 0.0f;
 
 // Moves the running references, if need be, before a block's scores are weighed: only when a
 // score passes what one was moved to by 2^8. Weights stay in range without it, and most blocks need neither the
-// exchange nor the scaling.
+// exchange nor the scaling. By how much it passes one is computed as its weight is: where scores are so large that
+// neighbouring numbers lie far apart, a rounded bound would let weights in half past their range.
 template <int HW, bool Half, int Parts>
 __device__ __forceinline__ void settle(const Launch& l, const f32x4 (&score)[Parts][2], Sums<HW> (&sums)[Parts])
 {
@@ -438,16 +439,18 @@ __device__ __forceinline__ void settle(const Launch& l, const f32x4 (&score)[Par
         const f32x4 a = score[t][0], b = score[t][1];
         // Of scores that are not numbers it is none either, and so is the row.
         most[t] = maximum(maximum(maximum(a[0], a[1], a[2]), a[3], b[0]), maximum(b[1], b[2], b[3]), b[3]);
-        // Not a product with -infinity, which a scale of 0 would make no number.
-        most[t] = most[t] == minus_infinity ? most[t] : most[t] * l.scale_log2;
-        move = move || most[t] > sums[t].reference + (8.0f + weight_log2<Half>);
+        // Of -infinity alone it is no number, or less.
+        move = move || __builtin_fmaf(most[t], l.scale_log2, -sums[t].reference) > 8.0f + weight_log2<Half>;
     }
     if (__any(move))
     {
 #pragma unroll
         for (int t = 0; t < Parts; ++t)
         {
-            sums[t].move(fmaxf(query_max(most[t]) - weight_log2<Half>, sums[t].reference));
+            const float score = query_max(most[t]);
+            // Not a product with -infinity, which a scale of 0 would make no number.
+            const float to = score == minus_infinity ? score : score * l.scale_log2 - weight_log2<Half>;
+            sums[t].move(fmaxf(to, sums[t].reference));
         }
     }
 }
