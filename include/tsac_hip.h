@@ -638,6 +638,172 @@ int tsac_hip_verify_drafts(const void* target, size_t target_stride, const void*
                            const float* draws, int32_t* path, int32_t* accepted, int32_t* next, void* workspace,
                            size_t workspace_bytes, void* stream);
 
+/* ---- a model's step around that attention -----------------------------------------
+ * No counterpart in the reference, whose model has one fixed form. What a program with
+ * a model of its own puts between the attention over its pages and the verification
+ * of its drafts: the norms before and after a block, products of 8-bit integers with a
+ * scale for each token and each channel (the projections above have one for every 256
+ * inputs, with sums in a fixed order of floats), rotated positions on the way into the
+ * cache, and the rules on logits. Calls are as in the section above: ordered on
+ * `stream`, on the current device, without allocating or waiting, and may be captured.
+ * Arithmetic is in 32 bits; values are rounded once, as they are stored. Types are
+ * TSAC_HIP_TYPE_BF16, _FP16 and, where it says so, _FP32. */
+
+/* y[m][n] = type((sum_k q[m][k] values[n][k]) * (token_scales[m] * scales[n]) + bias[n]). */
+typedef struct tsac_hip_channel_linear tsac_hip_channel_linear;
+
+/* Copies values [N][K], scales [N] and bias [N] (or NULL) to the current device, from host
+ * memory or from device memory that work in front on `stream` has written, and waits for
+ * it. K at most 131071, so that sums fit 32 bits; N at most 2^24. */
+int tsac_hip_channel_linear_create(const int8_t* values, const float* scales, const float* bias, size_t K, size_t N,
+                                   void* stream, tsac_hip_channel_linear** linear);
+void tsac_hip_channel_linear_destroy(tsac_hip_channel_linear* linear);
+
+/* Rows of 16- or 32-bit numbers to 8 bits and a scale each, q[m][k] = x[m][k] / scales[m]
+ * to the nearest, ties to even, at most 127 in size; scales[m] = max_k |x[m][k]| times
+ * 1/127, a float and a product of 32 bits; the quotient is taken without rounding. A row
+ * of zeros has the scale 0; one with a number that is not finite zeros and the scale NaN,
+ * which makes its row of the product NaN. K at most 65536. Strides in elements; q and its
+ * stride multiples of 16. */
+int tsac_hip_quantize_tokens(const void* x, size_t x_stride, int type, size_t rows, size_t K, int8_t* q,
+                             size_t q_stride, float* scales, void* stream);
+
+/* The product of M rows q [M][K] (stride and address multiples of 16; what stands behind
+ * the K-th byte, up to the next multiple of 16, is read and does not matter) to y [M][N]
+ * of `type` (FP32 too), strides in elements. Sums are exact, so that a row's result is
+ * the same in every batch. The linear's own device has to be current. Workspace: at least
+ * tsac_hip_channel_linear_workspace bytes of device memory, 16-byte aligned, not shared
+ * by calls that overlap. */
+size_t tsac_hip_channel_linear_workspace(const tsac_hip_channel_linear* linear, size_t M);
+int tsac_hip_channel_linear_apply(const tsac_hip_channel_linear* linear, const int8_t* q, size_t q_stride,
+                                  const float* token_scales, size_t M, void* y, size_t y_stride, int type,
+                                  void* workspace, size_t workspace_bytes, void* stream);
+
+/* u = scale * gate * post(input); s = residual + u; out = norm(s), with
+ * rms(x) = x / sqrt(mean x^2 + epsilon) * gain + bias and layer(x) = rms of x less its mean,
+ * for each row of `width` (1 to 65536) elements. A member that is NULL or TSAC_HIP_NORM_NONE
+ * leaves its part out. input, gains, biases, gate and out are of `type` (BF16, FP16, FP32),
+ * residual and sum of residual_type, which is `type` or FP32. Where out_scales is given, out
+ * is int8 [rows][width] and quantised as by tsac_hip_quantize_tokens. out is the norm of s
+ * as it is in 32 bits, before it is rounded for `sum`. sum may be the residual, sum or out
+ * the input, of the same type and stride; nothing else may overlap. Strides in elements. */
+#define TSAC_HIP_NORM_NONE 0
+#define TSAC_HIP_NORM_RMS 1
+#define TSAC_HIP_NORM_LAYER 2
+typedef struct tsac_hip_block_rows
+{
+    size_t rows, width;
+    int32_t type, residual_type;
+    const void* input;
+    size_t input_stride;
+    int32_t post; /* TSAC_HIP_NORM_* */
+    const void* post_gain; /* [width] */
+    const void* post_bias;
+    const void* gate; /* [rows][width] or, of stride 0, [width] */
+    size_t gate_stride;
+    float scale;
+    const void* residual;
+    size_t residual_stride;
+    void* sum;
+    size_t sum_stride;
+    int32_t norm;
+    const void* gain;
+    const void* bias;
+    float epsilon;
+    void* out;
+    size_t out_stride;
+    float* out_scales; /* [rows] */
+} tsac_hip_block_rows;
+int tsac_hip_block_norm(const tsac_hip_block_rows* rows, void* stream);
+
+/* Frequencies of rotated positions, in radians a position, for the pairs of `rotary` elements (even, 2 to
+ * 128) of a head: f[i] = base^(-2 i / rotary), host memory [rotary / 2]. scaling: NONE; LINEAR, divided by
+ * factor; BASE, of a base times factor^(rotary / (rotary - 2)) (rotary above 2), which leaves the first as it is and divides
+ * the last; TURNS, those of at most `slow` turns over `context` positions divided by factor, those of at
+ * least `fast` as they are, others between the two in proportion to their turns. */
+#define TSAC_HIP_ROTARY_NONE 0
+#define TSAC_HIP_ROTARY_LINEAR 1
+#define TSAC_HIP_ROTARY_BASE 2
+#define TSAC_HIP_ROTARY_TURNS 3
+int tsac_hip_rotary_frequencies(size_t rotary, double base, int scaling, double factor, double context, double slow,
+                                double fast, double* frequencies);
+
+/* tsac_hip_pages_write of one layer with rotated keys, and the rotated queries of the same rows: of each head the
+ * pairs (i, i + rotary / 2) or, interleaved, (2 i, 2 i + 1) of its first `rotary` (even) elements are turned by
+ * position * frequencies[i] (device, 64-bit: angles of far positions) and taken times amplitude. A row's position is
+ * positions[row] or, with NULL, the sequence's length and how far the row is down its line: the bits of its
+ * mask [rows][words] (tsac_hip_tree_mask) less 1 or, with NULL too, its place in the sequence. query and out
+ * [rows][heads][head_width] of the cache's type, at their strides; out may be query. heads may be 0. A row that has
+ * no page is not written (INVALID), its query is; rows past max_rows of a sequence and of no sequence are left. */
+typedef struct tsac_hip_rotary_rows
+{
+    const void* query;
+    size_t query_stride;
+    void* out;
+    size_t out_stride;
+    size_t heads;
+    const void* keys;
+    const void* values;
+    size_t row_stride; /* of keys and values */
+    size_t rows, max_rows;
+    const int32_t* starts;
+    const int32_t* positions;
+    const uint64_t* mask;
+    size_t words;
+    const double* frequencies;
+    size_t rotary;
+    int32_t interleaved;
+    float amplitude;
+} tsac_hip_rotary_rows;
+int tsac_hip_pages_append(const tsac_hip_paged_cache* cache, uint32_t layer, const tsac_hip_rotary_rows* rows,
+                          int32_t* status, void* stream);
+
+/* Rules on the logits of rows starts[s] .. starts[s+1]-1 of sequence s, in this order; device memory, every
+ * pointer but starts may be NULL. A token was had if it is among the first history_lengths[s] of history[s]
+ * or, with `tokens`, is that of a node on the row's line: rows of its sequence whose bit is set in
+ * mask[row][words] or, with mask NULL, the row itself and those in front of it. Its count leaves out the first
+ * prompt_lengths[s] of the history.
+ *   repetition[s] r: a token that was had, x > 0 ? x / r : x r
+ *   frequency[s], presence[s]: x - frequency * count, and - presence where the count is not 0
+ *   bias_values[i] for i from bias_starts[s] to bias_starts[s+1]: added to token bias_tokens[i]; of a token
+ *     that is listed twice the last one
+ *   allowed: bit t % 32 of word t / 32 of a row's, allowed_stride words apart (0: one for all rows); a token
+ *     without it is -infinity, whatever its logit
+ *   temperature[s] (probabilities only; NULL: 1)
+ * Tokens out of range are passed over, lengths are taken as 0 to what there is room for. */
+typedef struct tsac_hip_logit_rules
+{
+    const int32_t* starts; /* [sequences + 1], ascending */
+    size_t sequences;
+    const int32_t* history; /* [sequences][history_stride] */
+    size_t history_stride;
+    const int32_t* history_lengths;
+    const int32_t* prompt_lengths;
+    const int32_t* tokens; /* [rows] */
+    const uint64_t* mask;
+    size_t words;
+    const float* repetition;
+    const float* presence;
+    const float* frequency;
+    const int32_t* bias_starts; /* [sequences + 1] */
+    const int32_t* bias_tokens; /* [biases] */
+    const float* bias_values;
+    size_t biases;
+    const uint32_t* allowed;
+    size_t allowed_stride;
+    const float* temperature;
+} tsac_hip_logit_rules;
+
+/* out [rows][alphabet] of out_type = the logits of `type` (FP32 too) under the rules or, with `probabilities`, their
+ * softmax (x - max) / temperature. A temperature of 0 (or below) gives 1 to the lowest token of the largest x. A
+ * row in which nothing is above -infinity is 0; one with an allowed NaN is NaN, and so is one with +infinity at a temperature
+ * above 0. out may be the logits, of the same type and stride; rows of no sequence are left as they were. At
+ * most 2^20 tokens. Workspace as for tsac_hip_channel_linear_apply. */
+size_t tsac_hip_adjust_logits_workspace(size_t rows, size_t alphabet);
+int tsac_hip_adjust_logits(const void* logits, size_t stride, int type, size_t rows, size_t alphabet,
+                           const tsac_hip_logit_rules* rules, int probabilities, void* out, size_t out_stride,
+                           int out_type, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- calibration (no counterpart in the reference) ------------------------- */
 
 /* The attainable rates roofline fractions are read against, for benchmarks on

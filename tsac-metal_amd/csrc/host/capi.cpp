@@ -1,6 +1,7 @@
 // C ABI of the probability model (include/tsac_hip.h). Exceptions stop here and
 // become a nonzero status plus a thread-local message.
 #include "../../../include/tsac_hip.h"
+#include "../kernels/model_step.hpp"
 #include "../kernels/paged.hpp"
 #include "audio.hpp"
 #include "runtime.hpp"
@@ -8,11 +9,13 @@
 #include "wave.hpp"
 
 #include <algorithm>
+#include <cmath>
 #include <cstdlib>
 #include <cstring>
 #include <map>
 #include <mutex>
 #include <new>
+#include <numbers>
 #include <optional>
 #include <utility>
 
@@ -682,7 +685,56 @@ Drafts drafts_of(std::size_t sequences, std::size_t max_nodes, std::size_t alpha
     d.max_nodes = int(max_nodes);
     return d;
 }
+Type value_type(int type, const char* message)
+{
+    require(type >= TSAC_HIP_TYPE_BF16 && type <= TSAC_HIP_TYPE_FP32, message);
+    return type == TSAC_HIP_TYPE_BF16 ? Type::bf16 : type == TSAC_HIP_TYPE_FP16 ? Type::half : Type::single;
+}
+
+// Elements at multiples of their size, rows apart.
+void require_rows(const void* pointer, std::size_t stride, std::size_t rows, std::size_t width, Type type,
+                  const char* message)
+{
+    const std::size_t size = type == Type::single ? 4 : 2;
+    require(reinterpret_cast<std::uintptr_t>(pointer) % size == 0 && (rows <= 1 || stride >= width) &&
+                stride < (std::size_t(1) << 40),
+            message);
+}
+
+void require_token_rows(const int8_t* q, std::size_t stride, std::size_t rows, std::size_t width, const char* message)
+{
+    require(reinterpret_cast<std::uintptr_t>(q) % 16 == 0 && stride % 16 == 0 && (rows <= 1 || stride >= width) &&
+                stride < (std::size_t(1) << 40),
+            message);
+}
+
+NormRule norm_rule(int32_t norm, const void* gain, const void* bias)
+{
+    require(norm >= TSAC_HIP_NORM_NONE && norm <= TSAC_HIP_NORM_LAYER, "block norm: invalid norm");
+    return NormRule{norm == TSAC_HIP_NORM_NONE  ? Norm::none
+                    : norm == TSAC_HIP_NORM_RMS ? Norm::rms
+                                                : Norm::layer,
+                    gain, bias};
+}
+
+LogitRows logit_rows(std::size_t rows, std::size_t alphabet, bool probabilities)
+{
+    require(rows < max_new_rows, "logits: too many rows");
+    require(alphabet > 0 && alphabet <= max_alphabet_tokens, "logits: alphabets of 1 to 2^20 tokens");
+    LogitRows r;
+    r.rows = int(rows);
+    r.alphabet = int(alphabet);
+    r.probabilities = probabilities;
+    return r;
+}
 } // namespace
+
+struct tsac_hip_channel_linear
+{
+    DeviceBuffer values, constants;
+    ChannelWeights weights;
+    int device = 0;
+};
 
 extern "C"
 {
@@ -1602,6 +1654,321 @@ int tsac_hip_verify_drafts(const void* target, size_t target_stride, const void*
             d.accepted = accepted;
             d.next = next;
             verify_drafts(d, workspace, workspace_bytes, as_stream(stream));
+        });
+}
+
+int tsac_hip_channel_linear_create(const int8_t* values, const float* scales, const float* bias, size_t K, size_t N,
+                                   void* stream, tsac_hip_channel_linear** linear)
+{
+    return guarded(
+        [&]
+        {
+            require(values && scales && linear, "missing argument");
+            require(K > 0 && K <= channel_linear_max_inputs && N > 0 && N <= channel_linear_max_outputs,
+                    "channel linear: 1 to 131071 inputs, 1 to 2^24 outputs");
+            const hipStream_t s = as_stream(stream);
+            hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+            check_hip(hipStreamIsCapturing(s, &capture), "hipStreamIsCapturing");
+            require(capture == hipStreamCaptureStatusNone, "channel linear: a linear cannot be made in a capture");
+            auto l = std::make_unique<tsac_hip_channel_linear>();
+            check_hip(hipGetDevice(&l->device), "hipGetDevice");
+            l->values = DeviceBuffer(channel_tiles_bytes(K, N));
+            const std::size_t constant = (N * 4 + 255) / 256 * 256;
+            l->constants = DeviceBuffer(2 * constant);
+            const DeviceBuffer canonical(N * K);
+            auto* c = l->constants.as<uint8_t>();
+            hipError_t e = hipMemcpyAsync(canonical.get(), values, N * K, hipMemcpyDefault, s);
+            e = e != hipSuccess ? e : hipMemcpyAsync(c, scales, N * 4, hipMemcpyDefault, s);
+            e = e != hipSuccess || !bias ? e : hipMemcpyAsync(c + constant, bias, N * 4, hipMemcpyDefault, s);
+            if (e == hipSuccess)
+            {
+                channel_tiles(canonical.as<int8_t>(), K, N, l->values.as<int8_t>(), s);
+            }
+            // Waited for in any case: what has been queued uses the buffers.
+            const hipError_t waited = hipStreamSynchronize(s);
+            check_hip(e, "upload");
+            check_hip(waited, "upload");
+            l->weights.values = l->values.as<int8_t>();
+            l->weights.scales = reinterpret_cast<const float*>(c);
+            l->weights.bias = bias ? reinterpret_cast<const float*>(c + constant) : nullptr;
+            l->weights.inputs = int(K);
+            l->weights.outputs = int(N);
+            *linear = l.release();
+        });
+}
+
+void tsac_hip_channel_linear_destroy(tsac_hip_channel_linear* linear)
+{
+    delete linear;
+}
+
+int tsac_hip_quantize_tokens(const void* x, size_t x_stride, int type, size_t rows, size_t K, int8_t* q,
+                             size_t q_stride, float* scales, void* stream)
+{
+    return guarded(
+        [&]
+        {
+            require((x && q && scales) || !rows, "missing argument");
+            require(rows < max_new_rows && K > 0 && K <= max_norm_width, "quantize tokens: size out of range");
+            BlockRows r;
+            r.type = r.residual_type = value_type(type, "quantize tokens: invalid type");
+            require_rows(x, x_stride, rows, K, r.type, "quantize tokens: rows overlap or are misaligned");
+            require_token_rows(q, q_stride, rows, K, "quantize tokens: rows of q must be 16-byte aligned and apart");
+            r.rows = int(rows);
+            r.width = int(K);
+            r.input = x;
+            r.input_stride = x_stride;
+            r.out = q;
+            r.out_stride = q_stride;
+            r.out_scales = scales;
+            block_norm(r, as_stream(stream));
+        });
+}
+
+size_t tsac_hip_channel_linear_workspace(const tsac_hip_channel_linear* linear, size_t M)
+{
+    size_t bytes = 0;
+    guarded(
+        [&]
+        {
+            require(linear && M < max_new_rows, "channel linear: size out of range");
+            bytes = channel_linear_workspace(linear->weights, M);
+        });
+    return bytes;
+}
+
+int tsac_hip_channel_linear_apply(const tsac_hip_channel_linear* linear, const int8_t* q, size_t q_stride,
+                                  const float* token_scales, size_t M, void* y, size_t y_stride, int type,
+                                  void* workspace, size_t workspace_bytes, void* stream)
+{
+    return guarded(
+        [&]
+        {
+            require(linear && ((q && token_scales && y) || !M), "missing argument");
+            require(M < max_new_rows, "channel linear: too many rows");
+            int device = 0;
+            check_hip(hipGetDevice(&device), "hipGetDevice");
+            require(device == linear->device, "channel linear: made on another device");
+            ChannelRows r;
+            r.type = value_type(type, "channel linear: invalid type");
+            require_token_rows(q, q_stride, M, std::size_t(linear->weights.inputs),
+                               "channel linear: rows of q must be 16-byte aligned and apart");
+            require_rows(y, y_stride, M, std::size_t(linear->weights.outputs), r.type,
+                         "channel linear: rows of y overlap or are misaligned");
+            require(reinterpret_cast<std::uintptr_t>(workspace) % 16 == 0,
+                    "channel linear: the workspace must be 16-byte aligned");
+            r.q = q;
+            r.q_stride = q_stride;
+            r.scales = token_scales;
+            r.out = y;
+            r.out_stride = y_stride;
+            r.rows = int(M);
+            channel_linear(linear->weights, r, workspace, workspace_bytes, as_stream(stream));
+        });
+}
+
+int tsac_hip_block_norm(const tsac_hip_block_rows* rows, void* stream)
+{
+    return guarded(
+        [&]
+        {
+            require(rows != nullptr, "missing argument");
+            const tsac_hip_block_rows& b = *rows;
+            require(b.rows < max_new_rows && b.width > 0 && b.width <= max_norm_width, "block norm: size out of range");
+            BlockRows r;
+            r.type = value_type(b.type, "block norm: invalid type");
+            r.residual_type = value_type(b.residual_type, "block norm: invalid type");
+            require(r.residual_type == r.type || r.residual_type == Type::single,
+                    "block norm: the residual is of the same type or FP32");
+            require(b.input || !b.rows, "missing argument");
+            require(b.out || !b.out_scales, "block norm: scales of no output");
+            const char* const message = "block norm: rows overlap or are misaligned";
+            require_rows(b.input, b.input_stride, b.rows, b.width, r.type, message);
+            require_rows(b.gate, b.gate_stride, b.gate_stride ? b.rows : 0, b.width, r.type, message);
+            require_rows(b.residual, b.residual_stride, b.residual ? b.rows : 0, b.width, r.residual_type, message);
+            require_rows(b.sum, b.sum_stride, b.sum ? b.rows : 0, b.width, r.residual_type, message);
+            for (const void* p : {b.post_gain, b.post_bias, b.gain, b.bias})
+            {
+                require_rows(p, 0, 0, b.width, r.type, message);
+            }
+            if (b.out_scales)
+            {
+                require_token_rows(static_cast<const int8_t*>(b.out), b.out_stride, b.rows, b.width,
+                                   "block norm: rows of 8 bits must be 16-byte aligned and apart");
+            }
+            else
+            {
+                require_rows(b.out, b.out_stride, b.out ? b.rows : 0, b.width, r.type, message);
+            }
+            r.rows = int(b.rows);
+            r.width = int(b.width);
+            r.input = b.input;
+            r.input_stride = b.input_stride;
+            r.post = norm_rule(b.post, b.post_gain, b.post_bias);
+            r.gate = b.gate;
+            r.gate_stride = b.gate_stride;
+            r.scale = b.scale;
+            r.residual = b.residual;
+            r.residual_stride = b.residual_stride;
+            r.sum = b.sum;
+            r.sum_stride = b.sum_stride;
+            r.norm = norm_rule(b.norm, b.gain, b.bias);
+            r.epsilon = b.epsilon;
+            r.out = b.out;
+            r.out_stride = b.out_stride;
+            r.out_scales = b.out_scales;
+            block_norm(r, as_stream(stream));
+        });
+}
+
+int tsac_hip_rotary_frequencies(size_t rotary, double base, int scaling, double factor, double context, double slow,
+                                double fast, double* frequencies)
+{
+    return guarded(
+        [&]
+        {
+            require(frequencies != nullptr, "missing argument");
+            require(rotary >= 2 && rotary <= 128 && rotary % 2 == 0, "rotary: an even number of elements, 2 to 128");
+            require(scaling >= TSAC_HIP_ROTARY_NONE && scaling <= TSAC_HIP_ROTARY_TURNS, "rotary: invalid scaling");
+            require(std::isfinite(base) && base > 0, "rotary: the base must be above 0");
+            require(scaling == TSAC_HIP_ROTARY_NONE || (std::isfinite(factor) && factor > 0),
+                    "rotary: the factor must be above 0");
+            require(scaling != TSAC_HIP_ROTARY_BASE || rotary > 2, "rotary: one pair has no base to scale");
+            require(scaling != TSAC_HIP_ROTARY_TURNS ||
+                        (std::isfinite(context) && context > 0 && slow >= 0 && slow < fast && std::isfinite(fast)),
+                    "rotary: a context above 0, and fewer slow turns than fast ones");
+            const double width = double(rotary);
+            const double b = scaling == TSAC_HIP_ROTARY_BASE ? base * std::pow(factor, width / (width - 2)) : base;
+            for (std::size_t i = 0; i < rotary / 2; ++i)
+            {
+                double f = std::pow(b, -2.0 * double(i) / width);
+                if (scaling == TSAC_HIP_ROTARY_LINEAR)
+                {
+                    f /= factor;
+                }
+                else if (scaling == TSAC_HIP_ROTARY_TURNS)
+                {
+                    const double turns = context * f / (2 * std::numbers::pi);
+                    const double keep = std::clamp((turns - slow) / (fast - slow), 0.0, 1.0);
+                    f *= keep + (1 - keep) / factor;
+                }
+                frequencies[i] = f;
+            }
+        });
+}
+
+int tsac_hip_pages_append(const tsac_hip_paged_cache* cache, uint32_t layer, const tsac_hip_rotary_rows* rows,
+                          int32_t* status, void* stream)
+{
+    return guarded(
+        [&]
+        {
+            const PagedCache c = paged_cache_of(cache);
+            require(rows != nullptr, "missing argument");
+            const tsac_hip_rotary_rows& a = *rows;
+            require(layer < unsigned(c.layers), "pages append: layer out of range");
+            require(a.rows < max_new_rows && a.max_rows < max_new_rows, "pages append: too many rows in one call");
+            require(a.heads <= 65536, "pages append: too many heads");
+            require(a.rotary >= 2 && a.rotary <= std::size_t(c.head_width) && a.rotary % 2 == 0,
+                    "pages append: an even number of rotated elements, at most a head's");
+            require(a.starts && a.frequencies && ((a.keys && a.values) || !a.rows) &&
+                        ((a.query && a.out) || !a.rows || !a.heads),
+                    "missing argument");
+            require(!a.positions || !a.mask, "pages append: positions or a mask, not both");
+            require(!a.mask || (a.words > 0 && a.words <= 1024), "pages append: 1 to 1024 mask words a row");
+            const std::size_t wide = a.heads * std::size_t(c.head_width), row = std::size_t(c.heads) * c.head_width;
+            require_aligned(a.keys, a.row_stride, "pages append: rows must be 16-byte aligned");
+            require_aligned(a.values, a.row_stride, "pages append: rows must be 16-byte aligned");
+            require(a.rows <= 1 || a.row_stride >= row, "pages append: rows overlap");
+            if (a.heads)
+            {
+                require_aligned(a.query, a.query_stride, "pages append: rows must be 16-byte aligned");
+                require_aligned(a.out, a.out_stride, "pages append: rows must be 16-byte aligned");
+                require(a.rows <= 1 || (a.query_stride >= wide && a.out_stride >= wide), "pages append: rows overlap");
+            }
+            RotaryRows r;
+            r.query = static_cast<const uint16_t*>(a.query);
+            r.query_stride = a.query_stride;
+            r.out = static_cast<uint16_t*>(a.out);
+            r.out_stride = a.out_stride;
+            r.heads = int(a.heads);
+            r.keys = static_cast<const uint16_t*>(a.keys);
+            r.values = static_cast<const uint16_t*>(a.values);
+            r.row_stride = a.row_stride;
+            r.rows = int(a.rows);
+            r.max_rows = int(std::min(a.rows, a.max_rows));
+            r.starts = a.starts;
+            r.positions = a.positions;
+            r.mask = a.mask;
+            r.words = a.words;
+            r.frequencies = a.frequencies;
+            r.rotary = int(a.rotary);
+            r.interleaved = a.interleaved != 0;
+            r.amplitude = a.amplitude;
+            pages_append(c, int(layer), r, status, as_stream(stream));
+        });
+}
+
+size_t tsac_hip_adjust_logits_workspace(size_t rows, size_t alphabet)
+{
+    size_t bytes = 0;
+    guarded([&] { bytes = logits_workspace(logit_rows(rows, alphabet, true)); });
+    return bytes;
+}
+
+int tsac_hip_adjust_logits(const void* logits, size_t stride, int type, size_t rows, size_t alphabet,
+                           const tsac_hip_logit_rules* rules, int probabilities, void* out, size_t out_stride,
+                           int out_type, void* workspace, size_t workspace_bytes, void* stream)
+{
+    return guarded(
+        [&]
+        {
+            LogitRows r = logit_rows(rows, alphabet, probabilities != 0);
+            require(rules && ((logits && out) || !rows), "missing argument");
+            const tsac_hip_logit_rules& a = *rules;
+            require(a.starts != nullptr, "missing argument");
+            require(a.sequences <= std::size_t(max_sequences), "logits: too many sequences");
+            require(!a.history || (a.history_lengths && a.history_stride < (std::size_t(1) << 40)),
+                    "logits: a history needs its lengths");
+            require(!a.mask || (a.words > 0 && a.words <= std::size_t(1024)), "logits: 1 to 1024 mask words a row");
+            require(!a.bias_starts || ((a.bias_tokens && a.bias_values) || !a.biases), "logits: biases need tokens and values");
+            require(a.biases < (std::size_t(1) << 31), "logits: too many biases");
+            require(!a.allowed || !a.allowed_stride || a.allowed_stride >= (alphabet + 31) / 32,
+                    "logits: rows of allowed tokens overlap");
+            require(!a.temperature || probabilities, "logits: a temperature is that of probabilities");
+            r.type = value_type(type, "logits: invalid type");
+            r.out_type = value_type(out_type, "logits: invalid type");
+            require_rows(logits, stride, rows, alphabet, r.type, "logits: rows overlap or are misaligned");
+            require_rows(out, out_stride, rows, alphabet, r.out_type, "logits: rows overlap or are misaligned");
+            require(out != logits || (type == out_type && (rows <= 1 || stride == out_stride)),
+                    "logits: in place they are of one type and stride");
+            require(reinterpret_cast<std::uintptr_t>(workspace) % 16 == 0,
+                    "logits: the workspace must be 16-byte aligned");
+            r.logits = logits;
+            r.stride = stride;
+            r.out = out;
+            r.out_stride = out_stride;
+            LogitRules l;
+            l.starts = a.starts;
+            l.sequences = int(a.sequences);
+            l.history = a.history;
+            l.history_stride = a.history_stride;
+            l.history_lengths = a.history_lengths;
+            l.prompt_lengths = a.prompt_lengths;
+            l.tokens = a.tokens;
+            l.mask = a.mask;
+            l.words = a.words;
+            l.repetition = a.repetition;
+            l.presence = a.presence;
+            l.frequency = a.frequency;
+            l.bias_starts = a.bias_starts;
+            l.bias_tokens = a.bias_tokens;
+            l.bias_values = a.bias_values;
+            l.biases = int(a.biases);
+            l.allowed = a.allowed;
+            l.allowed_stride = a.allowed_stride;
+            l.temperature = a.temperature;
+            adjust_logits(r, l, workspace, workspace_bytes, as_stream(stream));
         });
 }
 

@@ -1,0 +1,326 @@
+// The rows between two blocks of a model, in one pass over them:
+//
+//   u = scale * gate * post(x)      s = residual + u      h = norm(s)
+//
+//   rms(x)   = x / sqrt(mean x^2 + epsilon) * gain + bias
+//   layer(x) = (x - m) / sqrt(mean (x - m)^2 + epsilon) * gain + bias,   m = mean x
+//
+// s leaves in the residual's type, h in 16 bits or, for a product of 8-bit integers, as whole numbers
+// q of 8 bits and a scale a row: scale = max |h| * fl(1 / 127), q = h / scale to the nearest, ties to even.
+// Nothing is rounded in between: h is the norm of the sum before it is rounded for its store.
+//
+// A row's values stay in the registers of its threads, so that the mean, the squares around it and
+// the largest value each are a pass over registers, in 32 bits and in an order that depends on the
+// width alone. What bounds it is memory; a row of few values one wave, which needs no barrier.
+#include "model_step.hpp"
+#include "values.hpp"
+
+namespace tsac_hip
+{
+namespace
+{
+constexpr int lanes = 64;
+
+template <int Threads, class Join> __device__ __forceinline__ float joined(float value, float* shared, Join join)
+{
+#pragma unroll
+    for (int step = 1; step < lanes; step *= 2)
+    {
+        value = join(value, __shfl_xor(value, step));
+    }
+    if constexpr (Threads > lanes)
+    {
+        __syncthreads(); // the last one's values have been read
+        if (threadIdx.x % lanes == 0)
+        {
+            shared[threadIdx.x / lanes] = value;
+        }
+        __syncthreads();
+        value = shared[0];
+#pragma unroll
+        for (int i = 1; i < Threads / lanes; ++i)
+        {
+            value = join(value, shared[i]);
+        }
+    }
+    return value;
+}
+
+template <int Threads> __device__ __forceinline__ float row_sum(float value, float* shared)
+{
+    return joined<Threads>(value, shared, [](float a, float b) { return a + b; });
+}
+
+// Of bit patterns without their signs, which order numbers, then infinities, then what is no number.
+template <int Threads> __device__ __forceinline__ unsigned row_max_bits(unsigned value, float* shared)
+{
+    return __float_as_uint(joined<Threads>(__uint_as_float(value), shared,
+                                           [](float a, float b)
+                                           {
+                                               const unsigned x = __float_as_uint(a), y = __float_as_uint(b);
+                                               return __uint_as_float(x > y ? x : y);
+                                           }));
+}
+
+template <Type T, int Vectors, int Threads>
+__device__ __forceinline__ void normalise(float (&v)[Vectors][8], const NormRule& rule, bool aligned, int width,
+                                          float epsilon, int thread, float* shared)
+{
+    if (rule.norm == Norm::none)
+    {
+        return;
+    }
+    float mean = 0.0f;
+    if (rule.norm == Norm::layer)
+    {
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < Vectors; ++i)
+        {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+            {
+                sum += v[i][e]; // 0 past the width
+            }
+        }
+        mean = row_sum<Threads>(sum, shared) / float(width);
+    }
+    float squares = 0.0f;
+#pragma unroll
+    for (int i = 0; i < Vectors; ++i)
+    {
+        const int count = width - 8 * (i * Threads + thread);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+        {
+            v[i][e] = e < count ? v[i][e] - mean : 0.0f;
+            squares = __builtin_fmaf(v[i][e], v[i][e], squares);
+        }
+    }
+    const float factor = 1.0f / __builtin_sqrtf(row_sum<Threads>(squares, shared) / float(width) + epsilon);
+#pragma unroll
+    for (int i = 0; i < Vectors; ++i)
+    {
+        const int at = 8 * (i * Threads + thread), count = width - at;
+        float gain[8], bias[8];
+        if (count > 0 && rule.gain)
+        {
+            load8<T>(static_cast<const value_t<T>*>(rule.gain) + at, count, aligned, 0.0f, gain);
+        }
+        if (count > 0 && rule.bias)
+        {
+            load8<T>(static_cast<const value_t<T>*>(rule.bias) + at, count, aligned, 0.0f, bias);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+        {
+            float x = v[i][e] * factor;
+            x = rule.gain ? x * gain[e] : x;
+            x = rule.bias ? x + bias[e] : x;
+            v[i][e] = e < count ? x : 0.0f;
+        }
+    }
+}
+
+// x / scale to the nearest whole number, a tie to the even one. The product with the reciprocal is off by
+// less than half a step, and x - r scale, which 24 bits hold, tells on which side of a border x is.
+__device__ __forceinline__ int nearest(float x, float scale, float reciprocal)
+{
+    float r = __builtin_rintf(x * reciprocal);
+    const float rest = __builtin_fmaf(-r, scale, x), half = 0.5f * scale;
+    const bool odd = int(r) & 1;
+    if (__builtin_fabsf(rest) > half || (__builtin_fabsf(rest) == half && odd))
+    {
+        r += __builtin_copysignf(1.0f, rest);
+    }
+    return int(__builtin_fminf(__builtin_fmaxf(r, -127.0f), 127.0f));
+}
+
+// Which pointers of a row's are at multiples of 16 bytes, with their strides.
+enum Aligned
+{
+    input_aligned = 1,
+    gate_aligned = 2,
+    residual_aligned = 4,
+    sum_aligned = 8,
+    out_aligned = 16,
+    post_aligned = 32,
+    norm_aligned = 64
+};
+
+// T: the values; R: the residual. A row is taken by Threads threads, each Vectors times eight values.
+template <Type T, Type R, int Vectors, int Threads>
+__global__ __launch_bounds__(Threads > 256 ? Threads : 256) void block_norm_kernel(BlockRows p, int aligned)
+{
+    constexpr int together = Threads < 256 ? 256 / Threads : 1; // rows of a workgroup
+    __shared__ float shared[Threads > lanes ? Threads / lanes : 1];
+    const int thread = threadIdx.x % Threads;
+    const int row = blockIdx.x * together + threadIdx.x / Threads;
+    if (row >= p.rows) // whole waves: a row of several has its workgroup for itself
+    {
+        return;
+    }
+    float v[Vectors][8];
+    const auto* x = static_cast<const value_t<T>*>(p.input) + std::size_t(row) * p.input_stride;
+#pragma unroll
+    for (int i = 0; i < Vectors; ++i)
+    {
+        const int at = 8 * (i * Threads + thread);
+        load8<T>(x + at, p.width - at, aligned & input_aligned, 0.0f, v[i]);
+    }
+    float before[Vectors][8];
+    const auto* residual = static_cast<const value_t<R>*>(p.residual) + std::size_t(row) * p.residual_stride;
+    if (p.residual)
+    {
+#pragma unroll
+        for (int i = 0; i < Vectors; ++i)
+        {
+            const int at = 8 * (i * Threads + thread);
+            load8<R>(residual + at, p.width - at, aligned & residual_aligned, 0.0f, before[i]);
+        }
+    }
+    normalise<T, Vectors, Threads>(v, p.post, aligned & post_aligned, p.width, p.epsilon, thread, shared);
+    const auto* gate = static_cast<const value_t<T>*>(p.gate) + std::size_t(row) * p.gate_stride;
+    auto* sum = static_cast<value_t<R>*>(p.sum) + std::size_t(row) * p.sum_stride;
+#pragma unroll
+    for (int i = 0; i < Vectors; ++i)
+    {
+        const int at = 8 * (i * Threads + thread), count = p.width - at;
+        float gates[8];
+        if (p.gate)
+        {
+            load8<T>(gate + at, count, aligned & gate_aligned, 0.0f, gates);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+        {
+            float u = p.gate ? v[i][e] * gates[e] : v[i][e];
+            u *= p.scale;
+            u = p.residual ? before[i][e] + u : u;
+            v[i][e] = e < count ? u : 0.0f;
+        }
+        if (p.sum && count > 0)
+        {
+            store8<R>(sum + at, count, aligned & sum_aligned, v[i]);
+        }
+    }
+    if (!p.out)
+    {
+        return;
+    }
+    normalise<T, Vectors, Threads>(v, p.norm, aligned & norm_aligned, p.width, p.epsilon, thread, shared);
+    if (!p.out_scales)
+    {
+        auto* out = static_cast<value_t<T>*>(p.out) + std::size_t(row) * p.out_stride;
+#pragma unroll
+        for (int i = 0; i < Vectors; ++i)
+        {
+            const int at = 8 * (i * Threads + thread), count = p.width - at;
+            if (count > 0)
+            {
+                store8<T>(out + at, count, aligned & out_aligned, v[i]);
+            }
+        }
+        return;
+    }
+    unsigned top = 0;
+#pragma unroll
+    for (int i = 0; i < Vectors; ++i)
+    {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+        {
+            const unsigned bits = __float_as_uint(v[i][e]) & 0x7fffffffu;
+            top = bits > top ? bits : top;
+        }
+    }
+    top = row_max_bits<Threads>(top, shared);
+    const bool finite = top < 0x7f800000u;
+    const float most = __uint_as_float(top), scale = most * (1.0f / 127.0f);
+    if (thread == 0)
+    {
+        p.out_scales[row] = finite ? scale : __uint_as_float(0x7fc00000u);
+    }
+    // Small rows are taken times 2^64, which changes no quotient, so that the reciprocal is finite and half
+    // the scale exact.
+    const float lift = most < 0x1p-60f ? 0x1p64f : 1.0f;
+    const float lifted = scale * lift, reciprocal = 1.0f / lifted;
+    const bool zero = !finite || scale == 0.0f;
+    auto* q = static_cast<int8_t*>(p.out) + std::size_t(row) * p.out_stride;
+#pragma unroll
+    for (int i = 0; i < Vectors; ++i)
+    {
+        const int at = 8 * (i * Threads + thread), count = p.width - at;
+        uint64_t packed = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+        {
+            const int n = zero ? 0 : nearest(v[i][e] * lift, lifted, reciprocal);
+            packed |= uint64_t(uint8_t(n)) << 8 * e;
+        }
+        if (count >= 8) // rows of 8-bit integers begin at multiples of 16 bytes
+        {
+            *reinterpret_cast<uint64_t*>(q + at) = packed;
+        }
+        else
+        {
+            for (int e = 0; e < count; ++e)
+            {
+                q[at + e] = int8_t(packed >> 8 * e);
+            }
+        }
+    }
+}
+
+template <Type T, Type R> void launch(const BlockRows& p, int aligned, hipStream_t stream)
+{
+    const auto go = [&](auto kernel, int threads)
+    {
+        const int together = threads < 256 ? 256 / threads : 1;
+        kernel<<<unsigned((p.rows + together - 1) / together), threads * together, 0, stream>>>(p, aligned);
+    };
+    // By the width alone, so that a row's result does not depend on how many there are.
+    const int w = p.width;
+    w <= 512      ? go(block_norm_kernel<T, R, 1, 64>, 64)
+    : w <= 1024   ? go(block_norm_kernel<T, R, 2, 64>, 64)
+    : w <= 2048   ? go(block_norm_kernel<T, R, 1, 256>, 256)
+    : w <= 4096   ? go(block_norm_kernel<T, R, 2, 256>, 256)
+    : w <= 8192   ? go(block_norm_kernel<T, R, 4, 256>, 256)
+    : w <= 16384  ? go(block_norm_kernel<T, R, 2, 1024>, 1024)
+    : w <= 32768  ? go(block_norm_kernel<T, R, 4, 1024>, 1024)
+                  : go(block_norm_kernel<T, R, 8, 1024>, 1024);
+    check_hip(hipGetLastError(), "block norm launch");
+}
+} // namespace
+
+void block_norm(const BlockRows& p, hipStream_t stream)
+{
+    require(p.width > 0 && std::size_t(p.width) <= max_norm_width, "block norm: width out of range");
+    if (!p.rows)
+    {
+        return;
+    }
+    const auto whole = [](const void* pointer, std::size_t stride, std::size_t size)
+    { return reinterpret_cast<std::uintptr_t>(pointer) % 16 == 0 && stride * size % 16 == 0; };
+    const std::size_t size = p.type == Type::single ? 4 : 2, wide = p.residual_type == Type::single ? 4 : 2;
+    int aligned = 0;
+    aligned |= whole(p.input, p.input_stride, size) ? input_aligned : 0;
+    aligned |= whole(p.gate, p.gate_stride, size) ? gate_aligned : 0;
+    aligned |= whole(p.residual, p.residual_stride, wide) ? residual_aligned : 0;
+    aligned |= whole(p.sum, p.sum_stride, wide) ? sum_aligned : 0;
+    aligned |= whole(p.out, p.out_stride, p.out_scales ? 1 : size) ? out_aligned : 0;
+    aligned |= whole(p.post.gain, 0, size) && whole(p.post.bias, 0, size) ? post_aligned : 0;
+    aligned |= whole(p.norm.gain, 0, size) && whole(p.norm.bias, 0, size) ? norm_aligned : 0;
+    const bool wider = p.residual_type == Type::single;
+    switch (p.type)
+    {
+    case Type::bf16:
+        return wider ? launch<Type::bf16, Type::single>(p, aligned, stream)
+                     : launch<Type::bf16, Type::bf16>(p, aligned, stream);
+    case Type::half:
+        return wider ? launch<Type::half, Type::single>(p, aligned, stream)
+                     : launch<Type::half, Type::half>(p, aligned, stream);
+    default: return launch<Type::single, Type::single>(p, aligned, stream);
+    }
+}
+} // namespace tsac_hip

@@ -4,7 +4,7 @@
 // ones, in the order of their list, from one workgroup that scans the counts: what a
 // sequence gets depends on the counts and the list alone, on no order of atomics and no
 // history of calls.
-#include "paged.hpp"
+#include "paged_device.hpp"
 
 #include <algorithm>
 
@@ -14,14 +14,6 @@ namespace
 {
 constexpr int most_threads = 1024; // of a workgroup that takes pages
 constexpr int scanned = 4;         // reference counts a thread reads at a time
-
-__device__ __forceinline__ void report(int* status, int what)
-{
-    if (status)
-    {
-        *status = what;
-    }
-}
 
 // Lanes below this one whose bit is set.
 __device__ __forceinline__ int lanes_below(uint64_t bits)
@@ -489,42 +481,6 @@ __global__ __launch_bounds__(copying_threads) void free_kernel(PagedCache cache,
             report(status, status_invalid);
         }
     }
-}
-
-// The page of a position that its sequence may write, -1 if there is none: covered by what the
-// sequence holds, and held by it alone.
-__device__ __forceinline__ int writable_page(const PagedCache& cache, int s, long long position)
-{
-    const long long index = position / cache.page_rows;
-    if (position < 0 || index >= cache.held[s] || std::size_t(index) >= cache.table_stride)
-    {
-        return -1;
-    }
-    const int page = cache.table[s * cache.table_stride + index];
-    return page >= 0 && page < cache.pages && cache.references[page] == 1 ? page : -1;
-}
-
-// A sequence's rows among `rows`, from the ascending starts.
-__device__ __forceinline__ int rows_of(const int* starts, int s, int rows, int& first)
-{
-    first = starts[s];
-    const int end = starts[s + 1] < rows ? starts[s + 1] : rows;
-    return first < 0 || end < first ? 0 : end - first;
-}
-
-// The last sequence that starts at or in front of a row, by a wave: 64 starts at a time.
-__device__ __forceinline__ int sequence_of(const int* starts, int sequences, int row)
-{
-    const int lane = threadIdx.x % 64;
-    int low = 0, high = sequences;
-    while (high - low > 1)
-    {
-        const int step = (high - low + 63) / 64, i = low + lane * step;
-        const uint64_t bits = __ballot(i < high && starts[i] <= row);
-        low += bits ? (63 - __builtin_clzll(bits)) * step : 0;
-        high = min(low + step, high);
-    }
-    return low;
 }
 
 // blockIdx: a row's place in its sequence, the sequence, the layer; or (`Find`) a row of all, 0, the layer. 64

@@ -44,12 +44,18 @@ EXPORTS = (
     "tsac_hip_pages_reserve", "tsac_hip_pages_fork", "tsac_hip_pages_free", "tsac_hip_pages_write",
     "tsac_hip_pages_keep", "tsac_hip_tree_mask", "tsac_hip_attention_paged_workspace", "tsac_hip_attention_paged",
     "tsac_hip_verify_drafts_workspace", "tsac_hip_verify_drafts",
+    "tsac_hip_channel_linear_create", "tsac_hip_channel_linear_destroy", "tsac_hip_quantize_tokens",
+    "tsac_hip_channel_linear_workspace", "tsac_hip_channel_linear_apply", "tsac_hip_block_norm",
+    "tsac_hip_rotary_frequencies", "tsac_hip_pages_append", "tsac_hip_adjust_logits_workspace",
+    "tsac_hip_adjust_logits",
 )
 
 PATH_AUTO, PATH_GEMV, PATH_GEMM, PATH_GEMM_TILES, PATH_SMALL = 0, 1, 2, 3, 4
 PASS_ENCODE, PASS_DECODE = 0, 1
 TYPE_BF16, TYPE_FP16, TYPE_FP32 = 0, 1, 2
 PAGES_INVALID, PAGES_EXHAUSTED = 1, 2
+NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
+ROTARY_NONE, ROTARY_LINEAR, ROTARY_BASE, ROTARY_TURNS = 0, 1, 2, 3
 
 
 class HipError(RuntimeError):
@@ -136,6 +142,28 @@ class PagedCacheDesc(C.Structure):
                 ("layers", C.c_uint32), ("pages", C.c_uint32), ("page_rows", C.c_uint32), ("heads", C.c_uint32),
                 ("head_width", C.c_uint32), ("type", C.c_int32), ("table", vp), ("table_stride", sz), ("held", vp),
                 ("lengths", vp), ("references", vp), ("sequences", C.c_uint32)]
+
+
+class BlockRows(C.Structure):
+    _fields_ = [("rows", sz), ("width", sz), ("type", C.c_int32), ("residual_type", C.c_int32), ("input", vp),
+                ("input_stride", sz), ("post", C.c_int32), ("post_gain", vp), ("post_bias", vp), ("gate", vp),
+                ("gate_stride", sz), ("scale", C.c_float), ("residual", vp), ("residual_stride", sz), ("sum", vp),
+                ("sum_stride", sz), ("norm", C.c_int32), ("gain", vp), ("bias", vp), ("epsilon", C.c_float), ("out", vp),
+                ("out_stride", sz), ("out_scales", vp)]
+
+
+class RotaryRows(C.Structure):
+    _fields_ = [("query", vp), ("query_stride", sz), ("out", vp), ("out_stride", sz), ("heads", sz), ("keys", vp),
+                ("values", vp), ("row_stride", sz), ("rows", sz), ("max_rows", sz), ("starts", vp), ("positions", vp),
+                ("mask", vp), ("words", sz), ("frequencies", vp), ("rotary", sz), ("interleaved", C.c_int32),
+                ("amplitude", C.c_float)]
+
+
+class LogitRules(C.Structure):
+    _fields_ = [("starts", vp), ("sequences", sz), ("history", vp), ("history_stride", sz), ("history_lengths", vp),
+                ("prompt_lengths", vp), ("tokens", vp), ("mask", vp), ("words", sz), ("repetition", vp), ("presence", vp),
+                ("frequency", vp), ("bias_starts", vp), ("bias_tokens", vp), ("bias_values", vp), ("biases", sz),
+                ("allowed", vp), ("allowed_stride", sz), ("temperature", vp)]
 
 
 def header(frames, batch, groups, codebooks, model_channels=2, method=1) -> Header:
@@ -235,6 +263,21 @@ def library() -> C.CDLL:
         lib.tsac_hip_verify_drafts_workspace.restype = sz
         lib.tsac_hip_verify_drafts.argtypes = [vp, sz, vp, sz, C.c_int, sz, sz, vp, vp, vp, sz, sz, vp, vp, vp, vp, vp,
                                                vp, sz, vp]
+        lib.tsac_hip_channel_linear_create.argtypes = [vp, vp, vp, sz, sz, vp, C.POINTER(vp)]
+        lib.tsac_hip_channel_linear_destroy.argtypes = [vp]
+        lib.tsac_hip_channel_linear_destroy.restype = None
+        lib.tsac_hip_quantize_tokens.argtypes = [vp, sz, C.c_int, sz, sz, vp, sz, vp, vp]
+        lib.tsac_hip_channel_linear_workspace.argtypes = [vp, sz]
+        lib.tsac_hip_channel_linear_workspace.restype = sz
+        lib.tsac_hip_channel_linear_apply.argtypes = [vp, vp, sz, vp, sz, vp, sz, C.c_int, vp, sz, vp]
+        lib.tsac_hip_block_norm.argtypes = [C.POINTER(BlockRows), vp]
+        lib.tsac_hip_rotary_frequencies.argtypes = [sz, C.c_double, C.c_int, C.c_double, C.c_double, C.c_double, C.c_double,
+                                                    vp]
+        lib.tsac_hip_pages_append.argtypes = [cache, C.c_uint32, C.POINTER(RotaryRows), vp, vp]
+        lib.tsac_hip_adjust_logits_workspace.argtypes = [sz, sz]
+        lib.tsac_hip_adjust_logits_workspace.restype = sz
+        lib.tsac_hip_adjust_logits.argtypes = [vp, sz, C.c_int, sz, sz, C.POINTER(LogitRules), C.c_int, vp, sz, C.c_int, vp,
+                                               sz, vp]
         _lib = lib
     return _lib
 
@@ -856,7 +899,7 @@ def _need(condition, message):
         raise HipError(message)
 
 
-_INT, _FLOAT, _LONG = "torch.int32", "torch.float32", "torch.int64"
+_INT, _FLOAT, _LONG, _DOUBLE = "torch.int32", "torch.float32", "torch.int64", "torch.float64"
 #: Element types by dtype; int16 holds BF16 bits, as in the other operators.
 _ROW_TYPES = {"torch.bfloat16": TYPE_BF16, "torch.int16": TYPE_BF16, "torch.float16": TYPE_FP16}
 _PROBABILITY_TYPES = dict(_ROW_TYPES, **{"torch.float32": TYPE_FP32})
@@ -981,6 +1024,30 @@ class PagedCache:
             strides[1] if rows > 1 else heads * width, rows, self._ints(starts, self.sequences + 1, "starts"), max_rows,
             self._status(status), _current(self.device)))
 
+    def append(self, layer, query, keys, values, starts, max_rows, frequencies, out, interleaved=False, amplitude=1.0,
+               positions=None, mask=None, status=None):
+        """New rows of one layer behind each sequence's length, keys [rows][heads][head_width] rotated, and the
+        rows' queries [rows][query heads][head_width] rotated to out (which may be query). frequencies: float64
+        [pairs], radians a position (rotary_frequencies). Positions: positions int32 [rows], or down the lines of mask
+        int64 [rows][words] (tree_mask), or one after the other."""
+        device, rows, heads, width = self.device, query.shape[0], query.shape[1], self.head_width
+        q, q_stride = _rows(query, device, heads, width, self.type, "query")
+        o, o_stride = _rows(out, device, heads, width, self.type, "out")
+        k, stride = _rows(keys, device, self.heads, width, self.type, "keys")
+        v, v_stride = _rows(values, device, self.heads, width, self.type, "values")
+        if out.shape[0] != rows or keys.shape[0] != rows or values.shape[0] != rows or stride != v_stride:
+            raise HipError("query, out, keys and values: as many rows, keys and values laid out alike")
+        if mask is not None and mask.dim() != 2:
+            raise HipError("mask: must be [rows][words]")
+        words, pairs = 0 if mask is None else mask.shape[1], frequencies.numel()
+        desc = RotaryRows(
+            q, q_stride, o, o_stride, heads, k, v, stride, rows, max_rows,
+            self._ints(starts, self.sequences + 1, "starts"),
+            None if positions is None else self._ints(positions, rows, "positions"),
+            None if mask is None else _array(mask, device, _LONG, rows * words, "mask"), words,
+            _array(frequencies, device, _DOUBLE, pairs, "frequencies"), 2 * pairs, interleaved, amplitude)
+        check(library().tsac_hip_pages_append(self._desc, layer, C.byref(desc), self._status(status), _current(device)))
+
     def keep(self, starts, path, accepted, lengths=None, status=None):
         """Moves each sequence's accepted rows (path [sequences][nodes], accepted) to the front of the
         new ones, in every layer; lengths (the cache's own, if None) takes the new lengths."""
@@ -1064,6 +1131,175 @@ def verify_drafts(target, draft, tokens, parents, starts, max_nodes, uniforms, d
         _array(uniforms, device, _FLOAT, rows, "uniforms"), _array(draws, device, _FLOAT, sequences, "draws"),
         _array(path, device, _INT, sequences * max_nodes, "path"), _array(accepted, device, _INT, sequences, "accepted"),
         _array(next, device, _INT, sequences, "next"), space, size, _current(device)))
+    del keep
+
+
+# ---------------------------------------------------------------- a model's step around the paged attention
+
+_VALUE_TYPES = _PROBABILITY_TYPES
+
+
+def _matrix(tensor, device, rows, width, name, types=_VALUE_TYPES):
+    """(address, row stride, type) of [rows][width], the elements of a row one after the other."""
+    shape, strides, type_ = tensor.shape, tensor.stride(), types.get(_kind(tensor))
+    if tensor.device != device or type_ is None:
+        raise HipError(f"{name}: another device or type")
+    if len(shape) != 2 or shape[0] != rows or shape[1] != width or (rows and width > 1 and strides[1] != 1):
+        raise HipError(f"{name}: must be [{rows}][{width}], rows contiguous")
+    return tensor.data_ptr(), strides[0] if rows > 1 else -(-width // 16) * 16, type_
+
+
+_BYTES = {"torch.int8": 3}
+
+
+class ChannelLinear:
+    """A projection of 8-bit integers with a scale for each output: values int8 [N][K], scales float32 [N] and bias
+    float32 [N] or None, numpy arrays or tensors on the host or the current device."""
+
+    def __init__(self, values, scales, bias=None):
+        import torch
+
+        values, scales, bias = (torch.from_numpy(a) if isinstance(a, np.ndarray) else a for a in (values, scales, bias))
+        _need(values.dim() == 2 and _kind(values) == "torch.int8", "values: must be int8 [outputs][inputs]")
+        self.N, self.K = values.shape
+        for name, t in (("scales", scales), ("bias", bias)):
+            _need(t is None or (_kind(t) == _FLOAT and t.shape == (self.N,)), f"{name}: must be float32 [outputs]")
+        _need(scales is not None, "scales: missing")
+        parts = [None if t is None else t.contiguous() for t in (values, scales, bias)]
+        for t in parts:
+            if t is not None and t.device.type != "cpu":
+                _current(t.device)
+        handle = vp()
+        check(library().tsac_hip_channel_linear_create(*(None if t is None else t.data_ptr() for t in parts), self.K, self.N,
+                                                       _stream(None), C.byref(handle)))
+        self.handle, self._library = handle, library()
+        self._workspaces = {}  # bytes by rows
+
+    def __del__(self, release=_release):  # bound now: module globals are cleared at shutdown
+        release(self, "tsac_hip_channel_linear_destroy")
+
+    def workspace(self, rows) -> int:
+        """Bytes that apply() needs for as many rows."""
+        need = self._workspaces.get(rows)
+        if need is None:
+            if len(self._workspaces) >= 1024:
+                self._workspaces.clear()
+            need = self._workspaces[rows] = int(library().tsac_hip_channel_linear_workspace(self.handle, rows))
+        return need
+
+    def apply(self, q, scales, out, workspace=None):
+        """q int8 [rows][K] and its scales float32 [rows] (quantize_tokens, block_norm) to out [rows][N]. A new
+        workspace a call, if none is given and one is needed."""
+        device, rows = q.device, q.shape[0]
+        a, a_stride, _ = _matrix(q, device, rows, self.K, "q", _BYTES)
+        o, o_stride, type_ = _matrix(out, device, rows, self.N, "out")
+        space, size, keep = _workspace(self.workspace(rows), workspace, device)
+        check(library().tsac_hip_channel_linear_apply(
+            self.handle, a, a_stride, _array(scales, device, _FLOAT, rows, "scales"), rows, o, o_stride, type_, space, size,
+            _current(device)))
+        del keep
+
+
+def quantize_tokens(x, q, scales):
+    """Rows of x to 8 bits, q int8 [rows][K] at a stride of a multiple of 16, and a scale each, float32 [rows]."""
+    device, (rows, width) = x.device, x.shape
+    a, a_stride, type_ = _matrix(x, device, rows, width, "x")
+    o, o_stride, _ = _matrix(q, device, rows, width, "q", _BYTES)
+    check(library().tsac_hip_quantize_tokens(a, a_stride, type_, rows, width, o, o_stride,
+                                             _array(scales, device, _FLOAT, rows, "scales"), _current(device)))
+
+
+def block_norm(x, post=NORM_NONE, post_gain=None, post_bias=None, gate=None, scale=1.0, residual=None, sum=None,
+               norm=NORM_NONE, gain=None, bias=None, epsilon=1e-5, out=None, out_scales=None):
+    """s = residual + scale * gate * post(x) to sum, norm(s) to out: of x's type, or int8 with out_scales float32
+    [rows]. gate [rows][width] or [1][width]; gains and biases [width], of x's type."""
+    device, (rows, width) = x.device, x.shape
+    a, a_stride, type_ = _matrix(x, device, rows, width, "x")
+    kind = _kind(x)
+
+    def vector(tensor, name):
+        if tensor is None:
+            return None
+        if tensor.dim() != 1:
+            raise HipError(f"{name}: must be [{width}]")
+        return _array(tensor, device, kind, width, name)
+
+    def same(tensor, name, of=None):
+        if tensor is None:
+            return None, 0
+        at, stride, t = _matrix(tensor, device, rows, width, name)
+        if t != (type_ if of is None else of):
+            raise HipError(f"{name}: another type")
+        return at, stride
+
+    g, g_stride = None, 0
+    if gate is not None:
+        one = gate.shape[0] == 1 and rows != 1
+        g, g_stride, g_type = _matrix(gate, device, 1 if one else rows, width, "gate")
+        _need(g_type == type_, "gate: another type")
+        g_stride = 0 if one else g_stride
+    wide = next((_VALUE_TYPES.get(_kind(t)) for t in (residual, sum) if t is not None), type_)
+    r, r_stride = same(residual, "residual", wide)
+    s, s_stride = same(sum, "sum", wide)
+    if out_scales is None:
+        o, o_stride = same(out, "out")
+    else:
+        _need(out is not None, "out: missing")
+        o, o_stride, _ = _matrix(out, device, rows, width, "out", _BYTES)
+        out_scales = _array(out_scales, device, _FLOAT, rows, "out_scales")
+    desc = BlockRows(rows, width, type_, -1 if wide is None else wide, a, a_stride, post, vector(post_gain, "post_gain"),
+                     vector(post_bias, "post_bias"), g, g_stride, scale, r, r_stride, s, s_stride, norm,
+                     vector(gain, "gain"), vector(bias, "bias"), epsilon, o, o_stride, out_scales)
+    check(library().tsac_hip_block_norm(C.byref(desc), _current(device)))
+
+
+def rotary_frequencies(rotary, base=10000.0, scaling=ROTARY_NONE, factor=1.0, context=0.0, slow=1.0, fast=32.0) -> np.ndarray:
+    """float64 [rotary / 2] for PagedCache.append, scaled for contexts `factor` times as long."""
+    out = np.zeros(max(int(rotary) // 2, 1))
+    check(library().tsac_hip_rotary_frequencies(rotary, base, scaling, factor, context, slow, fast, out.ctypes.data))
+    return out
+
+
+def adjust_logits(logits, out, starts, probabilities=True, history=None, history_lengths=None, prompt_lengths=None,
+                  tokens=None, mask=None, repetition=None, presence=None, frequency=None, bias_starts=None,
+                  bias_tokens=None, bias_values=None, allowed=None, temperature=None, workspace=None):
+    """The logits [rows][alphabet] of sequences' rows (starts) under the rules given, or their probabilities, to out
+    (which may be the logits). history int32 [sequences][most] with history_lengths and prompt_lengths; tokens int32
+    [rows] and mask int64 [rows][words] of drafted nodes; repetition, presence, frequency and temperature float32
+    [sequences]; bias_tokens int32 and bias_values float32, sequence s's from bias_starts[s] on; allowed int32 [rows]
+    [words], or [1][words] for all rows."""
+    device, (rows, alphabet), n = logits.device, logits.shape, starts.numel() - 1
+    a, a_stride, type_ = _matrix(logits, device, rows, alphabet, "logits")
+    o, o_stride, out_type = _matrix(out, device, rows, alphabet, "out")
+
+    def array(tensor, kind, count, name):
+        return None if tensor is None else _array(tensor, device, kind, count, name)
+
+    for name, tensor in (("history", history), ("mask", mask), ("allowed", allowed)):
+        if tensor is not None and tensor.dim() != 2:
+            raise HipError(f"{name}: must have two axes")
+    words = (alphabet + 31) // 32
+    stride = 0
+    if allowed is not None:
+        if allowed.shape[1] < words or allowed.shape[0] not in (1, rows):
+            raise HipError(f"allowed: must be [{rows}][{words}] or [1][{words}]")
+        stride = allowed.shape[1] if allowed.shape[0] == rows and rows > 1 else 0
+    biases = 0 if bias_tokens is None else bias_tokens.numel()
+    held = 0 if history is None else history.shape[1]
+    mask_words = 0 if mask is None else mask.shape[1]
+    rules = LogitRules(
+        _array(starts, device, _INT, 1, "starts"), n, array(history, _INT, n * held, "history"), held,
+        array(history_lengths, _INT, n, "history_lengths"), array(prompt_lengths, _INT, n, "prompt_lengths"),
+        array(tokens, _INT, rows, "tokens"), array(mask, _LONG, rows * mask_words, "mask"), mask_words,
+        array(repetition, _FLOAT, n, "repetition"), array(presence, _FLOAT, n, "presence"),
+        array(frequency, _FLOAT, n, "frequency"), array(bias_starts, _INT, n + 1, "bias_starts"),
+        array(bias_tokens, _INT, biases, "bias_tokens"), array(bias_values, _FLOAT, biases, "bias_values"), biases,
+        array(allowed, _INT, 0, "allowed"), stride, array(temperature, _FLOAT, n, "temperature"))
+    lib = library()
+    need = lib.tsac_hip_adjust_logits_workspace(rows, alphabet) if probabilities else 0
+    space, size, keep = _workspace(need, workspace, device)
+    check(lib.tsac_hip_adjust_logits(a, a_stride, type_, rows, alphabet, C.byref(rules), probabilities, o, o_stride,
+                                     out_type, space, size, _current(device)))
     del keep
 
 
