@@ -704,7 +704,7 @@ void require_rows(const void* pointer, std::size_t stride, std::size_t rows, std
 void require_token_rows(const int8_t* q, std::size_t stride, std::size_t rows, std::size_t width, const char* message)
 {
     require(reinterpret_cast<std::uintptr_t>(q) % 16 == 0 && stride % 16 == 0 && (rows <= 1 || stride >= width) &&
-                stride < (std::size_t(1) << 40),
+                stride < (std::size_t(1) << 23),
             message);
 }
 
