@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import pathlib
+import struct
 
 import numpy as np
 
@@ -270,14 +271,14 @@ def library() -> C.CDLL:
         lib.tsac_hip_channel_linear_workspace.argtypes = [vp, sz]
         lib.tsac_hip_channel_linear_workspace.restype = sz
         lib.tsac_hip_channel_linear_apply.argtypes = [vp, vp, sz, vp, sz, vp, sz, C.c_int, vp, sz, vp]
-        lib.tsac_hip_block_norm.argtypes = [C.POINTER(BlockRows), vp]
+        lib.tsac_hip_block_norm.argtypes = [vp, vp]  # BlockRows
         lib.tsac_hip_rotary_frequencies.argtypes = [sz, C.c_double, C.c_int, C.c_double, C.c_double, C.c_double, C.c_double,
                                                     vp]
-        lib.tsac_hip_pages_append.argtypes = [cache, C.c_uint32, C.POINTER(RotaryRows), vp, vp]
+        lib.tsac_hip_pages_append.argtypes = [cache, C.c_uint32, vp, vp, vp]  # RotaryRows
         lib.tsac_hip_adjust_logits_workspace.argtypes = [sz, sz]
         lib.tsac_hip_adjust_logits_workspace.restype = sz
-        lib.tsac_hip_adjust_logits.argtypes = [vp, sz, C.c_int, sz, sz, C.POINTER(LogitRules), C.c_int, vp, sz, C.c_int, vp,
-                                               sz, vp]
+        lib.tsac_hip_adjust_logits.argtypes = [vp, sz, C.c_int, sz, sz, vp, C.c_int, vp, sz, C.c_int, vp,
+                                               sz, vp]  # LogitRules
         _lib = lib
     return _lib
 
@@ -899,7 +900,7 @@ def _need(condition, message):
         raise HipError(message)
 
 
-_INT, _FLOAT, _LONG, _DOUBLE = "torch.int32", "torch.float32", "torch.int64", "torch.float64"
+_INT, _FLOAT, _LONG = "torch.int32", "torch.float32", "torch.int64"
 #: Element types by dtype; int16 holds BF16 bits, as in the other operators.
 _ROW_TYPES = {"torch.bfloat16": TYPE_BF16, "torch.int16": TYPE_BF16, "torch.float16": TYPE_FP16}
 _PROBABILITY_TYPES = dict(_ROW_TYPES, **{"torch.float32": TYPE_FP32})
@@ -928,14 +929,18 @@ def _array(tensor, device, kind, count, name):
 _cuda = None  # (current device, current stream's handle by device), once torch is imported
 
 
+def _load_cuda():
+    global _cuda
+    import torch
+
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    _cuda = (torch.cuda.current_device, raw or (lambda index: torch.cuda.current_stream(index).cuda_stream))
+
+
 def _current(device):
     """The current stream's handle; the tensors have to be on the current device."""
-    global _cuda
     if _cuda is None:
-        import torch
-
-        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-        _cuda = (torch.cuda.current_device, raw or (lambda index: torch.cuda.current_stream(index).cuda_stream))
+        _load_cuda()
     if device.type != "cuda" or device.index != _cuda[0]():
         raise HipError(f"tensors are on {device}, which is not the current device")
     return _cuda[1](device.index)
@@ -953,6 +958,9 @@ def _rows(tensor, device, heads, width, type_, name):
     return tensor.data_ptr(), strides[0] if shape[0] > 1 else heads * width
 
 
+_rotary_rows = struct.Struct("@PNPNNPPNNNPPPNPNif").pack  # RotaryRows
+
+
 class PagedCache:
     """A paged cache over a program's own tensors (tsac_hip_paged_cache): keys and values
     [layers][pages][page_rows][heads][head_width] of one type and layout, table
@@ -965,6 +973,7 @@ class PagedCache:
         _need(_kind(keys) in _ROW_TYPES, "keys and values: must be bfloat16, float16 or int16")
         self.layers, self.pages, self.page_rows, self.heads, self.head_width = shape
         self.type, self.device, self.sequences = _ROW_TYPES[_kind(keys)], keys.device, table.shape[0]
+        self.index = keys.get_device()
         _need(strides[4] == 1 and (shape[3] == 1 or strides[3] == shape[4]), "keys and values: heads must be contiguous")
         _need(values.device == keys.device and table.dim() == 2, "table: must be [sequences][pages a sequence]")
         self.tensors = (keys, values, table, held, lengths, references)  # what the addresses below belong to
@@ -1030,23 +1039,40 @@ class PagedCache:
         rows' queries [rows][query heads][head_width] rotated to out (which may be query). frequencies: float64
         [pairs], radians a position (rotary_frequencies). Positions: positions int32 [rows], or down the lines of mask
         int64 [rows][words] (tree_mask), or one after the other."""
-        device, rows, heads, width = self.device, query.shape[0], query.shape[1], self.head_width
-        q, q_stride = _rows(query, device, heads, width, self.type, "query")
-        o, o_stride = _rows(out, device, heads, width, self.type, "out")
-        k, stride = _rows(keys, device, self.heads, width, self.type, "keys")
-        v, v_stride = _rows(values, device, self.heads, width, self.type, "values")
-        if out.shape[0] != rows or keys.shape[0] != rows or values.shape[0] != rows or stride != v_stride:
-            raise HipError("query, out, keys and values: as many rows, keys and values laid out alike")
-        if mask is not None and mask.dim() != 2:
-            raise HipError("mask: must be [rows][words]")
-        words, pairs = 0 if mask is None else mask.shape[1], frequencies.numel()
-        desc = RotaryRows(
+        heads, width, index = query.shape[1], self.head_width, self.index
+        rows = query.shape[0]
+        q, q_stride = self._heads(query, rows, heads, "query")
+        o, o_stride = (q, q_stride) if out is query else self._heads(out, rows, heads, "out")
+        k, stride = self._heads(keys, rows, self.heads, "keys")
+        v, v_stride = self._heads(values, rows, self.heads, "values")
+        if stride != v_stride:
+            raise HipError("keys and values: must be laid out alike")
+        words, pairs = 0, frequencies.numel()
+        if mask is not None:
+            if mask.dim() != 2:
+                raise HipError("mask: must be [rows][words]")
+            words = mask.shape[1]
+        desc = _rotary_rows(
             q, q_stride, o, o_stride, heads, k, v, stride, rows, max_rows,
-            self._ints(starts, self.sequences + 1, "starts"),
-            None if positions is None else self._ints(positions, rows, "positions"),
-            None if mask is None else _array(mask, device, _LONG, rows * words, "mask"), words,
-            _array(frequencies, device, _DOUBLE, pairs, "frequencies"), 2 * pairs, interleaved, amplitude)
-        check(library().tsac_hip_pages_append(self._desc, layer, C.byref(desc), self._status(status), _current(device)))
+            _vector(starts, index, _int32, self.sequences + 1, "starts"),
+            0 if positions is None else _vector(positions, index, _int32, rows, "positions"),
+            0 if mask is None else _vector(mask, index, _int64, rows * words, "mask"), words,
+            _vector(frequencies, index, _float64, pairs, "frequencies"), 2 * pairs, interleaved, amplitude)
+        status = (_lib or library()).tsac_hip_pages_append(self._desc, layer, desc, self._status(status), _stream_of(index))
+        if status:
+            check(status)
+
+    def _heads(self, tensor, rows, heads, name):
+        """(address, row stride) of [rows][heads][head_width] of the cache's type, heads contiguous."""
+        if tensor.get_device() != self.index or (_values or _load_values()).get(tensor.dtype) != self.type:
+            raise HipError(f"{name}: another device or type")
+        shape = (rows, heads, self.head_width)
+        if tensor.shape != shape:
+            raise HipError(f"{name}: must be {list(shape)}")
+        row, head, one = tensor.stride()
+        if rows and (one != 1 or (heads > 1 and head != shape[2])):
+            raise HipError(f"{name}: heads must be contiguous")
+        return tensor.data_ptr(), row if rows > 1 else heads * shape[2]
 
     def keep(self, starts, path, accepted, lengths=None, status=None):
         """Moves each sequence's accepted rows (path [sequences][nodes], accepted) to the front of the
@@ -1136,20 +1162,66 @@ def verify_drafts(target, draft, tokens, parents, starts, max_nodes, uniforms, d
 
 # ---------------------------------------------------------------- a model's step around the paged attention
 
-_VALUE_TYPES = _PROBABILITY_TYPES
+# The kernels of small calls take few microseconds, and so may what is in front of them: types by dtype, one look at each
+# property, and structures packed at once.
+_values = None  # element types by dtype, once torch is imported
+_int8 = _int32 = _int64 = _float32 = _float64 = None
 
 
-def _matrix(tensor, device, rows, width, name, types=_VALUE_TYPES):
-    """(address, row stride, type) of [rows][width], the elements of a row one after the other."""
-    shape, strides, type_ = tensor.shape, tensor.stride(), types.get(_kind(tensor))
-    if tensor.device != device or type_ is None:
-        raise HipError(f"{name}: another device or type")
-    if len(shape) != 2 or shape[0] != rows or shape[1] != width or (rows and width > 1 and strides[1] != 1):
-        raise HipError(f"{name}: must be [{rows}][{width}], rows contiguous")
-    return tensor.data_ptr(), strides[0] if rows > 1 else -(-width // 16) * 16, type_
+def _load_values():
+    global _values, _int8, _int32, _int64, _float32, _float64
+    import torch
+
+    _int8, _int32, _int64 = torch.int8, torch.int32, torch.int64
+    _float32, _float64 = torch.float32, torch.float64
+    _values = {torch.bfloat16: TYPE_BF16, torch.int16: TYPE_BF16, torch.float16: TYPE_FP16, torch.float32: TYPE_FP32}
+    return _values
 
 
-_BYTES = {"torch.int8": 3}
+def _matrix(tensor, index, shape, name):
+    """(address, row stride) of [rows][width], the elements of a row one after the other, on device `index`."""
+    if tensor.get_device() != index:
+        raise HipError(f"{name}: on {tensor.device}, not on the others' device")
+    if tensor.shape != shape:
+        raise HipError(f"{name}: must be {list(shape)}")
+    rows, width = shape
+    if rows <= 1 or width == 0:
+        stride = -(-width // 16) * 16  # of no importance: whole vectors
+    elif tensor.is_contiguous():
+        return tensor.data_ptr(), width
+    else:
+        stride = tensor.stride(0)
+    if width > 1 and rows and tensor.stride(1) != 1:
+        raise HipError(f"{name}: rows must be contiguous")
+    return tensor.data_ptr(), stride
+
+
+def _rows_of(tensor, name):
+    """(shape, type) of a matrix of 16- or 32-bit numbers."""
+    type_, shape = (_values or _load_values()).get(tensor.dtype), tensor.shape
+    if type_ is None or len(shape) != 2:
+        raise HipError(f"{name}: must be bfloat16, float16 or float32 of two axes")
+    return shape, type_
+
+
+def _vector(tensor, index, dtype, count, name):
+    """The address of a contiguous vector of `count` elements at least."""
+    if tensor.get_device() != index:
+        raise HipError(f"{name}: on {tensor.device}, not on the others' device")
+    if tensor.dtype is not dtype or not tensor.is_contiguous():
+        raise HipError(f"{name}: must be contiguous {dtype}")
+    if tensor.numel() < count:
+        raise HipError(f"{name}: {tensor.numel()} elements, {count} needed")
+    return tensor.data_ptr()
+
+
+def _stream_of(index):
+    """The current stream's handle on device `index`, which has to be the current one."""
+    if _cuda is None:
+        _load_cuda()
+    if index < 0 or index != _cuda[0]():
+        raise HipError(f"tensors are on device {index}, which is not the current one")
+    return _cuda[1](index)
 
 
 class ChannelLinear:
@@ -1159,6 +1231,7 @@ class ChannelLinear:
     def __init__(self, values, scales, bias=None):
         import torch
 
+        _load_values()
         values, scales, bias = (torch.from_numpy(a) if isinstance(a, np.ndarray) else a for a in (values, scales, bias))
         _need(values.dim() == 2 and _kind(values) == "torch.int8", "values: must be int8 [outputs][inputs]")
         self.N, self.K = values.shape
@@ -1184,73 +1257,92 @@ class ChannelLinear:
         if need is None:
             if len(self._workspaces) >= 1024:
                 self._workspaces.clear()
-            need = self._workspaces[rows] = int(library().tsac_hip_channel_linear_workspace(self.handle, rows))
+            need = self._workspaces[rows] = int(self._library.tsac_hip_channel_linear_workspace(self.handle, rows))
         return need
 
     def apply(self, q, scales, out, workspace=None):
         """q int8 [rows][K] and its scales float32 [rows] (quantize_tokens, block_norm) to out [rows][N]. A new
         workspace a call, if none is given and one is needed."""
-        device, rows = q.device, q.shape[0]
-        a, a_stride, _ = _matrix(q, device, rows, self.K, "q", _BYTES)
-        o, o_stride, type_ = _matrix(out, device, rows, self.N, "out")
-        space, size, keep = _workspace(self.workspace(rows), workspace, device)
-        check(library().tsac_hip_channel_linear_apply(
-            self.handle, a, a_stride, _array(scales, device, _FLOAT, rows, "scales"), rows, o, o_stride, type_, space, size,
-            _current(device)))
+        shape, type_ = _rows_of(out, "out")
+        index, rows = q.get_device(), shape[0]
+        if q.dtype is not _int8 or shape[1] != self.N:
+            raise HipError(f"q: must be int8, out [rows][{self.N}]")
+        a, a_stride = _matrix(q, index, (rows, self.K), "q")
+        o, o_stride = _matrix(out, index, shape, "out")
+        space, size, keep = None, 0, None
+        need = self._workspaces.get(rows)
+        if need is None:
+            need = self.workspace(rows)
+        if need or workspace is not None:
+            space, size, keep = _workspace(need, workspace, q.device)
+        status = self._library.tsac_hip_channel_linear_apply(
+            self.handle, a, a_stride, _vector(scales, index, _float32, rows, "scales"), rows, o, o_stride, type_, space,
+            size, _stream_of(index))
+        if status:
+            check(status)
         del keep
 
 
 def quantize_tokens(x, q, scales):
     """Rows of x to 8 bits, q int8 [rows][K] at a stride of a multiple of 16, and a scale each, float32 [rows]."""
-    device, (rows, width) = x.device, x.shape
-    a, a_stride, type_ = _matrix(x, device, rows, width, "x")
-    o, o_stride, _ = _matrix(q, device, rows, width, "q", _BYTES)
-    check(library().tsac_hip_quantize_tokens(a, a_stride, type_, rows, width, o, o_stride,
-                                             _array(scales, device, _FLOAT, rows, "scales"), _current(device)))
+    shape, type_ = _rows_of(x, "x")
+    index, (rows, width) = x.get_device(), shape
+    a, a_stride = _matrix(x, index, shape, "x")
+    if q.dtype is not _int8:
+        raise HipError("q: must be int8")
+    o, o_stride = _matrix(q, index, shape, "q")
+    status = (_lib or library()).tsac_hip_quantize_tokens(
+        a, a_stride, type_, rows, width, o, o_stride, _vector(scales, index, _float32, rows, "scales"), _stream_of(index))
+    if status:
+        check(status)
+
+
+_block_rows = struct.Struct("@NNiiPNiPPPNfPNPNiPPfPNP").pack  # BlockRows
 
 
 def block_norm(x, post=NORM_NONE, post_gain=None, post_bias=None, gate=None, scale=1.0, residual=None, sum=None,
                norm=NORM_NONE, gain=None, bias=None, epsilon=1e-5, out=None, out_scales=None):
     """s = residual + scale * gate * post(x) to sum, norm(s) to out: of x's type, or int8 with out_scales float32
-    [rows]. gate [rows][width] or [1][width]; gains and biases [width], of x's type."""
-    device, (rows, width) = x.device, x.shape
-    a, a_stride, type_ = _matrix(x, device, rows, width, "x")
-    kind = _kind(x)
-
-    def vector(tensor, name):
-        if tensor is None:
-            return None
-        if tensor.dim() != 1:
-            raise HipError(f"{name}: must be [{width}]")
-        return _array(tensor, device, kind, width, name)
-
-    def same(tensor, name, of=None):
-        if tensor is None:
-            return None, 0
-        at, stride, t = _matrix(tensor, device, rows, width, name)
-        if t != (type_ if of is None else of):
-            raise HipError(f"{name}: another type")
-        return at, stride
-
-    g, g_stride = None, 0
+    [rows]. gate [rows][width] or [1][width]; gains and biases [width], of x's type; residual and sum of x's type or
+    float32."""
+    shape, type_ = _rows_of(x, "x")
+    index, dtype, (rows, width) = x.get_device(), x.dtype, shape
+    a, a_stride = _matrix(x, index, shape, "x")
+    g = g_stride = r = r_stride = s = s_stride = o = o_stride = scales = 0
     if gate is not None:
-        one = gate.shape[0] == 1 and rows != 1
-        g, g_stride, g_type = _matrix(gate, device, 1 if one else rows, width, "gate")
-        _need(g_type == type_, "gate: another type")
+        one = gate.shape != shape
+        g, g_stride = _matrix(gate, index, (1, width) if one else shape, "gate")
+        if gate.dtype is not dtype:
+            raise HipError("gate: another type")
         g_stride = 0 if one else g_stride
-    wide = next((_VALUE_TYPES.get(_kind(t)) for t in (residual, sum) if t is not None), type_)
-    r, r_stride = same(residual, "residual", wide)
-    s, s_stride = same(sum, "sum", wide)
-    if out_scales is None:
-        o, o_stride = same(out, "out")
-    else:
-        _need(out is not None, "out: missing")
-        o, o_stride, _ = _matrix(out, device, rows, width, "out", _BYTES)
-        out_scales = _array(out_scales, device, _FLOAT, rows, "out_scales")
-    desc = BlockRows(rows, width, type_, -1 if wide is None else wide, a, a_stride, post, vector(post_gain, "post_gain"),
-                     vector(post_bias, "post_bias"), g, g_stride, scale, r, r_stride, s, s_stride, norm,
-                     vector(gain, "gain"), vector(bias, "bias"), epsilon, o, o_stride, out_scales)
-    check(library().tsac_hip_block_norm(C.byref(desc), _current(device)))
+    wide = type_
+    if residual is not None:
+        r, r_stride = _matrix(residual, index, shape, "residual")
+        wide = _values.get(residual.dtype, -1)
+    if sum is not None:
+        s, s_stride = _matrix(sum, index, shape, "sum")
+        if residual is not None and sum.dtype is not residual.dtype:
+            raise HipError("sum: another type than the residual")
+        wide = _values.get(sum.dtype, -1)
+    if out is not None:
+        o, o_stride = _matrix(out, index, shape, "out")
+        if out.dtype is not (dtype if out_scales is None else _int8):
+            raise HipError("out: must be of the input's type, or int8 with scales")
+    if out_scales is not None:
+        scales = _vector(out_scales, index, _float32, rows, "out_scales")
+    for tensor in (post_gain, post_bias, gain, bias):
+        if tensor is not None and tensor.dim() != 1:
+            raise HipError(f"gains and biases: must be [{width}]")
+    status = (_lib or library()).tsac_hip_block_norm(_block_rows(
+        rows, width, type_, wide, a, a_stride, post,
+        0 if post_gain is None else _vector(post_gain, index, dtype, width, "post_gain"),
+        0 if post_bias is None else _vector(post_bias, index, dtype, width, "post_bias"),
+        g, g_stride, scale, r, r_stride, s, s_stride, norm,
+        0 if gain is None else _vector(gain, index, dtype, width, "gain"),
+        0 if bias is None else _vector(bias, index, dtype, width, "bias"), epsilon, o, o_stride, scales),
+        _stream_of(index))
+    if status:
+        check(status)
 
 
 def rotary_frequencies(rotary, base=10000.0, scaling=ROTARY_NONE, factor=1.0, context=0.0, slow=1.0, fast=32.0) -> np.ndarray:
@@ -1258,6 +1350,9 @@ def rotary_frequencies(rotary, base=10000.0, scaling=ROTARY_NONE, factor=1.0, co
     out = np.zeros(max(int(rotary) // 2, 1))
     check(library().tsac_hip_rotary_frequencies(rotary, base, scaling, factor, context, slow, fast, out.ctypes.data))
     return out
+
+
+_logit_rules = struct.Struct("@PNPNPPPPNPPPPPPNPNP").pack  # LogitRules
 
 
 def adjust_logits(logits, out, starts, probabilities=True, history=None, history_lengths=None, prompt_lengths=None,
@@ -1268,38 +1363,54 @@ def adjust_logits(logits, out, starts, probabilities=True, history=None, history
     [rows] and mask int64 [rows][words] of drafted nodes; repetition, presence, frequency and temperature float32
     [sequences]; bias_tokens int32 and bias_values float32, sequence s's from bias_starts[s] on; allowed int32 [rows]
     [words], or [1][words] for all rows."""
-    device, (rows, alphabet), n = logits.device, logits.shape, starts.numel() - 1
-    a, a_stride, type_ = _matrix(logits, device, rows, alphabet, "logits")
-    o, o_stride, out_type = _matrix(out, device, rows, alphabet, "out")
-
-    def array(tensor, kind, count, name):
-        return None if tensor is None else _array(tensor, device, kind, count, name)
-
-    for name, tensor in (("history", history), ("mask", mask), ("allowed", allowed)):
-        if tensor is not None and tensor.dim() != 2:
-            raise HipError(f"{name}: must have two axes")
-    words = (alphabet + 31) // 32
-    stride = 0
+    shape, type_ = _rows_of(logits, "logits")
+    index, (rows, alphabet), n = logits.get_device(), shape, starts.numel() - 1
+    a, a_stride = _matrix(logits, index, shape, "logits")
+    o, o_stride = _matrix(out, index, shape, "out")
+    out_type = _values.get(out.dtype)
+    if out_type is None:
+        raise HipError("out: must be bfloat16, float16 or float32")
+    stride = held = words = biases = 0
+    if history is not None:
+        if history.dim() != 2:
+            raise HipError("history: must be [sequences][tokens]")
+        held = history.shape[1]
+    if mask is not None:
+        if mask.dim() != 2:
+            raise HipError("mask: must be [rows][words]")
+        words = mask.shape[1]
     if allowed is not None:
-        if allowed.shape[1] < words or allowed.shape[0] not in (1, rows):
-            raise HipError(f"allowed: must be [{rows}][{words}] or [1][{words}]")
+        if allowed.dim() != 2 or allowed.shape[1] < (alphabet + 31) // 32 or allowed.shape[0] not in (1, rows):
+            raise HipError(f"allowed: must be [{rows}][{(alphabet + 31) // 32}], or of one row")
         stride = allowed.shape[1] if allowed.shape[0] == rows and rows > 1 else 0
-    biases = 0 if bias_tokens is None else bias_tokens.numel()
-    held = 0 if history is None else history.shape[1]
-    mask_words = 0 if mask is None else mask.shape[1]
-    rules = LogitRules(
-        _array(starts, device, _INT, 1, "starts"), n, array(history, _INT, n * held, "history"), held,
-        array(history_lengths, _INT, n, "history_lengths"), array(prompt_lengths, _INT, n, "prompt_lengths"),
-        array(tokens, _INT, rows, "tokens"), array(mask, _LONG, rows * mask_words, "mask"), mask_words,
-        array(repetition, _FLOAT, n, "repetition"), array(presence, _FLOAT, n, "presence"),
-        array(frequency, _FLOAT, n, "frequency"), array(bias_starts, _INT, n + 1, "bias_starts"),
-        array(bias_tokens, _INT, biases, "bias_tokens"), array(bias_values, _FLOAT, biases, "bias_values"), biases,
-        array(allowed, _INT, 0, "allowed"), stride, array(temperature, _FLOAT, n, "temperature"))
-    lib = library()
+    if bias_starts is not None:
+        if bias_tokens is None or bias_values is None:
+            raise HipError("biases: need starts, tokens and values")
+        biases = bias_tokens.numel()
+    rules = _logit_rules(
+        _vector(starts, index, _int32, 1, "starts"), n,
+        0 if history is None else _vector(history, index, _int32, n * held, "history"), held,
+        0 if history_lengths is None else _vector(history_lengths, index, _int32, n, "history_lengths"),
+        0 if prompt_lengths is None else _vector(prompt_lengths, index, _int32, n, "prompt_lengths"),
+        0 if tokens is None else _vector(tokens, index, _int32, rows, "tokens"),
+        0 if mask is None else _vector(mask, index, _int64, rows * words, "mask"), words,
+        0 if repetition is None else _vector(repetition, index, _float32, n, "repetition"),
+        0 if presence is None else _vector(presence, index, _float32, n, "presence"),
+        0 if frequency is None else _vector(frequency, index, _float32, n, "frequency"),
+        0 if bias_starts is None else _vector(bias_starts, index, _int32, n + 1, "bias_starts"),
+        0 if bias_starts is None else _vector(bias_tokens, index, _int32, biases, "bias_tokens"),
+        0 if bias_starts is None else _vector(bias_values, index, _float32, biases, "bias_values"), biases,
+        0 if allowed is None else _vector(allowed, index, _int32, 0, "allowed"), stride,
+        0 if temperature is None else _vector(temperature, index, _float32, n, "temperature"))
+    lib = _lib or library()
+    space, size, keep = None, 0, None
     need = lib.tsac_hip_adjust_logits_workspace(rows, alphabet) if probabilities else 0
-    space, size, keep = _workspace(need, workspace, device)
-    check(lib.tsac_hip_adjust_logits(a, a_stride, type_, rows, alphabet, C.byref(rules), probabilities, o, o_stride,
-                                     out_type, space, size, _current(device)))
+    if need or workspace is not None:
+        space, size, keep = _workspace(need, workspace, logits.device)
+    status = lib.tsac_hip_adjust_logits(a, a_stride, type_, rows, alphabet, rules, probabilities, o, o_stride, out_type,
+                                        space, size, _stream_of(index))
+    if status:
+        check(status)
     del keep
 
 
