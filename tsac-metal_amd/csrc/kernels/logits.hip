@@ -13,19 +13,23 @@
 //
 // A row of up to 32,768 tokens is one workgroup's, held in registers between its maximum, its sum and its
 // store. Longer ones are divided: one launch leaves each part's maximum and sum, another joins them in
-// ascending order and computes the part again.
+// ascending order and computes the part again. Logits are asked for before anything is counted.
+#include "lanes.hpp"
 #include "model_step.hpp"
 #include "paged_device.hpp"
 #include "values.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace tsac_hip
 {
 namespace
 {
 constexpr int lanes = 64;
-constexpr int most_threads = 512;
+constexpr int most_threads = 1024;
+constexpr int most_vectors = 4; // eights of a thread
+constexpr int asked = 8;        // tokens of the history that a thread has in flight
 constexpr float minus_infinity = -__builtin_inff();
 constexpr float log2e = 1.44269504f;
 
@@ -44,155 +48,70 @@ struct Launch
     int splits;   // of a row
     int width;    // tokens of a split
     bool aligned; // logits and outputs in whole vectors
+    bool counted; // there is a history, or there are drafted tokens
 };
 
-// What a workgroup works on.
-struct Place
+// What a token has had, in a word of LDS or two: twice the times it was said and 1 more if the prompt has it; and the
+// place in its sequence's list of biases and 1, or 0. One word has 16 bits of each, where no count reaches 2^15 and no
+// place 2^16.
+template <bool Narrow> struct Words
 {
-    int row, sequence, node; // node: the row's place in its sequence
-    int first, count;        // the sequence's rows
-    int from, to;            // tokens
+    static constexpr int each = Narrow ? 1 : 2;
+    unsigned* memory; // counts (and biases), then the biases of wide words
+    int chunk;
+
+    __device__ __forceinline__ void clear(int at) const
+    {
+#pragma unroll
+        for (int i = 0; i < each; ++i)
+        {
+            *reinterpret_cast<uint4*>(memory + i * chunk + at) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(memory + i * chunk + at + 4) = make_uint4(0, 0, 0, 0);
+        }
+    }
+    // Before counts are added to the same words.
+    __device__ __forceinline__ void bias(unsigned token, unsigned place) const
+    {
+        atomicMax(memory + (Narrow ? 0 : chunk) + token, Narrow ? place << 16 : place);
+    }
+    __device__ __forceinline__ void count(unsigned token, bool said) const
+    {
+        said ? (void)atomicAdd(memory + token, 2u) : (void)atomicOr(memory + token, 1u);
+    }
+    __device__ __forceinline__ void read(int at, unsigned (&said)[8], unsigned (&bias)[8]) const
+    {
+        eight(memory + at, said);
+        if constexpr (!Narrow)
+        {
+            eight(memory + chunk + at, bias);
+        }
+#pragma unroll
+        for (int e = 0; Narrow && e < 8; ++e)
+        {
+            bias[e] = said[e] >> 16;
+            said[e] &= 0xffffu;
+        }
+    }
+    static __device__ __forceinline__ void eight(const unsigned* from, unsigned (&to)[8])
+    {
+        const uint4 a = *reinterpret_cast<const uint4*>(from), b = *reinterpret_cast<const uint4*>(from + 4);
+        to[0] = a.x, to[1] = a.y, to[2] = a.z, to[3] = a.w;
+        to[4] = b.x, to[5] = b.y, to[6] = b.z, to[7] = b.w;
+    }
 };
 
-__device__ __forceinline__ bool place_of(const Launch& l, Place& p)
+template <class V, class Join> __device__ __forceinline__ V joined(V value, V* shared, Join join)
 {
-    p.row = blockIdx.x / l.splits;
-    p.sequence = sequence_of(l.rules.starts, l.rules.sequences, p.row);
-    p.count = rows_of(l.rules.starts, p.sequence, l.rows.rows, p.first);
-    p.node = p.row - p.first;
-    p.from = int(blockIdx.x % l.splits) * l.width;
-    p.to = min(p.from + l.width, l.rows.alphabet);
-    return p.node >= 0 && p.node < p.count;
-}
-
-// Counts of a chunk's tokens: twice the number of times they were said, and 1 more if the prompt had them.
-struct Counts
-{
-    unsigned* said; // [chunk]
-    unsigned* bias; // [chunk]: place in the list of biases and 1, or 0; null without biases
-};
-
-__device__ void count_chunk(const Launch& l, const Place& p, int base, int chunk, const Counts& counts)
-{
-    const LogitRules& r = l.rules;
-    for (int i = threadIdx.x; i < chunk; i += blockDim.x)
-    {
-        counts.said[i] = 0;
-        if (counts.bias)
-        {
-            counts.bias[i] = 0;
-        }
-    }
-    __syncthreads();
-    if (r.history)
-    {
-        const int held = int(min(r.history_stride, std::size_t(1) << 30));
-        const int length = max(0, min(r.history_lengths[p.sequence], held));
-        const int prompt = r.prompt_lengths ? max(0, min(r.prompt_lengths[p.sequence], length)) : 0;
-        const int* history = r.history + p.sequence * r.history_stride;
-        for (int i = threadIdx.x; i < length; i += blockDim.x)
-        {
-            const unsigned t = unsigned(history[i]) - unsigned(base);
-            if (t < unsigned(chunk))
-            {
-                i < prompt ? (void)atomicOr(&counts.said[t], 1u) : (void)atomicAdd(&counts.said[t], 2u);
-            }
-        }
-    }
-    if (r.tokens)
-    {
-        const uint64_t* line = r.mask ? r.mask + std::size_t(p.row) * r.words : nullptr;
-        const int nodes = r.mask ? int(min(std::size_t(p.count), 64 * r.words)) : p.node + 1;
-        for (int j = threadIdx.x; j < nodes; j += blockDim.x)
-        {
-            const unsigned t = unsigned(r.tokens[p.first + j]) - unsigned(base);
-            if (t < unsigned(chunk) && (!line || (line[j / 64] >> j % 64 & 1)))
-            {
-                atomicAdd(&counts.said[t], 2u);
-            }
-        }
-    }
-    if (counts.bias)
-    {
-        const int begin = max(0, min(r.bias_starts[p.sequence], r.biases));
-        const int end = min(r.bias_starts[p.sequence + 1], r.biases);
-        for (int i = begin + int(threadIdx.x); i < end; i += blockDim.x)
-        {
-            const unsigned t = unsigned(r.bias_tokens[i]) - unsigned(base);
-            if (t < unsigned(chunk))
-            {
-                atomicMax(&counts.bias[t], unsigned(i) + 1);
-            }
-        }
-    }
-    __syncthreads();
-}
-
-struct Penalties
-{
-    float repetition, presence, frequency;
-};
-
-// Eight tokens from `token` on, `at` from the chunk's first.
-template <Type T>
-__device__ __forceinline__ void adjusted(const Launch& l, const Place& p, const Penalties& k, const Counts& counts, int token,
-                                         int at, float (&x)[8])
-{
-    const auto* logits = static_cast<const value_t<T>*>(l.rows.logits) + std::size_t(p.row) * l.rows.stride;
-    const int count = p.to - token;
-    load8<T>(logits + token, count, l.aligned, minus_infinity, x);
-    const uint4 low = *reinterpret_cast<const uint4*>(counts.said + at), high = *reinterpret_cast<const uint4*>(counts.said + at + 4);
-    const unsigned said[8] = {low.x, low.y, low.z, low.w, high.x, high.y, high.z, high.w};
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-    {
-        if (said[e] && e < count)
-        {
-            const float times = float(said[e] >> 1);
-            x[e] = x[e] > 0.0f ? x[e] / k.repetition : x[e] * k.repetition;
-            x[e] -= k.frequency * times;
-            x[e] -= times > 0.0f ? k.presence : 0.0f;
-        }
-    }
-    if (counts.bias)
-    {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-        {
-            if (const unsigned i = counts.bias[at + e]; i && e < count)
-            {
-                x[e] += l.rules.bias_values[i - 1];
-            }
-        }
-    }
-    if (l.rules.allowed && count > 0)
-    {
-        // Tokens come in eights, so that their bits are in one word.
-        const uint32_t word = l.rules.allowed[p.row * l.rules.allowed_stride + token / 32] >> token % 32;
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-        {
-            x[e] = word >> e & 1 ? x[e] : minus_infinity;
-        }
-    }
-}
-
-template <class Join, class V> __device__ __forceinline__ V joined(V value, V* shared, Join join)
-{
-#pragma unroll
-    for (int step = 1; step < lanes; step *= 2)
-    {
-        value = join(value, __shfl_xor(value, step));
-    }
+    value = over_lanes(value, join);
     const int waves = int(blockDim.x) / lanes;
     if (waves > 1)
     {
-        __syncthreads(); // the last one's values have been read
+        lds_barrier(); // the last one's values have been read
         if (threadIdx.x % lanes == 0)
         {
             shared[threadIdx.x / lanes] = value;
         }
-        __syncthreads();
+        lds_barrier();
         value = shared[0];
         for (int i = 1; i < waves; ++i)
         {
@@ -220,9 +139,10 @@ __device__ __forceinline__ float factor_of(float temperature)
     return __builtin_fminf(log2e / temperature, 3.402823466e38f);
 }
 
-// What is known of values held in registers: the largest and its lowest place, the sum of weights.
+// What is known of values held in registers: the largest and its lowest place, the sum of weights, which stand in the
+// values' place afterwards.
 template <int Vectors>
-__device__ __forceinline__ Part part_of(const float (&x)[Vectors][8], int from, float temperature, Exchange& shared)
+__device__ __forceinline__ Part part_of(float (&x)[Vectors][8], int from, float temperature, Exchange& shared)
 {
     Part part;
     float top = minus_infinity;
@@ -249,7 +169,8 @@ __device__ __forceinline__ Part part_of(const float (&x)[Vectors][8], int from, 
 #pragma unroll
             for (int e = 0; e < 8; ++e)
             {
-                sum += weight(x[i][e], top, factor);
+                x[i][e] = weight(x[i][e], top, factor);
+                sum += x[i][e];
             }
         }
         part.sum = joined(sum, shared.f, [](float a, float b) { return a + b; });
@@ -301,43 +222,215 @@ enum class Step
     finish  // the softmax from these
 };
 
-template <Type T, Type O, Step S, int Vectors>
+// Eight logits as they are asked for.
+template <bool Wide> struct Raw
+{
+    uint4 v[Wide ? 2 : 1];
+};
+
+// Rounds: how often LDS holds the words of a part of the workgroup's tokens.
+template <Step S, bool Wide, int Vectors, int Rounds, bool Narrow>
 __global__ __launch_bounds__(most_threads) void logits_kernel(Launch l)
 {
-    extern __shared__ unsigned memory[]; // the counts of a chunk, and its biases
+    constexpr int held = Vectors / Rounds; // eights of a thread in a round
+    extern __shared__ __attribute__((aligned(16))) unsigned memory[];
     __shared__ Exchange shared;
-    Place p;
-    if (!place_of(l, p))
+    const int thread = threadIdx.x, threads = blockDim.x;
+    const int row = blockIdx.x / l.splits, from = int(blockIdx.x - row * l.splits) * l.width;
+    const int to = min(from + l.width, l.rows.alphabet);
+    const LogitRules& r = l.rules;
+    const int s = __builtin_amdgcn_readfirstlane(sequence_of(r.starts, r.sequences, row));
+    int first;
+    const int count = rows_of(r.starts, s, l.rows.rows, first), node = row - first;
+    if (node < 0 || node >= count)
     {
         return;
     }
-    const int chunk = 8 * blockDim.x;
-    const Counts counts = {memory, l.rules.bias_starts ? memory + chunk : nullptr};
-    const LogitRules& r = l.rules;
-    const Penalties k = {r.repetition ? r.repetition[p.sequence] : 1.0f, r.presence ? r.presence[p.sequence] : 0.0f,
-                         r.frequency ? r.frequency[p.sequence] : 0.0f};
-    float x[Vectors][8];
+
+    // The first of the history, then the logits: loads complete in the order of issue.
+    int length = 0, prompt = 0;
+    int past[asked];
+    const int* const history = r.history + std::size_t(s) * r.history_stride;
+    if (r.history)
+    {
+        const int room = int(min(r.history_stride, std::size_t(1) << 30));
+        length = max(0, min(r.history_lengths[s], room));
+        prompt = r.prompt_lengths ? max(0, min(r.prompt_lengths[s], length)) : 0;
+#pragma unroll
+        for (int i = 0; i < asked; ++i)
+        {
+            const int at = thread + i * threads;
+            past[i] = at < length ? history[at] : -1;
+        }
+    }
+    const std::size_t begin = std::size_t(row) * l.rows.stride;
+    Raw<Wide> raw[Vectors];
 #pragma unroll
     for (int i = 0; i < Vectors; ++i)
     {
-        const int base = p.from + i * chunk;
-        if (i)
+        const int token = from + 8 * (i * threads + thread);
+        if (l.aligned && token + 8 <= to)
         {
-            __syncthreads(); // the last chunk's counts have been read
+            raw[i] = *reinterpret_cast<const Raw<Wide>*>(static_cast<const char*>(l.rows.logits) +
+                                                         (begin + token) * (Wide ? 4 : 2));
         }
-        count_chunk(l, p, base, chunk, counts);
-        adjusted<T>(l, p, k, counts, base + 8 * int(threadIdx.x), 8 * int(threadIdx.x), x[i]);
     }
+
+    const float repetition = r.repetition ? r.repetition[s] : 1.0f, presence = r.presence ? r.presence[s] : 0.0f;
+    const float frequency = r.frequency ? r.frequency[s] : 0.0f;
+    const int bias_begin = r.bias_starts ? max(0, min(r.bias_starts[s], r.biases)) : 0;
+    const int bias_end = r.bias_starts ? min(r.bias_starts[s + 1], r.biases) : 0;
+    const bool edited = l.counted || bias_begin < bias_end;
+    const Words<Narrow> words = {memory, 8 * threads * held};
+    float x[Vectors][8];
+#pragma unroll
+    for (int round = 0; round < Rounds; ++round)
+    {
+        const int base = from + round * words.chunk;
+        if (edited)
+        {
+#pragma unroll
+            for (int i = 0; i < held; ++i)
+            {
+                words.clear(8 * (i * threads + thread)); // the words that this thread reads
+            }
+            lds_barrier();
+            if (bias_begin < bias_end)
+            {
+                for (int i = bias_begin + thread; i < bias_end; i += threads)
+                {
+                    const unsigned t = unsigned(r.bias_tokens[i]) - unsigned(base);
+                    if (t < unsigned(words.chunk))
+                    {
+                        words.bias(t, unsigned(i - bias_begin) + 1);
+                    }
+                }
+                lds_barrier();
+            }
+            const auto had = [&](int token, bool said)
+            {
+                const unsigned t = unsigned(token) - unsigned(base);
+                if (t < unsigned(words.chunk))
+                {
+                    words.count(t, said);
+                }
+            };
+            if (r.history)
+            {
+#pragma unroll
+                for (int i = 0; i < asked; ++i)
+                {
+                    if (const int at = thread + i * threads; at < length)
+                    {
+                        had(past[i], at >= prompt);
+                    }
+                }
+                for (int later = asked * threads; later < length; later += asked * threads)
+                {
+                    int more[asked];
+#pragma unroll
+                    for (int i = 0; i < asked; ++i)
+                    {
+                        const int at = later + thread + i * threads;
+                        more[i] = at < length ? history[at] : -1;
+                    }
+#pragma unroll
+                    for (int i = 0; i < asked; ++i)
+                    {
+                        if (const int at = later + thread + i * threads; at < length)
+                        {
+                            had(more[i], at >= prompt);
+                        }
+                    }
+                }
+            }
+            if (r.tokens)
+            {
+                const uint64_t* const line = r.mask ? r.mask + std::size_t(row) * r.words : nullptr;
+                const int nodes = r.mask ? int(min(std::size_t(count), 64 * r.words)) : node + 1;
+                for (int j = thread; j < nodes; j += threads)
+                {
+                    if (!line || (line[j / 64] >> j % 64 & 1))
+                    {
+                        had(r.tokens[first + j], true);
+                    }
+                }
+            }
+            lds_barrier();
+        }
+#pragma unroll
+        for (int h = 0; h < held; ++h)
+        {
+            const int i = round * held + h, token = from + 8 * (i * threads + thread), there = to - token;
+            const auto widened = [&](auto type)
+            {
+                constexpr Type T = decltype(type)::value;
+                if (l.aligned && there >= 8)
+                {
+                    const Eight<T> eight = __builtin_bit_cast(Eight<T>, raw[i]);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                    {
+                        x[i][e] = widen<T>(eight.v[e]);
+                    }
+                }
+                else
+                {
+                    load8<T>(static_cast<const value_t<T>*>(l.rows.logits) + begin + token, there, false, minus_infinity, x[i]);
+                }
+            };
+            if constexpr (Wide)
+            {
+                widened(std::integral_constant<Type, Type::single>{});
+            }
+            else
+            {
+                l.rows.type == Type::bf16 ? widened(std::integral_constant<Type, Type::bf16>{})
+                                          : widened(std::integral_constant<Type, Type::half>{});
+            }
+            if (edited)
+            {
+                unsigned said[8], bias[8];
+                words.read(8 * (h * threads + thread), said, bias);
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                {
+                    if (said[e] && e < there)
+                    {
+                        const float times = float(said[e] >> 1);
+                        x[i][e] = x[i][e] > 0.0f ? x[i][e] / repetition : x[i][e] * repetition;
+                        x[i][e] -= frequency * times;
+                        x[i][e] -= times > 0.0f ? presence : 0.0f;
+                    }
+                    if (bias[e] && e < there)
+                    {
+                        x[i][e] += r.bias_values[bias_begin + int(bias[e]) - 1];
+                    }
+                }
+            }
+            if (r.allowed && there > 0)
+            {
+                // Tokens come in eights, so that their bits are in one word.
+                const uint32_t bits = r.allowed[std::size_t(row) * r.allowed_stride + token / 32] >> token % 32;
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                {
+                    x[i][e] = bits >> e & 1 ? x[i][e] : minus_infinity;
+                }
+            }
+        }
+    }
+
     float scale = 1.0f, top = 0.0f, factor = 0.0f;
     Part part = {};
     bool soft = false;
     if constexpr (S != Step::adjust)
     {
-        const float temperature = r.temperature ? r.temperature[p.sequence] : 1.0f;
+        const float temperature = r.temperature ? r.temperature[s] : 1.0f;
         soft = temperature > 0.0f;
         if constexpr (S == Step::finish)
         {
-            const Part* parts = l.parts + std::size_t(p.row) * l.splits;
+            const Part* const parts = l.parts + std::size_t(row) * l.splits;
             part = parts[0];
             for (int i = 1; i < l.splits; ++i)
             {
@@ -346,11 +439,11 @@ __global__ __launch_bounds__(most_threads) void logits_kernel(Launch l)
         }
         else
         {
-            part = part_of<Vectors>(x, p.from, temperature, shared);
+            part = part_of<Vectors>(x, from, temperature, shared);
         }
         if constexpr (S == Step::parts)
         {
-            if (threadIdx.x == 0)
+            if (thread == 0)
             {
                 l.parts[blockIdx.x] = part;
             }
@@ -360,12 +453,12 @@ __global__ __launch_bounds__(most_threads) void logits_kernel(Launch l)
         factor = factor_of(temperature);
         scale = part.sum == 0.0f ? 0.0f : 1.0f / part.sum;
     }
-    auto* out = static_cast<value_t<O>*>(l.rows.out) + std::size_t(p.row) * l.rows.out_stride;
+    const std::size_t at = std::size_t(row) * l.rows.out_stride;
 #pragma unroll
     for (int i = 0; i < Vectors; ++i)
     {
-        const int token = p.from + i * chunk + 8 * int(threadIdx.x);
-        if (token >= p.to)
+        const int token = from + 8 * (i * threads + thread);
+        if (token >= to)
         {
             break;
         }
@@ -374,65 +467,86 @@ __global__ __launch_bounds__(most_threads) void logits_kernel(Launch l)
 #pragma unroll
             for (int e = 0; e < 8; ++e)
             {
-                x[i][e] = soft          ? weight(x[i][e], top, factor) * scale
-                          : part.broken ? __uint_as_float(0x7fc00000u)
-                                        : (token + e == part.first ? 1.0f : 0.0f);
+                if (soft)
+                {
+                    x[i][e] = (S == Step::whole ? x[i][e] : weight(x[i][e], top, factor)) * scale;
+                }
+                else
+                {
+                    x[i][e] = part.broken ? __uint_as_float(0x7fc00000u) : token + e == part.first ? 1.0f : 0.0f;
+                }
             }
         }
-        store8<O>(out + token, p.to - token, l.aligned, x[i]);
+        const auto store = [&](auto type)
+        {
+            constexpr Type T = decltype(type)::value;
+            store8<T>(static_cast<value_t<T>*>(l.rows.out) + at + token, to - token, l.aligned, x[i]);
+        };
+        l.rows.out_type == Type::single ? store(std::integral_constant<Type, Type::single>{})
+        : l.rows.out_type == Type::bf16 ? store(std::integral_constant<Type, Type::bf16>{})
+                                        : store(std::integral_constant<Type, Type::half>{});
     }
 }
 
-// Threads and eights a thread, of a row or a part of one.
+// Threads, eights of a thread, parts of a row.
 struct Shape
 {
     int threads, vectors, splits, width;
 };
-Shape shape_of(int alphabet)
+Shape shape_of(const LogitRows& rows, std::size_t history)
 {
-    const int eights = (alphabet + 7) / 8;
+    const int eights = (rows.alphabet + 7) / 8;
     Shape s;
-    s.threads = std::min(most_threads, (eights + lanes - 1) / lanes * lanes);
+    // Threads for the tokens or, where these are few and the history is long, for that.
+    const std::size_t wanted = std::max(std::size_t(eights), std::min<std::size_t>(history / asked, most_threads));
+    s.threads = int(std::min<std::size_t>(most_threads, (wanted + lanes - 1) / lanes * lanes));
     const int rounds = (eights + s.threads - 1) / s.threads;
-    s.vectors = rounds <= 1 ? 1 : rounds <= 2 ? 2 : rounds <= 4 ? 4 : 8;
+    s.vectors = rounds <= 1 ? 1 : rounds <= 2 ? 2 : most_vectors;
+    if (rounds > most_vectors || !rows.probabilities)
+    {
+        // Parts, then, of fewer tokens where rows are few: two workgroups a unit at least, if there are as many.
+        const int units = compute_units();
+        while (s.vectors > 1 && std::size_t(rows.rows) * ((rounds + s.vectors - 1) / s.vectors) < std::size_t(2 * units))
+        {
+            s.vectors /= 2;
+        }
+    }
     s.width = 8 * s.threads * s.vectors;
-    s.splits = (alphabet + s.width - 1) / s.width;
+    s.splits = (rows.alphabet + s.width - 1) / s.width;
     return s;
 }
 
-template <Type T, Type O, Step S> void launch(const Launch& l, const Shape& s, hipStream_t stream)
+template <Step S> void launch(const Launch& l, const Shape& s, bool narrow, hipStream_t stream)
 {
     const unsigned grid = unsigned(l.rows.rows) * unsigned(l.splits);
-    const std::size_t bytes = std::size_t(8 * s.threads) * 4 * (l.rules.bias_starts ? 2 : 1);
-    const auto go = [&](auto kernel) { kernel<<<grid, unsigned(s.threads), bytes, stream>>>(l); };
-    s.vectors == 1   ? go(logits_kernel<T, O, S, 1>)
-    : s.vectors == 2 ? go(logits_kernel<T, O, S, 2>)
-    : s.vectors == 4 ? go(logits_kernel<T, O, S, 4>)
-                     : go(logits_kernel<T, O, S, 8>);
-    check_hip(hipGetLastError(), "logits launch");
-}
-
-template <Type T, Type O> void steps(const Launch& l, const Shape& s, hipStream_t stream)
-{
-    if (!l.rows.probabilities)
+    const auto go = [&](auto kernel, int held, int each)
     {
-        launch<T, O, Step::adjust>(l, s, stream);
-    }
-    else if (s.splits == 1)
+        const std::size_t bytes = std::size_t(8 * s.threads) * held * each * 4;
+        kernel<<<grid, unsigned(s.threads), bytes, stream>>>(l);
+    };
+    const auto of = [&](auto wide, auto few)
     {
-        launch<T, O, Step::whole>(l, s, stream);
+        constexpr bool W = decltype(wide)::value, N = decltype(few)::value;
+        constexpr int each = Words<N>::each;
+        s.vectors == 1   ? go(logits_kernel<S, W, 1, 1, N>, 1, each)
+        : s.vectors == 2 ? go(logits_kernel<S, W, 2, 2, N>, 1, each)
+                         : go(logits_kernel<S, W, 4, 4, N>, 1, each);
+    };
+    if (l.rows.type == Type::single)
+    {
+        narrow ? of(std::true_type{}, std::true_type{}) : of(std::true_type{}, std::false_type{});
     }
     else
     {
-        launch<T, O, Step::parts>(l, s, stream);
-        launch<T, O, Step::finish>(l, s, stream);
+        narrow ? of(std::false_type{}, std::true_type{}) : of(std::false_type{}, std::false_type{});
     }
+    check_hip(hipGetLastError(), "logits launch");
 }
 } // namespace
 
 std::size_t logits_workspace(const LogitRows& rows)
 {
-    const Shape s = shape_of(rows.alphabet);
+    const Shape s = shape_of(rows, 0); // a history changes the threads of rows in one part alone
     return rows.probabilities && s.splits > 1 ? std::size_t(rows.rows) * s.splits * sizeof(Part) : 0;
 }
 
@@ -443,28 +557,33 @@ void adjust_logits(const LogitRows& rows, const LogitRules& rules, void* workspa
     {
         return;
     }
-    const Shape s = shape_of(rows.alphabet);
+    const std::size_t history = rules.history ? rules.history_stride : 0;
+    const Shape s = shape_of(rows, history);
     require(std::size_t(rows.rows) * s.splits < (std::size_t(1) << 31), "logits: too many rows");
     require(bytes >= logits_workspace(rows) && (workspace || !logits_workspace(rows)), "logits: workspace too small");
     const auto whole = [](const void* pointer, std::size_t stride, Type type)
     { return reinterpret_cast<std::uintptr_t>(pointer) % 16 == 0 && stride * (type == Type::single ? 4 : 2) % 16 == 0; };
-    const Launch l = {rows, rules, static_cast<Part*>(workspace), s.splits, s.width,
-                      whole(rows.logits, rows.stride, rows.type) && whole(rows.out, rows.out_stride, rows.out_type)};
-    const auto to = [&](auto in)
+    const Launch l = {rows,
+                      rules,
+                      static_cast<Part*>(workspace),
+                      s.splits,
+                      s.width,
+                      whole(rows.logits, rows.stride, rows.type) && whole(rows.out, rows.out_stride, rows.out_type),
+                      rules.history || rules.tokens};
+    const std::size_t nodes = !rules.tokens ? 0 : rules.mask ? 64 * rules.words : std::size_t(rows.rows);
+    const bool narrow = history + nodes < (1u << 15) && std::size_t(rules.biases) < (1u << 16);
+    if (!rows.probabilities)
     {
-        constexpr Type T = decltype(in)::value;
-        switch (rows.out_type)
-        {
-        case Type::bf16: return steps<T, Type::bf16>(l, s, stream);
-        case Type::half: return steps<T, Type::half>(l, s, stream);
-        default: return steps<T, Type::single>(l, s, stream);
-        }
-    };
-    switch (rows.type)
+        launch<Step::adjust>(l, s, narrow, stream);
+    }
+    else if (s.splits == 1)
     {
-    case Type::bf16: return to(std::integral_constant<Type, Type::bf16>{});
-    case Type::half: return to(std::integral_constant<Type, Type::half>{});
-    default: return to(std::integral_constant<Type, Type::single>{});
+        launch<Step::whole>(l, s, narrow, stream);
+    }
+    else
+    {
+        launch<Step::parts>(l, s, narrow, stream);
+        launch<Step::finish>(l, s, narrow, stream);
     }
 }
 } // namespace tsac_hip
