@@ -681,7 +681,8 @@ class Logits:
                         seen[t] = True
                 v, w = x[r].copy(), e[r]
                 v = np.where(seen, np.where(v > 0, v / float(self.repetition[s]), v * float(self.repetition[s])), v)
-                w = w + np.where(seen, H * np.abs(v), 0)
+                # A positive one is taken times a reciprocal: two roundings, (1 + H)^2 - 1 < 2.01 H.
+                w = w + np.where(seen, 2.01 * H * np.abs(v), 0)
                 f = float(self.frequency[s]) * count
                 v = v - f
                 w = w + np.where(count > 0, H * np.abs(f) + H * np.abs(v), 0)

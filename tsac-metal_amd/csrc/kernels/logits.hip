@@ -1,7 +1,7 @@
 // What a program does to a model's logits before it samples or verifies drafts: penalties for tokens that a
 // sequence has had already, biases, a grammar's mask, and the softmax at a temperature.
 //
-//   x = logit; where the token was had: x / r if x > 0, else x r        (repetition r)
+//   x = logit; where the token was had: x * fl(1 / r) if x > 0, else x r (repetition r)
 //   x = x - f count - (count > 0 ? g : 0)                                (frequency f, presence g)
 //   x = x + bias;  -infinity where the grammar has no bit
 //   p = e^((x - m) / t) / sum e^((x - m) / t),  m = max x;   t = 0: 1 at the lowest of the largest
@@ -27,8 +27,8 @@ namespace tsac_hip
 namespace
 {
 constexpr int lanes = 64;
-constexpr int most_threads = 1024;
-constexpr int most_vectors = 4; // eights of a thread
+constexpr int most_threads = 512;
+constexpr int most_vectors = 8; // eights of a thread
 constexpr int asked = 8;        // tokens of the history that a thread has in flight
 constexpr float minus_infinity = -__builtin_inff();
 constexpr float log2e = 1.44269504f;
@@ -85,12 +85,25 @@ template <bool Narrow> struct Words
         {
             eight(memory + chunk + at, bias);
         }
-#pragma unroll
-        for (int e = 0; Narrow && e < 8; ++e)
+        else
         {
-            bias[e] = said[e] >> 16;
-            said[e] &= 0xffffu;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+            {
+                bias[e] = said[e];
+                said[e] &= 0xffffu;
+            }
         }
+    }
+    // Whether one of eight has a bias, and its place.
+    static __device__ __forceinline__ bool biased(const unsigned (&bias)[8])
+    {
+        const unsigned any = bias[0] | bias[1] | bias[2] | bias[3] | bias[4] | bias[5] | bias[6] | bias[7];
+        return Narrow ? any > 0xffffu : any != 0;
+    }
+    static __device__ __forceinline__ unsigned place(unsigned bias)
+    {
+        return Narrow ? bias >> 16 : bias;
     }
     static __device__ __forceinline__ void eight(const unsigned* from, unsigned (&to)[8])
     {
@@ -127,16 +140,23 @@ struct Exchange
     int i[most_threads / lanes];
 };
 
-// e^((x - top) / t) as a power of two. -infinity gives 0, what is not a number and +infinity no number.
+// e^((x - top) / t) as a power of two, of a finite top. -infinity gives 0, what is not a number and +infinity no number.
 __device__ __forceinline__ float weight(float x, float top, float per_log2)
 {
-    return x == minus_infinity ? 0.0f : __builtin_amdgcn_exp2f((x - top) * per_log2);
+    return __builtin_amdgcn_exp2f((x - top) * per_log2);
 }
 
-// A temperature's factor; so small that it overflows, it is the largest number: 0 times it is still 0.
+// What stands for the largest of a row in which nothing is above -infinity: its weights are 0, or no numbers.
+__device__ __forceinline__ float reference(float top)
+{
+    return top == minus_infinity ? 0.0f : top;
+}
+
+// A temperature's factor; where that would be infinite the largest number, which times 0 is still 0, where it would be 0 a
+// small one, which times -infinity is still that.
 __device__ __forceinline__ float factor_of(float temperature)
 {
-    return __builtin_fminf(log2e / temperature, 3.402823466e38f);
+    return __builtin_fmaxf(__builtin_fminf(log2e / temperature, 0x1.fffffep127f), 0x1p-126f);
 }
 
 // What is known of values held in registers: the largest and its lowest place, the sum of weights, which stand in the
@@ -169,7 +189,7 @@ __device__ __forceinline__ Part part_of(float (&x)[Vectors][8], int from, float 
 #pragma unroll
             for (int e = 0; e < 8; ++e)
             {
-                x[i][e] = weight(x[i][e], top, factor);
+                x[i][e] = weight(x[i][e], reference(top), factor);
                 sum += x[i][e];
             }
         }
@@ -230,7 +250,7 @@ template <bool Wide> struct Raw
 
 // Rounds: how often LDS holds the words of a part of the workgroup's tokens.
 template <Step S, bool Wide, int Vectors, int Rounds, bool Narrow>
-__global__ __launch_bounds__(most_threads) void logits_kernel(Launch l)
+__global__ __launch_bounds__(most_threads, 4) void logits_kernel(Launch l)
 {
     constexpr int held = Vectors / Rounds; // eights of a thread in a round
     extern __shared__ __attribute__((aligned(16))) unsigned memory[];
@@ -277,7 +297,7 @@ __global__ __launch_bounds__(most_threads) void logits_kernel(Launch l)
     }
 
     const float repetition = r.repetition ? r.repetition[s] : 1.0f, presence = r.presence ? r.presence[s] : 0.0f;
-    const float frequency = r.frequency ? r.frequency[s] : 0.0f;
+    const float frequency = r.frequency ? r.frequency[s] : 0.0f, reciprocal = 1.0f / repetition;
     const int bias_begin = r.bias_starts ? max(0, min(r.bias_starts[s], r.biases)) : 0;
     const int bias_end = r.bias_starts ? min(r.bias_starts[s + 1], r.biases) : 0;
     const bool edited = l.counted || bias_begin < bias_end;
@@ -392,19 +412,25 @@ __global__ __launch_bounds__(most_threads) void logits_kernel(Launch l)
             {
                 unsigned said[8], bias[8];
                 words.read(8 * (h * threads + thread), said, bias);
+                // Without branches: with a long history most waves have a token of it in each place. Past the last token
+                // nothing is counted, and -infinity stays what it is.
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
                 {
-                    if (said[e] && e < there)
+                    const float times = float(said[e] >> 1);
+                    x[i][e] *= said[e] ? (x[i][e] > 0.0f ? reciprocal : repetition) : 1.0f;
+                    x[i][e] = __builtin_fmaf(-frequency, times, x[i][e]);
+                    x[i][e] = __builtin_fmaf(-presence, __builtin_fminf(times, 1.0f), x[i][e]);
+                }
+                if (words.biased(bias))
+                {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
                     {
-                        const float times = float(said[e] >> 1);
-                        x[i][e] = x[i][e] > 0.0f ? x[i][e] / repetition : x[i][e] * repetition;
-                        x[i][e] -= frequency * times;
-                        x[i][e] -= times > 0.0f ? presence : 0.0f;
-                    }
-                    if (bias[e] && e < there)
-                    {
-                        x[i][e] += r.bias_values[bias_begin + int(bias[e]) - 1];
+                        if (const unsigned place = words.place(bias[e]); place && e < there)
+                        {
+                            x[i][e] += r.bias_values[bias_begin + int(place) - 1];
+                        }
                     }
                 }
             }
@@ -415,7 +441,8 @@ __global__ __launch_bounds__(most_threads) void logits_kernel(Launch l)
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
                 {
-                    x[i][e] = bits >> e & 1 ? x[i][e] : minus_infinity;
+                    const int keep = int(bits << (31 - e)) >> 31; // all bits or none
+                    x[i][e] = __uint_as_float((__float_as_uint(x[i][e]) & keep) | (0xff800000u & ~keep));
                 }
             }
         }
@@ -449,7 +476,7 @@ __global__ __launch_bounds__(most_threads) void logits_kernel(Launch l)
             }
             return;
         }
-        top = part.top;
+        top = reference(part.top);
         factor = factor_of(temperature);
         scale = part.sum == 0.0f ? 0.0f : 1.0f / part.sum;
     }
@@ -501,7 +528,7 @@ Shape shape_of(const LogitRows& rows, std::size_t history)
     const std::size_t wanted = std::max(std::size_t(eights), std::min<std::size_t>(history / asked, most_threads));
     s.threads = int(std::min<std::size_t>(most_threads, (wanted + lanes - 1) / lanes * lanes));
     const int rounds = (eights + s.threads - 1) / s.threads;
-    s.vectors = rounds <= 1 ? 1 : rounds <= 2 ? 2 : most_vectors;
+    s.vectors = rounds <= 1 ? 1 : rounds <= 2 ? 2 : rounds <= 4 ? 4 : most_vectors;
     if (rounds > most_vectors || !rows.probabilities)
     {
         // Parts, then, of fewer tokens where rows are few: two workgroups a unit at least, if there are as many.
@@ -528,9 +555,12 @@ template <Step S> void launch(const Launch& l, const Shape& s, bool narrow, hipS
     {
         constexpr bool W = decltype(wide)::value, N = decltype(few)::value;
         constexpr int each = Words<N>::each;
+        // Words of at most 64 KiB at a time, so that a unit has two workgroups.
+        constexpr int most = N ? 4 : 2;
         s.vectors == 1   ? go(logits_kernel<S, W, 1, 1, N>, 1, each)
-        : s.vectors == 2 ? go(logits_kernel<S, W, 2, 2, N>, 1, each)
-                         : go(logits_kernel<S, W, 4, 4, N>, 1, each);
+        : s.vectors == 2 ? go(logits_kernel<S, W, 2, 1, N>, 2, each)
+        : s.vectors == 4 ? go(logits_kernel<S, W, 4, 4 / most, N>, most, each)
+                         : go(logits_kernel<S, W, 8, 8 / most, N>, most, each);
     };
     if (l.rows.type == Type::single)
     {
