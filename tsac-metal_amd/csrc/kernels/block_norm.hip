@@ -12,8 +12,12 @@
 // A row's values stay in the registers of its threads, so that the mean, the squares around it and
 // the largest value each are a pass over registers, in 32 bits and in an order that depends on the
 // width alone. What bounds it is memory; a row of few values one wave, which needs no barrier.
+#include "lanes.hpp"
 #include "model_step.hpp"
 #include "values.hpp"
+
+#include <algorithm>
+#include <type_traits>
 
 namespace tsac_hip
 {
@@ -23,19 +27,15 @@ constexpr int lanes = 64;
 
 template <int Threads, class Join> __device__ __forceinline__ float joined(float value, float* shared, Join join)
 {
-#pragma unroll
-    for (int step = 1; step < lanes; step *= 2)
-    {
-        value = join(value, __shfl_xor(value, step));
-    }
+    value = over_lanes(value, join);
     if constexpr (Threads > lanes)
     {
-        __syncthreads(); // the last one's values have been read
+        lds_barrier(); // the last one's values have been read
         if (threadIdx.x % lanes == 0)
         {
             shared[threadIdx.x / lanes] = value;
         }
-        __syncthreads();
+        lds_barrier();
         value = shared[0];
 #pragma unroll
         for (int i = 1; i < Threads / lanes; ++i)
@@ -62,7 +62,40 @@ template <int Threads> __device__ __forceinline__ unsigned row_max_bits(unsigned
                                            }));
 }
 
-template <Type T, int Vectors, int Threads>
+// Eight values from `at` on, of which `count` there are, as they lie in memory; 0 behind them. `Whole`: there are eight or
+// none, at a multiple of 16 bytes.
+template <bool Whole, Type T>
+__device__ __forceinline__ Eight<T> fetch8(const value_t<T>* at, int count, bool aligned)
+{
+    Eight<T> eight = {};
+    if (Whole ? count > 0 : aligned && count >= 8)
+    {
+        eight = *reinterpret_cast<const Eight<T>*>(at);
+    }
+    else if constexpr (!Whole)
+    {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+        {
+            if (i < count)
+            {
+                eight.v[i] = at[i];
+            }
+        }
+    }
+    return eight;
+}
+
+template <bool Whole, Type T>
+__device__ __forceinline__ void put8(value_t<T>* at, int count, bool aligned, const float (&in)[8])
+{
+    if (count > 0)
+    {
+        store8<T>(at, Whole ? 8 : count, Whole || aligned, in);
+    }
+}
+
+template <bool Whole, Type T, int Vectors, int Threads>
 __device__ __forceinline__ void normalise(float (&v)[Vectors][8], const NormRule& rule, bool aligned, int width,
                                           float epsilon, int thread, float* shared)
 {
@@ -93,7 +126,7 @@ __device__ __forceinline__ void normalise(float (&v)[Vectors][8], const NormRule
 #pragma unroll
         for (int e = 0; e < 8; ++e)
         {
-            v[i][e] = e < count ? v[i][e] - mean : 0.0f;
+            v[i][e] = (Whole ? 0 : e) < count ? v[i][e] - mean : 0.0f;
             squares = __builtin_fmaf(v[i][e], v[i][e], squares);
         }
     }
@@ -102,22 +135,22 @@ __device__ __forceinline__ void normalise(float (&v)[Vectors][8], const NormRule
     for (int i = 0; i < Vectors; ++i)
     {
         const int at = 8 * (i * Threads + thread), count = width - at;
-        float gain[8], bias[8];
-        if (count > 0 && rule.gain)
+        Eight<T> gain = {}, bias = {};
+        if (rule.gain)
         {
-            load8<T>(static_cast<const value_t<T>*>(rule.gain) + at, count, aligned, 0.0f, gain);
+            gain = fetch8<Whole, T>(static_cast<const value_t<T>*>(rule.gain) + at, count, aligned);
         }
-        if (count > 0 && rule.bias)
+        if (rule.bias)
         {
-            load8<T>(static_cast<const value_t<T>*>(rule.bias) + at, count, aligned, 0.0f, bias);
+            bias = fetch8<Whole, T>(static_cast<const value_t<T>*>(rule.bias) + at, count, aligned);
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e)
         {
             float x = v[i][e] * factor;
-            x = rule.gain ? x * gain[e] : x;
-            x = rule.bias ? x + bias[e] : x;
-            v[i][e] = e < count ? x : 0.0f;
+            x = rule.gain ? x * widen<T>(gain.v[e]) : x;
+            x = rule.bias ? x + widen<T>(bias.v[e]) : x;
+            v[i][e] = (Whole ? 0 : e) < count ? x : 0.0f;
         }
     }
 }
@@ -148,67 +181,104 @@ enum Aligned
     norm_aligned = 64
 };
 
-// T: the values; R: the residual. A row is taken by Threads threads, each Vectors times eight values.
-template <Type T, Type R, int Vectors, int Threads>
-__global__ __launch_bounds__(Threads > 256 ? Threads : 256) void block_norm_kernel(BlockRows p, int aligned)
+// T: the values; R: the residual. A row is taken by Threads threads, each Vectors times eight values. With `Whole` a
+// workgroup takes rows one after the other, and the next one's are on their way while one is worked on: they pass
+// barriers, which are for LDS alone. 8190 rows of 8192 to 8 bits: ...
+template <Type T, Type R, int Vectors, int Threads, bool Whole>
+__global__ __launch_bounds__(Threads > 256 ? Threads : 256, 4) void block_norm_kernel(BlockRows p, int aligned)
 {
     constexpr int together = Threads < 256 ? 256 / Threads : 1; // rows of a workgroup
     __shared__ float shared[Threads > lanes ? Threads / lanes : 1];
-    const int thread = threadIdx.x % Threads;
-    const int row = blockIdx.x * together + threadIdx.x / Threads;
-    if (row >= p.rows) // whole waves: a row of several has its workgroup for itself
+    const int thread = threadIdx.x % Threads, stride = gridDim.x * together;
+    int row = blockIdx.x * together + threadIdx.x / Threads;
+    Eight<T> inputs[Vectors];
+    Eight<R> residuals[Vectors];
+    const auto ask_input = [&](int from)
     {
-        return;
-    }
-    float v[Vectors][8];
-    const auto* x = static_cast<const value_t<T>*>(p.input) + std::size_t(row) * p.input_stride;
-#pragma unroll
-    for (int i = 0; i < Vectors; ++i)
-    {
-        const int at = 8 * (i * Threads + thread);
-        load8<T>(x + at, p.width - at, aligned & input_aligned, 0.0f, v[i]);
-    }
-    float before[Vectors][8];
-    const auto* residual = static_cast<const value_t<R>*>(p.residual) + std::size_t(row) * p.residual_stride;
-    if (p.residual)
-    {
+        const auto* x = static_cast<const value_t<T>*>(p.input) + std::size_t(from) * p.input_stride;
 #pragma unroll
         for (int i = 0; i < Vectors; ++i)
         {
             const int at = 8 * (i * Threads + thread);
-            load8<R>(residual + at, p.width - at, aligned & residual_aligned, 0.0f, before[i]);
+            inputs[i] = fetch8<Whole, T>(x + at, p.width - at, aligned & input_aligned);
+        }
+    };
+    const auto ask_residual = [&](int from)
+    {
+        const auto* x = static_cast<const value_t<R>*>(p.residual) + std::size_t(from) * p.residual_stride;
+#pragma unroll
+        for (int i = 0; p.residual && i < Vectors; ++i)
+        {
+            const int at = 8 * (i * Threads + thread);
+            residuals[i] = fetch8<Whole, R>(x + at, p.width - at, aligned & residual_aligned);
+        }
+    };
+    // Whole waves end together: a row of several has its workgroup for itself.
+    if (Whole && row < p.rows)
+    {
+        ask_input(row);
+        ask_residual(row);
+    }
+    for (; row < p.rows; row += stride)
+    {
+    if constexpr (!Whole)
+    {
+        ask_input(row);
+    }
+    float v[Vectors][8], before[Whole ? Vectors : 1][8];
+#pragma unroll
+    for (int i = 0; i < Vectors; ++i)
+    {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+        {
+            v[i][e] = widen<T>(inputs[i].v[e]);
+            if (Whole && p.residual)
+            {
+                before[Whole ? i : 0][e] = widen<R>(residuals[i].v[e]);
+            }
         }
     }
-    normalise<T, Vectors, Threads>(v, p.post, aligned & post_aligned, p.width, p.epsilon, thread, shared);
+    if constexpr (Whole)
+    {
+        const int next = min(row + stride, p.rows - 1); // the last one's once more, at the end
+        ask_input(next);
+        ask_residual(next);
+    }
+    normalise<Whole, T, Vectors, Threads>(v, p.post, aligned & post_aligned, p.width, p.epsilon, thread, shared);
+    if constexpr (!Whole)
+    {
+        ask_residual(row);
+    }
     const auto* gate = static_cast<const value_t<T>*>(p.gate) + std::size_t(row) * p.gate_stride;
     auto* sum = static_cast<value_t<R>*>(p.sum) + std::size_t(row) * p.sum_stride;
 #pragma unroll
     for (int i = 0; i < Vectors; ++i)
     {
         const int at = 8 * (i * Threads + thread), count = p.width - at;
-        float gates[8];
+        Eight<T> gates = {};
         if (p.gate)
         {
-            load8<T>(gate + at, count, aligned & gate_aligned, 0.0f, gates);
+            gates = fetch8<Whole, T>(gate + at, count, aligned & gate_aligned);
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e)
         {
-            float u = p.gate ? v[i][e] * gates[e] : v[i][e];
+            float u = p.gate ? v[i][e] * widen<T>(gates.v[e]) : v[i][e];
             u *= p.scale;
-            u = p.residual ? before[i][e] + u : u;
-            v[i][e] = e < count ? u : 0.0f;
+            u = !p.residual ? u : (Whole ? before[Whole ? i : 0][e] : widen<R>(residuals[i].v[e])) + u;
+            v[i][e] = (Whole ? 0 : e) < count ? u : 0.0f;
         }
-        if (p.sum && count > 0)
+        if (p.sum)
         {
-            store8<R>(sum + at, count, aligned & sum_aligned, v[i]);
+            put8<Whole, R>(sum + at, count, aligned & sum_aligned, v[i]);
         }
     }
     if (!p.out)
     {
-        return;
+        continue;
     }
-    normalise<T, Vectors, Threads>(v, p.norm, aligned & norm_aligned, p.width, p.epsilon, thread, shared);
+    normalise<Whole, T, Vectors, Threads>(v, p.norm, aligned & norm_aligned, p.width, p.epsilon, thread, shared);
     if (!p.out_scales)
     {
         auto* out = static_cast<value_t<T>*>(p.out) + std::size_t(row) * p.out_stride;
@@ -216,12 +286,9 @@ __global__ __launch_bounds__(Threads > 256 ? Threads : 256) void block_norm_kern
         for (int i = 0; i < Vectors; ++i)
         {
             const int at = 8 * (i * Threads + thread), count = p.width - at;
-            if (count > 0)
-            {
-                store8<T>(out + at, count, aligned & out_aligned, v[i]);
-            }
+            put8<Whole, T>(out + at, count, aligned & out_aligned, v[i]);
         }
-        return;
+        continue;
     }
     unsigned top = 0;
 #pragma unroll
@@ -258,11 +325,11 @@ __global__ __launch_bounds__(Threads > 256 ? Threads : 256) void block_norm_kern
             const int n = zero ? 0 : nearest(v[i][e] * lift, lifted, reciprocal);
             packed |= uint64_t(uint8_t(n)) << 8 * e;
         }
-        if (count >= 8) // rows of 8-bit integers begin at multiples of 16 bytes
+        if (Whole ? count > 0 : count >= 8) // rows of 8-bit integers begin at multiples of 16 bytes
         {
             *reinterpret_cast<uint64_t*>(q + at) = packed;
         }
-        else
+        else if constexpr (!Whole)
         {
             for (int e = 0; e < count; ++e)
             {
@@ -270,25 +337,35 @@ __global__ __launch_bounds__(Threads > 256 ? Threads : 256) void block_norm_kern
             }
         }
     }
+    }
 }
 
 template <Type T, Type R> void launch(const BlockRows& p, int aligned, hipStream_t stream)
 {
-    const auto go = [&](auto kernel, int threads)
+    // A workgroup takes several rows where there are more than are worked on at a time.
+    const auto go = [&](auto kernel, int threads, int a_unit)
     {
         const int together = threads < 256 ? 256 / threads : 1;
-        kernel<<<unsigned((p.rows + together - 1) / together), threads * together, 0, stream>>>(p, aligned);
+        const int groups = std::min<long>((p.rows + together - 1) / together, long(compute_units()) * a_unit);
+        kernel<<<unsigned(groups), threads * together, 0, stream>>>(p, aligned);
     };
-    // By the width alone, so that a row's result does not depend on how many there are.
-    const int w = p.width;
-    w <= 512      ? go(block_norm_kernel<T, R, 1, 64>, 64)
-    : w <= 1024   ? go(block_norm_kernel<T, R, 2, 64>, 64)
-    : w <= 2048   ? go(block_norm_kernel<T, R, 1, 256>, 256)
-    : w <= 4096   ? go(block_norm_kernel<T, R, 2, 256>, 256)
-    : w <= 8192   ? go(block_norm_kernel<T, R, 4, 256>, 256)
-    : w <= 16384  ? go(block_norm_kernel<T, R, 2, 1024>, 1024)
-    : w <= 32768  ? go(block_norm_kernel<T, R, 4, 1024>, 1024)
-                  : go(block_norm_kernel<T, R, 8, 1024>, 1024);
+    const auto of = [&](auto is_whole)
+    {
+        constexpr bool W = decltype(is_whole)::value;
+        const auto a_unit = [](int groups) { return W ? groups : 1 << 20; };
+        // By the width alone, so that a row's result does not depend on how many there are.
+        const int w = p.width;
+        w <= 512      ? go(block_norm_kernel<T, R, 1, 64, W>, 64, a_unit(8))
+        : w <= 1024   ? go(block_norm_kernel<T, R, 2, 64, W>, 64, a_unit(4))
+        : w <= 2048   ? go(block_norm_kernel<T, R, 1, 256, W>, 256, a_unit(8))
+        : w <= 4096   ? go(block_norm_kernel<T, R, 2, 256, W>, 256, a_unit(4))
+        : w <= 8192   ? go(block_norm_kernel<T, R, 2, 512, W>, 512, a_unit(2))
+        : w <= 16384  ? go(block_norm_kernel<T, R, 2, 1024, W>, 1024, a_unit(1))
+        : w <= 32768  ? go(block_norm_kernel<T, R, 4, 1024, false>, 1024, 1 << 20)
+                      : go(block_norm_kernel<T, R, 8, 1024, false>, 1024, 1 << 20);
+    };
+    constexpr int every = input_aligned | gate_aligned | residual_aligned | sum_aligned | out_aligned | post_aligned | norm_aligned;
+    aligned == every && p.width % 8 == 0 ? of(std::true_type{}) : of(std::false_type{});
     check_hip(hipGetLastError(), "block norm launch");
 }
 } // namespace

@@ -29,7 +29,11 @@ namespace
 constexpr int lanes = 64;
 constexpr int most_threads = 512;
 constexpr int most_vectors = 8; // eights of a thread
-constexpr int asked = 8;        // tokens of the history that a thread has in flight
+// Tokens of the history that a thread has in flight.
+constexpr int asked_for(int vectors)
+{
+    return vectors <= 2 ? 16 : 8;
+}
 constexpr float minus_infinity = -__builtin_inff();
 constexpr float log2e = 1.44269504f;
 
@@ -253,6 +257,7 @@ template <Step S, bool Wide, int Vectors, int Rounds, bool Narrow>
 __global__ __launch_bounds__(most_threads, 4) void logits_kernel(Launch l)
 {
     constexpr int held = Vectors / Rounds; // eights of a thread in a round
+    constexpr int asked = asked_for(Vectors);
     extern __shared__ __attribute__((aligned(16))) unsigned memory[];
     __shared__ Exchange shared;
     const int thread = threadIdx.x, threads = blockDim.x;
@@ -267,7 +272,11 @@ __global__ __launch_bounds__(most_threads, 4) void logits_kernel(Launch l)
         return;
     }
 
-    // The first of the history, then the logits: loads complete in the order of issue.
+    // Everything that is read is asked for at once, in the order of its use, in which loads complete: the first biases,
+    // what of the history and of the line's nodes a thread can hold, the logits, the grammar's bits.
+    const int bias_begin = r.bias_starts ? max(0, min(r.bias_starts[s], r.biases)) : 0;
+    const int bias_end = r.bias_starts ? min(r.bias_starts[s + 1], r.biases) : 0;
+    const int bias_token = bias_begin + thread < bias_end ? r.bias_tokens[bias_begin + thread] : -1;
     int length = 0, prompt = 0;
     int past[asked];
     const int* const history = r.history + std::size_t(s) * r.history_stride;
@@ -283,8 +292,18 @@ __global__ __launch_bounds__(most_threads, 4) void logits_kernel(Launch l)
             past[i] = at < length ? history[at] : -1;
         }
     }
+    const uint64_t* const line = r.mask ? r.mask + std::size_t(row) * r.words : nullptr;
+    const int nodes = !r.tokens ? 0 : r.mask ? int(min(std::size_t(count), 64 * r.words)) : node + 1;
+    int drafted = -1;
+    uint64_t lined = ~uint64_t(0);
+    if (thread < nodes)
+    {
+        drafted = r.tokens[first + thread];
+        lined = line ? line[thread / 64] : lined;
+    }
     const std::size_t begin = std::size_t(row) * l.rows.stride;
     Raw<Wide> raw[Vectors];
+    uint8_t grammar[Vectors]; // tokens come in eights, so that their bits are a byte
 #pragma unroll
     for (int i = 0; i < Vectors; ++i)
     {
@@ -294,12 +313,14 @@ __global__ __launch_bounds__(most_threads, 4) void logits_kernel(Launch l)
             raw[i] = *reinterpret_cast<const Raw<Wide>*>(static_cast<const char*>(l.rows.logits) +
                                                          (begin + token) * (Wide ? 4 : 2));
         }
+        if (r.allowed && token < to)
+        {
+            grammar[i] = reinterpret_cast<const uint8_t*>(r.allowed + std::size_t(row) * r.allowed_stride)[token / 8];
+        }
     }
 
     const float repetition = r.repetition ? r.repetition[s] : 1.0f, presence = r.presence ? r.presence[s] : 0.0f;
     const float frequency = r.frequency ? r.frequency[s] : 0.0f, reciprocal = 1.0f / repetition;
-    const int bias_begin = r.bias_starts ? max(0, min(r.bias_starts[s], r.biases)) : 0;
-    const int bias_end = r.bias_starts ? min(r.bias_starts[s + 1], r.biases) : 0;
     const bool edited = l.counted || bias_begin < bias_end;
     const Words<Narrow> words = {memory, 8 * threads * held};
     float x[Vectors][8];
@@ -317,13 +338,21 @@ __global__ __launch_bounds__(most_threads, 4) void logits_kernel(Launch l)
             lds_barrier();
             if (bias_begin < bias_end)
             {
-                for (int i = bias_begin + thread; i < bias_end; i += threads)
+                const auto add = [&](int token, int i)
                 {
-                    const unsigned t = unsigned(r.bias_tokens[i]) - unsigned(base);
+                    const unsigned t = unsigned(token) - unsigned(base);
                     if (t < unsigned(words.chunk))
                     {
                         words.bias(t, unsigned(i - bias_begin) + 1);
                     }
+                };
+                if (const int i = bias_begin + thread; i < bias_end)
+                {
+                    add(bias_token, i);
+                }
+                for (int i = bias_begin + threads + thread; i < bias_end; i += threads)
+                {
+                    add(r.bias_tokens[i], i);
                 }
                 lds_barrier();
             }
@@ -364,16 +393,15 @@ __global__ __launch_bounds__(most_threads, 4) void logits_kernel(Launch l)
                     }
                 }
             }
-            if (r.tokens)
+            if (thread < nodes && (lined >> thread % 64 & 1))
             {
-                const uint64_t* const line = r.mask ? r.mask + std::size_t(row) * r.words : nullptr;
-                const int nodes = r.mask ? int(min(std::size_t(count), 64 * r.words)) : node + 1;
-                for (int j = thread; j < nodes; j += threads)
+                had(drafted, true);
+            }
+            for (int j = thread + threads; j < nodes; j += threads)
+            {
+                if (!line || (line[j / 64] >> j % 64 & 1))
                 {
-                    if (!line || (line[j / 64] >> j % 64 & 1))
-                    {
-                        had(r.tokens[first + j], true);
-                    }
+                    had(r.tokens[first + j], true);
                 }
             }
             lds_barrier();
@@ -436,12 +464,10 @@ __global__ __launch_bounds__(most_threads, 4) void logits_kernel(Launch l)
             }
             if (r.allowed && there > 0)
             {
-                // Tokens come in eights, so that their bits are in one word.
-                const uint32_t bits = r.allowed[std::size_t(row) * r.allowed_stride + token / 32] >> token % 32;
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
                 {
-                    const int keep = int(bits << (31 - e)) >> 31; // all bits or none
+                    const int keep = int(unsigned(grammar[i]) << (31 - e)) >> 31; // all bits or none
                     x[i][e] = __uint_as_float((__float_as_uint(x[i][e]) & keep) | (0xff800000u & ~keep));
                 }
             }
@@ -525,15 +551,17 @@ Shape shape_of(const LogitRows& rows, std::size_t history)
     const int eights = (rows.alphabet + 7) / 8;
     Shape s;
     // Threads for the tokens or, where these are few and the history is long, for that.
-    const std::size_t wanted = std::max(std::size_t(eights), std::min<std::size_t>(history / asked, most_threads));
+    const std::size_t wanted = std::max(std::size_t(eights), std::min<std::size_t>(history / asked_for(1), most_threads));
     s.threads = int(std::min<std::size_t>(most_threads, (wanted + lanes - 1) / lanes * lanes));
     const int rounds = (eights + s.threads - 1) / s.threads;
     s.vectors = rounds <= 1 ? 1 : rounds <= 2 ? 2 : rounds <= 4 ? 4 : most_vectors;
     if (rounds > most_vectors || !rows.probabilities)
     {
-        // Parts, then, of fewer tokens where rows are few: two workgroups a unit at least, if there are as many.
+        // Parts, then: of four eights a thread (902 rows of 32,000, adjusted: 40 us, of eight 51, of two 49), of fewer
+        // where rows are few, for a workgroup a unit at least, if there are as many.
         const int units = compute_units();
-        while (s.vectors > 1 && std::size_t(rows.rows) * ((rounds + s.vectors - 1) / s.vectors) < std::size_t(2 * units))
+        s.vectors = std::min(s.vectors, 4);
+        while (s.vectors > 1 && std::size_t(rows.rows) * ((rounds + s.vectors - 1) / s.vectors) < std::size_t(units))
         {
             s.vectors /= 2;
         }
