@@ -169,6 +169,33 @@ __device__ __forceinline__ int nearest(float x, float scale, float reciprocal)
     return int(__builtin_fminf(__builtin_fmaxf(r, -127.0f), 127.0f));
 }
 
+// Eight of them, a byte each. x / scale + 1.5 2^23 has the whole number in its lowest bits; where the rest of one is half a step
+// or more, which takes a border within 2^-15 of a step, all are done with care.
+__device__ __forceinline__ uint2 nearest8(const float (&x)[8], float scale, float reciprocal)
+{
+    constexpr float whole = 0x1.8p23f;
+    float worst = 0.0f;
+    unsigned bits[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+    {
+        const float shifted = __builtin_fmaf(x[e], reciprocal, whole);
+        bits[e] = __float_as_uint(shifted);
+        worst = __builtin_fmaxf(worst, __builtin_fabsf(__builtin_fmaf(whole - shifted, scale, x[e])));
+    }
+    if (worst >= 0.5f * scale)
+    {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+        {
+            bits[e] = unsigned(nearest(x[e], scale, reciprocal));
+        }
+    }
+    const auto four = [](const unsigned* b)
+    { return __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u) | __builtin_amdgcn_perm(b[3], b[2], 0x04000c0cu); };
+    return make_uint2(four(bits), four(bits + 4));
+}
+
 // Which pointers of a row's are at multiples of 16 bytes, with their strides.
 enum Aligned
 {
@@ -310,30 +337,38 @@ __global__ __launch_bounds__(Threads > 256 ? Threads : 256, 4) void block_norm_k
     }
     // Small rows are taken times 2^64, which changes no quotient, so that the reciprocal is finite and half
     // the scale exact.
-    const float lift = most < 0x1p-60f ? 0x1p64f : 1.0f;
-    const float lifted = scale * lift, reciprocal = 1.0f / lifted;
-    const bool zero = !finite || scale == 0.0f;
+    const bool small = most < 0x1p-60f, zero = !finite || scale == 0.0f;
+    const float lifted = small ? scale * 0x1p64f : scale, reciprocal = 1.0f / lifted;
     auto* q = static_cast<int8_t*>(p.out) + std::size_t(row) * p.out_stride;
 #pragma unroll
     for (int i = 0; i < Vectors; ++i)
     {
         const int at = 8 * (i * Threads + thread), count = p.width - at;
-        uint64_t packed = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
+        uint2 packed = {};
+        if (!zero && small)
         {
-            const int n = zero ? 0 : nearest(v[i][e] * lift, lifted, reciprocal);
-            packed |= uint64_t(uint8_t(n)) << 8 * e;
+            // A scale of few bits may leave quotients past 127.
+            uint64_t bytes = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+            {
+                bytes |= uint64_t(uint8_t(nearest(v[i][e] * 0x1p64f, lifted, reciprocal))) << 8 * e;
+            }
+            packed = make_uint2(unsigned(bytes), unsigned(bytes >> 32));
+        }
+        else if (!zero)
+        {
+            packed = nearest8(v[i], lifted, reciprocal);
         }
         if (Whole ? count > 0 : count >= 8) // rows of 8-bit integers begin at multiples of 16 bytes
         {
-            *reinterpret_cast<uint64_t*>(q + at) = packed;
+            *reinterpret_cast<uint2*>(q + at) = packed;
         }
         else if constexpr (!Whole)
         {
             for (int e = 0; e < count; ++e)
             {
-                q[at + e] = int8_t(packed >> 8 * e);
+                q[at + e] = int8_t((e < 4 ? packed.x : packed.y) >> e % 4 * 8);
             }
         }
     }
