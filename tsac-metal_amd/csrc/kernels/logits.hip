@@ -27,6 +27,7 @@ namespace tsac_hip
 namespace
 {
 constexpr int lanes = 64;
+constexpr int units = 256; // of the card: a workspace is asked for where there is none, too
 constexpr int most_threads = 512;
 constexpr int most_vectors = 8; // eights of a thread
 // Tokens of the history that a thread has in flight.
@@ -559,7 +560,6 @@ Shape shape_of(const LogitRows& rows, std::size_t history)
     {
         // Parts, then: of four eights a thread (902 rows of 32,000, adjusted: 40 us, of eight 51, of two 49), of fewer
         // where rows are few, for a workgroup a unit at least, if there are as many.
-        const int units = compute_units();
         s.vectors = std::min(s.vectors, 4);
         while (s.vectors > 1 && std::size_t(rows.rows) * ((rounds + s.vectors - 1) / s.vectors) < std::size_t(units))
         {

@@ -934,7 +934,8 @@ def _load_cuda():
     import torch
 
     raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    _cuda = (torch.cuda.current_device, raw or (lambda index: torch.cuda.current_stream(index).cuda_stream))
+    device = getattr(torch._C, "_cuda_getDevice", None) if torch.cuda.is_initialized() else None
+    _cuda = (device or torch.cuda.current_device, raw or (lambda index: torch.cuda.current_stream(index).cuda_stream))
 
 
 def _current(device):
@@ -1297,6 +1298,12 @@ def quantize_tokens(x, q, scales):
         check(status)
 
 
+def _of_width(tensor, index, dtype, width, name):
+    if tensor.dim() != 1:
+        raise HipError(f"{name}: must be [{width}]")
+    return _vector(tensor, index, dtype, width, name)
+
+
 _block_rows = struct.Struct("@NNiiPNiPPPNfPNPNiPPfPNP").pack  # BlockRows
 
 
@@ -1330,16 +1337,13 @@ def block_norm(x, post=NORM_NONE, post_gain=None, post_bias=None, gate=None, sca
             raise HipError("out: must be of the input's type, or int8 with scales")
     if out_scales is not None:
         scales = _vector(out_scales, index, _float32, rows, "out_scales")
-    for tensor in (post_gain, post_bias, gain, bias):
-        if tensor is not None and tensor.dim() != 1:
-            raise HipError(f"gains and biases: must be [{width}]")
     status = (_lib or library()).tsac_hip_block_norm(_block_rows(
         rows, width, type_, wide, a, a_stride, post,
-        0 if post_gain is None else _vector(post_gain, index, dtype, width, "post_gain"),
-        0 if post_bias is None else _vector(post_bias, index, dtype, width, "post_bias"),
+        0 if post_gain is None else _of_width(post_gain, index, dtype, width, "post_gain"),
+        0 if post_bias is None else _of_width(post_bias, index, dtype, width, "post_bias"),
         g, g_stride, scale, r, r_stride, s, s_stride, norm,
-        0 if gain is None else _vector(gain, index, dtype, width, "gain"),
-        0 if bias is None else _vector(bias, index, dtype, width, "bias"), epsilon, o, o_stride, scales),
+        0 if gain is None else _of_width(gain, index, dtype, width, "gain"),
+        0 if bias is None else _of_width(bias, index, dtype, width, "bias"), epsilon, o, o_stride, scales),
         _stream_of(index))
     if status:
         check(status)
