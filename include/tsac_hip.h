@@ -686,7 +686,10 @@ int tsac_hip_channel_linear_apply(const tsac_hip_channel_linear* linear, const i
  * residual and sum of residual_type, which is `type` or FP32. Where out_scales is given, out
  * is int8 [rows][width] and quantised as by tsac_hip_quantize_tokens. out is the norm of s
  * as it is in 32 bits, before it is rounded for `sum`. sum may be the residual, sum or out
- * the input, of the same type and stride; nothing else may overlap. Strides in elements. */
+ * the input, of the same type and stride; nothing else may overlap. Strides in elements. Where
+ * all of them are 16-byte aligned, rows and gains are read in pieces of 16 bytes: what stands
+ * behind a last element, up to the next multiple of 16 bytes, does not matter. The same goes
+ * for the rows of tsac_hip_quantize_tokens. */
 #define TSAC_HIP_NORM_NONE 0
 #define TSAC_HIP_NORM_RMS 1
 #define TSAC_HIP_NORM_LAYER 2

@@ -27,7 +27,7 @@ constexpr int lanes = 64;
 
 template <int Threads, class Join> __device__ __forceinline__ float joined(float value, float* shared, Join join)
 {
-    value = over_lanes(value, join);
+    value = over_lanes<(Threads < lanes ? Threads : lanes)>(value, join);
     if constexpr (Threads > lanes)
     {
         lds_barrier(); // the last one's values have been read
@@ -62,40 +62,65 @@ template <int Threads> __device__ __forceinline__ unsigned row_max_bits(unsigned
                                            }));
 }
 
-// Eight values from `at` on, of which `count` there are, as they lie in memory; 0 behind them. `Whole`: there are eight or
-// none, at a multiple of 16 bytes.
-template <bool Whole, Type T>
+// What is known of rows: all of their eights are whole and at multiples of 16 bytes; all but the last of a row; nothing.
+enum class Rows
+{
+    whole,
+    ragged,
+    any
+};
+
+// Eight values from `at` on, of which `count` there are, as they lie in memory; 0 behind them. The last ones of a ragged row
+// are read in pieces of 16 bytes that have one of them, so that no element of its own is asked for.
+template <Rows M, Type T>
 __device__ __forceinline__ Eight<T> fetch8(const value_t<T>* at, int count, bool aligned)
 {
     Eight<T> eight = {};
-    if (Whole ? count > 0 : aligned && count >= 8)
+    if constexpr (M == Rows::any)
     {
-        eight = *reinterpret_cast<const Eight<T>*>(at);
+        if (!aligned || count < 8)
+        {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+            {
+                if (i < count)
+                {
+                    eight.v[i] = at[i];
+                }
+            }
+            return eight;
+        }
     }
-    else if constexpr (!Whole)
+    constexpr int piece = 16 / int(sizeof(value_t<T>));
+#pragma unroll
+    for (int i = 0; i < 8; i += piece)
+    {
+        if (i < count)
+        {
+            __builtin_memcpy(eight.v + i, __builtin_assume_aligned(at + i, 16), 16);
+        }
+    }
+    if constexpr (M == Rows::ragged)
     {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 1; i < 8; ++i)
         {
-            if (i < count)
-            {
-                eight.v[i] = at[i];
-            }
+            eight.v[i] = i < count ? eight.v[i] : value_t<T>(0);
         }
     }
     return eight;
 }
 
-template <bool Whole, Type T>
+template <Rows M, Type T>
 __device__ __forceinline__ void put8(value_t<T>* at, int count, bool aligned, const float (&in)[8])
 {
     if (count > 0)
     {
-        store8<T>(at, Whole ? 8 : count, Whole || aligned, in);
+        store8<T>(at, M == Rows::whole ? 8 : count, M != Rows::any || aligned, in);
     }
 }
 
-template <bool Whole, Type T, int Vectors, int Threads>
+template <Rows M, Type T, int Vectors, int Threads>
 __device__ __forceinline__ void normalise(float (&v)[Vectors][8], const NormRule& rule, bool aligned, int width,
                                           float epsilon, int thread, float* shared)
 {
@@ -126,7 +151,7 @@ __device__ __forceinline__ void normalise(float (&v)[Vectors][8], const NormRule
 #pragma unroll
         for (int e = 0; e < 8; ++e)
         {
-            v[i][e] = (Whole ? 0 : e) < count ? v[i][e] - mean : 0.0f;
+            v[i][e] = (M == Rows::whole ? 0 : e) < count ? v[i][e] - mean : 0.0f;
             squares = __builtin_fmaf(v[i][e], v[i][e], squares);
         }
     }
@@ -138,11 +163,11 @@ __device__ __forceinline__ void normalise(float (&v)[Vectors][8], const NormRule
         Eight<T> gain = {}, bias = {};
         if (rule.gain)
         {
-            gain = fetch8<Whole, T>(static_cast<const value_t<T>*>(rule.gain) + at, count, aligned);
+            gain = fetch8<M, T>(static_cast<const value_t<T>*>(rule.gain) + at, count, aligned);
         }
         if (rule.bias)
         {
-            bias = fetch8<Whole, T>(static_cast<const value_t<T>*>(rule.bias) + at, count, aligned);
+            bias = fetch8<M, T>(static_cast<const value_t<T>*>(rule.bias) + at, count, aligned);
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e)
@@ -150,7 +175,7 @@ __device__ __forceinline__ void normalise(float (&v)[Vectors][8], const NormRule
             float x = v[i][e] * factor;
             x = rule.gain ? x * widen<T>(gain.v[e]) : x;
             x = rule.bias ? x + widen<T>(bias.v[e]) : x;
-            v[i][e] = (Whole ? 0 : e) < count ? x : 0.0f;
+            v[i][e] = (M == Rows::whole ? 0 : e) < count ? x : 0.0f;
         }
     }
 }
@@ -208,12 +233,13 @@ enum Aligned
     norm_aligned = 64
 };
 
-// T: the values; R: the residual. A row is taken by Threads threads, each Vectors times eight values. With `Whole` a
+// T: the values; R: the residual. A row is taken by Threads threads, each Vectors times eight values. Unless they are `any`, a
 // workgroup takes rows one after the other, and the next one's are on their way while one is worked on: they pass
 // barriers, which are for LDS alone. 8190 rows of 8192 to 8 bits: ...
-template <Type T, Type R, int Vectors, int Threads, bool Whole>
+template <Type T, Type R, int Vectors, int Threads, Rows M>
 __global__ __launch_bounds__(Threads > 256 ? Threads : 256, 4) void block_norm_kernel(BlockRows p, int aligned)
 {
+    constexpr bool Ahead = M != Rows::any;
     constexpr int together = Threads < 256 ? 256 / Threads : 1; // rows of a workgroup
     __shared__ float shared[Threads > lanes ? Threads / lanes : 1];
     const int thread = threadIdx.x % Threads, stride = gridDim.x * together;
@@ -227,7 +253,7 @@ __global__ __launch_bounds__(Threads > 256 ? Threads : 256, 4) void block_norm_k
         for (int i = 0; i < Vectors; ++i)
         {
             const int at = 8 * (i * Threads + thread);
-            inputs[i] = fetch8<Whole, T>(x + at, p.width - at, aligned & input_aligned);
+            inputs[i] = fetch8<M, T>(x + at, p.width - at, aligned & input_aligned);
         }
     };
     const auto ask_residual = [&](int from)
@@ -237,22 +263,22 @@ __global__ __launch_bounds__(Threads > 256 ? Threads : 256, 4) void block_norm_k
         for (int i = 0; p.residual && i < Vectors; ++i)
         {
             const int at = 8 * (i * Threads + thread);
-            residuals[i] = fetch8<Whole, R>(x + at, p.width - at, aligned & residual_aligned);
+            residuals[i] = fetch8<M, R>(x + at, p.width - at, aligned & residual_aligned);
         }
     };
-    // Whole waves end together: a row of several has its workgroup for itself.
-    if (Whole && row < p.rows)
+    // A row's lanes end together, and where it has several waves these are the workgroup.
+    if (Ahead && row < p.rows)
     {
         ask_input(row);
         ask_residual(row);
     }
     for (; row < p.rows; row += stride)
     {
-    if constexpr (!Whole)
+    if constexpr (!Ahead)
     {
         ask_input(row);
     }
-    float v[Vectors][8], before[Whole ? Vectors : 1][8];
+    float v[Vectors][8], before[Ahead ? Vectors : 1][8];
 #pragma unroll
     for (int i = 0; i < Vectors; ++i)
     {
@@ -260,20 +286,20 @@ __global__ __launch_bounds__(Threads > 256 ? Threads : 256, 4) void block_norm_k
         for (int e = 0; e < 8; ++e)
         {
             v[i][e] = widen<T>(inputs[i].v[e]);
-            if (Whole && p.residual)
+            if (Ahead && p.residual)
             {
-                before[Whole ? i : 0][e] = widen<R>(residuals[i].v[e]);
+                before[Ahead ? i : 0][e] = widen<R>(residuals[i].v[e]);
             }
         }
     }
-    if constexpr (Whole)
+    if constexpr (Ahead)
     {
         const int next = min(row + stride, p.rows - 1); // the last one's once more, at the end
         ask_input(next);
         ask_residual(next);
     }
-    normalise<Whole, T, Vectors, Threads>(v, p.post, aligned & post_aligned, p.width, p.epsilon, thread, shared);
-    if constexpr (!Whole)
+    normalise<M, T, Vectors, Threads>(v, p.post, aligned & post_aligned, p.width, p.epsilon, thread, shared);
+    if constexpr (!Ahead)
     {
         ask_residual(row);
     }
@@ -286,26 +312,26 @@ __global__ __launch_bounds__(Threads > 256 ? Threads : 256, 4) void block_norm_k
         Eight<T> gates = {};
         if (p.gate)
         {
-            gates = fetch8<Whole, T>(gate + at, count, aligned & gate_aligned);
+            gates = fetch8<M, T>(gate + at, count, aligned & gate_aligned);
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e)
         {
             float u = p.gate ? v[i][e] * widen<T>(gates.v[e]) : v[i][e];
             u *= p.scale;
-            u = !p.residual ? u : (Whole ? before[Whole ? i : 0][e] : widen<R>(residuals[i].v[e])) + u;
-            v[i][e] = (Whole ? 0 : e) < count ? u : 0.0f;
+            u = !p.residual ? u : (Ahead ? before[Ahead ? i : 0][e] : widen<R>(residuals[i].v[e])) + u;
+            v[i][e] = (M == Rows::whole ? 0 : e) < count ? u : 0.0f;
         }
         if (p.sum)
         {
-            put8<Whole, R>(sum + at, count, aligned & sum_aligned, v[i]);
+            put8<M, R>(sum + at, count, aligned & sum_aligned, v[i]);
         }
     }
     if (!p.out)
     {
         continue;
     }
-    normalise<Whole, T, Vectors, Threads>(v, p.norm, aligned & norm_aligned, p.width, p.epsilon, thread, shared);
+    normalise<M, T, Vectors, Threads>(v, p.norm, aligned & norm_aligned, p.width, p.epsilon, thread, shared);
     if (!p.out_scales)
     {
         auto* out = static_cast<value_t<T>*>(p.out) + std::size_t(row) * p.out_stride;
@@ -313,7 +339,7 @@ __global__ __launch_bounds__(Threads > 256 ? Threads : 256, 4) void block_norm_k
         for (int i = 0; i < Vectors; ++i)
         {
             const int at = 8 * (i * Threads + thread), count = p.width - at;
-            put8<Whole, T>(out + at, count, aligned & out_aligned, v[i]);
+            put8<M, T>(out + at, count, aligned & out_aligned, v[i]);
         }
         continue;
     }
@@ -360,11 +386,11 @@ __global__ __launch_bounds__(Threads > 256 ? Threads : 256, 4) void block_norm_k
         {
             packed = nearest8(v[i], lifted, reciprocal);
         }
-        if (Whole ? count > 0 : count >= 8) // rows of 8-bit integers begin at multiples of 16 bytes
+        if (M == Rows::whole ? count > 0 : count >= 8) // rows of 8-bit integers begin at multiples of 16 bytes
         {
             *reinterpret_cast<uint2*>(q + at) = packed;
         }
-        else if constexpr (!Whole)
+        else if constexpr (M != Rows::whole)
         {
             for (int e = 0; e < count; ++e)
             {
@@ -384,23 +410,27 @@ template <Type T, Type R> void launch(const BlockRows& p, int aligned, hipStream
         const int groups = std::min<long>((p.rows + together - 1) / together, long(compute_units()) * a_unit);
         kernel<<<unsigned(groups), threads * together, 0, stream>>>(p, aligned);
     };
-    const auto of = [&](auto is_whole)
+    const auto of = [&](auto rows)
     {
-        constexpr bool W = decltype(is_whole)::value;
-        const auto a_unit = [](int groups) { return W ? groups : 1 << 20; };
+        constexpr Rows W = decltype(rows)::value;
+        const auto a_unit = [](int groups) { return W != Rows::any ? groups : 1 << 20; };
         // By the width alone, so that a row's result does not depend on how many there are.
         const int w = p.width;
-        w <= 512      ? go(block_norm_kernel<T, R, 1, 64, W>, 64, a_unit(8))
+        w <= 128      ? go(block_norm_kernel<T, R, 1, 16, W>, 16, a_unit(8))
+        : w <= 256    ? go(block_norm_kernel<T, R, 1, 32, W>, 32, a_unit(8))
+        : w <= 512    ? go(block_norm_kernel<T, R, 1, 64, W>, 64, a_unit(8))
         : w <= 1024   ? go(block_norm_kernel<T, R, 2, 64, W>, 64, a_unit(4))
         : w <= 2048   ? go(block_norm_kernel<T, R, 1, 256, W>, 256, a_unit(8))
         : w <= 4096   ? go(block_norm_kernel<T, R, 2, 256, W>, 256, a_unit(4))
         : w <= 8192   ? go(block_norm_kernel<T, R, 2, 512, W>, 512, a_unit(2))
         : w <= 16384  ? go(block_norm_kernel<T, R, 2, 1024, W>, 1024, a_unit(1))
-        : w <= 32768  ? go(block_norm_kernel<T, R, 4, 1024, false>, 1024, 1 << 20)
-                      : go(block_norm_kernel<T, R, 8, 1024, false>, 1024, 1 << 20);
+        : w <= 32768  ? go(block_norm_kernel<T, R, 4, 1024, Rows::any>, 1024, 1 << 20)
+                      : go(block_norm_kernel<T, R, 8, 1024, Rows::any>, 1024, 1 << 20);
     };
     constexpr int every = input_aligned | gate_aligned | residual_aligned | sum_aligned | out_aligned | post_aligned | norm_aligned;
-    aligned == every && p.width % 8 == 0 ? of(std::true_type{}) : of(std::false_type{});
+    aligned != every     ? of(std::integral_constant<Rows, Rows::any>{})
+    : p.width % 8 != 0   ? of(std::integral_constant<Rows, Rows::ragged>{})
+                         : of(std::integral_constant<Rows, Rows::whole>{});
     check_hip(hipGetLastError(), "block norm launch");
 }
 } // namespace

@@ -29,13 +29,21 @@ template <int stride, class V, class Join> __device__ __forceinline__ V join_nei
     }
 }
 
-// All lanes' values joined, in every lane.
-template <class V, class Join> __device__ __forceinline__ V over_lanes(V value, Join join)
+// The values of all lanes, or of each group of 16 or 32, joined, in every lane of them.
+template <int Lanes = 64, class V, class Join> __device__ __forceinline__ V over_lanes(V value, Join join)
 {
-    static_assert(sizeof(V) == 4);
+    static_assert(sizeof(V) == 4 && (Lanes == 16 || Lanes == 32 || Lanes == 64));
     value = join_neighbours<2>(join_neighbours<1>(value, join), join);
     value = join_neighbours<8>(join_neighbours<4>(value, join), join);
-    return join_neighbours<32>(join_neighbours<16>(value, join), join);
+    if constexpr (Lanes > 16)
+    {
+        value = join_neighbours<16>(value, join);
+    }
+    if constexpr (Lanes > 32)
+    {
+        value = join_neighbours<32>(value, join);
+    }
+    return value;
 }
 
 // A workgroup's barrier for what lies in LDS.
