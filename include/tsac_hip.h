@@ -668,16 +668,14 @@ void tsac_hip_channel_linear_destroy(tsac_hip_channel_linear* linear);
 int tsac_hip_quantize_tokens(const void* x, size_t x_stride, int type, size_t rows, size_t K, int8_t* q,
                              size_t q_stride, float* scales, void* stream);
 
-/* The product of M rows q [M][K] (stride and address multiples of 16; what stands behind
- * the K-th byte, up to the next multiple of 16, is read and does not matter) to y [M][N]
- * of `type` (FP32 too), strides in elements. Sums are exact, so that a row's result is
- * the same in every batch. The linear's own device has to be current. Workspace: at least
- * tsac_hip_channel_linear_workspace bytes of device memory, 16-byte aligned, not shared
- * by calls that overlap. */
-size_t tsac_hip_channel_linear_workspace(const tsac_hip_channel_linear* linear, size_t M);
+/* The product of M rows q [M][K] (address and stride multiples of 16, rows less than 8 MiB
+ * apart; what stands behind the K-th byte, up to the next multiple of 16, is read and does
+ * not matter) to y [M][N] of `type` (FP32 too), strides in elements, which overlaps nothing.
+ * Sums are exact, so that a row's result is the same in every batch. The linear's own
+ * device has to be current. Calls of one linear may overlap. */
 int tsac_hip_channel_linear_apply(const tsac_hip_channel_linear* linear, const int8_t* q, size_t q_stride,
                                   const float* token_scales, size_t M, void* y, size_t y_stride, int type,
-                                  void* workspace, size_t workspace_bytes, void* stream);
+                                  void* stream);
 
 /* u = scale * gate * post(input); s = residual + u; out = norm(s), with
  * rms(x) = x / sqrt(mean x^2 + epsilon) * gain + bias and layer(x) = rms of x less its mean,
@@ -801,7 +799,7 @@ typedef struct tsac_hip_logit_rules
  * softmax (x - max) / temperature. A temperature of 0 (or below) gives 1 to the lowest token of the largest x. A
  * row in which nothing is above -infinity is 0; one with an allowed NaN is NaN, and so is one with +infinity at a temperature
  * above 0. out may be the logits, of the same type and stride; rows of no sequence are left as they were. At
- * most 2^20 tokens. Workspace as for tsac_hip_channel_linear_apply. */
+ * most 2^20 tokens. Workspace as for tsac_hip_attention_paged. */
 size_t tsac_hip_adjust_logits_workspace(size_t rows, size_t alphabet);
 int tsac_hip_adjust_logits(const void* logits, size_t stride, int type, size_t rows, size_t alphabet,
                            const tsac_hip_logit_rules* rules, int probabilities, void* out, size_t out_stride,

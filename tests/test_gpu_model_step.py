@@ -165,11 +165,11 @@ def product(torch, q, s, w, c, b, kind):
     return y, 3.01 * H * exact.abs() + H * y.abs() + UNIT[kind] * (1 + 4 * H) * y.abs() + TINY[kind]
 
 
-def check_product(torch, native, rows, inputs, outputs, kind, seed=0, bias=True, linear=None, workspace=None):
+def check_product(torch, native, rows, inputs, outputs, kind, seed=0, bias=True, linear=None):
     linear, w, c, b = linear or linear_of(torch, native, outputs, inputs, seed, bias)
     q, s = tokens_of(torch, rows, inputs, seed + 1)
     out = Inside(torch, rows, outputs, kind, offset=3 if rows % 2 else 0)
-    linear.apply(q, s, out.view, workspace=workspace)
+    linear.apply(q, s, out.view)
     y, room = product(torch, q, s, w, c, b, kind)
     near(torch, out.view, y, room)
     out.rest_stays()
@@ -898,8 +898,7 @@ class Step:
         self.accepted, self.next = ints(torch, [0] * len(counts)), ints(torch, [0] * len(counts))
         self.longest = max(a + b for a, b in zip(lengths, counts))
         self.spaces = [torch.empty(max(n, 16), dtype=torch.uint8, device="cuda") for n in (
-            self.qkv_linear[0].workspace(rows), native.attention_paged_workspace(p.cache, rows, heads, p.max_rows, self.longest),
-            self.out_linear[0].workspace(rows), self.head[0].workspace(rows),
+            native.attention_paged_workspace(p.cache, rows, heads, p.max_rows, self.longest),
             native.library().tsac_hip_adjust_logits_workspace(rows, alphabet),
             native.library().tsac_hip_verify_drafts_workspace(len(counts), alphabet))]
 
@@ -907,21 +906,21 @@ class Step:
         native, p, (width, heads, kv, hw) = self.native, self.p, self.dims
         native.tree_mask(self.parents_t, p.starts, p.max_rows, self.mask)
         native.block_norm(self.x.bfloat16(), norm=native.NORM_RMS, gain=self.gain, out=self.q, out_scales=self.s)
-        self.qkv_linear[0].apply(self.q, self.s, self.qkv, workspace=self.spaces[0])
+        self.qkv_linear[0].apply(self.q, self.s, self.qkv)
         parts = self.qkv.view(-1, heads + 2 * kv, hw)
         p.cache.append(0, parts[:, :heads], parts[:, heads:heads + kv], parts[:, heads + kv:], p.starts, p.max_rows,
                        self.frequencies, self.turned, mask=self.mask)
         native.attention_paged(p.cache, 0, self.turned, p.starts, p.max_rows, self.longest, self.mask, 0.125, self.mixed,
-                               workspace=self.spaces[1])
+                               workspace=self.spaces[0])
         native.quantize_tokens(self.mixed.view(-1, heads * hw), self.q2, self.s2)
-        self.out_linear[0].apply(self.q2, self.s2, self.block, workspace=self.spaces[2])
+        self.out_linear[0].apply(self.q2, self.s2, self.block)
         native.block_norm(self.block, post=native.NORM_RMS, post_gain=self.gain, scale=0.5, residual=self.x, sum=self.after,
                           norm=native.NORM_LAYER, out=self.q3, out_scales=self.s3)
-        self.head[0].apply(self.q3, self.s3, self.logits, workspace=self.spaces[3])
+        self.head[0].apply(self.q3, self.s3, self.logits)
         native.adjust_logits(self.logits, self.probs, p.starts, history=self.history, history_lengths=self.history_lengths,
-                             tokens=self.tokens, mask=self.mask, repetition=self.penalty, workspace=self.spaces[4])
+                             tokens=self.tokens, mask=self.mask, repetition=self.penalty, workspace=self.spaces[1])
         native.verify_drafts(self.probs, None, self.tokens, self.parents_t, p.starts, p.max_rows, self.uniforms, self.draws,
-                             self.path, self.accepted, self.next, workspace=self.spaces[5])
+                             self.path, self.accepted, self.next, workspace=self.spaces[2])
 
     def results(self):
         return [t.clone() for t in (self.qkv, self.turned, self.p.keys, self.p.values, self.mixed, self.block, self.after,

@@ -1725,21 +1725,9 @@ int tsac_hip_quantize_tokens(const void* x, size_t x_stride, int type, size_t ro
         });
 }
 
-size_t tsac_hip_channel_linear_workspace(const tsac_hip_channel_linear* linear, size_t M)
-{
-    size_t bytes = 0;
-    guarded(
-        [&]
-        {
-            require(linear && M < max_new_rows, "channel linear: size out of range");
-            bytes = channel_linear_workspace(linear->weights, M);
-        });
-    return bytes;
-}
-
 int tsac_hip_channel_linear_apply(const tsac_hip_channel_linear* linear, const int8_t* q, size_t q_stride,
                                   const float* token_scales, size_t M, void* y, size_t y_stride, int type,
-                                  void* workspace, size_t workspace_bytes, void* stream)
+                                  void* stream)
 {
     return guarded(
         [&]
@@ -1755,15 +1743,13 @@ int tsac_hip_channel_linear_apply(const tsac_hip_channel_linear* linear, const i
                                "channel linear: rows of q must be 16-byte aligned and apart");
             require_rows(y, y_stride, M, std::size_t(linear->weights.outputs), r.type,
                          "channel linear: rows of y overlap or are misaligned");
-            require(reinterpret_cast<std::uintptr_t>(workspace) % 16 == 0,
-                    "channel linear: the workspace must be 16-byte aligned");
             r.q = q;
             r.q_stride = q_stride;
             r.scales = token_scales;
             r.out = y;
             r.out_stride = y_stride;
             r.rows = int(M);
-            channel_linear(linear->weights, r, workspace, workspace_bytes, as_stream(stream));
+            channel_linear(linear->weights, r, as_stream(stream));
         });
 }
 

@@ -274,146 +274,149 @@ __global__ __launch_bounds__(Threads > 256 ? Threads : 256, 4) void block_norm_k
     }
     for (; row < p.rows; row += stride)
     {
-    if constexpr (!Ahead)
-    {
-        ask_input(row);
-    }
-    float v[Vectors][8], before[Ahead ? Vectors : 1][8];
-#pragma unroll
-    for (int i = 0; i < Vectors; ++i)
-    {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
+        if constexpr (!Ahead)
         {
-            v[i][e] = widen<T>(inputs[i].v[e]);
-            if (Ahead && p.residual)
+            ask_input(row);
+        }
+        float v[Vectors][8], before[Ahead ? Vectors : 1][8];
+#pragma unroll
+        for (int i = 0; i < Vectors; ++i)
+        {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
             {
-                before[Ahead ? i : 0][e] = widen<R>(residuals[i].v[e]);
+                v[i][e] = widen<T>(inputs[i].v[e]);
+                if (Ahead && p.residual)
+                {
+                    before[Ahead ? i : 0][e] = widen<R>(residuals[i].v[e]);
+                }
             }
         }
-    }
-    if constexpr (Ahead)
-    {
-        const int next = min(row + stride, p.rows - 1); // the last one's once more, at the end
-        ask_input(next);
-        ask_residual(next);
-    }
-    normalise<M, T, Vectors, Threads>(v, p.post, aligned & post_aligned, p.width, p.epsilon, thread, shared);
-    if constexpr (!Ahead)
-    {
-        ask_residual(row);
-    }
-    const auto* gate = static_cast<const value_t<T>*>(p.gate) + std::size_t(row) * p.gate_stride;
-    auto* sum = static_cast<value_t<R>*>(p.sum) + std::size_t(row) * p.sum_stride;
-#pragma unroll
-    for (int i = 0; i < Vectors; ++i)
-    {
-        const int at = 8 * (i * Threads + thread), count = p.width - at;
-        Eight<T> gates = {};
-        if (p.gate)
+        if constexpr (Ahead)
         {
-            gates = fetch8<M, T>(gate + at, count, aligned & gate_aligned);
+            if (row + stride < p.rows)
+            {
+                ask_input(row + stride);
+                ask_residual(row + stride);
+            }
         }
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
+        normalise<M, T, Vectors, Threads>(v, p.post, aligned & post_aligned, p.width, p.epsilon, thread, shared);
+        if constexpr (!Ahead)
         {
-            float u = p.gate ? v[i][e] * widen<T>(gates.v[e]) : v[i][e];
-            u *= p.scale;
-            u = !p.residual ? u : (Ahead ? before[Ahead ? i : 0][e] : widen<R>(residuals[i].v[e])) + u;
-            v[i][e] = (M == Rows::whole ? 0 : e) < count ? u : 0.0f;
+            ask_residual(row);
         }
-        if (p.sum)
-        {
-            put8<M, R>(sum + at, count, aligned & sum_aligned, v[i]);
-        }
-    }
-    if (!p.out)
-    {
-        continue;
-    }
-    normalise<M, T, Vectors, Threads>(v, p.norm, aligned & norm_aligned, p.width, p.epsilon, thread, shared);
-    if (!p.out_scales)
-    {
-        auto* out = static_cast<value_t<T>*>(p.out) + std::size_t(row) * p.out_stride;
+        const auto* gate = static_cast<const value_t<T>*>(p.gate) + std::size_t(row) * p.gate_stride;
+        auto* sum = static_cast<value_t<R>*>(p.sum) + std::size_t(row) * p.sum_stride;
 #pragma unroll
         for (int i = 0; i < Vectors; ++i)
         {
             const int at = 8 * (i * Threads + thread), count = p.width - at;
-            put8<M, T>(out + at, count, aligned & out_aligned, v[i]);
-        }
-        continue;
-    }
-    unsigned top = 0;
-#pragma unroll
-    for (int i = 0; i < Vectors; ++i)
-    {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-        {
-            const unsigned bits = __float_as_uint(v[i][e]) & 0x7fffffffu;
-            top = bits > top ? bits : top;
-        }
-    }
-    top = row_max_bits<Threads>(top, shared);
-    const bool finite = top < 0x7f800000u;
-    const float most = __uint_as_float(top), scale = most * (1.0f / 127.0f);
-    if (thread == 0)
-    {
-        p.out_scales[row] = finite ? scale : __uint_as_float(0x7fc00000u);
-    }
-    // Small rows are taken times 2^64, which changes no quotient, so that the reciprocal is finite and half
-    // the scale exact.
-    const bool small = most < 0x1p-60f, zero = !finite || scale == 0.0f;
-    const float lifted = small ? scale * 0x1p64f : scale, reciprocal = 1.0f / lifted;
-    auto* q = static_cast<int8_t*>(p.out) + std::size_t(row) * p.out_stride;
-#pragma unroll
-    for (int i = 0; i < Vectors; ++i)
-    {
-        const int at = 8 * (i * Threads + thread), count = p.width - at;
-        uint2 packed = {};
-        if (!zero && small)
-        {
-            // A scale of few bits may leave quotients past 127.
-            uint64_t bytes = 0;
+            Eight<T> gates = {};
+            if (p.gate)
+            {
+                gates = fetch8<M, T>(gate + at, count, aligned & gate_aligned);
+            }
 #pragma unroll
             for (int e = 0; e < 8; ++e)
             {
-                bytes |= uint64_t(uint8_t(nearest(v[i][e] * 0x1p64f, lifted, reciprocal))) << 8 * e;
+                float u = p.gate ? v[i][e] * widen<T>(gates.v[e]) : v[i][e];
+                u *= p.scale;
+                u = !p.residual ? u : (Ahead ? before[Ahead ? i : 0][e] : widen<R>(residuals[i].v[e])) + u;
+                v[i][e] = (M == Rows::whole ? 0 : e) < count ? u : 0.0f;
             }
-            packed = make_uint2(unsigned(bytes), unsigned(bytes >> 32));
-        }
-        else if (!zero)
-        {
-            packed = nearest8(v[i], lifted, reciprocal);
-        }
-        if (M == Rows::whole ? count > 0 : count >= 8) // rows of 8-bit integers begin at multiples of 16 bytes
-        {
-            *reinterpret_cast<uint2*>(q + at) = packed;
-        }
-        else if constexpr (M != Rows::whole)
-        {
-            for (int e = 0; e < count; ++e)
+            if (p.sum)
             {
-                q[at + e] = int8_t((e < 4 ? packed.x : packed.y) >> e % 4 * 8);
+                put8<M, R>(sum + at, count, aligned & sum_aligned, v[i]);
             }
         }
-    }
+        if (!p.out)
+        {
+            continue;
+        }
+        normalise<M, T, Vectors, Threads>(v, p.norm, aligned & norm_aligned, p.width, p.epsilon, thread, shared);
+        if (!p.out_scales)
+        {
+            auto* out = static_cast<value_t<T>*>(p.out) + std::size_t(row) * p.out_stride;
+#pragma unroll
+            for (int i = 0; i < Vectors; ++i)
+            {
+                const int at = 8 * (i * Threads + thread), count = p.width - at;
+                put8<M, T>(out + at, count, aligned & out_aligned, v[i]);
+            }
+            continue;
+        }
+        unsigned top = 0;
+#pragma unroll
+        for (int i = 0; i < Vectors; ++i)
+        {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+            {
+                const unsigned bits = __float_as_uint(v[i][e]) & 0x7fffffffu;
+                top = bits > top ? bits : top;
+            }
+        }
+        top = row_max_bits<Threads>(top, shared);
+        const bool finite = top < 0x7f800000u;
+        const float most = __uint_as_float(top), scale = most * (1.0f / 127.0f);
+        if (thread == 0)
+        {
+            p.out_scales[row] = finite ? scale : __uint_as_float(0x7fc00000u);
+        }
+        // Small rows are taken times 2^64, which changes no quotient, so that the reciprocal is finite and half
+        // the scale exact.
+        const bool small = most < 0x1p-60f, zero = !finite || scale == 0.0f;
+        const float lifted = small ? scale * 0x1p64f : scale, reciprocal = 1.0f / lifted;
+        auto* q = static_cast<int8_t*>(p.out) + std::size_t(row) * p.out_stride;
+#pragma unroll
+        for (int i = 0; i < Vectors; ++i)
+        {
+            const int at = 8 * (i * Threads + thread), count = p.width - at;
+            uint2 packed = {};
+            if (!zero && small)
+            {
+                // A scale of few bits may leave quotients past 127.
+                uint64_t bytes = 0;
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                {
+                    bytes |= uint64_t(uint8_t(nearest(v[i][e] * 0x1p64f, lifted, reciprocal))) << 8 * e;
+                }
+                packed = make_uint2(unsigned(bytes), unsigned(bytes >> 32));
+            }
+            else if (!zero)
+            {
+                packed = nearest8(v[i], lifted, reciprocal);
+            }
+            if (M == Rows::whole ? count > 0 : count >= 8) // rows of 8-bit integers begin at multiples of 16 bytes
+            {
+                *reinterpret_cast<uint2*>(q + at) = packed;
+            }
+            else if constexpr (M != Rows::whole)
+            {
+                for (int e = 0; e < count; ++e)
+                {
+                    q[at + e] = int8_t((e < 4 ? packed.x : packed.y) >> e % 4 * 8);
+                }
+            }
+        }
     }
 }
 
 template <Type T, Type R> void launch(const BlockRows& p, int aligned, hipStream_t stream)
 {
-    // A workgroup takes several rows where there are more than are worked on at a time.
+    // A workgroup takes several rows where there are more than are worked on at a time, or than a launch has room for.
+    constexpr int most_groups = 1 << 13; // a unit's
     const auto go = [&](auto kernel, int threads, int a_unit)
     {
         const int together = threads < 256 ? 256 / threads : 1;
-        const int groups = std::min<long>((p.rows + together - 1) / together, long(compute_units()) * a_unit);
+        const int groups = std::min({(p.rows + together - 1) / together, compute_units() * a_unit, 1 << 21});
         kernel<<<unsigned(groups), threads * together, 0, stream>>>(p, aligned);
     };
     const auto of = [&](auto rows)
     {
         constexpr Rows W = decltype(rows)::value;
-        const auto a_unit = [](int groups) { return W != Rows::any ? groups : 1 << 20; };
+        const auto a_unit = [](int groups) { return W != Rows::any ? groups : most_groups; };
         // By the width alone, so that a row's result does not depend on how many there are.
         const int w = p.width;
         w <= 128      ? go(block_norm_kernel<T, R, 1, 16, W>, 16, a_unit(8))
@@ -424,8 +427,8 @@ template <Type T, Type R> void launch(const BlockRows& p, int aligned, hipStream
         : w <= 4096   ? go(block_norm_kernel<T, R, 2, 256, W>, 256, a_unit(4))
         : w <= 8192   ? go(block_norm_kernel<T, R, 2, 512, W>, 512, a_unit(2))
         : w <= 16384  ? go(block_norm_kernel<T, R, 2, 1024, W>, 1024, a_unit(1))
-        : w <= 32768  ? go(block_norm_kernel<T, R, 4, 1024, Rows::any>, 1024, 1 << 20)
-                      : go(block_norm_kernel<T, R, 8, 1024, Rows::any>, 1024, 1 << 20);
+        : w <= 32768  ? go(block_norm_kernel<T, R, 4, 1024, Rows::any>, 1024, most_groups)
+                      : go(block_norm_kernel<T, R, 8, 1024, Rows::any>, 1024, most_groups);
     };
     constexpr int every = input_aligned | gate_aligned | residual_aligned | sum_aligned | out_aligned | post_aligned | norm_aligned;
     aligned != every     ? of(std::integral_constant<Rows, Rows::any>{})

@@ -131,21 +131,20 @@ template <int Pieces, int Ring> struct Shape
 } // namespace narrow
 
 template <Type T, int Pieces, int Ring>
-__global__ __launch_bounds__(narrow::waves * lanes) void narrow_kernel(Launch l, int row_tiles)
+__global__ __launch_bounds__(narrow::waves * lanes) void narrow_kernel(Launch l)
 {
     using namespace narrow;
     using S = Shape<Pieces, Ring>;
     extern __shared__ __attribute__((aligned(1024))) int8_t lds[];
     const int lane = threadIdx.x % lanes, warp = __builtin_amdgcn_readfirstlane(threadIdx.x / lanes);
-    const int column = blockIdx.x / row_tiles, n0 = column * tile, m0 = int(blockIdx.x - column * row_tiles) * S::rows;
-    const int8_t* const weights = l.weights + std::size_t(column) * l.steps * S::weight_bytes;
-    const int8_t* const rows = l.q + std::size_t(m0) * l.q_stride;
+    const int n0 = blockIdx.x * tile;
+    const int8_t* const weights = l.weights + std::size_t(blockIdx.x) * l.steps * S::weight_bytes;
     int8_t* const mine = lds + warp * Ring * S::step_bytes;
     unsigned row_offset[Pieces];
 #pragma unroll
     for (int j = 0; j < Pieces; ++j)
     {
-        row_offset[j] = unsigned(min(8 * j + lane / 8, l.rows - 1 - m0)) * unsigned(l.q_stride);
+        row_offset[j] = unsigned(min(8 * j + lane / 8, l.rows - 1)) * unsigned(l.q_stride);
     }
     const auto ask = [&](int s, int slot)
     {
@@ -161,7 +160,7 @@ __global__ __launch_bounds__(narrow::waves * lanes) void narrow_kernel(Launch l,
         {
             // The lane's row is 8 j + lane / 8; the piece of 16 bytes that belongs into place lane % 8 of it.
             const int piece = (lane % 8 ^ lane / 8 ^ j % 2) * 16;
-            load16_to_lds<false>(rows, row_offset[j] + unsigned(min(s * step + piece, l.last_piece)),
+            load16_to_lds<false>(l.q, row_offset[j] + unsigned(min(s * step + piece, l.last_piece)),
                                  to + S::weight_bytes + j * 1024);
         }
     };
@@ -221,8 +220,8 @@ __global__ __launch_bounds__(narrow::waves * lanes) void narrow_kernel(Launch l,
         __syncthreads();
         for (int i = threadIdx.x; i < tile * tile; i += waves * lanes)
         {
-            const int row = g * tile + i / tile, m = m0 + row, n = n0 + i % tile;
-            if (row >= S::rows || m >= l.rows || n >= l.outputs)
+            const int m = g * tile + i / tile, n = n0 + i % tile;
+            if (m >= l.rows || n >= l.outputs)
             {
                 continue;
             }
@@ -587,22 +586,20 @@ __global__ __launch_bounds__(tiled::threads, PerUnit) void tiled_kernel(Launch l
 __global__ void tiles_kernel(const int8_t* __restrict__ canonical, int inputs, int outputs, int steps,
                              int8_t* __restrict__ tiled, std::size_t pieces)
 {
-    const std::size_t piece = std::size_t(blockIdx.x) * blockDim.x + threadIdx.x;
-    if (piece >= pieces)
+    const std::size_t across = std::size_t(steps) * slices, threads = std::size_t(gridDim.x) * blockDim.x;
+    for (std::size_t piece = std::size_t(blockIdx.x) * blockDim.x + threadIdx.x; piece < pieces; piece += threads)
     {
-        return;
-    }
-    const int lane = piece % lanes;
-    const std::size_t t = piece / lanes, across = std::size_t(steps) * slices;
-    const std::size_t n = t / across * tile + lane % tile;
-    const int k = int(t % across) * tile + lane / tile * 16;
-    int8_t v[16];
+        const int lane = piece % lanes;
+        const std::size_t t = piece / lanes, n = t / across * tile + lane % tile;
+        const int k = int(t % across) * tile + lane / tile * 16;
+        int8_t v[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-    {
-        v[i] = n < std::size_t(outputs) && k + i < inputs ? canonical[n * inputs + k + i] : int8_t(0);
+        for (int i = 0; i < 16; ++i)
+        {
+            v[i] = n < std::size_t(outputs) && k + i < inputs ? canonical[n * inputs + k + i] : int8_t(0);
+        }
+        __builtin_memcpy(tiled + 16 * piece, v, 16);
     }
-    __builtin_memcpy(tiled + 16 * piece, v, 16);
 }
 
 int steps_of(std::size_t inputs)
@@ -610,14 +607,22 @@ int steps_of(std::size_t inputs)
     return int((inputs + step - 1) / step);
 }
 
+template <class Kernel> void allow_lds(Kernel kernel, int bytes)
+{
+    if (bytes > 65536)
+    {
+        check_hip(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                      bytes),
+                  "channel linear LDS");
+    }
+}
+
 template <Type T, int JN, int JM, int Depth, int Ring, int PerUnit> void launch_tiled(const Launch& l, hipStream_t stream)
 {
     using S = tiled::Shape<JN, JM, Depth, Ring>;
     static_assert(S::lds_bytes * PerUnit <= 160 * 1024);
     const auto kernel = tiled_kernel<T, JN, JM, Depth, Ring, PerUnit>;
-    static const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                                          hipFuncAttributeMaxDynamicSharedMemorySize, S::lds_bytes);
-    check_hip(allowed, "channel linear LDS");
+    allow_lds(kernel, S::lds_bytes);
     const int row_tiles = (l.rows + S::m - 1) / S::m, column_tiles = (l.outputs + S::n - 1) / S::n;
     const std::size_t total = std::size_t(row_tiles) * column_tiles;
     require(total < (std::size_t(1) << 30), "channel linear: too many tiles");
@@ -632,11 +637,8 @@ template <Type T, int Pieces, int Ring> void launch_narrow(const Launch& l, hipS
 {
     using S = narrow::Shape<Pieces, Ring>;
     const auto kernel = narrow_kernel<T, Pieces, Ring>;
-    static const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                                          hipFuncAttributeMaxDynamicSharedMemorySize, S::lds_bytes);
-    check_hip(allowed, "channel linear LDS");
-    const int row_tiles = (l.rows + S::rows - 1) / S::rows;
-    kernel<<<unsigned((l.outputs + tile - 1) / tile * row_tiles), narrow::waves * lanes, S::lds_bytes, stream>>>(l, row_tiles);
+    allow_lds(kernel, S::lds_bytes);
+    kernel<<<unsigned((l.outputs + tile - 1) / tile), narrow::waves * lanes, S::lds_bytes, stream>>>(l);
     check_hip(hipGetLastError(), "channel linear launch");
 }
 
@@ -700,21 +702,13 @@ std::size_t channel_tiles_bytes(std::size_t inputs, std::size_t outputs)
 void channel_tiles(const int8_t* canonical, std::size_t inputs, std::size_t outputs, int8_t* tiled, hipStream_t stream)
 {
     const std::size_t pieces = channel_tiles_bytes(inputs, outputs) / 16;
-    tiles_kernel<<<unsigned((pieces + 255) / 256), 256, 0, stream>>>(canonical, int(inputs), int(outputs),
-                                                                     steps_of(inputs), tiled, pieces);
+    const std::size_t groups = std::min<std::size_t>((pieces + 255) / 256, 1 << 20);
+    tiles_kernel<<<unsigned(groups), 256, 0, stream>>>(canonical, int(inputs), int(outputs), steps_of(inputs), tiled, pieces);
     check_hip(hipGetLastError(), "channel linear tiles launch");
 }
 
-std::size_t channel_linear_workspace(const ChannelWeights&, std::size_t)
+void channel_linear(const ChannelWeights& weights, const ChannelRows& rows, hipStream_t stream)
 {
-    return 0;
-}
-
-void channel_linear(const ChannelWeights& weights, const ChannelRows& rows, void* workspace, std::size_t bytes,
-                    hipStream_t stream)
-{
-    const std::size_t need = channel_linear_workspace(weights, std::size_t(rows.rows));
-    require(bytes >= need && (workspace || !need), "channel linear: workspace too small");
     if (!rows.rows)
     {
         return;

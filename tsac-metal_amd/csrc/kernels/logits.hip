@@ -617,7 +617,8 @@ void adjust_logits(const LogitRows& rows, const LogitRules& rules, void* workspa
     }
     const std::size_t history = rules.history ? rules.history_stride : 0;
     const Shape s = shape_of(rows, history);
-    require(std::size_t(rows.rows) * s.splits < (std::size_t(1) << 31), "logits: too many rows");
+    // 2^32 work-items are a launch's limit.
+    require(std::size_t(rows.rows) * s.splits < (std::size_t(1) << 32) / s.threads, "logits: too many rows");
     require(bytes >= logits_workspace(rows) && (workspace || !logits_workspace(rows)), "logits: workspace too small");
     const auto whole = [](const void* pointer, std::size_t stride, Type type)
     { return reinterpret_cast<std::uintptr_t>(pointer) % 16 == 0 && stride * (type == Type::single ? 4 : 2) % 16 == 0; };

@@ -41,9 +41,7 @@ struct ChannelRows
     int rows = 0;
     Type type = Type::bf16;
 };
-std::size_t channel_linear_workspace(const ChannelWeights& weights, std::size_t rows);
-void channel_linear(const ChannelWeights& weights, const ChannelRows& rows, void* workspace, std::size_t bytes,
-                    hipStream_t stream);
+void channel_linear(const ChannelWeights& weights, const ChannelRows& rows, hipStream_t stream);
 
 // ---- norms around a block, tokens to 8 bits (block_norm.hip) -------------------
 enum class Norm

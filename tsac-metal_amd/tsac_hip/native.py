@@ -46,7 +46,7 @@ EXPORTS = (
     "tsac_hip_pages_keep", "tsac_hip_tree_mask", "tsac_hip_attention_paged_workspace", "tsac_hip_attention_paged",
     "tsac_hip_verify_drafts_workspace", "tsac_hip_verify_drafts",
     "tsac_hip_channel_linear_create", "tsac_hip_channel_linear_destroy", "tsac_hip_quantize_tokens",
-    "tsac_hip_channel_linear_workspace", "tsac_hip_channel_linear_apply", "tsac_hip_block_norm",
+    "tsac_hip_channel_linear_apply", "tsac_hip_block_norm",
     "tsac_hip_rotary_frequencies", "tsac_hip_pages_append", "tsac_hip_adjust_logits_workspace",
     "tsac_hip_adjust_logits",
 )
@@ -268,9 +268,7 @@ def library() -> C.CDLL:
         lib.tsac_hip_channel_linear_destroy.argtypes = [vp]
         lib.tsac_hip_channel_linear_destroy.restype = None
         lib.tsac_hip_quantize_tokens.argtypes = [vp, sz, C.c_int, sz, sz, vp, sz, vp, vp]
-        lib.tsac_hip_channel_linear_workspace.argtypes = [vp, sz]
-        lib.tsac_hip_channel_linear_workspace.restype = sz
-        lib.tsac_hip_channel_linear_apply.argtypes = [vp, vp, sz, vp, sz, vp, sz, C.c_int, vp, sz, vp]
+        lib.tsac_hip_channel_linear_apply.argtypes = [vp, vp, sz, vp, sz, vp, sz, C.c_int, vp]
         lib.tsac_hip_block_norm.argtypes = [vp, vp]  # BlockRows
         lib.tsac_hip_rotary_frequencies.argtypes = [sz, C.c_double, C.c_int, C.c_double, C.c_double, C.c_double, C.c_double,
                                                     vp]
@@ -1247,41 +1245,23 @@ class ChannelLinear:
         check(library().tsac_hip_channel_linear_create(*(None if t is None else t.data_ptr() for t in parts), self.K, self.N,
                                                        _stream(None), C.byref(handle)))
         self.handle, self._library = handle, library()
-        self._workspaces = {}  # bytes by rows
 
     def __del__(self, release=_release):  # bound now: module globals are cleared at shutdown
         release(self, "tsac_hip_channel_linear_destroy")
 
-    def workspace(self, rows) -> int:
-        """Bytes that apply() needs for as many rows."""
-        need = self._workspaces.get(rows)
-        if need is None:
-            if len(self._workspaces) >= 1024:
-                self._workspaces.clear()
-            need = self._workspaces[rows] = int(self._library.tsac_hip_channel_linear_workspace(self.handle, rows))
-        return need
-
-    def apply(self, q, scales, out, workspace=None):
-        """q int8 [rows][K] and its scales float32 [rows] (quantize_tokens, block_norm) to out [rows][N]. A new
-        workspace a call, if none is given and one is needed."""
+    def apply(self, q, scales, out):
+        """q int8 [rows][K] and its scales float32 [rows] (quantize_tokens, block_norm) to out [rows][N]."""
         shape, type_ = _rows_of(out, "out")
         index, rows = q.get_device(), shape[0]
         if q.dtype is not _int8 or shape[1] != self.N:
             raise HipError(f"q: must be int8, out [rows][{self.N}]")
         a, a_stride = _matrix(q, index, (rows, self.K), "q")
         o, o_stride = _matrix(out, index, shape, "out")
-        space, size, keep = None, 0, None
-        need = self._workspaces.get(rows)
-        if need is None:
-            need = self.workspace(rows)
-        if need or workspace is not None:
-            space, size, keep = _workspace(need, workspace, q.device)
         status = self._library.tsac_hip_channel_linear_apply(
-            self.handle, a, a_stride, _vector(scales, index, _float32, rows, "scales"), rows, o, o_stride, type_, space,
-            size, _stream_of(index))
+            self.handle, a, a_stride, _vector(scales, index, _float32, rows, "scales"), rows, o, o_stride, type_,
+            _stream_of(index))
         if status:
             check(status)
-        del keep
 
 
 def quantize_tokens(x, q, scales):
