@@ -14,6 +14,11 @@
 // A row of up to 32,768 tokens is one workgroup's, held in registers between its maximum, its sum and its
 // store. Longer ones are divided: one launch leaves each part's maximum and sum, another joins them in
 // ascending order and computes the part again. Logits are asked for before anything is counted.
+//
+// 902 rows of 32,000 with a history of 4,093, BF16 to half: 63 us, where a copy of their bytes takes 25; without
+// rules 34, adjusted without a softmax 40 (27 without rules). What is left is some 30 instructions a token and the waits between the
+// phases of two workgroups a unit. Rows in 1,024 threads left one workgroup a unit or spilled (100 us); spilled registers
+// alone cost 5 us, penalties by branches 25, since most waves have a token of the history in each place.
 #include "lanes.hpp"
 #include "model_step.hpp"
 #include "paged_device.hpp"
@@ -33,7 +38,7 @@ constexpr int most_vectors = 8; // eights of a thread
 // Tokens of the history that a thread has in flight.
 constexpr int asked_for(int vectors)
 {
-    return vectors <= 2 ? 16 : 8;
+    return vectors <= 2 ? 16 : vectors <= 4 ? 8 : 4;
 }
 constexpr float minus_infinity = -__builtin_inff();
 constexpr float log2e = 1.44269504f;
@@ -304,7 +309,11 @@ __global__ __launch_bounds__(most_threads, 4) void logits_kernel(Launch l)
     }
     const std::size_t begin = std::size_t(row) * l.rows.stride;
     Raw<Wide> raw[Vectors];
-    uint8_t grammar[Vectors]; // tokens come in eights, so that their bits are a byte
+    // Tokens come in eights, so that their bits are a byte. Of eight eights they are read where they are used: there is no
+    // register left.
+    constexpr bool early = Vectors < most_vectors;
+    const auto* const bits = reinterpret_cast<const uint8_t*>(r.allowed + std::size_t(row) * r.allowed_stride);
+    uint8_t grammar[Vectors];
 #pragma unroll
     for (int i = 0; i < Vectors; ++i)
     {
@@ -314,9 +323,9 @@ __global__ __launch_bounds__(most_threads, 4) void logits_kernel(Launch l)
             raw[i] = *reinterpret_cast<const Raw<Wide>*>(static_cast<const char*>(l.rows.logits) +
                                                          (begin + token) * (Wide ? 4 : 2));
         }
-        if (r.allowed && token < to)
+        if (early && r.allowed && token < to)
         {
-            grammar[i] = reinterpret_cast<const uint8_t*>(r.allowed + std::size_t(row) * r.allowed_stride)[token / 8];
+            grammar[i] = bits[token / 8];
         }
     }
 
@@ -465,10 +474,11 @@ __global__ __launch_bounds__(most_threads, 4) void logits_kernel(Launch l)
             }
             if (r.allowed && there > 0)
             {
+                const unsigned byte = early ? grammar[i] : bits[token / 8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
                 {
-                    const int keep = int(unsigned(grammar[i]) << (31 - e)) >> 31; // all bits or none
+                    const int keep = int(byte << (31 - e)) >> 31; // all bits or none
                     x[i][e] = __uint_as_float((__float_as_uint(x[i][e]) & keep) | (0xff800000u & ~keep));
                 }
             }
@@ -558,8 +568,9 @@ Shape shape_of(const LogitRows& rows, std::size_t history)
     s.vectors = rounds <= 1 ? 1 : rounds <= 2 ? 2 : rounds <= 4 ? 4 : most_vectors;
     if (rounds > most_vectors || !rows.probabilities)
     {
-        // Parts, then: of four eights a thread (902 rows of 32,000, adjusted: 40 us, of eight 51, of two 49), of fewer
-        // where rows are few, for a workgroup a unit at least, if there are as many.
+        // Parts, then: of four eights a thread (902 rows of 32,000, adjusted alone: 40 us, of eight 51, of two 49), of
+        // fewer where rows are few, for a workgroup a unit at least, if there are as many (24 rows of 128,001 in parts
+        // of 16,384, 8,192 and 4,096: 27.2 us of 8,192, 31.5 of 4,096).
         s.vectors = std::min(s.vectors, 4);
         while (s.vectors > 1 && std::size_t(rows.rows) * ((rounds + s.vectors - 1) / s.vectors) < std::size_t(units))
         {
@@ -585,10 +596,16 @@ template <Step S> void launch(const Launch& l, const Shape& s, bool narrow, hipS
         constexpr int each = Words<N>::each;
         // Words of at most 64 KiB at a time, so that a unit has two workgroups.
         constexpr int most = N ? 4 : 2;
+        if constexpr (S == Step::whole)
+        {
+            if (s.vectors == most_vectors)
+            {
+                return go(logits_kernel<S, W, most_vectors, most_vectors / most, N>, most, each);
+            }
+        }
         s.vectors == 1   ? go(logits_kernel<S, W, 1, 1, N>, 1, each)
         : s.vectors == 2 ? go(logits_kernel<S, W, 2, 1, N>, 2, each)
-        : s.vectors == 4 ? go(logits_kernel<S, W, 4, 4 / most, N>, most, each)
-                         : go(logits_kernel<S, W, 8, 8 / most, N>, most, each);
+                         : go(logits_kernel<S, W, 4, 4 / most, N>, most, each);
     };
     if (l.rows.type == Type::single)
     {
