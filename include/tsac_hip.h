@@ -679,7 +679,8 @@ int tsac_hip_channel_linear_apply(const tsac_hip_channel_linear* linear, const i
 
 /* u = scale * gate * post(input); s = residual + u; out = norm(s), with
  * rms(x) = x / sqrt(mean x^2 + epsilon) * gain + bias and layer(x) = rms of x less its mean,
- * for each row of `width` (1 to 65536) elements. A member that is NULL or TSAC_HIP_NORM_NONE
+ * for each row of `width` (1 to 65536) elements, below 2^55 in size, so that 32 bits hold their
+ * squares' sum. A row's result is the same in every batch. A member that is NULL or TSAC_HIP_NORM_NONE
  * leaves its part out. input, gains, biases, gate and out are of `type` (BF16, FP16, FP32),
  * residual and sum of residual_type, which is `type` or FP32. Where out_scales is given, out
  * is int8 [rows][width] and quantised as by tsac_hip_quantize_tokens. out is the norm of s
@@ -798,7 +799,8 @@ typedef struct tsac_hip_logit_rules
 /* out [rows][alphabet] of out_type = the logits of `type` (FP32 too) under the rules or, with `probabilities`, their
  * softmax (x - max) / temperature. A temperature of 0 (or below) gives 1 to the lowest token of the largest x. A
  * row in which nothing is above -infinity is 0; one with an allowed NaN is NaN, and so is one with +infinity at a temperature
- * above 0. out may be the logits, of the same type and stride; rows of no sequence are left as they were. At
+ * above 0. Sums are 32-bit and of one order for the same sizes. out may be the logits, of the same type and stride, and
+ * overlaps nothing else; rows of no sequence are left as they were. At
  * most 2^20 tokens. Workspace as for tsac_hip_attention_paged. */
 size_t tsac_hip_adjust_logits_workspace(size_t rows, size_t alphabet);
 int tsac_hip_adjust_logits(const void* logits, size_t stride, int type, size_t rows, size_t alphabet,

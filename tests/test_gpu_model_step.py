@@ -400,6 +400,38 @@ def test_norms_without_their_parts_and_in_place(torch, native):
     assert torch.equal(b.r, kept) and torch.equal(b.x, want)
 
 
+@pytest.mark.parametrize("width", [60, 130, 512, 1000, 2048, 4100, 8192, 10000])
+def test_norms_are_the_same_in_every_batch(torch, native, width):
+    """A row alone, among others, and in rows that lie at odd places: the same bits."""
+    b = Block(torch, 5000, width, "bfloat16", "float32", 2, 2, 1, 4)
+    total, out = torch.empty(5000, width, device="cuda"), torch.empty(5000, width, dtype=torch.bfloat16, device="cuda")
+    b.run(native, total, out)
+    x, r, gate = b.x, b.r, b.gate
+    for first, rows in ((0, 1), (3, 2), (4000, 999)):
+        part = slice(first, first + rows)
+        for odd in (False, True):
+            place = (lambda t: torch.nn.functional.pad(t, (1, 2))[:, 1:-2]) if odd else (lambda t: t)  # noqa: E731
+            b.x, b.r, b.gate = place(x[part]), place(r[part]), place(gate)
+            some, other = torch.empty_like(total[part]), torch.empty_like(out[part])
+            b.run(native, some, other)
+            assert torch.equal(some, total[part]) and torch.equal(other, out[part]), (first, odd)
+
+
+def test_calls_of_no_rows(torch, native):
+    """Nothing is written, and nothing is refused."""
+    empty = lambda *shape, kind=torch.bfloat16: torch.empty(*shape, dtype=kind, device="cuda")  # noqa: E731
+    native.quantize_tokens(empty(0, 64), empty(0, 64, kind=torch.int8), empty(0, kind=torch.float32))
+    linear, *_ = linear_of(torch, native, 32, 64, 1)
+    linear.apply(empty(0, 64, kind=torch.int8), empty(0, kind=torch.float32), empty(0, 32))
+    native.block_norm(empty(0, 64), norm=native.NORM_RMS, out=empty(0, 64))
+    native.adjust_logits(empty(0, 100), empty(0, 100), ints(torch, [0, 0, 0]))
+    logits = normal(torch, (3, 100), 1, "float32")
+    out = torch.full((3, 100), 7.0, device="cuda")
+    native.adjust_logits(logits, out, ints(torch, [0]))  # no sequence
+    native.adjust_logits(logits, out, ints(torch, [2, 2, 2]))  # none with a row
+    assert bool((out == 7).all())
+
+
 def test_norms_of_more_than_2_to_the_31_elements(torch, native):
     rows, width = 270000, 8192
     x = torch.zeros(rows, width, dtype=torch.bfloat16, device="cuda")
