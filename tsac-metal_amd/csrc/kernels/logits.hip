@@ -570,7 +570,7 @@ Shape shape_of(const LogitRows& rows, std::size_t history)
     {
         // Parts, then: of four eights a thread (902 rows of 32,000, adjusted alone: 40 us, of eight 51, of two 49), of
         // fewer where rows are few, for a workgroup a unit at least, if there are as many (24 rows of 128,001 in parts
-        // of 16,384, 8,192 and 4,096: 27.2 us of 8,192, 31.5 of 4,096).
+        // of 16,384, 8,192 and 4,096 tokens: 27.4, 26.9 and 43 us).
         s.vectors = std::min(s.vectors, 4);
         while (s.vectors > 1 && std::size_t(rows.rows) * ((rounds + s.vectors - 1) / s.vectors) < std::size_t(units))
         {
