@@ -12,7 +12,7 @@
 // A row's values stay in the registers of its threads, so that the mean, the squares around it and
 // the largest value each are a pass over registers, in 32 bits and in an order that depends on the
 // width alone; a row of up to 1,024 values is one wave's, or a part of one's, which needs no barrier. What bounds it is
-// memory: 8190 rows of 8192, BF16, with a residual of 32 bits in 171 us, where a copy of their bytes takes 169; to 8 bits in 47 (42).
+// memory: 8190 rows of 8192, BF16, with a residual of 32 bits in 166 us, where a copy of their bytes takes 169; to 8 bits in 48 (42).
 #include "lanes.hpp"
 #include "model_step.hpp"
 #include "values.hpp"
@@ -236,7 +236,7 @@ enum Aligned
 
 // T: the values; R: the residual. A row is taken by Threads threads, each Vectors times eight values. Unless they are `any`, a
 // workgroup takes rows one after the other, and the next one's are on their way while one is worked on: they pass
-// barriers, which are for LDS alone. 8190 rows of 8192 with a residual of 32 bits: 171 us, a row a workgroup 204.
+// barriers, which are for LDS alone. 8190 rows of 8192 with a residual of 32 bits: 166 us, a row a workgroup 204.
 template <Type T, Type R, int Vectors, int Threads, Rows M>
 __global__ __launch_bounds__(Threads > 256 ? Threads : 256, 4) void block_norm_kernel(BlockRows p, int aligned)
 {
@@ -293,6 +293,9 @@ __global__ __launch_bounds__(Threads > 256 ? Threads : 256, 4) void block_norm_k
                 }
             }
         }
+        // Hidden from the compiler, which otherwise holds gains, biases and gates of all rows in registers and spills others
+        // for it (8190 rows of 8192: 176 us for 166); read again, they come from the caches.
+        asm volatile("" : "+s"(p.gate), "+s"(p.post.gain), "+s"(p.post.bias), "+s"(p.norm.gain), "+s"(p.norm.bias));
         if constexpr (Ahead)
         {
             if (row + stride < p.rows)
