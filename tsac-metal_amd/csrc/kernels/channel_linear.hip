@@ -56,9 +56,9 @@ template <Type T> __device__ __forceinline__ value_t<T> finished(int sum, float 
 }
 
 // 16 (or 4) bytes a lane, from `offset` bytes behind `from`, to `to`, lane after lane; the wave waits for it with
-// its other loads (s_waitcnt vmcnt). `Once`: past the caches. Written out because the compiler would wait for it before any other read of
-// LDS. A load to LDS needs a wait state behind a write of M0, which the compiler does not put into assembly. M0 is
-// reserved, so that clang warns where it is named; nothing else uses it.
+// its other loads (s_waitcnt vmcnt). `Once`: past the caches. Written out because the compiler would wait for it before
+// any other read of LDS. A load to LDS needs a wait state behind a write of M0, which the compiler does not put into
+// assembly. M0 is reserved, so that clang warns where it is named; nothing else uses it.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ unsigned lds_address(const void* p)
@@ -241,13 +241,14 @@ __global__ __launch_bounds__(narrow::waves * lanes) void narrow_kernel(Launch l)
 // ------------------------------------------------------------------ many rows
 //
 // Workgroups of four waves, 2 x 2, take tiles of 64 JN outputs x 64 JM rows one after the other, each wave JN x JM
-// results of 32 x 32. A stage is 64 or 128 inputs of a tile's operands. Stages pass from memory straight into a ring in LDS, across the tiles' borders: while a tile is stored the next one's first stages are on their way. At
-// a stage's barrier the next one has landed, so that its first operands are read from LDS under the stage's last products.
+// results of 32 x 32. A stage is 64 or 128 inputs of a tile's operands. Stages pass from memory straight into a ring in
+// LDS, across the tiles' borders: while a tile is stored the next one's first stages are on their way. At a stage's
+// barrier the next one has landed, so that its first operands are read from LDS under the stage's last products.
 //
 // Activation rows lie in LDS with their 16-byte pieces exchanged by row, so that lanes that read one piece of
 // consecutive rows meet different banks; weights lie as they are read.
 //
-// 8192 x 8192 x 8192: 480 us, 2,290 TOP/s, matrix units busy 58% at about 1.9 GHz. With weights of zero, which cost no power,
+// 8192 x 8192 x 8192: 480 us, 2,290 TOP/s, matrix units busy 56%, the clock held down to about 1.9 GHz. With weights of zero, which cost no power,
 // 352 us; without the loads, in a copy, 354, without the barriers too 343; with all loads from one tile 475, so that it is
 // their way into LDS that costs, not memory. Results by way of LDS, in whole lines, were slower (525 us).
 //
