@@ -731,7 +731,7 @@ LogitRows logit_rows(std::size_t rows, std::size_t alphabet, bool probabilities)
 
 struct tsac_hip_channel_linear
 {
-    DeviceBuffer values, constants;
+    DeviceBuffer memory; // operand tiles, scales, bias
     ChannelWeights weights;
     int device = 0;
 };
@@ -1672,23 +1672,28 @@ int tsac_hip_channel_linear_create(const int8_t* values, const float* scales, co
             require(capture == hipStreamCaptureStatusNone, "channel linear: a linear cannot be made in a capture");
             auto l = std::make_unique<tsac_hip_channel_linear>();
             check_hip(hipGetDevice(&l->device), "hipGetDevice");
-            l->values = DeviceBuffer(channel_tiles_bytes(K, N));
-            const std::size_t constant = (N * 4 + 255) / 256 * 256;
-            l->constants = DeviceBuffer(2 * constant);
-            const DeviceBuffer canonical(N * K);
-            auto* c = l->constants.as<uint8_t>();
-            hipError_t e = hipMemcpyAsync(canonical.get(), values, N * K, hipMemcpyDefault, s);
+            const std::size_t tiles = channel_tiles_bytes(K, N), constant = (N * 4 + 255) / 256 * 256;
+            l->memory = DeviceBuffer(tiles + 2 * constant);
+            auto* const tiled = l->memory.as<int8_t>();
+            auto* const c = l->memory.as<uint8_t>() + tiles; // tiles are a multiple of 4 KiB
+            // What lies on this device is laid out from where it is.
+            hipPointerAttribute_t place{};
+            const bool here = hipPointerGetAttributes(&place, values) == hipSuccess &&
+                              place.type == hipMemoryTypeDevice && place.device == l->device;
+            (void)hipGetLastError(); // of memory that is the host's alone
+            const DeviceBuffer canonical = here ? DeviceBuffer() : DeviceBuffer(N * K);
+            hipError_t e = here ? hipSuccess : hipMemcpyAsync(canonical.get(), values, N * K, hipMemcpyDefault, s);
             e = e != hipSuccess ? e : hipMemcpyAsync(c, scales, N * 4, hipMemcpyDefault, s);
             e = e != hipSuccess || !bias ? e : hipMemcpyAsync(c + constant, bias, N * 4, hipMemcpyDefault, s);
             if (e == hipSuccess)
             {
-                channel_tiles(canonical.as<int8_t>(), K, N, l->values.as<int8_t>(), s);
+                channel_tiles(here ? values : canonical.as<int8_t>(), K, N, tiled, s);
             }
             // Waited for in any case: what has been queued uses the buffers.
             const hipError_t waited = hipStreamSynchronize(s);
             check_hip(e, "upload");
             check_hip(waited, "upload");
-            l->weights.values = l->values.as<int8_t>();
+            l->weights.values = tiled;
             l->weights.scales = reinterpret_cast<const float*>(c);
             l->weights.bias = bias ? reinterpret_cast<const float*>(c + constant) : nullptr;
             l->weights.inputs = int(K);
