@@ -12,7 +12,8 @@
 // A row's values stay in the registers of its threads, so that the mean, the squares around it and
 // the largest value each are a pass over registers, in 32 bits and in an order that depends on the
 // width alone; a row of up to 1,024 values is one wave's, or a part of one's, which needs no barrier. What bounds it is
-// memory: 8190 rows of 8192, BF16, with a residual of 32 bits in 166 us, where a copy of their bytes takes 169; to 8 bits in 48 (42).
+// memory: 8190 rows of 8192, BF16, with a residual of 32 bits in 167 us, where a copy of their bytes takes 169; to 8 bits
+// in 49 (42).
 #include "lanes.hpp"
 #include "model_step.hpp"
 #include "values.hpp"
@@ -195,8 +196,8 @@ __device__ __forceinline__ int nearest(float x, float scale, float reciprocal)
     return int(__builtin_fminf(__builtin_fmaxf(r, -127.0f), 127.0f));
 }
 
-// Eight of them, a byte each. x / scale + 1.5 2^23 has the whole number in its lowest bits; where the rest of one is half a step
-// or more, which takes a border within 2^-15 of a step, all are done with care.
+// Eight of them, a byte each. x / scale + 1.5 2^23 has the whole number in its lowest bits; where the rest of one is half a
+// step or more, which takes a border within 2^-15 of a step, all are done with care.
 __device__ __forceinline__ uint2 nearest8(const float (&x)[8], float scale, float reciprocal)
 {
     constexpr float whole = 0x1.8p23f;
@@ -234,9 +235,9 @@ enum Aligned
     norm_aligned = 64
 };
 
-// T: the values; R: the residual. A row is taken by Threads threads, each Vectors times eight values. Unless they are `any`, a
-// workgroup takes rows one after the other, and the next one's are on their way while one is worked on: they pass
-// barriers, which are for LDS alone. 8190 rows of 8192 with a residual of 32 bits: 166 us, a row a workgroup 204.
+// T: the values; R: the residual. A row is taken by Threads threads, each Vectors times eight values. Unless they are
+// `any`, a workgroup takes rows one after the other, and the next one's are on their way while one is worked on: they pass
+// barriers, which are for LDS alone. 8190 rows of 8192 with a residual of 32 bits: 167 us, a row a workgroup 204.
 template <Type T, Type R, int Vectors, int Threads, Rows M>
 __global__ __launch_bounds__(Threads > 256 ? Threads : 256, 4) void block_norm_kernel(BlockRows p, int aligned)
 {
@@ -434,7 +435,8 @@ template <Type T, Type R> void launch(const BlockRows& p, int aligned, hipStream
         : w <= 32768  ? go(block_norm_kernel<T, R, 4, 1024, Rows::any>, 1024, most_groups)
                       : go(block_norm_kernel<T, R, 8, 1024, Rows::any>, 1024, most_groups);
     };
-    constexpr int every = input_aligned | gate_aligned | residual_aligned | sum_aligned | out_aligned | post_aligned | norm_aligned;
+    constexpr int every =
+        input_aligned | gate_aligned | residual_aligned | sum_aligned | out_aligned | post_aligned | norm_aligned;
     aligned != every     ? of(std::integral_constant<Rows, Rows::any>{})
     : p.width % 8 != 0   ? of(std::integral_constant<Rows, Rows::ragged>{})
                          : of(std::integral_constant<Rows, Rows::whole>{});

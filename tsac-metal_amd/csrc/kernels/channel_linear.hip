@@ -108,8 +108,8 @@ __device__ __forceinline__ void ring_barrier()
 // ------------------------------------------------------------------ few rows
 //
 // What costs is reading the weights. A workgroup takes 32 outputs and up to 8 Pieces rows, each of its waves every fourth
-// step of 128 inputs, through a ring of Ring steps in LDS of its own: it asks for a step as soon as it has read the one whose
-// place that takes, and waits for nobody until the waves' sums meet. Rows of activations come in whole lines of 128 bytes,
+// step of 128 inputs, through a ring of Ring steps in LDS of its own: it asks for a step as soon as it has read the one
+// whose place that takes, and waits for nobody until the waves' sums meet. Rows of activations come in whole lines of 128 bytes,
 // which straight into registers, 32 bytes of each of 32 rows at a time, they would not (48 rows, 8192 x 8192: 26 us
 // for 16 now, where reading the weights takes 11), their pieces exchanged by row so that eight rows' meet different banks.
 // More steps in flight, or eight waves, gain nothing (rings of 3 and 4: 17 us) and keep a unit from a second workgroup.
@@ -248,9 +248,10 @@ __global__ __launch_bounds__(narrow::waves * lanes) void narrow_kernel(Launch l)
 // Activation rows lie in LDS with their 16-byte pieces exchanged by row, so that lanes that read one piece of
 // consecutive rows meet different banks; weights lie as they are read.
 //
-// 8192 x 8192 x 8192: 480 us, 2,290 TOP/s, matrix units busy 56%, the clock held down to about 1.9 GHz. With weights of zero, which cost no power,
-// 352 us; without the loads, in a copy, 354, without the barriers too 343; with all loads from one tile 475, so that it is
-// their way into LDS that costs, not memory. Results by way of LDS, in whole lines, were slower (525 us).
+// 8192 x 8192 x 8192: 480 us, 2,290 TOP/s, matrix units busy 56%, the clock held down to about 1.9 GHz. With weights of
+// zero, which cost no power, 352 us; without the loads, in a copy, 354, without the barriers too 343; with all loads from
+// one tile 475, so that it is their way into LDS that costs, not memory. Results by way of LDS, in whole lines, were
+// slower (525 us).
 //
 // A die's workgroups take neighbouring tiles, four of rows by as many of outputs as there are, which share what they
 // read in its cache.
@@ -270,8 +271,8 @@ template <int JN, int JM, int Depth, int Ring> struct Shape
     static constexpr int loads = weight_loads + row_loads;
     static constexpr int constants = 2 * n + m;                     // scales and bias of a tile
     static constexpr int constant_loads = (constants / 64 + 3) / 4; // of a wave and tile
-    // With the fewest stages a tile, two of 64 or one of 128, the scales of the tile Ring / 2, or Ring - 1, further on arrive
-    // before this one is stored.
+    // With the fewest stages a tile, two of 64 or one of 128, the scales of the tile Ring / 2, or Ring - 1, further on
+    // arrive before this one is stored.
     static constexpr int constant_slots = Depth == 64 ? Ring / 2 + 1 : Ring;
     static constexpr int lds_bytes = ring * stage_bytes + 4 * constant_slots * constants;
     static constexpr int row_pieces = Depth / 16;
@@ -338,7 +339,10 @@ __device__ __forceinline__ void store_block(const v16i& sums, float token, const
     }
 }
 
-template <Type T, int JN, int JM, int Depth, int Ring, int PerUnit>
+// Once: all rows are in one row tile, so that each weight is read once and need not stay in a cache, where the results and
+// the rows then do. With six layers' weights in turn, 190 x 2043 x 32003 to FP32 in 28.7 us for 30.8, to BF16 26.2 for
+// 28.2, 256 x 4096 x 14336 26.8 for 26.6; one layer's again and again, 65 MB, as before.
+template <Type T, int JN, int JM, int Depth, int Ring, int PerUnit, bool Once>
 __global__ __launch_bounds__(tiled::threads, PerUnit) void tiled_kernel(Launch l, int row_tiles, int column_tiles)
 {
     using namespace tiled;
@@ -396,8 +400,8 @@ __global__ __launch_bounds__(tiled::threads, PerUnit) void tiled_kernel(Launch l
     };
     const auto ask_weights = [&](int slot, int j)
     {
-        load16_to_lds<false>(weights[j], unsigned(loading_stage) * (S::cuts * tile_bytes) + lane * 16,
-                             lds + slot * S::stage_bytes + (warp * S::weight_loads + j) * tile_bytes);
+        load16_to_lds<Once>(weights[j], unsigned(loading_stage) * (S::cuts * tile_bytes) + lane * 16,
+                            lds + slot * S::stage_bytes + (warp * S::weight_loads + j) * tile_bytes);
     };
     const auto ask_rows = [&](int slot, int j)
     {
@@ -627,9 +631,16 @@ template <Type T, int JN, int JM, int Depth, int Ring, int PerUnit> void launch_
 {
     using S = tiled::Shape<JN, JM, Depth, Ring>;
     static_assert(S::lds_bytes * PerUnit <= 160 * 1024);
-    const auto kernel = tiled_kernel<T, JN, JM, Depth, Ring, PerUnit>;
-    allow_lds(kernel, S::lds_bytes);
     const int row_tiles = (l.rows + S::m - 1) / S::m, column_tiles = (l.outputs + S::n - 1) / S::n;
+    auto kernel = tiled_kernel<T, JN, JM, Depth, Ring, PerUnit, false>;
+    if constexpr (S::m > 64) // fewer rows than 65 do not come here
+    {
+        if (row_tiles == 1)
+        {
+            kernel = tiled_kernel<T, JN, JM, Depth, Ring, PerUnit, true>;
+        }
+    }
+    allow_lds(kernel, S::lds_bytes);
     const std::size_t total = std::size_t(row_tiles) * column_tiles;
     require(total < (std::size_t(1) << 30), "channel linear: too many tiles");
     const std::size_t most = std::size_t(compute_units()) * PerUnit / tiled::dies * tiled::dies;

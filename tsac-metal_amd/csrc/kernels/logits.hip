@@ -16,9 +16,9 @@
 // ascending order and computes the part again. Logits are asked for before anything is counted.
 //
 // 902 rows of 32,000 with a history of 4,093, BF16 to half: 63 us, where a copy of their bytes takes 25; without
-// rules 34, adjusted without a softmax 40 (27 without rules). What is left is some 30 instructions a token and the waits between the
-// phases of two workgroups a unit. Rows in 1,024 threads left one workgroup a unit or spilled (100 us); spilled registers
-// alone cost 5 us, penalties by branches 25, since most waves have a token of the history in each place.
+// rules 34, adjusted without a softmax 40 (27 without rules). What is left is some 30 instructions a token and the waits
+// between the phases of two workgroups a unit. Rows in 1,024 threads left one workgroup a unit or spilled (100 us);
+// spilled registers alone cost 5 us, penalties by branches 25, since most waves have a token of the history in each place.
 #include "lanes.hpp"
 #include "model_step.hpp"
 #include "paged_device.hpp"
