@@ -799,9 +799,10 @@ typedef struct tsac_hip_logit_rules
 /* out [rows][alphabet] of out_type = the logits of `type` (FP32 too) under the rules or, with `probabilities`, their
  * softmax (x - max) / temperature. A temperature of 0 (or below) gives 1 to the lowest token of the largest x. A
  * row in which nothing is above -infinity is 0; one with an allowed NaN is NaN, and so is one with +infinity at a temperature
- * above 0. Sums are 32-bit and of one order for the same sizes. out may be the logits, of the same type and stride, and
- * overlaps nothing else; rows of no sequence are left as they were. At
- * most 2^20 tokens. Workspace as for tsac_hip_attention_paged. */
+ * above 0. Sums are 32-bit and of one order for the same sizes: a row's follows the alphabet, the history's stride and, past
+ * 32768 tokens, the number of rows. out may be the logits, of the same type and stride, and overlaps nothing else; rows of no
+ * sequence are left as they were. At most 2^20 tokens. Workspace as for tsac_hip_attention_paged; what the largest batch
+ * needs is enough for smaller ones. */
 size_t tsac_hip_adjust_logits_workspace(size_t rows, size_t alphabet);
 int tsac_hip_adjust_logits(const void* logits, size_t stride, int type, size_t rows, size_t alphabet,
                            const tsac_hip_logit_rules* rules, int probabilities, void* out, size_t out_stride,

@@ -882,6 +882,20 @@ def test_logits_in_place_and_rows_of_no_sequence(torch, native):
         assert bool((wide[[0, 6, 7]] == 7).all())
 
 
+@pytest.mark.parametrize("alphabet", [50001, 128001])
+def test_a_workspace_for_the_largest_batch(torch, native, alphabet):
+    """One workspace for batches that shrink, across the numbers of rows at which a row has another number of parts."""
+    need = native.library().tsac_hip_adjust_logits_workspace
+    space = torch.full((need(64, alphabet) + 16,), 77, dtype=torch.uint8, device="cuda")
+    for counts in ([40, 24], [63], [20, 17], [36], [31], [16], [15], [1]):
+        logits = Logits(torch, counts, alphabet, "bfloat16", seed=sum(counts), biases=0, allowed=None)
+        out = torch.empty(logits.rows, alphabet, device="cuda")
+        logits.run(native, out, workspace=space[:need(64, alphabet)])
+        want, room = logits.probabilities()
+        near(torch, out, want, room + H * want + TINY["float32"])
+        assert bool((space[-16:] == 77).all())
+
+
 def test_logits_past_2_to_the_31_elements(torch, native):
     rows, alphabet = 17000, 131072
     x = torch.zeros(rows, alphabet, dtype=torch.bfloat16, device="cuda")

@@ -119,6 +119,17 @@ def test_logit_rules(changes, call, text):
     assert lib.tsac_hip_adjust_logits_workspace(4, 0) == 0
 
 
+def test_workspaces_of_logits():
+    """One asked for once, for a program's largest batch, is enough for every smaller one; and the query grows with both sizes."""
+    need = native.library().tsac_hip_adjust_logits_workspace
+    for alphabet in (1, 32768, 32769, 50001, 65537, 128001, 1 << 20):
+        sizes = [need(rows, alphabet) for rows in range(600)]
+        assert all(a <= b for a, b in zip(sizes, sizes[1:])), alphabet
+    for rows in (1, 3, 15, 16, 31, 32, 63, 64, 255, 256, 5000):
+        sizes = [need(rows, alphabet) for alphabet in range(1, 1 << 20, 509)]
+        assert all(a <= b for a, b in zip(sizes, sizes[1:])), rows
+
+
 def test_frequencies():
     """Plain ones, divided ones, those of a larger base and those chosen by their turns, from the formulas."""
     for rotary in (2, 4, 20, 96, 128):

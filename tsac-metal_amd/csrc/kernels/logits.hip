@@ -619,10 +619,16 @@ template <Step S> void launch(const Launch& l, const Shape& s, bool narrow, hipS
 }
 } // namespace
 
+// Of the narrowest parts: how many parts a row has falls where there are more rows, and a workspace that a program keeps for
+// its largest batch has to do for smaller ones.
 std::size_t logits_workspace(const LogitRows& rows)
 {
-    const Shape s = shape_of(rows, 0); // a history changes the threads of rows in one part alone
-    return rows.probabilities && s.splits > 1 ? std::size_t(rows.rows) * s.splits * sizeof(Part) : 0;
+    if (!rows.probabilities || shape_of(rows, 0).splits == 1) // a history changes the threads of rows in one part alone
+    {
+        return 0;
+    }
+    constexpr std::size_t narrowest = 8 * most_threads;
+    return std::size_t(rows.rows) * ((rows.alphabet + narrowest - 1) / narrowest) * sizeof(Part);
 }
 
 void adjust_logits(const LogitRows& rows, const LogitRules& rules, void* workspace, std::size_t bytes,
