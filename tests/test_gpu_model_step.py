@@ -811,6 +811,28 @@ def test_lengths_of_histories_out_of_range(torch, native):
     logits.check(native, "float32")
 
 
+@pytest.mark.parametrize("alphabet", [50, 1000, 8200, 32001, 40001])
+def test_tokens_out_of_range_are_passed_over(torch, native, alphabet):
+    """In the history, among the nodes and among the biases, whatever the rules would make of them."""
+    x = normal(torch, (6, alphabet), 1, "float32", 4.0)
+    within = [0, alphabet // 2, alphabet - 1]
+    outside = [alphabet, alphabet + 1, alphabet + 6, alphabet + 9, -1, -alphabet, 2 ** 31 - 1, -2 ** 31]
+    starts, nodes = ints(torch, [0, 2, 4, 6]), ints(torch, [0, alphabet, 0, -1, 0, alphabet + 3])
+    for repetition in (0.0, -0.5, 1.5, math.nan):
+        rules = dict(repetition=floats(torch, [repetition] * 3), presence=floats(torch, [0.5] * 3),
+                     frequency=floats(torch, [0.25] * 3), bias_starts=ints(torch, [0, 2, 2, 4]),
+                     bias_tokens=ints(torch, [alphabet, alphabet + 2, 1, alphabet + 5]),
+                     bias_values=floats(torch, [math.nan, math.inf, 0.0, math.inf]))
+        lone = torch.where(torch.arange(6, device="cuda") % 2 == 0, 0, -1).int()  # the nodes that are of the alphabet
+        for probabilities in (False, True):
+            got, want = torch.empty_like(x), torch.empty_like(x)
+            for out, tokens, past in ((got, nodes, within + outside), (want, lone, within + [-1] * len(outside))):
+                native.adjust_logits(x, out, starts, probabilities=probabilities, history=ints(torch, [past] * 3),
+                                     history_lengths=ints(torch, [len(past)] * 3), tokens=tokens, **rules)
+            assert torch.equal(got.nan_to_num(-7.0), want.nan_to_num(-7.0)), (repetition, probabilities)
+            assert repetition not in (-0.5, 1.5) or not bool(want.isnan().any())
+
+
 @pytest.mark.parametrize("alphabet", [50, 1000, 40000])
 def test_the_likeliest_token(torch, native, alphabet):
     """Temperature 0 and below, ties, rows without a token, infinities and what is not a number."""

@@ -338,6 +338,7 @@ __global__ __launch_bounds__(most_threads, 4) void logits_kernel(Launch l)
     for (int round = 0; round < Rounds; ++round)
     {
         const int base = from + round * words.chunk;
+        const unsigned inside = unsigned(max(0, min(words.chunk, to - base))); // tokens of the alphabet among its words
         if (edited)
         {
 #pragma unroll
@@ -351,7 +352,7 @@ __global__ __launch_bounds__(most_threads, 4) void logits_kernel(Launch l)
                 const auto add = [&](int token, int i)
                 {
                     const unsigned t = unsigned(token) - unsigned(base);
-                    if (t < unsigned(words.chunk))
+                    if (t < inside)
                     {
                         words.bias(t, unsigned(i - bias_begin) + 1);
                     }
@@ -369,7 +370,7 @@ __global__ __launch_bounds__(most_threads, 4) void logits_kernel(Launch l)
             const auto had = [&](int token, bool said)
             {
                 const unsigned t = unsigned(token) - unsigned(base);
-                if (t < unsigned(words.chunk))
+                if (t < inside)
                 {
                     words.count(t, said);
                 }
@@ -465,7 +466,7 @@ __global__ __launch_bounds__(most_threads, 4) void logits_kernel(Launch l)
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
                     {
-                        if (const unsigned place = words.place(bias[e]); place && e < there)
+                        if (const unsigned place = words.place(bias[e]); place)
                         {
                             x[i][e] += r.bias_values[bias_begin + int(place) - 1];
                         }
