@@ -765,7 +765,7 @@ int tsac_hip_pages_append(const tsac_hip_paged_cache* cache, uint32_t layer, con
  * or, with `tokens`, is that of a node on the row's line: rows of its sequence whose bit is set in
  * mask[row][words] or, with mask NULL, the row itself and those in front of it. Its count leaves out the first
  * prompt_lengths[s] of the history.
- *   repetition[s] r: a token that was had, x > 0 ? x (1 / r) : x r
+ *   repetition[s] r: a token that was had, x > 0 ? x / r : x r
  *   frequency[s], presence[s], finite: x - frequency * count, and - presence where the count is not 0
  *   bias_values[i] for i from bias_starts[s] to bias_starts[s+1]: added to token bias_tokens[i]; of a token
  *     that is listed twice the last one

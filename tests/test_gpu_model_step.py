@@ -877,6 +877,44 @@ def test_rows_that_are_empty_or_broken(torch, native, alphabet):
     assert bool(((out[[2, 3]].double().sum(1) - 1).abs() < 1e-5).all())
 
 
+@pytest.mark.parametrize("alphabet", [4096, 32000, 70001])
+def test_shares_far_below_the_largest(torch, native, alphabet):
+    """A probability over the largest one, which leaves the sum out: e^((x - m) / t). The difference is rounded, and its product
+    with the factor: 2 h of the exponent. The exponential is off by 2^-22 at most and the factor, joined from two floats, by less
+    than h / 8 of the exponent; the largest's weight is 1, and both are rounded as they are scaled and stored, 4 h."""
+    temperatures = [0.3, 0.37, 0.5, 0.61, 0.7, 0.77, 0.9, 1.0, 1.1, 1.3, 1.7, 2.3]
+    x = normal(torch, (len(temperatures), alphabet), 7, "float32", 3.0)
+    out = torch.empty_like(x)
+    t = floats(torch, temperatures)
+    native.adjust_logits(x, out, ints(torch, list(range(len(temperatures) + 1))), temperature=t)
+    exponent = (x.double() - x.double().amax(1, keepdim=True)) / t.double()[:, None]
+    want = exponent.exp()
+    got = out.double() / out.double().amax(1, keepdim=True)
+    room = want * (2.125 * H * exponent.abs() + 2.0 ** -22 + 4 * H) * (1 + 2.0 ** -12)
+    normal_numbers = want > 2.0 ** -100
+    assert bool(((got - want).abs() <= room)[normal_numbers].all()), float(((got - want).abs() / room)[normal_numbers].max())
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_a_repeated_logit_is_divided(torch, native, kind):
+    """x / r of a positive one and x r of another are each rounded once; h / 64 for what stands in for the quotient."""
+    alphabet = 5000
+    factors = [1.0, 1.1, 1.15, 1.2, 1.3, 1.5, 2.0, 3.0, 0.7, 7.3]
+    x = normal(torch, (len(factors), alphabet), 9, kind, 4.0)
+    out = torch.empty(x.shape, device="cuda")
+    r = floats(torch, factors)
+    history = torch.arange(alphabet, dtype=torch.int32, device="cuda").repeat(len(factors), 1)
+    native.adjust_logits(x, out, ints(torch, list(range(len(factors) + 1))), probabilities=False, history=history,
+                         history_lengths=ints(torch, [alphabet] * len(factors)), repetition=r)
+    v, by = x.double(), r.double()[:, None]
+    want = torch.where(v > 0, v / by, v * by)
+    near(torch, out, want, H * (1 + 1 / 64) * want.abs())
+    x[:, ::7], x[:, 1::7], x[:, 2::7] = math.inf, -math.inf, 0.0
+    native.adjust_logits(x, out, ints(torch, list(range(len(factors) + 1))), probabilities=False, history=history,
+                         history_lengths=ints(torch, [alphabet] * len(factors)), repetition=r)
+    assert torch.equal(out.sign(), x.float().sign()) and torch.equal(out.isinf(), x.isinf())
+
+
 def test_temperatures_at_their_ends(torch, native):
     """So small that its reciprocal overflows: the largest share it all; so large that all are alike."""
     x = floats(torch, [[1.0, 3.0, 3.0, -2.0]] * 4)

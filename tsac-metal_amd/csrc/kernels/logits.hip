@@ -1,7 +1,7 @@
 // What a program does to a model's logits before it samples or verifies drafts: penalties for tokens that a
 // sequence has had already, biases, a grammar's mask, and the softmax at a temperature.
 //
-//   x = logit; where the token was had: x * fl(1 / r) if x > 0, else x r (repetition r)
+//   x = logit; where the token was had: x / r if x > 0, else x r (repetition r)
 //   x = x - f count - (count > 0 ? g : 0)                                (frequency f, presence g)
 //   x = x + bias;  -infinity where the grammar has no bit
 //   p = e^((x - m) / t) / sum e^((x - m) / t),  m = max x;   t = 0: 1 at the lowest of the largest
@@ -19,6 +19,8 @@
 // rules 34, adjusted without a softmax 40 (27 without rules). What is left is some 30 instructions a token and the waits
 // between the phases of two workgroups a unit. Rows in 1,024 threads left one workgroup a unit or spilled (100 us);
 // spilled registers alone cost 5 us, penalties by branches 25, since most waves have a token of the history in each place.
+// Quotients are products with factors of two floats, each rounded once (1 us; with factors of one float, probabilities far below
+// the largest were off by twice as much).
 #include "lanes.hpp"
 #include "model_step.hpp"
 #include "paged_device.hpp"
@@ -41,7 +43,8 @@ constexpr int asked_for(int vectors)
     return vectors <= 2 ? 16 : vectors <= 4 ? 8 : 4;
 }
 constexpr float minus_infinity = -__builtin_inff();
-constexpr float log2e = 1.44269504f;
+constexpr float log2e = 0x1.715476p0f, log2e_rest = 0x1.4ae0cp-26f;
+constexpr float little = 0x1p-126f;
 
 struct Part // of a row: what its softmax needs of it
 {
@@ -150,10 +153,31 @@ struct Exchange
     int i[most_threads / lanes];
 };
 
-// e^((x - top) / t) as a power of two, of a finite top. -infinity gives 0, what is not a number and +infinity no number.
-__device__ __forceinline__ float weight(float x, float top, float per_log2)
+// A factor as the sum of two floats, so that a product with it is rounded once: a rounded factor would be off in one direction
+// for all tokens of a row.
+struct Factor
 {
-    return __builtin_amdgcn_exp2f((x - top) * per_log2);
+    float high, low;
+};
+__device__ __forceinline__ float times(float x, const Factor& by)
+{
+    return __builtin_fmaf(x, by.high, x * by.low);
+}
+
+// (a + rest) / b of numbers above 0, from a / b. Both parts are above 0, so that infinities stay what they are; where a / b is far
+// out there is no second one to speak of.
+__device__ __forceinline__ Factor divided(float quotient, float a, float rest, float b)
+{
+    const bool near = quotient > 0x1p-100f && quotient < 0x1p100f;
+    const float high = near ? __uint_as_float(__float_as_uint(quotient) - 1) : quotient;
+    const float low = (__builtin_fmaf(-high, b, a) + rest) * __builtin_amdgcn_rcpf(b);
+    return {high, near ? __builtin_fmaxf(low, little) : little};
+}
+
+// e^((x - top) / t) as a power of two, of a finite top. -infinity gives 0, what is not a number and +infinity no number.
+__device__ __forceinline__ float weight(float x, float top, const Factor& per_log2)
+{
+    return __builtin_amdgcn_exp2f(times(x - top, per_log2));
 }
 
 // What stands for the largest of a row in which nothing is above -infinity: its weights are 0, or no numbers.
@@ -164,15 +188,17 @@ __device__ __forceinline__ float reference(float top)
 
 // A temperature's factor; where that would be infinite the largest number, which times 0 is still 0, where it would be 0 a
 // small one, which times -infinity is still that.
-__device__ __forceinline__ float factor_of(float temperature)
+__device__ __forceinline__ Factor factor_of(float temperature)
 {
-    return __builtin_fmaxf(__builtin_fminf(log2e / temperature, 0x1.fffffep127f), 0x1p-126f);
+    const float quotient = __builtin_fmaxf(__builtin_fminf(log2e / temperature, 0x1.fffffep127f), 0x1p-126f);
+    return divided(quotient, log2e, log2e_rest, temperature);
 }
 
 // What is known of values held in registers: the largest and its lowest place, the sum of weights, which stand in the
 // values' place afterwards.
 template <int Vectors>
-__device__ __forceinline__ Part part_of(float (&x)[Vectors][8], int from, float temperature, Exchange& shared)
+__device__ __forceinline__ Part part_of(float (&x)[Vectors][8], int from, bool soft, const Factor& factor,
+                                        Exchange& shared)
 {
     Part part;
     float top = minus_infinity;
@@ -189,9 +215,8 @@ __device__ __forceinline__ Part part_of(float (&x)[Vectors][8], int from, float 
     part.sum = 0.0f;
     part.first = 1 << 30;
     part.broken = 0;
-    if (temperature > 0.0f)
+    if (soft)
     {
-        const float factor = factor_of(temperature);
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < Vectors; ++i)
@@ -226,16 +251,15 @@ __device__ __forceinline__ Part part_of(float (&x)[Vectors][8], int from, float 
 }
 
 // A later part joined to what is in front of it.
-__device__ __forceinline__ Part join(const Part& a, const Part& b, float temperature)
+__device__ __forceinline__ Part join(const Part& a, const Part& b, bool soft, const Factor& factor)
 {
     Part r;
     r.top = __builtin_fmaxf(a.top, b.top);
     r.first = a.top >= b.top ? a.first : b.first;
     r.broken = a.broken | b.broken;
     r.sum = 0.0f;
-    if (temperature > 0.0f)
+    if (soft)
     {
-        const float factor = factor_of(temperature);
         // A part without a number above -infinity has a sum of 0, or none that is a number.
         const float wa = a.top == r.top ? 1.0f : weight(a.top, r.top, factor);
         const float wb = b.top == r.top ? 1.0f : weight(b.top, r.top, factor);
@@ -330,7 +354,13 @@ __global__ __launch_bounds__(most_threads, 4) void logits_kernel(Launch l)
     }
 
     const float repetition = r.repetition ? r.repetition[s] : 1.0f, presence = r.presence ? r.presence[s] : 0.0f;
-    const float frequency = r.frequency ? r.frequency[s] : 0.0f, reciprocal = 1.0f / repetition;
+    const float frequency = r.frequency ? r.frequency[s] : 0.0f;
+    const float temperature = S != Step::adjust && r.temperature ? r.temperature[s] : 1.0f;
+    const bool soft = temperature > 0.0f;
+    const Factor factor = factor_of(temperature);
+    const Factor inverse = divided(1.0f / __builtin_fabsf(repetition), 1.0f, 0.0f, __builtin_fabsf(repetition));
+    const float reciprocal = __builtin_copysignf(inverse.high, repetition);
+    const float reciprocal_rest = __builtin_copysignf(inverse.low, repetition);
     const bool edited = l.counted || bias_begin < bias_end;
     const Words<Narrow> words = {memory, 8 * threads * held};
     float x[Vectors][8];
@@ -456,10 +486,12 @@ __global__ __launch_bounds__(most_threads, 4) void logits_kernel(Launch l)
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
                 {
-                    const float times = float(said[e] >> 1);
-                    x[i][e] *= said[e] ? (x[i][e] > 0.0f ? reciprocal : repetition) : 1.0f;
-                    x[i][e] = __builtin_fmaf(-frequency, times, x[i][e]);
-                    x[i][e] = __builtin_fmaf(-presence, __builtin_fminf(times, 1.0f), x[i][e]);
+                    const float count = float(said[e] >> 1);
+                    const bool above = x[i][e] > 0.0f;
+                    const float rest = said[e] && above ? x[i][e] * reciprocal_rest : 0.0f;
+                    x[i][e] = __builtin_fmaf(x[i][e], said[e] ? (above ? reciprocal : repetition) : 1.0f, rest);
+                    x[i][e] = __builtin_fmaf(-frequency, count, x[i][e]);
+                    x[i][e] = __builtin_fmaf(-presence, __builtin_fminf(count, 1.0f), x[i][e]);
                 }
                 if (words.biased(bias))
                 {
@@ -486,25 +518,23 @@ __global__ __launch_bounds__(most_threads, 4) void logits_kernel(Launch l)
         }
     }
 
-    float scale = 1.0f, top = 0.0f, factor = 0.0f;
+    Factor scale = {};
+    float top = 0.0f;
     Part part = {};
-    bool soft = false;
     if constexpr (S != Step::adjust)
     {
-        const float temperature = r.temperature ? r.temperature[s] : 1.0f;
-        soft = temperature > 0.0f;
         if constexpr (S == Step::finish)
         {
             const Part* const parts = l.parts + std::size_t(row) * l.splits;
             part = parts[0];
             for (int i = 1; i < l.splits; ++i)
             {
-                part = join(part, parts[i], temperature);
+                part = join(part, parts[i], soft, factor);
             }
         }
         else
         {
-            part = part_of<Vectors>(x, from, temperature, shared);
+            part = part_of<Vectors>(x, from, soft, factor, shared);
         }
         if constexpr (S == Step::parts)
         {
@@ -515,8 +545,11 @@ __global__ __launch_bounds__(most_threads, 4) void logits_kernel(Launch l)
             return;
         }
         top = reference(part.top);
-        factor = factor_of(temperature);
-        scale = part.sum == 0.0f ? 0.0f : 1.0f / part.sum;
+        if (part.sum != 0.0f)
+        {
+            scale.high = 1.0f / part.sum;
+            scale.low = __builtin_fmaf(-scale.high, part.sum, 1.0f) * scale.high;
+        }
     }
     const std::size_t at = std::size_t(row) * l.rows.out_stride;
 #pragma unroll
@@ -534,7 +567,7 @@ __global__ __launch_bounds__(most_threads, 4) void logits_kernel(Launch l)
             {
                 if (soft)
                 {
-                    x[i][e] = (S == Step::whole ? x[i][e] : weight(x[i][e], top, factor)) * scale;
+                    x[i][e] = times(S == Step::whole ? x[i][e] : weight(x[i][e], top, factor), scale);
                 }
                 else
                 {
