@@ -197,3 +197,14 @@ def test_bindings_check_their_tensors():
                 dict(allowed=ints(3, 4)), dict(allowed=ints(4)), {}]:
         with pytest.raises(native.HipError):
             native.adjust_logits(**dict(dict(logits=logits, out=logits.clone(), starts=ints(3)), **bad))
+
+
+def test_biases_come_with_their_starts():
+    """Tokens and values alone are no biases of any sequence: refused, not passed over."""
+    torch = pytest.importorskip("torch")
+    logits, starts = torch.zeros(4, 100), torch.zeros(3, dtype=torch.int32)
+    tokens, values = torch.zeros(2, dtype=torch.int32), torch.zeros(2)
+    for some in (dict(bias_tokens=tokens, bias_values=values), dict(bias_tokens=tokens), dict(bias_values=values),
+                 dict(bias_starts=starts, bias_tokens=tokens), dict(bias_starts=starts, bias_values=values)):
+        with pytest.raises(native.HipError, match="biases"):
+            native.adjust_logits(logits, logits.clone(), starts, **some)

@@ -1367,8 +1367,8 @@ def adjust_logits(logits, out, starts, probabilities=True, history=None, history
         if allowed.dim() != 2 or allowed.shape[1] < (alphabet + 31) // 32 or allowed.shape[0] not in (1, rows):
             raise HipError(f"allowed: must be [{rows}][{(alphabet + 31) // 32}], or of one row")
         stride = allowed.shape[1] if allowed.shape[0] == rows and rows > 1 else 0
-    if bias_starts is not None:
-        if bias_tokens is None or bias_values is None:
+    if bias_starts is not None or bias_tokens is not None or bias_values is not None:
+        if bias_starts is None or bias_tokens is None or bias_values is None:
             raise HipError("biases: need starts, tokens and values")
         biases = bias_tokens.numel()
     rules = _logit_rules(
