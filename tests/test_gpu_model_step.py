@@ -194,6 +194,33 @@ def test_products_of_model_sizes(torch, native, kind, rows, inputs, outputs):
     check_product(torch, native, rows, inputs, outputs, kind, seed=5)
 
 
+# Sizes for which each variant of many rows has workgroups that go on from one tile to the next, of 256 units: tiles of outputs
+# x rows, and tiles a workgroup at most.
+SEVERAL_TILES = [(1000, 20000),  # 128 x 128, 5
+                 (128, 70000),  # 128 x 128, one row tile, 3
+                 (700, 30000),  # 128 x 256, 3
+                 (256, 90000),  # 128 x 256, one row tile, 3
+                 (8190, 4096),  # 256 x 256, 2
+                 (4999, 5001),  # 256 x 256, 2
+                 (240, 120000),  # 256 x 256, one row tile, 2
+                 (12000, 300)]  # 64 x 64, 2
+
+
+@pytest.mark.parametrize("rows,outputs", SEVERAL_TILES)
+def test_products_of_several_tiles_a_workgroup(torch, native, rows, outputs):
+    """Every element, of one stage a tile to more than a ring holds, in all types, stored in whole vectors and one by one."""
+    for i, inputs in enumerate((1, 64, 100, 128, 129, 256, 700)):
+        linear, w, c, b = linear_of(torch, native, outputs, inputs, i, bias=i % 2 == 0)
+        q, s = tokens_of(torch, rows, inputs, i + 1)
+        exact = (q.double() @ w.double().T) * (s.double()[:, None] * c.double())
+        y = exact if b is None else exact + b.double()
+        for j, kind in enumerate(KINDS):
+            out = Inside(torch, rows, outputs, kind, offset=3 if (i + j) % 4 == 3 else 0)
+            linear.apply(q, s, out.view)
+            near(torch, out.view, y, 3.01 * H * exact.abs() + H * y.abs() + UNIT[kind] * (1 + 4 * H) * y.abs() + TINY[kind])
+            out.rest_stays()
+
+
 @pytest.mark.parametrize("rows", [1, 40, 300])
 def test_products_of_the_longest_sums(torch, native, rows):
     """Sums up to 128 x 128 x 131071 = 2^31 - 16384."""
@@ -800,6 +827,52 @@ def test_rules_one_at_a_time(torch, native, aligned):
 def test_long_histories_and_many_nodes(torch, native):
     logits = Logits(torch, [200, 1, 90], 300, "float32", history=30000, seed=4, drafted="trees")
     logits.check(native, "float32")
+
+
+@pytest.mark.parametrize("past,words", [(32703, 1), (32704, 1), (32767, 0), (32768, 0)])
+def test_counts_at_the_end_of_16_bits(torch, native, past, words):
+    """One token all along a history, on both sides of the sizes at which a count and a bias no longer share a word."""
+    alphabet, rows = 300, 64 if words else 1
+    x = normal(torch, (rows, alphabet), past, "float32", 4.0)
+    rules = dict(history=ints(torch, [[7] * past]), history_lengths=ints(torch, [past]), frequency=floats(torch, [2.0 ** -10]),
+                 presence=floats(torch, [0.25]), bias_starts=ints(torch, [0, 2]), bias_tokens=ints(torch, [7, 8]),
+                 bias_values=floats(torch, [0.5, -0.5]))
+    if words:  # each node of the same token, on the line of those in front of it
+        mask = [(1 << (r + 1)) - 1 for r in range(rows)]
+        rules.update(tokens=ints(torch, [7] * rows), mask=torch.from_numpy(np.array(mask, np.uint64).view(np.int64))[:, None].cuda())
+    counts = past + (torch.arange(rows, device="cuda").double() + 1 if words else torch.zeros(1, device="cuda").double())
+    want = x.double()
+    want[:, 7] = want[:, 7] - counts / 1024 - 0.25 + 0.5
+    want[:, 8] -= 0.5
+    out = torch.empty_like(x)
+    native.adjust_logits(x, out, ints(torch, [0, rows]), probabilities=False, **rules)
+    # The count's product, then two sums more of numbers below 2^6.
+    near(torch, out, want, torch.full_like(want, 3 * H * 64))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("alphabet", [300, 8200, 16384, 32000, 50001, 128001])
+def test_histories_past_16_bits_of_count(torch, native, kind, alphabet):
+    """Counts and biases in words of their own, in each number of a thread's eights."""
+    logits = Logits(torch, [2, 1, 0, 3], alphabet, kind, history=40000, seed=alphabet, biases=300, drafted="trees",
+                    aligned=alphabet != 8200)
+    logits.check(native, "float32")
+    logits.check(native, kind, probabilities=False)
+
+
+def test_more_biases_than_16_bits(torch, native):
+    """Tokens that are listed many times, past the 65,535th bias of a sequence: the last one counts."""
+    logits = Logits(torch, [2, 1], 20000, "float32", history=100, seed=5, biases=0)
+    rng = np.random.default_rng(6)
+    starts, tokens = [0, 90000, 160000], rng.integers(0, 20002, 160000)
+    values = rng.normal(size=160000).astype(np.float32)
+    for s in range(2):
+        for i in range(starts[s], starts[s + 1]):
+            if tokens[i] < 20000:
+                logits.bias[s, tokens[i]] = values[i]
+    logits.rules.update(bias_starts=ints(torch, starts), bias_tokens=ints(torch, tokens), bias_values=floats(torch, values))
+    logits.check(native, "float32")
+    logits.check(native, "bfloat16", probabilities=False)
 
 
 def test_lengths_of_histories_out_of_range(torch, native):
