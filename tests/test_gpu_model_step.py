@@ -1155,6 +1155,61 @@ def test_a_step_of_a_model(torch, native):
     assert step.path[:, 0].tolist() == [0] * len(p.counts)
 
 
+def to_8_bits(q, scales, h, error):
+    """Rows h that are off by at most `error`, as 8 bits and a scale each."""
+    top = h.abs().amax(1)
+    assert bool(((scales.double() - top / 127).abs() <= error.amax(1) / 127 + 2 * H * top / 127 + 2.0 ** -149).all())
+    off = (q.double() * scales.double()[:, None] - h).abs()
+    assert bool((off <= (0.5 + 2.0 ** -16) * scales.double()[:, None] + error).all())
+
+
+def test_norms_rules_and_verification_of_a_step(torch, native):
+    """What one stage hands to the next, each held against its definition on what it was given."""
+    from test_gpu_drafts import verify_plain
+
+    step = Step(torch, native, seed=7, counts=(6, 1, 12))
+    p, (width, heads, kv, hw) = step.p, step.dims
+    step.run()
+    # Some drafted tokens are the likeliest behind their parents, so that there is something to accept.
+    likely = step.probs.argmax(1).tolist()
+    tokens = step.tokens.tolist()
+    for s, count in enumerate(p.counts):
+        for i in range(1, count, 2):
+            tokens[p.starts_list[s] + i] = likely[p.starts_list[s] + step.parents[p.starts_list[s] + i]]
+    step.tokens.copy_(ints(torch, tokens))
+    step.uniforms.mul_(2.0 ** -12)
+    step.run()
+    rms = step.x.bfloat16().double()
+    to_8_bits(step.q, step.s, *normed(torch, rms, torch.zeros_like(rms), native.NORM_RMS, step.gain, None, 1e-5))
+    block = step.block.double()
+    u, e = normed(torch, block, torch.zeros_like(block), native.NORM_RMS, step.gain, None, 1e-5)
+    total = step.x.double() + 0.5 * u
+    e = 0.5 * e + H * total.abs()  # halves are exact
+    near(torch, step.after, total, e + H * (total.abs() + e) + TINY["float32"])
+    to_8_bits(step.q3, step.s3, *normed(torch, total, e, native.NORM_LAYER, None, None, 1e-5))
+    rules = Logits(torch, p.counts, step.alphabet, "float32", biases=0, allowed=None, temperature=False, prompt=False)
+    n = len(p.counts)
+    rules.logits, rules.history, rules.lengths = step.logits, step.history.cpu().numpy(), step.history_lengths.cpu().numpy()
+    rules.prompts, rules.tokens, rules.lines = np.zeros(n, np.int64), np.array(tokens), []
+    for s, count in enumerate(p.counts):
+        lines = []
+        for i in range(count):
+            parent = step.parents[p.starts_list[s] + i]
+            lines.append({i} | (lines[parent] if parent >= 0 else set()))
+        rules.lines += lines
+    rules.repetition, rules.presence, rules.frequency = np.full(n, 1.2, np.float32), np.zeros(n), np.zeros(n)
+    want, room = rules.probabilities()
+    near(torch, step.probs, want, room + H * want + TINY["float32"])
+    probs, uniforms, draws = (t.cpu().numpy() for t in (step.probs, step.uniforms, step.draws))
+    for s, count in enumerate(p.counts):
+        part = slice(p.starts_list[s], p.starts_list[s] + count)
+        path, following = verify_plain(probs[part], None, tokens[part], step.parents[part], uniforms[part], draws[s])
+        got = int(step.accepted[s])
+        assert (step.path[s, :got].tolist(), int(step.next[s])) == (path, following)
+        assert step.path[s, got:].tolist() == [-1] * (p.max_rows - got)
+    assert int(step.accepted.max()) > 2
+
+
 def test_a_captured_step(torch, native):
     """Replays between other work give what the calls give, on new inputs too."""
     step = Step(torch, native, seed=3)
