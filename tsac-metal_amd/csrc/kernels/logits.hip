@@ -19,8 +19,8 @@
 // rules 34, adjusted without a softmax 40 (27 without rules). What is left is some 30 instructions a token and the waits
 // between the phases of two workgroups a unit. Rows in 1,024 threads left one workgroup a unit or spilled (100 us);
 // spilled registers alone cost 5 us, penalties by branches 25, since most waves have a token of the history in each place.
-// Quotients are products with factors of two floats, each rounded once (1 us; with factors of one float, probabilities far below
-// the largest were off by twice as much).
+// For results of 32 bits, quotients are products with factors of two floats, each rounded once (24 rows of 128,001: 1 us of 27; with
+// factors of one float, probabilities far below the largest were off by twice as much).
 #include "lanes.hpp"
 #include "model_step.hpp"
 #include "paged_device.hpp"
@@ -154,30 +154,30 @@ struct Exchange
 };
 
 // A factor as the sum of two floats, so that a product with it is rounded once: a rounded factor would be off in one direction
-// for all tokens of a row.
+// for all tokens of a row. Results of 16 bits, whose own rounding is 2^12 times as much at least, take the first float alone.
 struct Factor
 {
     float high, low;
 };
-__device__ __forceinline__ float times(float x, const Factor& by)
+template <bool Fine> __device__ __forceinline__ float times(float x, const Factor& by)
 {
-    return __builtin_fmaf(x, by.high, x * by.low);
+    return Fine ? __builtin_fmaf(x, by.high, x * by.low) : x * by.high;
 }
 
 // (a + rest) / b of numbers above 0, from a / b. Both parts are above 0, so that infinities stay what they are; where a / b is far
 // out there is no second one to speak of.
-__device__ __forceinline__ Factor divided(float quotient, float a, float rest, float b)
+template <bool Fine> __device__ __forceinline__ Factor divided(float quotient, float a, float rest, float b)
 {
-    const bool near = quotient > 0x1p-100f && quotient < 0x1p100f;
+    const bool near = Fine && quotient > 0x1p-100f && quotient < 0x1p100f;
     const float high = near ? __uint_as_float(__float_as_uint(quotient) - 1) : quotient;
     const float low = (__builtin_fmaf(-high, b, a) + rest) * __builtin_amdgcn_rcpf(b);
     return {high, near ? __builtin_fmaxf(low, little) : little};
 }
 
 // e^((x - top) / t) as a power of two, of a finite top. -infinity gives 0, what is not a number and +infinity no number.
-__device__ __forceinline__ float weight(float x, float top, const Factor& per_log2)
+template <bool Fine> __device__ __forceinline__ float weight(float x, float top, const Factor& per_log2)
 {
-    return __builtin_amdgcn_exp2f(times(x - top, per_log2));
+    return __builtin_amdgcn_exp2f(times<Fine>(x - top, per_log2));
 }
 
 // What stands for the largest of a row in which nothing is above -infinity: its weights are 0, or no numbers.
@@ -188,17 +188,16 @@ __device__ __forceinline__ float reference(float top)
 
 // A temperature's factor; where that would be infinite the largest number, which times 0 is still 0, where it would be 0 a
 // small one, which times -infinity is still that.
-__device__ __forceinline__ Factor factor_of(float temperature)
+template <bool Fine> __device__ __forceinline__ Factor factor_of(float temperature)
 {
     const float quotient = __builtin_fmaxf(__builtin_fminf(log2e / temperature, 0x1.fffffep127f), 0x1p-126f);
-    return divided(quotient, log2e, log2e_rest, temperature);
+    return divided<Fine>(quotient, log2e, log2e_rest, temperature);
 }
 
 // What is known of values held in registers: the largest and its lowest place, the sum of weights, which stand in the
 // values' place afterwards.
-template <int Vectors>
-__device__ __forceinline__ Part part_of(float (&x)[Vectors][8], int from, bool soft, const Factor& factor,
-                                        Exchange& shared)
+template <bool Fine, int Vectors>
+__device__ __forceinline__ Part part_of(float (&x)[Vectors][8], int from, bool soft, const Factor& factor, Exchange& shared)
 {
     Part part;
     float top = minus_infinity;
@@ -224,7 +223,7 @@ __device__ __forceinline__ Part part_of(float (&x)[Vectors][8], int from, bool s
 #pragma unroll
             for (int e = 0; e < 8; ++e)
             {
-                x[i][e] = weight(x[i][e], reference(top), factor);
+                x[i][e] = weight<Fine>(x[i][e], reference(top), factor);
                 sum += x[i][e];
             }
         }
@@ -251,7 +250,7 @@ __device__ __forceinline__ Part part_of(float (&x)[Vectors][8], int from, bool s
 }
 
 // A later part joined to what is in front of it.
-__device__ __forceinline__ Part join(const Part& a, const Part& b, bool soft, const Factor& factor)
+template <bool Fine> __device__ __forceinline__ Part join(const Part& a, const Part& b, bool soft, const Factor& factor)
 {
     Part r;
     r.top = __builtin_fmaxf(a.top, b.top);
@@ -261,8 +260,8 @@ __device__ __forceinline__ Part join(const Part& a, const Part& b, bool soft, co
     if (soft)
     {
         // A part without a number above -infinity has a sum of 0, or none that is a number.
-        const float wa = a.top == r.top ? 1.0f : weight(a.top, r.top, factor);
-        const float wb = b.top == r.top ? 1.0f : weight(b.top, r.top, factor);
+        const float wa = a.top == r.top ? 1.0f : weight<Fine>(a.top, r.top, factor);
+        const float wb = b.top == r.top ? 1.0f : weight<Fine>(b.top, r.top, factor);
         r.sum = (a.top == minus_infinity ? a.sum : a.sum * wa) + (b.top == minus_infinity ? b.sum : b.sum * wb);
     }
     return r;
@@ -282,8 +281,8 @@ template <bool Wide> struct Raw
     uint4 v[Wide ? 2 : 1];
 };
 
-// Rounds: how often LDS holds the words of a part of the workgroup's tokens.
-template <Step S, bool Wide, int Vectors, int Rounds, bool Narrow>
+// Rounds: how often LDS holds the words of a part of the workgroup's tokens. Wide: logits of 32 bits; Fine: results of 32 bits.
+template <Step S, bool Wide, int Vectors, int Rounds, bool Narrow, bool Fine>
 __global__ __launch_bounds__(most_threads, 4) void logits_kernel(Launch l)
 {
     constexpr int held = Vectors / Rounds; // eights of a thread in a round
@@ -357,8 +356,8 @@ __global__ __launch_bounds__(most_threads, 4) void logits_kernel(Launch l)
     const float frequency = r.frequency ? r.frequency[s] : 0.0f;
     const float temperature = S != Step::adjust && r.temperature ? r.temperature[s] : 1.0f;
     const bool soft = temperature > 0.0f;
-    const Factor factor = factor_of(temperature);
-    const Factor inverse = divided(1.0f / __builtin_fabsf(repetition), 1.0f, 0.0f, __builtin_fabsf(repetition));
+    const Factor factor = factor_of<Fine>(temperature);
+    const Factor inverse = divided<Fine>(1.0f / __builtin_fabsf(repetition), 1.0f, 0.0f, __builtin_fabsf(repetition));
     const float reciprocal = __builtin_copysignf(inverse.high, repetition);
     const float reciprocal_rest = __builtin_copysignf(inverse.low, repetition);
     const bool edited = l.counted || bias_begin < bias_end;
@@ -488,8 +487,9 @@ __global__ __launch_bounds__(most_threads, 4) void logits_kernel(Launch l)
                 {
                     const float count = float(said[e] >> 1);
                     const bool above = x[i][e] > 0.0f;
-                    const float rest = said[e] && above ? x[i][e] * reciprocal_rest : 0.0f;
-                    x[i][e] = __builtin_fmaf(x[i][e], said[e] ? (above ? reciprocal : repetition) : 1.0f, rest);
+                    const float rest = Fine && said[e] && above ? x[i][e] * reciprocal_rest : 0.0f;
+                    const float by = said[e] ? (above ? reciprocal : repetition) : 1.0f;
+                    x[i][e] = Fine ? __builtin_fmaf(x[i][e], by, rest) : x[i][e] * by;
                     x[i][e] = __builtin_fmaf(-frequency, count, x[i][e]);
                     x[i][e] = __builtin_fmaf(-presence, __builtin_fminf(count, 1.0f), x[i][e]);
                 }
@@ -529,12 +529,12 @@ __global__ __launch_bounds__(most_threads, 4) void logits_kernel(Launch l)
             part = parts[0];
             for (int i = 1; i < l.splits; ++i)
             {
-                part = join(part, parts[i], soft, factor);
+                part = join<Fine>(part, parts[i], soft, factor);
             }
         }
         else
         {
-            part = part_of<Vectors>(x, from, soft, factor, shared);
+            part = part_of<Fine>(x, from, soft, factor, shared);
         }
         if constexpr (S == Step::parts)
         {
@@ -567,7 +567,7 @@ __global__ __launch_bounds__(most_threads, 4) void logits_kernel(Launch l)
             {
                 if (soft)
                 {
-                    x[i][e] = times(S == Step::whole ? x[i][e] : weight(x[i][e], top, factor), scale);
+                    x[i][e] = times<Fine>(S == Step::whole ? x[i][e] : weight<Fine>(x[i][e], top, factor), scale);
                 }
                 else
                 {
@@ -580,9 +580,15 @@ __global__ __launch_bounds__(most_threads, 4) void logits_kernel(Launch l)
             constexpr Type T = decltype(type)::value;
             store8<T>(static_cast<value_t<T>*>(l.rows.out) + at + token, to - token, l.aligned, x[i]);
         };
-        l.rows.out_type == Type::single ? store(std::integral_constant<Type, Type::single>{})
-        : l.rows.out_type == Type::bf16 ? store(std::integral_constant<Type, Type::bf16>{})
-                                        : store(std::integral_constant<Type, Type::half>{});
+        if constexpr (Fine)
+        {
+            store(std::integral_constant<Type, Type::single>{});
+        }
+        else
+        {
+            l.rows.out_type == Type::bf16 ? store(std::integral_constant<Type, Type::bf16>{})
+                                          : store(std::integral_constant<Type, Type::half>{});
+        }
     }
 }
 
@@ -624,9 +630,9 @@ template <Step S> void launch(const Launch& l, const Shape& s, bool narrow, hipS
         const std::size_t bytes = std::size_t(8 * s.threads) * held * each * 4;
         kernel<<<grid, unsigned(s.threads), bytes, stream>>>(l);
     };
-    const auto of = [&](auto wide, auto few)
+    const auto of = [&](auto wide, auto few, auto fine)
     {
-        constexpr bool W = decltype(wide)::value, N = decltype(few)::value;
+        constexpr bool W = decltype(wide)::value, N = decltype(few)::value, F = decltype(fine)::value;
         constexpr int each = Words<N>::each;
         // Words of at most 64 KiB at a time, so that a unit has two workgroups.
         constexpr int most = N ? 4 : 2;
@@ -634,21 +640,21 @@ template <Step S> void launch(const Launch& l, const Shape& s, bool narrow, hipS
         {
             if (s.vectors == most_vectors)
             {
-                return go(logits_kernel<S, W, most_vectors, most_vectors / most, N>, most, each);
+                return go(logits_kernel<S, W, most_vectors, most_vectors / most, N, F>, most, each);
             }
         }
-        s.vectors == 1   ? go(logits_kernel<S, W, 1, 1, N>, 1, each)
-        : s.vectors == 2 ? go(logits_kernel<S, W, 2, 1, N>, 2, each)
-                         : go(logits_kernel<S, W, 4, 4 / most, N>, most, each);
+        s.vectors == 1   ? go(logits_kernel<S, W, 1, 1, N, F>, 1, each)
+        : s.vectors == 2 ? go(logits_kernel<S, W, 2, 1, N, F>, 2, each)
+                         : go(logits_kernel<S, W, 4, 4 / most, N, F>, most, each);
     };
-    if (l.rows.type == Type::single)
-    {
-        narrow ? of(std::true_type{}, std::true_type{}) : of(std::true_type{}, std::false_type{});
-    }
-    else
-    {
-        narrow ? of(std::false_type{}, std::true_type{}) : of(std::false_type{}, std::false_type{});
-    }
+    const auto chosen = [](bool yes, auto next) { yes ? next(std::true_type{}) : next(std::false_type{}); };
+    chosen(l.rows.type == Type::single,
+           [&](auto wide)
+           {
+               chosen(narrow,
+                      [&](auto few)
+                      { chosen(l.rows.out_type == Type::single, [&](auto fine) { of(wide, few, fine); }); });
+           });
     check_hip(hipGetLastError(), "logits launch");
 }
 } // namespace
