@@ -9,11 +9,15 @@
 // q of 8 bits and a scale a row: scale = max |h| * fl(1 / 127), q = h / scale to the nearest, ties to even.
 // Nothing is rounded in between: h is the norm of the sum before it is rounded for its store.
 //
-// A row's values stay in the registers of its threads, so that the mean, the squares around it and
+// Up to 16,384 values a row's stay in the registers of its threads, so that the mean, the squares around it and
 // the largest value each are a pass over registers, in 32 bits and in an order that depends on the
 // width alone; a row of up to 1,024 values is one wave's, or a part of one's, which needs no barrier. What bounds it is
-// memory: 8190 rows of 8192, BF16, with a residual of 32 bits in 167 us, where a copy of their bytes takes 169; to 8 bits
-// in 49 (42).
+// memory: 8190 rows of 8192, BF16, with a residual of 32 bits in 164 us, where a copy of their bytes takes 169; rows to 8 bits
+// in 46 (42), and with a norm in front of that 75.
+//
+// Longer rows do not fit a lane's 128 registers: 112 to 825 of a lane's values go through scratch memory, and rows are read as
+// those of any alignment. Odd widths past 8,192 leave 1 to 41 there, and in FP32 odd ones of 513 to 1,024 and from 4,097 on 1 to 6.
+// A norm of 67 M values, BF16, 57 us as a copy: 55 at width 16384, 98 at 12289, 370 at 16385, 217 at 32768, 610 at 65536.
 #include "lanes.hpp"
 #include "model_step.hpp"
 #include "values.hpp"
@@ -237,7 +241,7 @@ enum Aligned
 
 // T: the values; R: the residual. A row is taken by Threads threads, each Vectors times eight values. Unless they are
 // `any`, a workgroup takes rows one after the other, and the next one's are on their way while one is worked on: they pass
-// barriers, which are for LDS alone. 8190 rows of 8192 with a residual of 32 bits: 167 us, a row a workgroup 204.
+// barriers, which are for LDS alone. 8190 rows of 8192 with a residual of 32 bits: a row a workgroup, without that, 204 us for 167.
 template <Type T, Type R, int Vectors, int Threads, Rows M>
 __global__ __launch_bounds__(Threads > 256 ? Threads : 256, 4) void block_norm_kernel(BlockRows p, int aligned)
 {

@@ -111,7 +111,7 @@ __device__ __forceinline__ void ring_barrier()
 // step of 128 inputs, through a ring of Ring steps in LDS of its own: it asks for a step as soon as it has read the one
 // whose place that takes, and waits for nobody until the waves' sums meet. Rows of activations come in whole lines of 128 bytes,
 // which straight into registers, 32 bytes of each of 32 rows at a time, they would not (48 rows, 8192 x 8192: 26 us
-// for 16 now, where reading the weights takes 11), their pieces exchanged by row so that eight rows' meet different banks.
+// for 17 now, where reading the weights takes 10), their pieces exchanged by row so that eight rows' meet different banks.
 // More steps in flight, or eight waves, gain nothing (rings of 3 and 4: 17 us) and keep a unit from a second workgroup.
 namespace narrow
 {
@@ -668,10 +668,10 @@ struct Tiles
 constexpr Tiles tiles[] = {{256, 256, 0.85, 6.5}, {128, 256, 0.50, 3.7}, {128, 128, 0.29, 2.0}, {64, 64, 0.115, 0.8}};
 
 // Which of them: the least time by what one costs and how many of them the fullest compute unit has. Large tiles share
-// more of what they read, small ones are more of a few rows' work at once. Measured, us (256 x 256, 128 x 256, 128 x 128,
-// 64 x 64): 128 rows x 4096 x 4096 49, 30, 19, 10.8; 1024 x 1024 x 4096 20, 13.7, 10.6, 11.8; 512 x 8192 x 8192 101, 73,
-// 44, 70; 1024 x 8192 x 8192 103, 79, 83, 131; 4096 x 4096 x 4096 68, 75, 84, 113; 30960 x 1024 x 4096 165, 178, 198, 255.
-// By this rule: 10.8, 10.6, 44, 79, 68, 165.
+// more of what they read, small ones are more of a few rows' work at once. Measured with eight layers' weights in turn, us
+// (256 x 256, 128 x 256, 128 x 128, 64 x 64): 128 rows x 4096 x 4096 49, 30, 19, 10.8; 1024 x 1024 x 4096 20, 13.7, 10.6, 11.8;
+// 512 x 8192 x 8192 101, 73, 44, 70; 1024 x 8192 x 8192 103, 79, 83, 131; 4096 x 4096 x 4096 68, 75, 84, 113; 30960 x 1024 x
+// 4096 165, 178, 198, 255. By this rule: 10.8, 10.6, 44, 79, 68, 165.
 int tiles_for(const Launch& l)
 {
     int best = 0;

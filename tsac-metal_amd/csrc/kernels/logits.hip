@@ -15,10 +15,11 @@
 // store. Longer ones are divided: one launch leaves each part's maximum and sum, another joins them in
 // ascending order and computes the part again. Logits are asked for before anything is counted.
 //
-// 902 rows of 32,000 with a history of 4,093, BF16 to half: 63 us, where a copy of their bytes takes 25; without
-// rules 34, adjusted without a softmax 40 (27 without rules). What is left is some 30 instructions a token and the waits
-// between the phases of two workgroups a unit. Rows in 1,024 threads left one workgroup a unit or spilled (100 us);
-// spilled registers alone cost 5 us, penalties by branches 25, since most waves have a token of the history in each place.
+// 902 rows of 32,000 with a history of 4,093, BF16 to half, six batches in turn: 62 us, where a copy of their bytes
+// takes 25; without rules 40, adjusted without a softmax 48 (32 without rules). What is left is some 30 instructions a
+// token and the waits between the phases of two workgroups a unit. Rows in 1,024 threads left one workgroup a unit or
+// spilled (100 us); spilled registers alone cost 5 us, penalties by branches 25, since most waves have a token of the
+// history in each place.
 // For results of 32 bits, quotients are products with factors of two floats, each rounded once (24 rows of 128,001: 1 us of 27; with
 // factors of one float, probabilities far below the largest were off by twice as much).
 #include "lanes.hpp"
@@ -154,7 +155,8 @@ struct Exchange
 };
 
 // A factor as the sum of two floats, so that a product with it is rounded once: a rounded factor would be off in one direction
-// for all tokens of a row. Results of 16 bits, whose own rounding is 2^12 times as much at least, take the first float alone.
+// for all tokens of a row. Results of 16 bits, whose own rounding is at least 2^7 times what that makes of them, take the first
+// float alone.
 struct Factor
 {
     float high, low;
@@ -608,9 +610,9 @@ Shape shape_of(const LogitRows& rows, std::size_t history)
     s.vectors = rounds <= 1 ? 1 : rounds <= 2 ? 2 : rounds <= 4 ? 4 : most_vectors;
     if (rounds > most_vectors || !rows.probabilities)
     {
-        // Parts, then: of four eights a thread (902 rows of 32,000, adjusted alone: 40 us, of eight 51, of two 49), of
-        // fewer where rows are few, for a workgroup a unit at least, if there are as many (24 rows of 128,001 in parts
-        // of 16,384, 8,192 and 4,096 tokens: 27.4, 26.9 and 43 us).
+        // Parts, then: of four eights a thread (902 rows of 32,000, adjusted alone, one batch again and again: 40 us, of eight
+        // 51, of two 49), of fewer where rows are few, for a workgroup a unit at least, if there are as many (24 rows of
+        // 128,001 in parts of 16,384, 8,192 and 4,096 tokens: 27.4, 26.9 and 43 us).
         s.vectors = std::min(s.vectors, 4);
         while (s.vectors > 1 && std::size_t(rows.rows) * ((rounds + s.vectors - 1) / s.vectors) < std::size_t(units))
         {
